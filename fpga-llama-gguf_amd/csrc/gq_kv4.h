@@ -1,0 +1,77 @@
+// The 4-bit KV cache (Q4_0 blocks of 32 elements along head_dim): its layout, and the launch descriptors of the kernels on it.
+//
+// A block x[0..31]: m = its element of largest magnitude (the first of them), d = m / -8, q = min(15, int(x / d + 8.5)) with
+// x / d formed as x * (1 / d), all in FP32 (ggml's Q4_0); it holds fp16(d) and the sixteen values, and stands for fp16(d) * (q - 8).
+//
+// Per sequence and KV head the cache is a row of records of 32 positions each, NB = head_dim / 32 blocks a position:
+//   Kq  16 head_dim bytes  [sub 2][c][g 4][p 16][b][e 4]: byte of block 4 c + b (b < min(NB, 4)) at position 16 sub + p; low nibble
+//                          element 32 block + 4 g + e, high nibble the one 16 further (the two halves of a byte as in ggml)
+//   Vq  16 head_dim bytes  [c][g 4][n 16][b][sub 2][r 4]: byte of block 2 c + b (b < min(NB, 2)) at position 16 sub + 4 g + r; low
+//                          nibble element 32 block + n, high nibble the one 16 further
+//   Kd, Vd  2 head_dim bytes each  [g 4][block][sub 2][r 4]: fp16 scale of position 16 sub + 4 g + r
+// The order is that of the matrix instructions' operands (16x16x32): lane 16 g + p of a wave finds the key bytes of its position, and
+// lane 16 g + n the value bytes of its element at 8 positions, as consecutive 16-byte pieces, whole 1 KB lines a load. Every byte
+// belongs to one position, so a position is written without reading its neighbours.
+#pragma once
+#include "gq_kernels.h"
+
+namespace gq {
+
+constexpr int KV4_TILE = 32;  // positions of a record
+
+__host__ __device__ constexpr bool kv4_dim_ok(int hd) { return hd == 32 || hd == 64 || hd == 128 || hd == 256; }
+__host__ __device__ constexpr size_t kv4_record(int hd) { return size_t(36) * hd; }
+__host__ __device__ constexpr int kv4_tiles(int n_ctx) { return (n_ctx - 1) / KV4_TILE + 1; }
+
+// Offsets in a record of position p (0..31): the key byte of element e < 16 of block blk (its high nibble: element e + 16),
+// the value byte likewise, and the scale of the block (bytes from the start of Kd or Vd).
+template <int HD>
+struct Kv4Layout {
+    static constexpr int NB = HD / 32, KB = NB < 4 ? NB : 4, VB = NB < 2 ? NB : 2;
+    static constexpr int VQ = 16 * HD, KD = 32 * HD, VD = 34 * HD, RECORD = 36 * HD;
+    __device__ static int kq(int p, int blk, int e) {
+        return (p >> 4) * 8 * HD + (blk / KB) * 256 * KB + ((e >> 2) * 16 + (p & 15)) * 4 * KB + (blk % KB) * 4 + (e & 3);
+    }
+    __device__ static int vq(int p, int blk, int e) {
+        return VQ + (blk / VB) * 512 * VB + (((p & 15) >> 2) * 16 + e) * 8 * VB + (blk % VB) * 8 + (p >> 4) * 4 + (p & 3);
+    }
+    __device__ static int scale(int p, int blk) { return ((((p & 15) >> 2) * NB + blk) * 8 + (p >> 4) * 4 + (p & 3)) * 2; }
+};
+
+// Tokens t < num[s] (num NULL: n_tok) of sequence s are at positions pos[s * pos_stride] + t; the ones outside 0 .. n_ctx - 1 are
+// not touched.
+struct Kv4Tokens {
+    const int32_t * pos;
+    const int32_t * num;
+    int pos_stride, n_tok, n_seq;
+};
+
+struct Kv4Cache {
+    uint8_t * data;
+    int n_ctx, tiles, n_head_kv, head_dim;  // tiles: records of a sequence and KV head
+};
+
+struct Kv4RowsArgs {  // store or load: row (s * n_tok + t) of k and v at row_stride floats, KV heads packed
+    Kv4Cache c;
+    Kv4Tokens t;
+    float * k;
+    float * v;
+    long long row_stride;
+};
+
+struct Kv4AttnArgs {
+    Kv4Cache c;
+    Kv4Tokens t;
+    const float * q;  // row (s * n_tok + t) at q_row floats, head h at q_head floats
+    float * y;        // row (s * n_tok + t) at y_row floats, heads packed
+    long long q_row, q_head, y_row;
+    int n_head, window;  // window 0: every position up to the token's own
+    float scale;
+    const float * gate;  // NULL, or gate rows as q's (the output times sigmoid(gate))
+};
+
+hipError_t launch_kv4_store(const Kv4RowsArgs & a, hipStream_t s);
+hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s);
+hipError_t launch_kv4_attn(const Kv4AttnArgs & a, hipStream_t s);
+
+}  // namespace gq

@@ -3,8 +3,10 @@
 // buffers, are staged here in `scratch`, a fixed device array of this file (one copy per device, held until the
 // process ends). Nothing here allocates: the array's address on a device is looked up once, on the first call on
 // that device, and kept.
+// The 4-bit KV cache on caller-owned memory (gemvq_kv4_*_static): its arguments' checks and launches.
 #include "gemvq_hip.h"
 #include "gq_kernels.h"
+#include "gq_kv4.h"
 
 #include <hip/hip_runtime.h>
 
@@ -39,6 +41,40 @@ int scratch_on(int dev, uint8_t ** out) {
 }
 
 bool aligned(const void * p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+
+// Rows of floats that the kernels read and write in 16-byte pieces.
+bool rows_ok(const void * p, int64_t stride, int64_t least) {
+    return p && aligned(p, 16) && stride % 4 == 0 && stride >= least && stride <= (int64_t(1) << 40);
+}
+
+constexpr int GRID_MAX = 65535;
+
+bool kv4_ok(const gemvq_kv4 * c) {
+    return c && c->data && aligned(c->data, 256) && c->n_seq > 0 && c->n_seq <= GRID_MAX && c->n_ctx > 0 && c->n_head_kv > 0 &&
+           c->n_head_kv <= GRID_MAX && kv4_dim_ok(c->head_dim);
+}
+
+Kv4Cache kv4_cache(const gemvq_kv4 * c) {
+    return {static_cast<uint8_t *>(c->data), c->n_ctx, kv4_tiles(c->n_ctx), c->n_head_kv, c->head_dim};
+}
+
+bool kv4_tokens(const gemvq_kv4 * c, int n_tok, const int32_t * pos, const int32_t * num, Kv4Tokens & t) {
+    if (n_tok < 1 || n_tok > GEMVQ_KV4_MAX_TOK || !pos || !aligned(pos, 4) || !aligned(num, 4)) return false;
+    t = {pos, num, 1, n_tok, c->n_seq};
+    return true;
+}
+
+int kv4_rows(const gemvq_kv4 * c, const float * k, const float * v, int64_t row_stride, int n_tok, const int32_t * pos,
+             const int32_t * num, Kv4RowsArgs & a) {
+    if (!kv4_ok(c) || !kv4_tokens(c, n_tok, pos, num, a.t)) return GEMVQ_EINVAL;
+    const int64_t least = int64_t(c->n_head_kv) * c->head_dim;
+    if (!rows_ok(k, row_stride, least) || !rows_ok(v, row_stride, least)) return GEMVQ_EINVAL;
+    a.c = kv4_cache(c);
+    a.k = const_cast<float *>(k);
+    a.v = const_cast<float *>(v);
+    a.row_stride = row_stride;
+    return 0;
+}
 
 }  // namespace
 
@@ -85,3 +121,62 @@ extern "C" int gemvq_gemm_static(int type, int rows, int cols, const void * w, c
     if (e == hipSuccess) e = launch_gemm(g, type, s);
     return e == hipSuccess ? 0 : -int(e);
 }
+
+extern "C" {
+
+uint64_t gemvq_kv4_bytes(int n_seq, int n_ctx, int n_head_kv, int head_dim) {
+    if (n_seq < 1 || n_seq > GRID_MAX || n_ctx < 1 || n_head_kv < 1 || n_head_kv > GRID_MAX || !kv4_dim_ok(head_dim)) return 0;
+    return uint64_t(n_seq) * uint64_t(n_head_kv) * uint64_t(kv4_tiles(n_ctx)) * kv4_record(head_dim);
+}
+
+int gemvq_kv4_store_static(const gemvq_kv4 * kv, const float * k, const float * v, int64_t row_stride, int n_tok,
+                           const int32_t * pos, const int32_t * num, void * stream) {
+    Kv4RowsArgs a;
+    const int st = kv4_rows(kv, k, v, row_stride, n_tok, pos, num, a);
+    if (st) return st;
+    const hipError_t e = launch_kv4_store(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : -int(e);
+}
+
+int gemvq_kv4_load_static(const gemvq_kv4 * kv, float * k, float * v, int64_t row_stride, int n_tok, const int32_t * pos,
+                          const int32_t * num, void * stream) {
+    Kv4RowsArgs a;
+    const int st = kv4_rows(kv, k, v, row_stride, n_tok, pos, num, a);
+    if (st) return st;
+    const hipError_t e = launch_kv4_load(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : -int(e);
+}
+
+uint64_t gemvq_kv4_attn_work(const gemvq_kv4 * kv, int n_tok, int n_head) {
+    (void)kv;
+    (void)n_tok;
+    (void)n_head;
+    return 0;
+}
+
+int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
+                          int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,
+                          float scale, void * work, uint64_t work_bytes, void * stream) {
+    Kv4AttnArgs a{};
+    if (!kv4_ok(kv) || !kv4_tokens(kv, n_tok, pos, num, a.t)) return GEMVQ_EINVAL;
+    if (n_head < 1 || n_head > GRID_MAX || n_head % kv->n_head_kv || window < 0) return GEMVQ_EINVAL;
+    const uint64_t need = gemvq_kv4_attn_work(kv, n_tok, n_head);
+    if (work_bytes < need || (need && (!work || !aligned(work, 16)))) return GEMVQ_EINVAL;
+    const int64_t hd = kv->head_dim;
+    if (!rows_ok(q, q_stride, hd) || q_head_stride % 4 || q_head_stride < hd || q_head_stride > (int64_t(1) << 40) ||
+        !rows_ok(y, y_stride, n_head * hd))
+        return GEMVQ_EINVAL;
+    a.c = kv4_cache(kv);
+    a.q = q;
+    a.y = y;
+    a.q_row = q_stride;
+    a.q_head = q_head_stride;
+    a.y_row = y_stride;
+    a.n_head = n_head;
+    a.window = window;
+    a.scale = scale;
+    const hipError_t e = launch_kv4_attn(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : -int(e);
+}
+
+}  // extern "C"

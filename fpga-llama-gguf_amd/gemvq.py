@@ -137,6 +137,11 @@ _hip = None
 _synth = None
 
 
+class Kv4(C.Structure):  # gemvq_kv4
+    """A 4-bit KV cache on device memory: its address (kv4_bytes() bytes) and sizes."""
+    _fields_ = [("data", C.c_void_p)] + [(n, C.c_int32) for n in ("n_seq", "n_ctx", "n_head_kv", "head_dim")]
+
+
 class LaunchStat(C.Structure):  # gemvq_launch_stat
     _fields_ = [("name", C.c_char * 40), ("first_cmd", C.c_int32), ("n_cmds", C.c_int32), ("bytes", C.c_uint64),
                 ("us", C.c_double)]
@@ -189,6 +194,12 @@ def hip_lib() -> C.CDLL:
         _c_fn(lib, "gemvq_cr_expf", C.c_float, C.c_float)
         _c_fn(lib, "gemvq_cr_logf", C.c_float, C.c_float)
         _c_fn(lib, "gemvq_crmath_hash", C.c_int, vp, C.c_int, u64p)
+        i, i64, u64, kvp = C.c_int, C.c_int64, C.c_uint64, C.POINTER(Kv4)
+        _c_fn(lib, "gemvq_kv4_bytes", u64, i, i, i, i)
+        for name in ("gemvq_kv4_store_static", "gemvq_kv4_load_static"):
+            _c_fn(lib, name, i, kvp, vp, vp, i64, i, vp, vp, vp)
+        _c_fn(lib, "gemvq_kv4_attn_work", u64, kvp, i, i)
+        _c_fn(lib, "gemvq_kv4_attn_static", i, kvp, vp, i64, i64, vp, i64, i, i, vp, vp, i, C.c_float, vp, u64, vp)
         _hip = lib
     return _hip
 
@@ -266,6 +277,43 @@ def unpack(t: int, rows: int, cols: int, packed: np.ndarray) -> np.ndarray:
 # ---------------------------------------------------------------------------------------------------------------
 class GemvqError(RuntimeError):
     pass
+
+
+# ---------------------------------------------------------------------------------------------------------------
+# Operators on caller-owned device memory (gemvq_hip.h): pointers are addresses (a tensor's data_ptr(), say) on the
+# current device, stream is a hipStream_t's value (0: the null stream). A program that uses torch imports it before the
+# library is loaded, so that both work on one HIP runtime.
+def _ok(st: int, what: str) -> None:
+    if st:
+        raise GemvqError(f"{what}: " + ("bad argument" if st == EINVAL else f"status {st}"))
+
+
+def kv4_bytes(n_seq: int, n_ctx: int, n_head_kv: int, head_dim: int) -> int:
+    """Bytes of a 4-bit KV cache (0: sizes that are not served)."""
+    return hip_lib().gemvq_kv4_bytes(n_seq, n_ctx, n_head_kv, head_dim)
+
+
+def kv4_store_static(kv: Kv4, k: int, v: int, row_stride: int, n_tok: int, pos: int, num: int = 0, stream: int = 0) -> None:
+    """Stores the tokens' keys and values at positions pos[s] + t."""
+    _ok(hip_lib().gemvq_kv4_store_static(kv, k, v, row_stride, n_tok, pos, num, stream), "kv4 store")
+
+
+def kv4_load_static(kv: Kv4, k: int, v: int, row_stride: int, n_tok: int, pos: int, num: int = 0, stream: int = 0) -> None:
+    """Reads the keys and values at positions pos[s] + t as FP32."""
+    _ok(hip_lib().gemvq_kv4_load_static(kv, k, v, row_stride, n_tok, pos, num, stream), "kv4 load")
+
+
+def kv4_attn_work(kv: Kv4, n_tok: int, n_head: int) -> int:
+    """Bytes of workspace of kv4_attn_static."""
+    return hip_lib().gemvq_kv4_attn_work(kv, n_tok, n_head)
+
+
+def kv4_attn_static(kv: Kv4, q: int, q_stride: int, q_head_stride: int, y: int, y_stride: int, n_tok: int, n_head: int,
+                    pos: int, num: int = 0, window: int = 0, scale: float = 1.0, work: int = 0, work_bytes: int = 0,
+                    stream: int = 0) -> None:
+    """Attention of the tokens at positions pos[s] + t over the cache (their own keys and values stored before)."""
+    _ok(hip_lib().gemvq_kv4_attn_static(kv, q, q_stride, q_head_stride, y, y_stride, n_tok, n_head, pos, num, window, scale,
+                                        work, work_bytes, stream), "kv4 attention")
 
 
 class Context:

@@ -287,6 +287,42 @@ int gemvq_crmath_hash(gemvq_ctx * ctx, int fn, uint64_t * hashes);
 int gemvq_gemm_static(int type, int rows, int cols, const void * w, const float * x, int n_tok, int x_stride,
                       float * y, int y_stride, void * stream);
 
+/* No counterpart in the reference: a KV cache held in 4 bits (ggml's Q4_0 blocks of 32 along head_dim: 4.5 bits a value
+ * against F16's 16), on caller-owned device memory. `data` holds gemvq_kv4_bytes() bytes, 256-byte aligned: n_ctx positions of
+ * n_head_kv keys and values of head_dim (32, 64, 128 or 256) for each of n_seq sequences, in a layout of its own (records of 32
+ * positions of one KV head, csrc/gq_kv4.h). Nothing needs clearing: positions that were not stored are not read.
+ * All calls run on the current device, asynchronously on `stream` (a hipStream_t of that device; NULL for the null stream),
+ * allocate nothing and keep nothing: they can be captured into a graph, and calls overlap freely where their memory is apart.
+ * Tokens: row s * n_tok + t of k, v, q and y is token t of sequence s, at position pos[s] + t (pos: n_seq int32 in device
+ * memory). num (n_seq int32 in device memory, or NULL for n_tok each) says how many tokens of a sequence there are: the others,
+ * and tokens whose position is outside 0 .. n_ctx - 1, are neither stored nor read, and their rows of y, k and v are left as they
+ * were. 1 <= n_tok <= GEMVQ_KV4_MAX_TOK. Rows start at multiples of 16 bytes: pointers 16-byte aligned, strides (in floats)
+ * multiples of 4 and no smaller than a row. Outputs do not overlap inputs.
+ * Status: 0, GEMVQ_EINVAL (nothing launched) or a negated HIP error. */
+#define GEMVQ_KV4_MAX_TOK 65535
+typedef struct {
+    void * data;
+    int32_t n_seq, n_ctx, n_head_kv, head_dim;
+} gemvq_kv4;
+/* 0 for sizes that are not served. */
+uint64_t gemvq_kv4_bytes(int n_seq, int n_ctx, int n_head_kv, int head_dim);
+/* Quantizes the tokens' keys and values (KV head h of a row at h * head_dim) into the cache, in FP32 as ggml does: d the
+ * element of largest magnitude over -8, each value min(15, trunc(x * (1 / d) + 8.5)). */
+int gemvq_kv4_store_static(const gemvq_kv4 * kv, const float * k, const float * v, int64_t row_stride, int n_tok,
+                           const int32_t * pos, const int32_t * num, void * stream);
+/* The other way: what the cache holds at the tokens' positions, fp16(d) * (quant - 8). */
+int gemvq_kv4_load_static(const gemvq_kv4 * kv, float * k, float * v, int64_t row_stride, int n_tok, const int32_t * pos,
+                          const int32_t * num, void * stream);
+/* Attention: the token at position p gives y = sum_j softmax_j(scale * q . k_j) v_j over the positions j from 0, or from
+ * max(0, p - window + 1) with window > 0, to p (store the tokens' own keys and values first). q head h of a row starts at
+ * h * q_head_stride and reads KV head h / (n_head / n_head_kv); y's heads are packed. q enters as it is (no rounding to 16 bits);
+ * products, softmax and sums in FP32. work: gemvq_kv4_attn_work() bytes of device memory, 16-byte aligned, whose contents do
+ * not matter before or after; calls that may overlap need one each. */
+uint64_t gemvq_kv4_attn_work(const gemvq_kv4 * kv, int n_tok, int n_head);
+int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
+                          int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,
+                          float scale, void * work, uint64_t work_bytes, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -68,7 +68,13 @@ struct Kv4AttnArgs {
     int n_head, window;  // window 0: every position up to the token's own
     float scale;
     const float * gate;  // NULL, or gate rows as q's (the output times sigmoid(gate))
+    float * work;        // kv4_work_floats
+    int ranges;          // set at launch: ranges of records that the grid has workgroups for
 };
+
+constexpr int KV4_GROUPS = 1024;  // workgroups that a call's records are dealt to, where they are enough
+constexpr int KV4_LEAST = 4;      // records of a range at least: one a wave
+size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head);
 
 hipError_t launch_kv4_store(const Kv4RowsArgs & a, hipStream_t s);
 hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s);

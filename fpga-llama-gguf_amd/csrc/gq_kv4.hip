@@ -2,6 +2,7 @@
 #include "gq_device.h"
 #include "gq_kv4.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace gq {
@@ -96,48 +97,459 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
     }
 }
 
-// Workgroup (q head, token, sequence): records in order, 8 threads a position for the scores, a thread an element for the values.
+// ---- attention ----
+// A wave takes the rows (token, q head) of one KV head 16 at a time (NQ such groups) and records of 32 positions one after another:
+//   S^T = K Q^T   16x16x32 fp16 matrix instructions, a block of 32 elements each: the quants minus 8 are whole numbers, exact in fp16;
+//                 the query, scaled to its row's largest element, is the sum of two fp16 numbers (22 bits). Each block's sums are
+//                 multiplied by its scales in FP32.
+//   P = 2^(S - c) in FP32. Lane 16 g + q then holds query q's weights of the 8 positions that it feeds to
+//   O^T += V^T P^T: the value scales differ by position, so they go into the weights: p d as the sum of two fp16 numbers, against the
+//                 whole quants. The accumulators stay with the query's lanes, and nothing crosses lanes in the loop.
+// The reference c = m - e of a query: m its running maximum, taken anew only when a score passes it by 8 (the weights may be
+// 2^8), and e an exponent common to the wave that brings the largest value scale so far to 2^6..2^7, so p d < 2^15 has its fp16
+// parts' full precision (they are whole multiples of 2^-24: 2^-30 of what the largest scale gives). Both sums are taken relative to
+// c, so e cancels.
+// The four waves of a workgroup take the records of its range in turn and join at the end; ranges of one sequence are joined by
+// kv4_join_kernel.
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr float KV4_LOW = -1e30f;  // below every score: the maximum before the first one
+
+template <int N>
+__device__ __forceinline__ void load_words(const uint8_t * p, uint32_t * w) {
+    if constexpr (N == 4) {
+        const u32x4 x = *reinterpret_cast<const u32x4 *>(p);
+        for (int i = 0; i < 4; ++i) w[i] = x[i];
+    } else if constexpr (N == 2) {
+        const u32x2 x = *reinterpret_cast<const u32x2 *>(p);
+        w[0] = x[0];
+        w[1] = x[1];
+    } else {
+        w[0] = *reinterpret_cast<const uint32_t *>(p);
+    }
+}
+
+// What a lane holds of a record.
 template <int HD>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
-    __shared__ float qs[HD], pr[KV4_TILE];
-    const int hq = blockIdx.x, t = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, h = hq / (a.n_head / a.c.n_head_kv);
+struct Kv4Tile {
+    static constexpr int NB = HD / 32, KB = Kv4Layout<HD>::KB, VB = Kv4Layout<HD>::VB, NV = HD >= 128 ? HD / 128 : 1;
+    uint32_t k[2][NB];   // its position's key bytes, by half of the record and block
+    uint32_t v[NB][2];   // its element's value bytes at its 8 positions
+    uint32_t kd[NB][4];  // its 8 positions' scales, pairs
+    uint32_t vd[NB][4];
+    uint32_t any[NV];    // the lane's share of the record's value scales, for the largest one (HD 32 and 64: several lanes have the same)
+
+    __device__ static int any_word(int lane, int i) { return HD >= 128 ? lane * NV + i : lane & (HD / 2 - 1); }
+
+    __device__ __forceinline__ void load(const uint8_t * rec, int lane) {
+        using L = Kv4Layout<HD>;
+        const int g = lane >> 4;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int c = 0; c < NB / KB; ++c) load_words<KB>(rec + u * 8 * HD + c * 256 * KB + lane * 4 * KB, &k[u][c * KB]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) load_words<4>(rec + L::KD + (g * NB + b) * 16, kd[b]);
+#pragma unroll
+        for (int c = 0; c < NB / VB; ++c) load_words<2 * VB>(rec + L::VQ + c * 512 * VB + lane * 8 * VB, v[c * VB]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) load_words<4>(rec + L::VD + (g * NB + b) * 16, vd[b]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) any[i] = *reinterpret_cast<const uint32_t *>(rec + L::VD + any_word(lane, i) * 4);
+    }
+};
+
+__device__ __forceinline__ float half_of(uint32_t w, int hi) { return h2f((hi ? w >> 16 : w) & 0xffffu); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    const half2 h = {_Float16(a), _Float16(b)};
+    return __builtin_bit_cast(uint32_t, h);
+}
+
+// Two numbers as the sums of two fp16 numbers each: hi + lo, 22 bits. The empty asm makes the numbers exist (see f2h): folded into
+// the conversion, a product's nearest fp16 number can differ from the one that lo is formed against.
+__device__ __forceinline__ void split2(float a, float b, uint32_t & hi, uint32_t & lo) {
+    __asm__("" : "+v"(a), "+v"(b));
+    hi = pack2(a, b);
+    lo = pack2(a - half_of(hi, 0), b - half_of(hi, 1));
+}
+
+// The 8 nibbles of four bytes minus 8, as fp16: low nibbles of bytes 0, 2, 1, 3, then the high ones.
+__device__ __forceinline__ u32x4 nibbles(uint32_t w) {
+    const half2 c0 = {_Float16(-1032.0f), _Float16(-1032.0f)}, c1 = {_Float16(-72.0f), _Float16(-72.0f)};
+    const uint32_t x = w >> 8;
+    u32x4 r;
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (w & 0x000f000fu) | 0x64006400u) + c0);  // 1024 + n
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (x & 0x000f000fu) | 0x64006400u) + c0);
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (w & 0x00f000f0u) | 0x54005400u) + c1);  // 64 + n
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (x & 0x00f000f0u) | 0x54005400u) + c1);
+    return r;
+}
+
+__device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+
+__device__ __forceinline__ float wave_max(float x) {
+#pragma unroll
+    for (int s = 32; s >= 1; s >>= 1) x = fmaxf(x, __shfl_xor(x, s, WAVE));
+    return x;
+}
+
+// How the sequences' records are dealt to workgroups: a sequence's `tiles` records from `first` on, in ranges of `per`; its ranges
+// are number `slot` on of all. Every lane of a wave has the same.
+struct Kv4Range {
+    int first, tiles, per, slot, n;  // n: tokens of the sequence
     long long p0;
-    int n;
-    kv4_span(a.t, s, p0, n);
-    const long long pl = p0 + t;
-    if (t >= n || pl < 0 || pl >= a.c.n_ctx) return;
-    const int pos = int(pl), from = a.window && pos >= a.window ? pos - a.window + 1 : 0;
-    const size_t row = size_t(s) * a.t.n_tok + t;
-    if (tid < HD) qs[tid] = a.q[row * size_t(a.q_row) + size_t(hq) * size_t(a.q_head) + tid];
-    __syncthreads();
-    float m = -__builtin_inff(), l = 0.0f, o = 0.0f;
-    for (int tile = from / KV4_TILE; tile <= pos / KV4_TILE; ++tile) {
-        const uint8_t * rec = kv4_rec(a.c, s, h, tile);
-        const int p = tid >> 3, part = tid & 7, at = tile * KV4_TILE + p;
-        float dot = 0.0f;
-        for (int e = part; e < HD; e += 8) dot += qs[e] * kv4_key<HD>(rec, p, e);
-        dot += __shfl_xor(dot, 1, WAVE);
-        dot += __shfl_xor(dot, 2, WAVE);
-        dot += __shfl_xor(dot, 4, WAVE);
-        if (part == 0) pr[p] = at >= from && at <= pos ? dot * a.scale : -__builtin_inff();
-        __syncthreads();
-        float mt = m;
-        for (int j = 0; j < KV4_TILE; ++j) mt = fmaxf(mt, pr[j]);
-        const float f = expf_(m - mt);
-        l *= f;
-        o *= f;
-        m = mt;
-        for (int j = 0; j < KV4_TILE; ++j) {
-            if (pr[j] == -__builtin_inff()) continue;
-            const float w = expf_(pr[j] - m);
-            l += w;
-            if (tid < HD) o += w * kv4_value<HD>(rec, j, tid);
+};
+
+// Records that the tokens of a sequence see: from the first token's first position to the last one's own.
+__device__ __forceinline__ void kv4_seen(const Kv4AttnArgs & a, int s, Kv4Range & r) {
+    kv4_span(a.t, s, r.p0, r.n);
+    const long long lo = r.p0 < 0 ? 0 : r.p0, hi = r.p0 + r.n < a.c.n_ctx ? r.p0 + r.n : a.c.n_ctx;  // positions of live tokens
+    if (lo >= hi) {
+        r.first = r.tiles = 0;
+        return;
+    }
+    r.first = a.window && lo >= a.window ? int((lo - a.window + 1) / KV4_TILE) : 0;
+    r.tiles = int((hi - 1) / KV4_TILE) - r.first + 1;
+}
+
+// The ranges' length: all records over the ranges that the grid has room for, a sequence's last one being short.
+__device__ __forceinline__ int kv4_per(long long records, int ranges, int n_seq, int most) {
+    const long long per = ranges > n_seq ? (records + ranges - n_seq - 1) / (ranges - n_seq) : most;
+    return int(per > KV4_LEAST ? per : KV4_LEAST);
+}
+
+// All sequences' records (a wave's lanes scan them together): the ranges' length.
+__device__ __forceinline__ int kv4_length(const Kv4AttnArgs & a) {
+    long long sum = 0;
+    int most = 0;
+    Kv4Range x;
+    for (int i = threadIdx.x & 63; i < a.t.n_seq; i += 64) {
+        kv4_seen(a, i, x);
+        sum += x.tiles;
+        most = max(most, x.tiles);
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) {
+        sum += __shfl_xor(sum, d, WAVE);
+        most = max(most, __shfl_xor(most, d, WAVE));
+    }
+    return kv4_per(sum, a.ranges, a.t.n_seq, most);
+}
+
+// The sequence that range number `range` belongs to (BY_RANGE), or sequence s itself, with its ranges; false: no such range.
+template <bool BY_RANGE>
+__device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int & s, Kv4Range & r) {
+    if (a.t.n_seq == 1) {
+        s = 0;
+        kv4_seen(a, 0, r);
+        r.per = kv4_per(r.tiles, a.ranges, 1, r.tiles);
+        r.slot = 0;
+        return (long long)(BY_RANGE ? range : 0) * r.per < r.tiles;
+    }
+    const int lane = threadIdx.x & 63, per = kv4_length(a);
+    int before = 0;
+    for (int i0 = 0; i0 < a.t.n_seq; i0 += 64) {
+        Kv4Range x;
+        x.tiles = 0;
+        if (i0 + lane < a.t.n_seq) kv4_seen(a, i0 + lane, x);
+        const int mine = (x.tiles + per - 1) / per;
+        int upto = before + mine;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int y = __shfl_up(upto, d, WAVE);
+            if (lane >= d) upto += y - before;
         }
+        const int all = __shfl(upto, 63, WAVE);
+        if (BY_RANGE ? range < all : s < i0 + 64) {
+            const int l = BY_RANGE ? __ffsll(__ballot(upto > range)) - 1 : s - i0;
+            s = i0 + l;
+            r.slot = __shfl(upto - mine, l, WAVE);
+            kv4_seen(a, s, r);
+            r.per = per;
+            return r.tiles > 0;
+        }
+        before = all;
+    }
+    return false;
+}
+
+// Four elements of an output row.
+template <int HD>
+__device__ __forceinline__ void kv4_out(const Kv4AttnArgs & a, size_t row, int hq, int e, f32x4 y, float l) {
+    if (a.gate) {
+        const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + row * size_t(a.q_row) + size_t(hq) * size_t(a.q_head) + e);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = sigmoid_(g[i]) * (y[i] / l);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] = y[i] / l;
+    }
+    *reinterpret_cast<f32x4 *>(a.y + row * size_t(a.y_row) + size_t(hq) * HD + e) = y;
+}
+
+template <int HD, int NQ>
+__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
+    constexpr int NB = HD / 32, ROWS = 16 * NQ, PAD = 36;
+    __shared__ __align__(16) float part[4][ROWS][PAD];
+    __shared__ float cs[4][ROWS], ls[4][ROWS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
+    const int G = a.n_head / a.c.n_head_kv, groups = (a.t.n_tok * G + ROWS - 1) / ROWS;
+    const int h = blockIdx.x / groups, row0 = blockIdx.x % groups * ROWS;  // rows of the KV head: token row / G, q head row % G
+    const int range = blockIdx.y;
+    int s = 0;
+    Kv4Range r;
+    if (!kv4_find<true>(a, range, s, r)) return;
+    s = __builtin_amdgcn_readfirstlane(s);
+    const int p0 = __builtin_amdgcn_readfirstlane(int(r.p0));
+    const int live = min(__builtin_amdgcn_readfirstlane(r.n), a.c.n_ctx - p0);  // tokens -p0 (where p0 < 0) .. live - 1 have positions
+    const int t_lo = max(row0 / G, -p0), t_hi = min((row0 + ROWS - 1) / G, live - 1);
+    if (t_lo > t_hi) return;
+    // the group's positions: lo .. hi, the rows' own ranges within them
+    const int lo = a.window ? max(0, p0 + t_lo - a.window + 1) : 0, hi = p0 + t_hi;
+    const int j = range - r.slot, split = __builtin_amdgcn_readfirstlane((r.tiles + r.per - 1) / r.per);
+    const int first = __builtin_amdgcn_readfirstlane(max(r.first + j * r.per, lo / KV4_TILE));
+    const int last = __builtin_amdgcn_readfirstlane(min(r.first + min((j + 1) * r.per, r.tiles) - 1, hi / KV4_TILE));
+    if (first > last) return;  // none of the range's positions are seen
+    const uint8_t * head = a.c.data + (size_t(s) * a.c.n_head_kv + h) * size_t(a.c.tiles) * kv4_record(HD);
+
+    u32x4 q[NQ][NB][2];  // the queries' two parts, elements in the order of nibbles()
+    float kq[NQ];        // what brings the products back: scale * log2(e) over the row's power of two
+    int my_lo[NQ], my_hi[NQ];
+    f32x4 o[NQ][NB][2];
+    float c[NQ], l[NQ];
+    Kv4Tile<HD> tile;
+    int at = first + wave;
+    tile.load(head + size_t(min(at, last)) * kv4_record(HD), lane);
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int row = row0 + n * 16 + col, t = row / G;
+        const bool ok = t >= t_lo && t <= t_hi;
+        my_hi[n] = ok ? p0 + t : -1;
+        my_lo[n] = ok && a.window ? p0 + t - a.window + 1 : 0;
+        const float * src = a.q + (size_t(s) * a.t.n_tok + (ok ? t : t_lo)) * size_t(a.q_row) + size_t(h * G + (ok ? row % G : 0)) * size_t(a.q_head);
+        float x[NB][8], top = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            *reinterpret_cast<f32x4 *>(&x[b][0]) = *reinterpret_cast<const f32x4 *>(src + b * 32 + 4 * g);
+            *reinterpret_cast<f32x4 *>(&x[b][4]) = *reinterpret_cast<const f32x4 *>(src + b * 32 + 16 + 4 * g);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[b][i]));
+        }
+        top = fmaxf(top, __shfl_xor(top, 16, WAVE));
+        top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+        // the largest element to 2^13..2^14 (rows of zeros and the ends of FP32's range: some power of two that does not overflow)
+        const int e = min(max(int((__float_as_uint(top) >> 23) & 255), 40), 240);
+        const float up = __uint_as_float(uint32_t(127 + 13 + 127 - e) << 23);
+        kq[n] = a.scale * 1.44269504088896341f * __uint_as_float(uint32_t(e - 13) << 23);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            constexpr int order[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float u = x[b][order[2 * i]] * up, w = x[b][order[2 * i + 1]] * up;
+                uint32_t hi2, lo2;
+                split2(u, w, hi2, lo2);
+                q[n][b][0][i] = hi2;
+                q[n][b][1][i] = lo2;
+            }
+        }
+        c[n] = KV4_LOW;
+        l[n] = 0.0f;
+#pragma unroll
+        for (int b = 0; b < NB; ++b) o[n][b][0] = o[n][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+    int e = 30;  // the value scales' exponent, and their bound 2^(7 - e)
+    for (; at <= last; at += 4) {
+        Kv4Tile<HD> next;
+        const int ahead = min(at + 4, last);  // (the last one again where there is none)
+        next.load(head + size_t(ahead) * kv4_record(HD), lane);
+        const int from = at * KV4_TILE;
+        const bool edge = from < (a.window ? p0 + t_hi - a.window + 1 : 0) || from + KV4_TILE - 1 > p0 + t_lo;  // some row does not see all of it
+        if (edge) {  // positions that no row sees may never have been stored: their scales become 0
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int p = from + (i >> 2) * 16 + 4 * g + (i & 3);
+                if (p < lo || p > hi) {
+                    const uint32_t keep = i & 1 ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+                    for (int b = 0; b < NB; ++b) {
+                        tile.kd[b][i / 2] &= keep;
+                        tile.vd[b][i / 2] &= keep;
+                    }
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < Kv4Tile<HD>::NV * 2; ++i) {  // the same of the lane's share
+                const int w = Kv4Tile<HD>::any_word(lane, i / 2) * 2 + (i & 1);  // which scale of the record
+                const int p = from + ((w >> 2) & 1) * 16 + w / (8 * NB) * 4 + (w & 3);
+                if (p < lo || p > hi) tile.any[i / 2] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+            }
+        }
+        uint32_t dtop = 0;  // the largest value scale's magnitude, as fp16 bits
+#pragma unroll
+        for (int i = 0; i < Kv4Tile<HD>::NV; ++i) dtop = max(dtop, max(tile.any[i] & 0x7fffu, (tile.any[i] >> 16) & 0x7fffu));
+        bool again = __any(half_of(dtop, 0) >= __uint_as_float(uint32_t(127 + 7 - e) << 23));
+        float sc[NQ][8];
+        f32x4 acc[NQ][2];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                const u32x4 kk = nibbles(tile.k[u][b]);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    f32x4 x = mfma(kk, q[n][b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                    x = mfma(kk, q[n][b][1], x);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][u][i] = __builtin_fmaf(x[i], half_of(tile.kd[b][2 * u + i / 2], i & 1), acc[n][u][i]);
+                }
+            }
+        float top[NQ];
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sc[n][i] = acc[n][i >> 2][i & 3] * kq[n];
+            if (edge)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int p = from + (i >> 2) * 16 + 4 * g + (i & 3);
+                    if (p < my_lo[n] || p > my_hi[n]) sc[n][i] = -__builtin_inff();
+                }
+            top[n] = fmaxf(fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])), fmaxf(fmaxf(sc[n][4], sc[n][5]), fmaxf(sc[n][6], sc[n][7])));
+            again |= __any(top[n] > c[n] + float(e + 8));
+        }
+        if (again) {  // new maxima and scale exponent
+            const float dm = wave_max(half_of(dtop, 0));
+            const int de = 6 + 127 - int(__float_as_uint(dm) >> 23);  // brings dm to 2^6..2^7
+            const int e2 = max(min(e, de), -10);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                float m = fmaxf(top[n], __shfl_xor(top[n], 16, WAVE));
+                m = fmaxf(m, __shfl_xor(m, 32, WAVE));
+                m = fmaxf(m, c[n] + float(e));
+                const float c2 = m - float(e2), f = __builtin_amdgcn_exp2f(c[n] - c2);
+                c[n] = c2;
+                l[n] *= f;
+#pragma unroll
+                for (int b = 0; b < NB; ++b)
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) o[n][b][u] *= f;
+            }
+            e = e2;
+        }
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) sc[n][i] = __builtin_amdgcn_exp2f(sc[n][i] - c[n]);
+            l[n] += ((sc[n][0] + sc[n][1]) + (sc[n][2] + sc[n][3])) + ((sc[n][4] + sc[n][5]) + (sc[n][6] + sc[n][7]));
+        }
+#pragma unroll
+        for (int b = 0; b < NB; ++b) {
+            const u32x4 v0 = nibbles(tile.v[b][0]), v1 = nibbles(tile.v[b][1]);  // positions 0, 2, 1, 3 and 4, 6, 5, 7 of the lane's 8
+            const u32x4 lo4 = {v0[0], v0[1], v1[0], v1[1]}, hi4 = {v0[2], v0[3], v1[2], v1[3]};
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+                u32x4 ph, pl;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int i0 = (i >> 1) * 4 + (i & 1), i1 = i0 + 2;
+                    const float u = sc[n][i0] * half_of(tile.vd[b][i0 / 2], i0 & 1), w = sc[n][i1] * half_of(tile.vd[b][i1 / 2], i1 & 1);
+                    uint32_t hi2, lo2;
+                    split2(u, w, hi2, lo2);
+                    ph[i] = hi2;
+                    pl[i] = lo2;
+                }
+                o[n][b][0] = mfma(lo4, ph, o[n][b][0]);
+                o[n][b][1] = mfma(hi4, ph, o[n][b][1]);
+                o[n][b][0] = mfma(lo4, pl, o[n][b][0]);
+                o[n][b][1] = mfma(hi4, pl, o[n][b][1]);
+            }
+        }
+        tile = next;
+    }
+    // ---- the waves' sums joined, a block of 32 elements after another ----
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        l[n] += __shfl_xor(l[n], 16, WAVE);
+        l[n] += __shfl_xor(l[n], 32, WAVE);
+        if (g == 0) {
+            cs[wave][n * 16 + col] = c[n];
+            ls[wave][n * 16 + col] = l[n];
+        }
+    }
+    const int rj = tid >> 3, ej = (tid & 7) * 4;  // this thread's row (of 32) and elements of a block
+    const int row = row0 + rj, tj = row / G, hq = h * G + row % G;
+    const bool mine = rj < ROWS && tj >= t_lo && tj <= t_hi;
+    float f[4], C = 0.0f, L = 0.0f;
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+        if (b) __syncthreads();
+#pragma unroll
+        for (int n = 0; n < NQ; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) *reinterpret_cast<f32x4 *>(&part[wave][n * 16 + col][u * 16 + 4 * g]) = o[n][b][u];
         __syncthreads();
+        if (!mine) continue;
+        if (b == 0) {
+            C = fmaxf(fmaxf(cs[0][rj], cs[1][rj]), fmaxf(cs[2][rj], cs[3][rj]));
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                f[w] = __builtin_amdgcn_exp2f(cs[w][rj] - C);
+                L += ls[w][rj] * f[w];
+            }
+        }
+        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int w = 0; w < 4; ++w) y += *reinterpret_cast<const f32x4 *>(&part[w][rj][ej]) * f[w];
+        const size_t orow = size_t(s) * a.t.n_tok + tj;
+        if (split == 1) {
+            kv4_out<HD>(a, orow, hq, b * 32 + ej, y, L);
+        } else {  // this range's set: [range][token][head][HD + 4], C and L behind the sums
+            float * w = a.work + ((size_t(range) * a.t.n_tok + tj) * a.n_head + hq) * (HD + 4);
+            *reinterpret_cast<f32x4 *>(w + b * 32 + ej) = y;
+            if (b == 0 && ej == 0) {
+                w[HD] = C;
+                w[HD + 1] = L;
+            }
+        }
+    }
+}
+
+// Workgroup (q head, token, sequence): the sets of a sequence with several ranges, a thread an element.
+template <int HD>
+__global__ __launch_bounds__(HD < 64 ? 64 : HD) void kv4_join_kernel(Kv4AttnArgs a) {
+    const int hq = blockIdx.x, t = blockIdx.y, tid = threadIdx.x;
+    int s = blockIdx.z;
+    Kv4Range r;
+    if (!kv4_find<false>(a, 0, s, r)) return;
+    const long long p = r.p0 + t;
+    if (r.tiles <= r.per || t >= r.n || p < 0 || p >= a.c.n_ctx) return;
+    // the ranges that hold positions this token sees
+    const int lo = (a.window && p >= a.window ? int((p - a.window + 1) / KV4_TILE) : 0) - r.first, hi = int(p / KV4_TILE) - r.first;
+    const size_t step = size_t(a.t.n_tok) * a.n_head * (HD + 4);
+    const float * w = a.work + ((size_t(r.slot) * a.t.n_tok + t) * a.n_head + hq) * (HD + 4);
+    float C = KV4_LOW, L = 0.0f, o = 0.0f;
+    for (int j = lo / r.per; j <= hi / r.per; ++j) C = fmaxf(C, w[j * step + HD]);
+#pragma unroll 8
+    for (int j = lo / r.per; j <= hi / r.per; ++j) {
+        const float f = __builtin_amdgcn_exp2f(w[j * step + HD] - C);
+        L += w[j * step + HD + 1] * f;
+        o += w[j * step + min(tid, HD - 1)] * f;
     }
     if (tid < HD) {
-        const size_t g = row * size_t(a.q_row) + size_t(hq) * size_t(a.q_head) + tid;
-        a.y[row * size_t(a.y_row) + size_t(hq) * HD + tid] = a.gate ? sigmoid_(a.gate[g]) * (o / l) : o / l;
+        const size_t row = size_t(s) * a.t.n_tok + t;
+        const float y = o / L;
+        a.y[row * size_t(a.y_row) + size_t(hq) * HD + tid] =
+            a.gate ? sigmoid_(a.gate[row * size_t(a.q_row) + size_t(hq) * size_t(a.q_head) + tid]) * y : y;
     }
 }
 
@@ -168,9 +580,32 @@ hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s) {
     });
 }
 
-hipError_t launch_kv4_attn(const Kv4AttnArgs & a, hipStream_t s) {
+// Rows of a workgroup, and how many ranges a call's records are dealt to: about KV4_GROUPS workgroups in all, but at least one
+// range a sequence and no more than KV4_LEAST records each give.
+static int kv4_nq(int n_tok, int per_kv) { return n_tok * (long long)per_kv > 16 ? 2 : 1; }
+
+int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
+    const int per_kv = n_head / c.n_head_kv, rows = 16 * kv4_nq(n_tok, per_kv);
+    const long long units = (n_tok * (long long)per_kv + rows - 1) / rows * c.n_head_kv;
+    const long long most = (long long)n_seq * ((c.tiles + KV4_LEAST - 1) / KV4_LEAST);
+    return int(std::min<long long>(std::max<long long>(n_seq, std::min(KV4_GROUPS / units, most)), 65535));
+}
+
+size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
+    const int ranges = kv4_ranges(c, n_seq, n_tok, n_head);
+    return ranges > n_seq ? size_t(ranges) * n_tok * n_head * (c.head_dim + 4) : 0;
+}
+
+hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
+    Kv4AttnArgs a = args;
+    const int per_kv = a.n_head / a.c.n_head_kv, nq = kv4_nq(a.t.n_tok, per_kv);
+    a.ranges = kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head);
+    const dim3 grid(unsigned((a.t.n_tok * (long long)per_kv + 16 * nq - 1) / (16 * nq) * a.c.n_head_kv), unsigned(a.ranges));
     return by_dim(a.c.head_dim, [&](auto hd) {
-        GQ_LAUNCH(kv4_attn_kernel<hd.value>, dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
+        if (nq == 1) GQ_LAUNCH((kv4_attn_kernel<hd.value, 1>), grid, dim3(256), 0, s, a);
+        else GQ_LAUNCH((kv4_attn_kernel<hd.value, 2>), grid, dim3(256), 0, s, a);
+        if (a.ranges > a.t.n_seq)
+            GQ_LAUNCH(kv4_join_kernel<hd.value>, dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(hd.value < 64 ? 64 : hd.value), 0, s, a);
     });
 }
 

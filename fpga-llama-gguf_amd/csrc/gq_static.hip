@@ -49,10 +49,11 @@ bool rows_ok(const void * p, int64_t stride, int64_t least) {
 
 constexpr int GRID_MAX = 65535;
 
-bool kv4_ok(const gemvq_kv4 * c) {
-    return c && c->data && aligned(c->data, 256) && c->n_seq > 0 && c->n_seq <= GRID_MAX && c->n_ctx > 0 && c->n_head_kv > 0 &&
-           c->n_head_kv <= GRID_MAX && kv4_dim_ok(c->head_dim);
+bool kv4_sizes_ok(const gemvq_kv4 * c) {
+    return c && c->n_seq > 0 && c->n_seq <= GRID_MAX && c->n_ctx > 0 && c->n_head_kv > 0 && c->n_head_kv <= GRID_MAX &&
+           kv4_dim_ok(c->head_dim);
 }
+bool kv4_ok(const gemvq_kv4 * c) { return kv4_sizes_ok(c) && c->data && aligned(c->data, 256); }
 
 Kv4Cache kv4_cache(const gemvq_kv4 * c) {
     return {static_cast<uint8_t *>(c->data), c->n_ctx, kv4_tiles(c->n_ctx), c->n_head_kv, c->head_dim};
@@ -148,10 +149,9 @@ int gemvq_kv4_load_static(const gemvq_kv4 * kv, float * k, float * v, int64_t ro
 }
 
 uint64_t gemvq_kv4_attn_work(const gemvq_kv4 * kv, int n_tok, int n_head) {
-    (void)kv;
-    (void)n_tok;
-    (void)n_head;
-    return 0;
+    if (!kv4_sizes_ok(kv) || n_tok < 1 || n_tok > GEMVQ_KV4_MAX_TOK || n_head < 1 || n_head > GRID_MAX || n_head % kv->n_head_kv)
+        return 0;
+    return kv4_work_floats(kv4_cache(kv), kv->n_seq, n_tok, n_head) * sizeof(float);
 }
 
 int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
@@ -175,6 +175,7 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
     a.n_head = n_head;
     a.window = window;
     a.scale = scale;
+    a.work = static_cast<float *>(work);
     const hipError_t e = launch_kv4_attn(a, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : -int(e);
 }

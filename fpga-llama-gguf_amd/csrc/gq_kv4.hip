@@ -133,35 +133,49 @@ __device__ __forceinline__ void load_words(const uint8_t * p, uint32_t * w) {
     }
 }
 
-// What a lane holds of a record.
+// What a lane holds of a record: its quants in registers; the scales, which 16 lanes share, go through LDS (a lane loads and masks
+// 4 HD / 64 bytes of them: the keys' in lanes 0..31, the values' in 32..63).
 template <int HD>
 struct Kv4Tile {
-    static constexpr int NB = HD / 32, KB = Kv4Layout<HD>::KB, VB = Kv4Layout<HD>::VB, NV = HD >= 128 ? HD / 128 : 1;
-    uint32_t k[2][NB];   // its position's key bytes, by half of the record and block
-    uint32_t v[NB][2];   // its element's value bytes at its 8 positions
-    uint32_t kd[NB][4];  // its 8 positions' scales, pairs
-    uint32_t vd[NB][4];
-    uint32_t any[NV];    // the lane's share of the record's value scales, for the largest one (HD 32 and 64: several lanes have the same)
-
-    __device__ static int any_word(int lane, int i) { return HD >= 128 ? lane * NV + i : lane & (HD / 2 - 1); }
+    static constexpr int NB = HD / 32, KB = Kv4Layout<HD>::KB, VB = Kv4Layout<HD>::VB;
+    static constexpr int NS = HD / 32;              // scales a lane loads
+    static constexpr int NW = NS > 1 ? NS / 2 : 1;  // words of them
+    uint32_t k[2][NB];  // its position's key bytes, by half of the record and block
+    uint32_t v[NB][2];  // its element's value bytes at its 8 positions
+    uint32_t d[NW];
 
     __device__ __forceinline__ void load(const uint8_t * rec, int lane) {
         using L = Kv4Layout<HD>;
-        const int g = lane >> 4;
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int c = 0; c < NB / KB; ++c) load_words<KB>(rec + u * 8 * HD + c * 256 * KB + lane * 4 * KB, &k[u][c * KB]);
-#pragma unroll
-        for (int b = 0; b < NB; ++b) load_words<4>(rec + L::KD + (g * NB + b) * 16, kd[b]);
+        if constexpr (NS > 1) load_words<NW>(rec + L::KD + lane * 4 * NW, d);
+        else d[0] = *reinterpret_cast<const uint16_t *>(rec + L::KD + lane * 2);
 #pragma unroll
         for (int c = 0; c < NB / VB; ++c) load_words<2 * VB>(rec + L::VQ + c * 512 * VB + lane * 8 * VB, v[c * VB]);
+    }
+    // The position of the record that the lane's scale i belongs to.
+    __device__ static int at(int lane, int i) {
+        const int w = (lane & 31) * NS + i;
+        return ((w >> 2) & 1) * 16 + w / (8 * NB) * 4 + (w & 3);
+    }
+    __device__ __forceinline__ void stage(uint32_t * lds, int lane) const {
+        if constexpr (NS > 1) {
 #pragma unroll
-        for (int b = 0; b < NB; ++b) load_words<4>(rec + L::VD + (g * NB + b) * 16, vd[b]);
-#pragma unroll
-        for (int i = 0; i < NV; ++i) any[i] = *reinterpret_cast<const uint32_t *>(rec + L::VD + any_word(lane, i) * 4);
+            for (int i = 0; i < NW; ++i) lds[lane * NW + i] = d[i];
+        } else {
+            reinterpret_cast<uint16_t *>(lds)[lane] = uint16_t(d[0]);
+        }
     }
 };
+
+// Orders a wave's LDS writes before its other lanes' reads (a wave's LDS operations are carried out in order).
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
 
 __device__ __forceinline__ float half_of(uint32_t w, int hi) { return h2f((hi ? w >> 16 : w) & 0xffffu); }
 
@@ -295,10 +309,15 @@ __device__ __forceinline__ void kv4_out(const Kv4AttnArgs & a, size_t row, int h
 }
 
 template <int HD, int NQ>
-__global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(256, HD == 256 && NQ == 1 ? 2 : 1) void kv4_attn_kernel(Kv4AttnArgs a) {
     constexpr int NB = HD / 32, ROWS = 16 * NQ, PAD = 36;
     __shared__ __align__(16) float part[4][ROWS][PAD];
+    // head_dim 256: the queries' parts, the same for the four waves, stay in LDS (in registers they leave room for one wave a SIMD, or
+    // for 16 rows without spills)
+    constexpr bool QL = HD == 256;
+    __shared__ u32x4 ql[QL ? NQ * NB * 2 : 1][64];
     __shared__ float cs[4][ROWS], ls[4][ROWS];
+    __shared__ __align__(16) uint32_t scales[4][HD];  // a wave's record's key scales, then its value scales: [g][block][8] each
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
     const int G = a.n_head / a.c.n_head_kv, groups = (a.t.n_tok * G + ROWS - 1) / ROWS;
     const int h = blockIdx.x / groups, row0 = blockIdx.x % groups * ROWS;  // rows of the KV head: token row / G, q head row % G
@@ -319,7 +338,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
     if (first > last) return;  // none of the range's positions are seen
     const uint8_t * head = a.c.data + (size_t(s) * a.c.n_head_kv + h) * size_t(a.c.tiles) * kv4_record(HD);
 
-    u32x4 q[NQ][NB][2];  // the queries' two parts, elements in the order of nibbles()
+    u32x4 q[QL ? 1 : NQ][QL ? 1 : NB][2];  // the queries' two parts, elements in the order of nibbles()
     float kq[NQ];        // what brings the products back: scale * log2(e) over the row's power of two
     int my_lo[NQ], my_hi[NQ];
     f32x4 o[NQ][NB][2];
@@ -356,8 +375,12 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
                 const float u = x[b][order[2 * i]] * up, w = x[b][order[2 * i + 1]] * up;
                 uint32_t hi2, lo2;
                 split2(u, w, hi2, lo2);
-                q[n][b][0][i] = hi2;
-                q[n][b][1][i] = lo2;
+                q[QL ? 0 : n][QL ? 0 : b][0][i] = hi2;
+                q[QL ? 0 : n][QL ? 0 : b][1][i] = lo2;
+            }
+            if (QL && (b & 3) == wave) {
+                ql[(n * NB + b) * 2][lane] = q[0][0][0];
+                ql[(n * NB + b) * 2 + 1][lane] = q[0][0][1];
             }
         }
         c[n] = KV4_LOW;
@@ -365,6 +388,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
         for (int b = 0; b < NB; ++b) o[n][b][0] = o[n][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
+    if constexpr (QL) __syncthreads();
     int e = 30;  // the value scales' exponent, and their bound 2^(7 - e)
     for (; at <= last; at += 4) {
         Kv4Tile<HD> next;
@@ -374,45 +398,37 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
         const bool edge = from < (a.window ? p0 + t_hi - a.window + 1 : 0) || from + KV4_TILE - 1 > p0 + t_lo;  // some row does not see all of it
         if (edge) {  // positions that no row sees may never have been stored: their scales become 0
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int p = from + (i >> 2) * 16 + 4 * g + (i & 3);
-                if (p < lo || p > hi) {
-                    const uint32_t keep = i & 1 ? 0x0000ffffu : 0xffff0000u;
-#pragma unroll
-                    for (int b = 0; b < NB; ++b) {
-                        tile.kd[b][i / 2] &= keep;
-                        tile.vd[b][i / 2] &= keep;
-                    }
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < Kv4Tile<HD>::NV * 2; ++i) {  // the same of the lane's share
-                const int w = Kv4Tile<HD>::any_word(lane, i / 2) * 2 + (i & 1);  // which scale of the record
-                const int p = from + ((w >> 2) & 1) * 16 + w / (8 * NB) * 4 + (w & 3);
-                if (p < lo || p > hi) tile.any[i / 2] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+            for (int i = 0; i < Kv4Tile<HD>::NS; ++i) {
+                const int p = from + Kv4Tile<HD>::at(lane, i);
+                if (p < lo || p > hi) tile.d[i / 2] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
             }
         }
+        tile.stage(scales[wave], lane);
         uint32_t dtop = 0;  // the largest value scale's magnitude, as fp16 bits
 #pragma unroll
-        for (int i = 0; i < Kv4Tile<HD>::NV; ++i) dtop = max(dtop, max(tile.any[i] & 0x7fffu, (tile.any[i] >> 16) & 0x7fffu));
+        for (int i = 0; i < Kv4Tile<HD>::NW; ++i) dtop = max(dtop, max(tile.d[i] & 0x7fffu, (tile.d[i] >> 16) & 0x7fffu));
+        if (lane < 32) dtop = 0;
+        wave_sync();
         bool again = __any(half_of(dtop, 0) >= __uint_as_float(uint32_t(127 + 7 - e) << 23));
         float sc[NQ][8];
         f32x4 acc[NQ][2];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
+        for (int b = 0; b < NB; ++b) {
+            const u32x4 kd = *reinterpret_cast<const u32x4 *>(&scales[wave][(g * NB + b) * 4]);
 #pragma unroll
             for (int u = 0; u < 2; ++u) {
                 const u32x4 kk = nibbles(tile.k[u][b]);
 #pragma unroll
                 for (int n = 0; n < NQ; ++n) {
-                    f32x4 x = mfma(kk, q[n][b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                    x = mfma(kk, q[n][b][1], x);
+                    f32x4 x = mfma(kk, QL ? ql[(n * NB + b) * 2][lane] : q[QL ? 0 : n][QL ? 0 : b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                    x = mfma(kk, QL ? ql[(n * NB + b) * 2 + 1][lane] : q[QL ? 0 : n][QL ? 0 : b][1], x);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[n][u][i] = __builtin_fmaf(x[i], half_of(tile.kd[b][2 * u + i / 2], i & 1), acc[n][u][i]);
+                    for (int i = 0; i < 4; ++i) acc[n][u][i] = __builtin_fmaf(x[i], half_of(kd[2 * u + i / 2], i & 1), acc[n][u][i]);
                 }
             }
+        }
         float top[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -454,6 +470,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            const u32x4 vd = *reinterpret_cast<const u32x4 *>(&scales[wave][HD / 2 + (g * NB + b) * 4]);
             const u32x4 v0 = nibbles(tile.v[b][0]), v1 = nibbles(tile.v[b][1]);  // positions 0, 2, 1, 3 and 4, 6, 5, 7 of the lane's 8
             const u32x4 lo4 = {v0[0], v0[1], v1[0], v1[1]}, hi4 = {v0[2], v0[3], v1[2], v1[3]};
 #pragma unroll
@@ -462,7 +479,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int i0 = (i >> 1) * 4 + (i & 1), i1 = i0 + 2;
-                    const float u = sc[n][i0] * half_of(tile.vd[b][i0 / 2], i0 & 1), w = sc[n][i1] * half_of(tile.vd[b][i1 / 2], i1 & 1);
+                    const float u = sc[n][i0] * half_of(vd[i0 / 2], i0 & 1), w = sc[n][i1] * half_of(vd[i1 / 2], i1 & 1);
                     uint32_t hi2, lo2;
                     split2(u, w, hi2, lo2);
                     ph[i] = hi2;
@@ -475,6 +492,7 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
             }
         }
         tile = next;
+        wave_sync();  // the scales have been read
     }
     // ---- the waves' sums joined, a block of 32 elements after another ----
 #pragma unroll
@@ -524,33 +542,51 @@ __global__ __launch_bounds__(256) void kv4_attn_kernel(Kv4AttnArgs a) {
     }
 }
 
-// Workgroup (q head, token, sequence): the sets of a sequence with several ranges, a thread an element.
+// Workgroup (q head, token, sequence): the sets of a sequence with several ranges. The factors of all sets first, then HD / 4 threads
+// a set, 1024 / HD sets at a time.
 template <int HD>
-__global__ __launch_bounds__(HD < 64 ? 64 : HD) void kv4_join_kernel(Kv4AttnArgs a) {
-    const int hq = blockIdx.x, t = blockIdx.y, tid = threadIdx.x;
+__global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
+    constexpr int PER = HD / 4, SETS = 256 / PER;
+    __shared__ float f[KV4_GROUPS], red[2][4];
+    __shared__ __align__(16) float part[SETS][HD];
+    const int hq = blockIdx.x, t = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int s = blockIdx.z;
     Kv4Range r;
     if (!kv4_find<false>(a, 0, s, r)) return;
     const long long p = r.p0 + t;
     if (r.tiles <= r.per || t >= r.n || p < 0 || p >= a.c.n_ctx) return;
     // the ranges that hold positions this token sees
-    const int lo = (a.window && p >= a.window ? int((p - a.window + 1) / KV4_TILE) : 0) - r.first, hi = int(p / KV4_TILE) - r.first;
+    const int j0 = ((a.window && p >= a.window ? int((p - a.window + 1) / KV4_TILE) : 0) - r.first) / r.per;
+    const int n = (int(p / KV4_TILE) - r.first) / r.per - j0 + 1;
     const size_t step = size_t(a.t.n_tok) * a.n_head * (HD + 4);
-    const float * w = a.work + ((size_t(r.slot) * a.t.n_tok + t) * a.n_head + hq) * (HD + 4);
-    float C = KV4_LOW, L = 0.0f, o = 0.0f;
-    for (int j = lo / r.per; j <= hi / r.per; ++j) C = fmaxf(C, w[j * step + HD]);
+    const float * w = a.work + (size_t(r.slot + j0) * a.t.n_tok + t) * a.n_head * (HD + 4) + size_t(hq) * (HD + 4);
+    float C = KV4_LOW, L = 0.0f;
+    for (int j = tid; j < n; j += 256) {
+        f[j] = w[j * step + HD];
+        C = fmaxf(C, f[j]);
+    }
+    C = wave_max(C);
+    if (lane == 0) red[0][wave] = C;
+    __syncthreads();
+    C = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+    for (int j = tid; j < n; j += 256) {
+        f[j] = __builtin_amdgcn_exp2f(f[j] - C);
+        L += w[j * step + HD + 1] * f[j];
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) L += __shfl_xor(L, d, WAVE);
+    if (lane == 0) red[1][wave] = L;
+    __syncthreads();
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    const int e = tid % PER * 4;
 #pragma unroll 8
-    for (int j = lo / r.per; j <= hi / r.per; ++j) {
-        const float f = __builtin_amdgcn_exp2f(w[j * step + HD] - C);
-        L += w[j * step + HD + 1] * f;
-        o += w[j * step + min(tid, HD - 1)] * f;
-    }
-    if (tid < HD) {
-        const size_t row = size_t(s) * a.t.n_tok + t;
-        const float y = o / L;
-        a.y[row * size_t(a.y_row) + size_t(hq) * HD + tid] =
-            a.gate ? sigmoid_(a.gate[row * size_t(a.q_row) + size_t(hq) * size_t(a.q_head) + tid]) * y : y;
-    }
+    for (int j = tid / PER; j < n; j += SETS) y += *reinterpret_cast<const f32x4 *>(w + j * step + e) * f[j];
+    *reinterpret_cast<f32x4 *>(&part[tid / PER][e]) = y;
+    __syncthreads();
+    if (tid >= PER) return;
+#pragma unroll
+    for (int i = 1; i < SETS; ++i) y += *reinterpret_cast<const f32x4 *>(&part[i][e]);
+    kv4_out<HD>(a, size_t(s) * a.t.n_tok + t, hq, e, y, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
 }
 
 template <typename F>
@@ -605,7 +641,7 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
         if (nq == 1) GQ_LAUNCH((kv4_attn_kernel<hd.value, 1>), grid, dim3(256), 0, s, a);
         else GQ_LAUNCH((kv4_attn_kernel<hd.value, 2>), grid, dim3(256), 0, s, a);
         if (a.ranges > a.t.n_seq)
-            GQ_LAUNCH(kv4_join_kernel<hd.value>, dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(hd.value < 64 ? 64 : hd.value), 0, s, a);
+            GQ_LAUNCH(kv4_join_kernel<hd.value>, dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
     });
 }
 

@@ -102,20 +102,21 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 //   S^T = K Q^T   16x16x32 fp16 matrix instructions, a block of 32 elements each: the quants minus 8 are whole numbers, exact in fp16;
 //                 the query, scaled to its row's largest element, is the sum of two fp16 numbers (22 bits). Each block's sums are
 //                 multiplied by its scales in FP32.
-//   P = 2^(S - c) in FP32. Lane 16 g + q then holds query q's weights of the 8 positions that it feeds to
-//   O^T += V^T P^T: the value scales differ by position, so they go into the weights: p d as the sum of two fp16 numbers, against the
-//                 whole quants. The accumulators stay with the query's lanes, and nothing crosses lanes in the loop.
-// The reference c = m - e of a query: m its running maximum, taken anew only when a score passes it by 8 (the weights may be
-// 2^8), and e an exponent common to the wave that brings the largest value scale so far to 2^6..2^7, so p d < 2^15 has its fp16
-// parts' full precision (they are whole multiples of 2^-24: 2^-30 of what the largest scale gives). Both sums are taken relative to
-// c, so e cancels.
-// The four waves of a workgroup take the records of its range in turn and join at the end; ranges of one sequence are joined by
-// kv4_join_kernel.
+//   P = 2^(S - c) in FP32, c = m - 7 with m the query's running maximum, taken anew only when a score passes it by 8 (so P < 2^15).
+//                 P is the sum of two fp16 numbers, whole multiples of 2^-24 (2^-31 of the largest weight). Lane 16 g + q holds
+//                 query q's weights of the 8 positions that it feeds to
+//   O^T += V^T P^T: a value, quant minus 8 times scale, has 15 bits: the sum of two fp16 numbers again (the rounded product and, by a
+//                 fused multiply-add, what is missing). The scales are brought up by a power of two 2^e common to the wave, the
+//                 largest so far to 2^9..2^10, so that the second number is a multiple of 2^-24 too. Three of the four products of
+//                 parts are summed (the fourth is below 2^-22 of the first).
+// The accumulators stay with the query's lanes and nothing crosses lanes in the loop. The four waves of a workgroup take the
+// records of its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+typedef uint16_t __attribute__((may_alias)) half_word;  // 16 bits of memory that is read as words
 
 constexpr float KV4_LOW = -1e30f;  // below every score: the maximum before the first one
 
@@ -133,8 +134,8 @@ __device__ __forceinline__ void load_words(const uint8_t * p, uint32_t * w) {
     }
 }
 
-// What a lane holds of a record: its quants in registers; the scales, which 16 lanes share, go through LDS (a lane loads and masks
-// 4 HD / 64 bytes of them: the keys' in lanes 0..31, the values' in 32..63).
+// What a lane holds of a record: its quants in registers; the scales, which 16 lanes share, go through LDS (a lane loads, masks and
+// scales 4 HD / 64 bytes of them: the keys' in lanes 0..31, the values' in 32..63).
 template <int HD>
 struct Kv4Tile {
     static constexpr int NB = HD / 32, KB = Kv4Layout<HD>::KB, VB = Kv4Layout<HD>::VB;
@@ -144,28 +145,43 @@ struct Kv4Tile {
     uint32_t v[NB][2];  // its element's value bytes at its 8 positions
     uint32_t d[NW];
 
-    __device__ __forceinline__ void load(const uint8_t * rec, int lane) {
-        using L = Kv4Layout<HD>;
+    __device__ __forceinline__ void load_keys(const uint8_t * rec, int lane) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
             for (int c = 0; c < NB / KB; ++c) load_words<KB>(rec + u * 8 * HD + c * 256 * KB + lane * 4 * KB, &k[u][c * KB]);
-        if constexpr (NS > 1) load_words<NW>(rec + L::KD + lane * 4 * NW, d);
-        else d[0] = *reinterpret_cast<const uint16_t *>(rec + L::KD + lane * 2);
+    }
+    __device__ __forceinline__ void load_scales(const uint8_t * rec, int lane) {
+        if constexpr (NS > 1) load_words<NW>(rec + Kv4Layout<HD>::KD + lane * 4 * NW, d);
+        else d[0] = *reinterpret_cast<const uint16_t *>(rec + Kv4Layout<HD>::KD + lane * 2);
+    }
+    __device__ __forceinline__ void load_values(const uint8_t * rec, int lane) {
 #pragma unroll
-        for (int c = 0; c < NB / VB; ++c) load_words<2 * VB>(rec + L::VQ + c * 512 * VB + lane * 8 * VB, v[c * VB]);
+        for (int c = 0; c < NB / VB; ++c) load_words<2 * VB>(rec + Kv4Layout<HD>::VQ + c * 512 * VB + lane * 8 * VB, v[c * VB]);
     }
     // The position of the record that the lane's scale i belongs to.
     __device__ static int at(int lane, int i) {
         const int w = (lane & 31) * NS + i;
         return ((w >> 2) & 1) * 16 + w / (8 * NB) * 4 + (w & 3);
     }
-    __device__ __forceinline__ void stage(uint32_t * lds, int lane) const {
-        if constexpr (NS > 1) {
+    // Scales to LDS, each group of four in the order 0, 2, 1, 3 of nibbles(), times f (fp16 pairs; 1 for the keys').
+    __device__ __forceinline__ void stage(uint32_t * lds, int lane, half2 f) const {
+        uint32_t x[NW];
 #pragma unroll
-            for (int i = 0; i < NW; ++i) lds[lane * NW + i] = d[i];
+        for (int i = 0; i < NW; ++i) x[i] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, d[i]) * f);
+        if constexpr (NS >= 4) {
+#pragma unroll
+            for (int i = 0; i < NW; i += 2) {
+                lds[lane * NW + i] = __builtin_amdgcn_perm(x[i + 1], x[i], 0x05040100u);
+                lds[lane * NW + i + 1] = __builtin_amdgcn_perm(x[i + 1], x[i], 0x07060302u);
+            }
         } else {
-            reinterpret_cast<uint16_t *>(lds)[lane] = uint16_t(d[0]);
+            half_word * p = reinterpret_cast<half_word *>(lds);
+#pragma unroll
+            for (int i = 0; i < NS; ++i) {
+                const int w = lane * NS + i;
+                p[(w & ~3) + ((w & 1) << 1) + ((w >> 1) & 1)] = uint16_t(x[0] >> (16 * i));
+            }
         }
     }
 };
@@ -184,23 +200,38 @@ __device__ __forceinline__ uint32_t pack2(float a, float b) {
     return __builtin_bit_cast(uint32_t, h);
 }
 
-// Two numbers as the sums of two fp16 numbers each: hi + lo, 22 bits. The empty asm makes the numbers exist (see f2h): folded into
-// the conversion, a product's nearest fp16 number can differ from the one that lo is formed against.
-__device__ __forceinline__ void split2(float a, float b, uint32_t & hi, uint32_t & lo) {
+// Constants that the compiler is kept from seeing: masks and exponents whose and-or then is one instruction (two literals would not
+// fit it), and a -1 whose multiply-add with an fp16 operand is one.
+struct Kv4Const {
+    uint32_t m0, m1, x0, x1;
+    float minus;
+    __device__ __forceinline__ Kv4Const() {
+        __asm__("s_mov_b32 %0, 0x000f000f" : "=s"(m0));
+        __asm__("s_mov_b32 %0, 0x00f000f0" : "=s"(m1));
+        __asm__("v_mov_b32 %0, 0x64006400" : "=v"(x0));
+        __asm__("v_mov_b32 %0, 0x54005400" : "=v"(x1));
+        __asm__("s_mov_b32 %0, -1.0" : "=s"(minus));
+    }
+};
+
+// Two numbers as the sums of two fp16 numbers each: hi + lo, 22 bits. The empty asms make the numbers and their upper parts exist
+// (see f2h): folded into the conversion, a product's nearest fp16 number can differ from the one that lo is formed against.
+__device__ __forceinline__ void split2(float a, float b, uint32_t & hi, uint32_t & lo, const Kv4Const & k) {
     __asm__("" : "+v"(a), "+v"(b));
     hi = pack2(a, b);
-    lo = pack2(a - half_of(hi, 0), b - half_of(hi, 1));
+    __asm__("" : "+v"(hi));
+    lo = pack2(__builtin_fmaf(half_of(hi, 0), k.minus, a), __builtin_fmaf(half_of(hi, 1), k.minus, b));
 }
 
 // The 8 nibbles of four bytes minus 8, as fp16: low nibbles of bytes 0, 2, 1, 3, then the high ones.
-__device__ __forceinline__ u32x4 nibbles(uint32_t w) {
+__device__ __forceinline__ u32x4 nibbles(uint32_t w, const Kv4Const & k) {
     const half2 c0 = {_Float16(-1032.0f), _Float16(-1032.0f)}, c1 = {_Float16(-72.0f), _Float16(-72.0f)};
     const uint32_t x = w >> 8;
     u32x4 r;
-    r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (w & 0x000f000fu) | 0x64006400u) + c0);  // 1024 + n
-    r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (x & 0x000f000fu) | 0x64006400u) + c0);
-    r[2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (w & 0x00f000f0u) | 0x54005400u) + c1);  // 64 + n
-    r[3] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (x & 0x00f000f0u) | 0x54005400u) + c1);
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (w & k.m0) | k.x0) + c0);  // 1024 + n
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (x & k.m0) | k.x0) + c0);
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (w & k.m1) | k.x1) + c1);  // 64 + n
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(half2, (x & k.m1) | k.x1) + c1);
     return r;
 }
 
@@ -309,12 +340,11 @@ __device__ __forceinline__ void kv4_out(const Kv4AttnArgs & a, size_t row, int h
 }
 
 template <int HD, int NQ>
-__global__ __launch_bounds__(256, HD == 256 && NQ == 1 ? 2 : 1) void kv4_attn_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     constexpr int NB = HD / 32, ROWS = 16 * NQ, PAD = 36;
     __shared__ __align__(16) float part[4][ROWS][PAD];
-    // head_dim 256: the queries' parts, the same for the four waves, stay in LDS (in registers they leave room for one wave a SIMD, or
-    // for 16 rows without spills)
-    constexpr bool QL = HD == 256;
+    // the queries' parts, the same for the four waves: in LDS where registers would not leave room for two waves a SIMD
+    constexpr bool QL = HD * NQ > 128;
     __shared__ u32x4 ql[QL ? NQ * NB * 2 : 1][64];
     __shared__ float cs[4][ROWS], ls[4][ROWS];
     __shared__ __align__(16) uint32_t scales[4][HD];  // a wave's record's key scales, then its value scales: [g][block][8] each
@@ -337,15 +367,21 @@ __global__ __launch_bounds__(256, HD == 256 && NQ == 1 ? 2 : 1) void kv4_attn_ke
     const int last = __builtin_amdgcn_readfirstlane(min(r.first + min((j + 1) * r.per, r.tiles) - 1, hi / KV4_TILE));
     if (first > last) return;  // none of the range's positions are seen
     const uint8_t * head = a.c.data + (size_t(s) * a.c.n_head_kv + h) * size_t(a.c.tiles) * kv4_record(HD);
+    const Kv4Const k4;
 
     u32x4 q[QL ? 1 : NQ][QL ? 1 : NB][2];  // the queries' two parts, elements in the order of nibbles()
-    float kq[NQ];        // what brings the products back: scale * log2(e) over the row's power of two
+    float kq[NQ];  // what brings the products back: scale * log2(e) over the row's power of two
     int my_lo[NQ], my_hi[NQ];
     f32x4 o[NQ][NB][2];
     float c[NQ], l[NQ];
     Kv4Tile<HD> tile;
     int at = first + wave;
-    tile.load(head + size_t(min(at, last)) * kv4_record(HD), lane);
+    {
+        const uint8_t * rec = head + size_t(min(at, last)) * kv4_record(HD);
+        tile.load_scales(rec, lane);
+        tile.load_keys(rec, lane);
+        tile.load_values(rec, lane);
+    }
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         const int row = row0 + n * 16 + col, t = row / G;
@@ -369,18 +405,22 @@ __global__ __launch_bounds__(256, HD == 256 && NQ == 1 ? 2 : 1) void kv4_attn_ke
         kq[n] = a.scale * 1.44269504088896341f * __uint_as_float(uint32_t(e - 13) << 23);
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
+            if (QL && (b & 3) != wave && NB >= 4) continue;  // (each wave a quarter of the blocks)
             constexpr int order[8] = {0, 2, 1, 3, 4, 6, 5, 7};
+            u32x4 qh, qlo;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const float u = x[b][order[2 * i]] * up, w = x[b][order[2 * i + 1]] * up;
                 uint32_t hi2, lo2;
-                split2(u, w, hi2, lo2);
-                q[QL ? 0 : n][QL ? 0 : b][0][i] = hi2;
-                q[QL ? 0 : n][QL ? 0 : b][1][i] = lo2;
+                split2(x[b][order[2 * i]] * up, x[b][order[2 * i + 1]] * up, hi2, lo2, k4);
+                qh[i] = hi2;
+                qlo[i] = lo2;
             }
-            if (QL && (b & 3) == wave) {
-                ql[(n * NB + b) * 2][lane] = q[0][0][0];
-                ql[(n * NB + b) * 2 + 1][lane] = q[0][0][1];
+            if constexpr (QL) {
+                ql[(n * NB + b) * 2][lane] = qh;
+                ql[(n * NB + b) * 2 + 1][lane] = qlo;
+            } else {
+                q[n][b][0] = qh;
+                q[n][b][1] = qlo;
             }
         }
         c[n] = KV4_LOW;
@@ -389,11 +429,9 @@ __global__ __launch_bounds__(256, HD == 256 && NQ == 1 ? 2 : 1) void kv4_attn_ke
         for (int b = 0; b < NB; ++b) o[n][b][0] = o[n][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
     if constexpr (QL) __syncthreads();
-    int e = 30;  // the value scales' exponent, and their bound 2^(7 - e)
+    int e = 15;  // the value scales' exponent: the largest so far times 2^e is below 2^10 (scales below 2^-5 keep 2^15)
     for (; at <= last; at += 4) {
-        Kv4Tile<HD> next;
-        const int ahead = min(at + 4, last);  // (the last one again where there is none)
-        next.load(head + size_t(ahead) * kv4_record(HD), lane);
+        const uint8_t * ahead = head + size_t(min(at + 4, last)) * kv4_record(HD);  // (the last one again where there is none)
         const int from = at * KV4_TILE;
         const bool edge = from < (a.window ? p0 + t_hi - a.window + 1 : 0) || from + KV4_TILE - 1 > p0 + t_lo;  // some row does not see all of it
         if (edge) {  // positions that no row sees may never have been stored: their scales become 0
@@ -403,37 +441,61 @@ __global__ __launch_bounds__(256, HD == 256 && NQ == 1 ? 2 : 1) void kv4_attn_ke
                 if (p < lo || p > hi) tile.d[i / 2] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
             }
         }
-        tile.stage(scales[wave], lane);
         uint32_t dtop = 0;  // the largest value scale's magnitude, as fp16 bits
 #pragma unroll
         for (int i = 0; i < Kv4Tile<HD>::NW; ++i) dtop = max(dtop, max(tile.d[i] & 0x7fffu, (tile.d[i] >> 16) & 0x7fffu));
         if (lane < 32) dtop = 0;
+        if (__any(int(dtop >> 10) - 15 + e >= 10)) {  // a larger value scale: bring it to 2^9
+            int top = int(dtop >> 10);
+#pragma unroll
+            for (int d = 32; d >= 1; d >>= 1) top = max(top, __shfl_xor(top, d, WAVE));
+            const int e2 = 9 + 15 - top;
+            const float f = __uint_as_float(uint32_t(127 + e2 - e) << 23);
+            e = e2;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    o[n][b][0] *= f;
+                    o[n][b][1] *= f;
+                }
+        }
+        {
+            const _Float16 f = lane < 32 ? _Float16(1.0f) : _Float16(__uint_as_float(uint32_t(127 + e) << 23));
+            tile.stage(scales[wave], lane, half2{f, f});
+        }
         wave_sync();
-        bool again = __any(half_of(dtop, 0) >= __uint_as_float(uint32_t(127 + 7 - e) << 23));
+        tile.load_scales(ahead, lane);
         float sc[NQ][8];
-        f32x4 acc[NQ][2];
+        {
+            f32x4 acc[NQ][2];
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int n = 0; n < NQ; ++n) acc[n][0] = acc[n][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            const u32x4 kd = *reinterpret_cast<const u32x4 *>(&scales[wave][(g * NB + b) * 4]);
+            for (int b = 0; b < NB; ++b) {
+                const u32x4 kd = *reinterpret_cast<const u32x4 *>(&scales[wave][(g * NB + b) * 4]);
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                const u32x4 kk = nibbles(tile.k[u][b]);
+                for (int u = 0; u < 2; ++u) {
+                    const u32x4 kk = nibbles(tile.k[u][b], k4);
 #pragma unroll
-                for (int n = 0; n < NQ; ++n) {
-                    f32x4 x = mfma(kk, QL ? ql[(n * NB + b) * 2][lane] : q[QL ? 0 : n][QL ? 0 : b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                    x = mfma(kk, QL ? ql[(n * NB + b) * 2 + 1][lane] : q[QL ? 0 : n][QL ? 0 : b][1], x);
+                    for (int n = 0; n < NQ; ++n) {
+                        f32x4 x = mfma(kk, QL ? ql[(n * NB + b) * 2][lane] : q[QL ? 0 : n][QL ? 0 : b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                        x = mfma(kk, QL ? ql[(n * NB + b) * 2 + 1][lane] : q[QL ? 0 : n][QL ? 0 : b][1], x);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) acc[n][u][i] = __builtin_fmaf(x[i], half_of(kd[2 * u + i / 2], i & 1), acc[n][u][i]);
+                        for (int i = 0; i < 4; ++i) acc[n][u][i] = __builtin_fmaf(x[i], half_of(kd[2 * u + (i & 1)], i >> 1), acc[n][u][i]);
+                    }
                 }
             }
+            tile.load_keys(ahead, lane);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) sc[n][i] = acc[n][i >> 2][i & 3] * kq[n];
         }
+        bool again = false;
         float top[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) sc[n][i] = acc[n][i >> 2][i & 3] * kq[n];
             if (edge)
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -441,60 +503,65 @@ __global__ __launch_bounds__(256, HD == 256 && NQ == 1 ? 2 : 1) void kv4_attn_ke
                     if (p < my_lo[n] || p > my_hi[n]) sc[n][i] = -__builtin_inff();
                 }
             top[n] = fmaxf(fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])), fmaxf(fmaxf(sc[n][4], sc[n][5]), fmaxf(sc[n][6], sc[n][7])));
-            again |= __any(top[n] > c[n] + float(e + 8));
+            again |= bool(__any(top[n] > c[n] + 15.0f));
         }
-        if (again) {  // new maxima and scale exponent
-            const float dm = wave_max(half_of(dtop, 0));
-            const int de = 6 + 127 - int(__float_as_uint(dm) >> 23);  // brings dm to 2^6..2^7
-            const int e2 = max(min(e, de), -10);
+        if (again) {  // new maxima
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 float m = fmaxf(top[n], __shfl_xor(top[n], 16, WAVE));
                 m = fmaxf(m, __shfl_xor(m, 32, WAVE));
-                m = fmaxf(m, c[n] + float(e));
-                const float c2 = m - float(e2), f = __builtin_amdgcn_exp2f(c[n] - c2);
+                const float c2 = fmaxf(m - 7.0f, c[n]), f = __builtin_amdgcn_exp2f(c[n] - c2);
                 c[n] = c2;
                 l[n] *= f;
 #pragma unroll
-                for (int b = 0; b < NB; ++b)
-#pragma unroll
-                    for (int u = 0; u < 2; ++u) o[n][b][u] *= f;
+                for (int b = 0; b < NB; ++b) {
+                    o[n][b][0] *= f;
+                    o[n][b][1] *= f;
+                }
             }
-            e = e2;
         }
+        u32x4 ph[NQ], pl[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) sc[n][i] = __builtin_amdgcn_exp2f(sc[n][i] - c[n]);
             l[n] += ((sc[n][0] + sc[n][1]) + (sc[n][2] + sc[n][3])) + ((sc[n][4] + sc[n][5]) + (sc[n][6] + sc[n][7]));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int i0 = (i >> 1) * 4 + (i & 1);
+                uint32_t hi2, lo2;
+                split2(sc[n][i0], sc[n][i0 + 2], hi2, lo2, k4);
+                ph[n][i] = hi2;
+                pl[n][i] = lo2;
+            }
         }
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             const u32x4 vd = *reinterpret_cast<const u32x4 *>(&scales[wave][HD / 2 + (g * NB + b) * 4]);
-            const u32x4 v0 = nibbles(tile.v[b][0]), v1 = nibbles(tile.v[b][1]);  // positions 0, 2, 1, 3 and 4, 6, 5, 7 of the lane's 8
-            const u32x4 lo4 = {v0[0], v0[1], v1[0], v1[1]}, hi4 = {v0[2], v0[3], v1[2], v1[3]};
+            const u32x4 v0 = nibbles(tile.v[b][0], k4), v1 = nibbles(tile.v[b][1], k4);  // positions 0, 2, 1, 3 and 4, 6, 5, 7 of the lane's 8
 #pragma unroll
-            for (int n = 0; n < NQ; ++n) {
-                u32x4 ph, pl;
+            for (int u = 0; u < 2; ++u) {  // the lane's element, and the one 16 further
+                u32x4 vh, vl;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const int i0 = (i >> 1) * 4 + (i & 1), i1 = i0 + 2;
-                    const float u = sc[n][i0] * half_of(vd[i0 / 2], i0 & 1), w = sc[n][i1] * half_of(vd[i1 / 2], i1 & 1);
-                    uint32_t hi2, lo2;
-                    split2(u, w, hi2, lo2);
-                    ph[i] = hi2;
-                    pl[i] = lo2;
+                    const uint32_t w32 = i < 2 ? v0[2 * u + i] : v1[2 * u + i - 2], d32 = vd[i];
+                    const half2 w = __builtin_bit_cast(half2, w32), d = __builtin_bit_cast(half2, d32), p = w * d;
+                    vh[i] = __builtin_bit_cast(uint32_t, p);
+                    vl[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(w, d, -p));
                 }
-                o[n][b][0] = mfma(lo4, ph, o[n][b][0]);
-                o[n][b][1] = mfma(hi4, ph, o[n][b][1]);
-                o[n][b][0] = mfma(lo4, pl, o[n][b][0]);
-                o[n][b][1] = mfma(hi4, pl, o[n][b][1]);
+#pragma unroll
+                for (int n = 0; n < NQ; ++n) {
+                    o[n][b][u] = mfma(vh, ph[n], o[n][b][u]);
+                    o[n][b][u] = mfma(vh, pl[n], o[n][b][u]);
+                    o[n][b][u] = mfma(vl, ph[n], o[n][b][u]);
+                }
             }
         }
-        tile = next;
+        tile.load_values(ahead, lane);
         wave_sync();  // the scales have been read
     }
     // ---- the waves' sums joined, a block of 32 elements after another ----
+    const float down = __uint_as_float(uint32_t(127 - e) << 23);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         l[n] += __shfl_xor(l[n], 16, WAVE);
@@ -504,39 +571,38 @@ __global__ __launch_bounds__(256, HD == 256 && NQ == 1 ? 2 : 1) void kv4_attn_ke
             ls[wave][n * 16 + col] = l[n];
         }
     }
-    const int rj = tid >> 3, ej = (tid & 7) * 4;  // this thread's row (of 32) and elements of a block
-    const int row = row0 + rj, tj = row / G, hq = h * G + row % G;
-    const bool mine = rj < ROWS && tj >= t_lo && tj <= t_hi;
-    float f[4], C = 0.0f, L = 0.0f;
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
         if (b) __syncthreads();
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) *reinterpret_cast<f32x4 *>(&part[wave][n * 16 + col][u * 16 + 4 * g]) = o[n][b][u];
+            for (int u = 0; u < 2; ++u) *reinterpret_cast<f32x4 *>(&part[wave][n * 16 + col][u * 16 + 4 * g]) = o[n][b][u] * down;
         __syncthreads();
-        if (!mine) continue;
-        if (b == 0) {
-            C = fmaxf(fmaxf(cs[0][rj], cs[1][rj]), fmaxf(cs[2][rj], cs[3][rj]));
+#pragma unroll
+        for (int i = 0; i < (ROWS + 31) / 32; ++i) {
+            const int rj = (tid >> 3) + i * 32, ej = (tid & 7) * 4;  // this thread's row and elements of the block
+            const int row = row0 + rj, tj = row / G, hq = h * G + row % G;
+            if (rj >= ROWS || tj < t_lo || tj > t_hi) continue;
+            const float C = fmaxf(fmaxf(cs[0][rj], cs[1][rj]), fmaxf(cs[2][rj], cs[3][rj]));
+            f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+            float L = 0.0f;
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                f[w] = __builtin_amdgcn_exp2f(cs[w][rj] - C);
-                L += ls[w][rj] * f[w];
+                const float f = __builtin_amdgcn_exp2f(cs[w][rj] - C);
+                L += ls[w][rj] * f;
+                y += *reinterpret_cast<const f32x4 *>(&part[w][rj][ej]) * f;
             }
-        }
-        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int w = 0; w < 4; ++w) y += *reinterpret_cast<const f32x4 *>(&part[w][rj][ej]) * f[w];
-        const size_t orow = size_t(s) * a.t.n_tok + tj;
-        if (split == 1) {
-            kv4_out<HD>(a, orow, hq, b * 32 + ej, y, L);
-        } else {  // this range's set: [range][token][head][HD + 4], C and L behind the sums
-            float * w = a.work + ((size_t(range) * a.t.n_tok + tj) * a.n_head + hq) * (HD + 4);
-            *reinterpret_cast<f32x4 *>(w + b * 32 + ej) = y;
-            if (b == 0 && ej == 0) {
-                w[HD] = C;
-                w[HD + 1] = L;
+            const size_t orow = size_t(s) * a.t.n_tok + tj;
+            if (split == 1) {
+                kv4_out<HD>(a, orow, hq, b * 32 + ej, y, L);
+            } else {  // this range's set: [range][token][head][HD + 4], C and L behind the sums
+                float * w = a.work + ((size_t(range) * a.t.n_tok + tj) * a.n_head + hq) * (HD + 4);
+                *reinterpret_cast<f32x4 *>(w + b * 32 + ej) = y;
+                if (b == 0 && ej == 0) {
+                    w[HD] = C;
+                    w[HD + 1] = L;
+                }
             }
         }
     }
@@ -616,12 +682,16 @@ hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s) {
     });
 }
 
-// Rows of a workgroup, and how many ranges a call's records are dealt to: about KV4_GROUPS workgroups in all, but at least one
-// range a sequence and no more than KV4_LEAST records each give.
-static int kv4_nq(int n_tok, int per_kv) { return n_tok * (long long)per_kv > 16 ? 2 : 1; }
+// Groups of 16 rows that a workgroup takes: as many as there are, up to what the registers hold.
+static int kv4_nq(int hd, int n_tok, int per_kv) {
+    const long long rows = n_tok * (long long)per_kv;
+    return rows <= 16 ? 1 : rows <= 32 || hd == 256 ? 2 : 4;
+}
 
+// How many ranges a call's records are dealt to: about KV4_GROUPS workgroups in all, but at least one range a sequence and no more
+// than KV4_LEAST records each give.
 int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
-    const int per_kv = n_head / c.n_head_kv, rows = 16 * kv4_nq(n_tok, per_kv);
+    const int per_kv = n_head / c.n_head_kv, rows = 16 * kv4_nq(c.head_dim, n_tok, per_kv);
     const long long units = (n_tok * (long long)per_kv + rows - 1) / rows * c.n_head_kv;
     const long long most = (long long)n_seq * ((c.tiles + KV4_LEAST - 1) / KV4_LEAST);
     return int(std::min<long long>(std::max<long long>(n_seq, std::min(KV4_GROUPS / units, most)), 65535));
@@ -634,12 +704,13 @@ size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
 
 hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
     Kv4AttnArgs a = args;
-    const int per_kv = a.n_head / a.c.n_head_kv, nq = kv4_nq(a.t.n_tok, per_kv);
+    const int per_kv = a.n_head / a.c.n_head_kv, nq = kv4_nq(a.c.head_dim, a.t.n_tok, per_kv);
     a.ranges = kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head);
     const dim3 grid(unsigned((a.t.n_tok * (long long)per_kv + 16 * nq - 1) / (16 * nq) * a.c.n_head_kv), unsigned(a.ranges));
     return by_dim(a.c.head_dim, [&](auto hd) {
         if (nq == 1) GQ_LAUNCH((kv4_attn_kernel<hd.value, 1>), grid, dim3(256), 0, s, a);
-        else GQ_LAUNCH((kv4_attn_kernel<hd.value, 2>), grid, dim3(256), 0, s, a);
+        else if (nq == 2) GQ_LAUNCH((kv4_attn_kernel<hd.value, 2>), grid, dim3(256), 0, s, a);
+        else if constexpr (hd.value < 256) GQ_LAUNCH((kv4_attn_kernel<hd.value, 4>), grid, dim3(256), 0, s, a);
         if (a.ranges > a.t.n_seq)
             GQ_LAUNCH(kv4_join_kernel<hd.value>, dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
     });

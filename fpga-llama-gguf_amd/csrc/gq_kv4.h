@@ -70,6 +70,7 @@ struct Kv4AttnArgs {
     const float * gate;  // NULL, or gate rows as q's (the output times sigmoid(gate))
     float * work;        // kv4_work_floats
     int ranges;          // set at launch: ranges of records that the grid has workgroups for
+    int group;           // set at launch: n_head / n_head_kv
 };
 
 constexpr int KV4_GROUPS = 1024;  // workgroups that a call's records are dealt to, where they are enough

@@ -8,20 +8,34 @@
 namespace gq {
 namespace {
 
-// One block of 32 elements, one per lane of a half wave: returns the lane's quant and, in d, the block's fp16 scale.
-__device__ __forceinline__ uint32_t kv4_quantize(float x, uint32_t & d16) {
-    const int lane = threadIdx.x & 63;
-    float am = fabsf(x);
+// A block of 32 elements held by 8 lanes, lane j elements 4 j .. 4 j + 3: returns the lane's four quants as the low nibbles of four
+// bytes and, in d16, the block's fp16 scale.
+__device__ __forceinline__ uint32_t kv4_quantize(const float * x, uint32_t & d16) {
+    float am = fabsf(x[0]), m = x[0];
 #pragma unroll
-    for (int s = 16; s >= 1; s >>= 1) am = fmaxf(am, __shfl_xor(am, s, WAVE));
-    const unsigned long long at = __ballot(fabsf(x) == am);
-    const uint32_t half = lane < 32 ? uint32_t(at) : uint32_t(at >> 32);
-    const float m = __shfl(x, (lane & 32) + (half ? __ffs(int(half)) - 1 : 0), WAVE);
-    const float d = m / -8.0f;
-    const float id = d != 0.0f ? 1.0f / d : 0.0f;
-    const float v = x * id + 8.5f;
+    for (int i = 1; i < 4; ++i) {
+        const bool more = fabsf(x[i]) > am;
+        am = more ? fabsf(x[i]) : am;
+        m = more ? x[i] : m;
+    }
+    const int lane = threadIdx.x;
+    const auto take = [&](float am2, float m2, bool later) {  // the other lanes' largest; of equal ones the first
+        const bool other = am2 > am || (later && am2 == am);
+        am = other ? am2 : am;
+        m = other ? m2 : m;
+    };
+    take(dpp_f32<DPP_XOR1>(am), dpp_f32<DPP_XOR1>(m), lane & 1);
+    take(dpp_f32<DPP_XOR2>(am), dpp_f32<DPP_XOR2>(m), lane & 2);
+    take(dpp_f32<DPP_HALF_MIRROR>(am), dpp_f32<DPP_HALF_MIRROR>(m), lane & 4);
+    const float d = m / -8.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
     d16 = f2h(d);
-    return uint32_t(int(fminf(fmaxf(v, 0.0f), 15.0f)));
+    uint32_t q = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float v = x[i] * id + 8.5f;
+        q |= uint32_t(int(fminf(fmaxf(v, 0.0f), 15.0f))) << (8 * i);
+    }
+    return q;
 }
 
 // The sequence's first position and number of tokens.
@@ -34,37 +48,68 @@ __device__ __forceinline__ uint8_t * kv4_rec(const Kv4Cache & c, int s, int h, i
     return c.data + ((size_t(s) * c.n_head_kv + h) * c.tiles + tile) * kv4_record(c.head_dim);
 }
 
-// Workgroup (record of the tokens' span, KV head, sequence): half waves take the blocks of its positions in turn. A record that the
-// tokens fill is put together in LDS and written in 16-byte pieces; of the others only the tokens' own bytes are written.
+// Workgroup (record of the tokens' span; keys or values; four blocks | KV head | sequence): 8 lanes a block. A record that the tokens
+// fill is put together in LDS and written in 16-byte pieces; of the others only the tokens' own bytes are written. So small a share
+// of a record (2.3 KB) that a prompt of 512 tokens still has a few hundred workgroups, each with its 8 reads in flight together.
+constexpr int KV4_STORE = 128;  // threads
 template <int HD>
-__global__ __launch_bounds__(256) void kv4_store_kernel(Kv4RowsArgs a) {
+__global__ __launch_bounds__(KV4_STORE) void kv4_store_kernel(Kv4RowsArgs a) {
     using L = Kv4Layout<HD>;
-    __shared__ __align__(16) uint8_t img[L::RECORD];
-    const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, hw = tid >> 5, e = tid & 31;
+    constexpr int BG = L::NB < 4 ? L::NB : 4, GROUPS = L::NB / BG, UNITS = KV4_STORE / 8, ITER = KV4_TILE * BG / UNITS;
+    constexpr int QB = 512 * BG;  // bytes of the quants of BG blocks, keys or values
+    __shared__ __align__(16) uint8_t img[QB + 64 * BG];
+    const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, j = tid & 7;
+    const int val = blockIdx.x & 1, bg = (blockIdx.x >> 1) % GROUPS;
     long long p0;
     int n;
     kv4_span(a.t, s, p0, n);
     const long long lo = p0 < 0 ? 0 : p0, hi = p0 + n < a.c.n_ctx ? p0 + n : a.c.n_ctx;  // positions to store
-    const long long tile = lo / KV4_TILE + blockIdx.x;
-    if (lo >= hi || tile * KV4_TILE >= hi) return;
-    const int first = int(lo - tile * KV4_TILE > 0 ? lo - tile * KV4_TILE : 0);
-    const int end = int(hi - tile * KV4_TILE < KV4_TILE ? hi - tile * KV4_TILE : KV4_TILE);
-    uint8_t * rec = kv4_rec(a.c, s, h, int(tile));
+    const long long at = (lo / KV4_TILE + (blockIdx.x >> 1) / GROUPS) * KV4_TILE;        // the record's first position
+    if (lo >= hi || at >= hi) return;
+    const int first = int(lo - at > 0 ? lo - at : 0), end = int(hi - at < KV4_TILE ? hi - at : KV4_TILE);
+    uint8_t * rec = kv4_rec(a.c, s, h, int(at / KV4_TILE));
     const bool full = end - first == KV4_TILE;
-    uint8_t * out = full ? img : rec;
-    for (int u = hw; u < (end - first) * L::NB * 2; u += 8) {
-        const int p = first + u / (2 * L::NB), blk = u % L::NB;
-        const bool val = (u / L::NB) & 1;
-        const size_t row = size_t(s) * a.t.n_tok + size_t(tile * KV4_TILE + p - p0);
+    const float * src = (val ? a.v : a.k) + size_t(h) * HD + bg * 128 + j * 4;
+    const long long row0 = (long long)s * a.t.n_tok + (at - p0);
+    const int units = (end - first) * BG;
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    float x[ITER][4];
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int u = i * UNITS + (tid >> 3);
+        if (u < units) *reinterpret_cast<f32x4 *>(x[i]) = *reinterpret_cast<const f32x4 *>(src + (row0 + first + u / BG) * a.row_stride + u % BG * 32);
+    }
+#pragma unroll
+    for (int i = 0; i < ITER; ++i) {
+        const int u = i * UNITS + (tid >> 3);
+        if (u >= units) break;
+        const int p = first + u / BG, b = u % BG, blk = bg * BG + b;
         uint32_t d;
-        const uint32_t q = kv4_quantize((val ? a.v : a.k)[row * size_t(a.row_stride) + size_t(h) * HD + blk * 32 + e], d);
-        const uint32_t up = __shfl_xor(q, 16, WAVE);
-        if (e < 16) out[val ? L::vq(p, blk, e) : L::kq(p, blk, e)] = uint8_t(q | up << 4);
-        if (e == 0) *reinterpret_cast<uint16_t *>(out + (val ? L::VD : L::KD) + L::scale(p, blk)) = uint16_t(d);
+        const uint32_t q = kv4_quantize(x[i], d), bytes = q | uint32_t(dpp_i32<0x104>(int(q))) << 4;  // lanes j < 4: with those of lane j + 4
+        uint8_t * to = full ? img : rec;
+        if (j < 4) {
+            if (val) {
+                uint8_t * v = to + (full ? L::vq(p, blk, 4 * j) - L::VQ - bg * QB : L::vq(p, blk, 4 * j));
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e * 8 * L::VB] = uint8_t(bytes >> (8 * e));
+            } else {
+                uint8_t * k = to + (full ? L::kq(p, blk, 4 * j) - (p >> 4) * (8 * HD - 256 * BG) - bg * 256 * L::KB : L::kq(p, blk, 4 * j));
+                *reinterpret_cast<uint32_t *>(k) = bytes;
+            }
+        }
+        if (j == 0)
+            *reinterpret_cast<uint16_t *>(full ? img + QB + ((p & 15) >> 2) * 16 * BG + b * 16 + (p >> 4) * 8 + (p & 3) * 2
+                                               : rec + (val ? L::VD : L::KD) + L::scale(p, blk)) = uint16_t(d);
     }
     if (!full) return;
     __syncthreads();
-    for (int i = tid; i < L::RECORD / 16; i += 256) reinterpret_cast<uint4 *>(rec)[i] = reinterpret_cast<const uint4 *>(img)[i];
+    for (int i = tid; i < QB / 16; i += KV4_STORE) {
+        const int sub = i / (QB / 32);  // keys: the record's halves lie apart
+        const int to = val ? L::VQ + bg * QB + i * 16 : sub * 8 * HD + bg * 256 * L::KB + (i - sub * (QB / 32)) * 16;
+        *reinterpret_cast<uint4 *>(rec + to) = *reinterpret_cast<const uint4 *>(img + i * 16);
+    }
+    for (int i = tid; i < 4 * BG; i += KV4_STORE)
+        *reinterpret_cast<uint4 *>(rec + (val ? L::VD : L::KD) + (i / BG * L::NB + bg * BG + i % BG) * 16) = *reinterpret_cast<const uint4 *>(img + QB + i * 16);
 }
 
 template <int HD>
@@ -266,8 +311,12 @@ __device__ __forceinline__ void kv4_seen(const Kv4AttnArgs & a, int s, Kv4Range 
 
 // The ranges' length: all records over the ranges that the grid has room for, a sequence's last one being short.
 __device__ __forceinline__ int kv4_per(long long records, int ranges, int n_seq, int most) {
-    const long long per = ranges > n_seq ? (records + ranges - n_seq - 1) / (ranges - n_seq) : most;
-    return int(per > KV4_LEAST ? per : KV4_LEAST);
+    int per = most;
+    if (ranges > n_seq) {
+        if (n_seq == 1) per = int((unsigned(records) + unsigned(ranges) - 1u) / unsigned(ranges));
+        else per = int(ceil(double(records) / double(ranges - n_seq)));  // (quotients below 2^27 with fractions of at least 2^-16)
+    }
+    return per > KV4_LEAST ? per : KV4_LEAST;
 }
 
 // All sequences' records (a wave's lanes scan them together): the ranges' length.
@@ -341,39 +390,37 @@ __device__ __forceinline__ void kv4_out(const Kv4AttnArgs & a, size_t row, int h
 
 template <int HD, int NQ>
 __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
-    constexpr int NB = HD / 32, ROWS = 16 * NQ, PAD = 36;
-    __shared__ __align__(16) float part[4][ROWS][PAD];
-    // the queries' parts, the same for the four waves: in LDS where registers would not leave room for two waves a SIMD
-    constexpr bool QL = HD * NQ > 128;
-    __shared__ u32x4 ql[QL ? NQ * NB * 2 : 1][64];
-    __shared__ float cs[4][ROWS], ls[4][ROWS];
+    constexpr int NB = HD / 32, ROWS = 16 * NQ;
+    // Blocks of 32 elements that the waves' sums are joined in at a time; threads of a row there.
+    constexpr int JB = NQ == 1 ? NB : 1, PAD = 32 * JB + 4, JT = 256 / ROWS;
+    constexpr size_t QBYTES = size_t(NQ) * NB * 2 * 1024, JBYTES = size_t(4) * ROWS * PAD * 4;
+    __shared__ __align__(16) uint8_t both[QBYTES > JBYTES ? QBYTES : JBYTES];
+    u32x4(*ql)[64] = reinterpret_cast<u32x4(*)[64]>(both);              // the queries' parts
+    float(*part)[ROWS][PAD] = reinterpret_cast<float(*)[ROWS][PAD]>(both);  // later the waves' sums
+    constexpr bool QL = HD * NQ > 128;  // the queries stay in LDS where registers would not leave room for two waves a SIMD
+    __shared__ float kqs[ROWS], cs[4][ROWS], ls[4][ROWS];
     __shared__ __align__(16) uint32_t scales[4][HD];  // a wave's record's key scales, then its value scales: [g][block][8] each
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
-    const int G = a.n_head / a.c.n_head_kv, groups = (a.t.n_tok * G + ROWS - 1) / ROWS;
-    const int h = blockIdx.x / groups, row0 = blockIdx.x % groups * ROWS;  // rows of the KV head: token row / G, q head row % G
-    const int range = blockIdx.y;
+    const int G = a.group, h = blockIdx.y, row0 = blockIdx.x * ROWS;  // rows of the KV head: token row / G, q head row % G
+    const int range = blockIdx.z;
     int s = 0;
     Kv4Range r;
     if (!kv4_find<true>(a, range, s, r)) return;
     s = __builtin_amdgcn_readfirstlane(s);
     const int p0 = __builtin_amdgcn_readfirstlane(int(r.p0));
     const int live = min(__builtin_amdgcn_readfirstlane(r.n), a.c.n_ctx - p0);  // tokens -p0 (where p0 < 0) .. live - 1 have positions
-    const int t_lo = max(row0 / G, -p0), t_hi = min((row0 + ROWS - 1) / G, live - 1);
+    const int t_lo = max(int(unsigned(row0) / unsigned(G)), -p0), t_hi = min(int(unsigned(row0 + ROWS - 1) / unsigned(G)), live - 1);
     if (t_lo > t_hi) return;
     // the group's positions: lo .. hi, the rows' own ranges within them
     const int lo = a.window ? max(0, p0 + t_lo - a.window + 1) : 0, hi = p0 + t_hi;
-    const int j = range - r.slot, split = __builtin_amdgcn_readfirstlane((r.tiles + r.per - 1) / r.per);
+    const int j = range - r.slot;
+    const bool alone = __builtin_amdgcn_readfirstlane(int(r.tiles <= r.per));  // the sequence's one range
     const int first = __builtin_amdgcn_readfirstlane(max(r.first + j * r.per, lo / KV4_TILE));
     const int last = __builtin_amdgcn_readfirstlane(min(r.first + min((j + 1) * r.per, r.tiles) - 1, hi / KV4_TILE));
     if (first > last) return;  // none of the range's positions are seen
     const uint8_t * head = a.c.data + (size_t(s) * a.c.n_head_kv + h) * size_t(a.c.tiles) * kv4_record(HD);
     const Kv4Const k4;
 
-    u32x4 q[QL ? 1 : NQ][QL ? 1 : NB][2];  // the queries' two parts, elements in the order of nibbles()
-    float kq[NQ];  // what brings the products back: scale * log2(e) over the row's power of two
-    int my_lo[NQ], my_hi[NQ];
-    f32x4 o[NQ][NB][2];
-    float c[NQ], l[NQ];
     Kv4Tile<HD> tile;
     int at = first + wave;
     {
@@ -382,53 +429,69 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
         tile.load_keys(rec, lane);
         tile.load_values(rec, lane);
     }
+    // the queries to LDS, 16 threads a row with 4 elements at a time (elements in the order of nibbles())
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const int row = row0 + n * 16 + col, t = row / G;
+        constexpr int NP = HD >= 64 ? HD / 64 : 1;
+        const int row = row0 + n * 16 + (tid >> 4), t = int(unsigned(row) / unsigned(G)), pc = tid & 15;
         const bool ok = t >= t_lo && t <= t_hi;
-        my_hi[n] = ok ? p0 + t : -1;
-        my_lo[n] = ok && a.window ? p0 + t - a.window + 1 : 0;
-        const float * src = a.q + (size_t(s) * a.t.n_tok + (ok ? t : t_lo)) * size_t(a.q_row) + size_t(h * G + (ok ? row % G : 0)) * size_t(a.q_head);
-        float x[NB][8], top = 0.0f;
+        const float * src = a.q + (size_t(s) * a.t.n_tok + (ok ? t : t_lo)) * size_t(a.q_row) + size_t(h * G + (ok ? row - t * G : 0)) * size_t(a.q_head);
+        f32x4 x[NP];
+        float top = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            *reinterpret_cast<f32x4 *>(&x[b][0]) = *reinterpret_cast<const f32x4 *>(src + b * 32 + 4 * g);
-            *reinterpret_cast<f32x4 *>(&x[b][4]) = *reinterpret_cast<const f32x4 *>(src + b * 32 + 16 + 4 * g);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) top = fmaxf(top, fabsf(x[b][i]));
+        for (int i = 0; i < NP; ++i) {
+            x[i] = *reinterpret_cast<const f32x4 *>(src + ((pc + 16 * i) * 4 & (HD - 1)));
+            top = fmaxf(fmaxf(fmaxf(top, fabsf(x[i][0])), fmaxf(fabsf(x[i][1]), fabsf(x[i][2]))), fabsf(x[i][3]));
         }
-        top = fmaxf(top, __shfl_xor(top, 16, WAVE));
-        top = fmaxf(top, __shfl_xor(top, 32, WAVE));
+        top = fmaxf(top, dpp_f32<DPP_XOR1>(top));
+        top = fmaxf(top, dpp_f32<DPP_XOR2>(top));
+        top = fmaxf(top, dpp_f32<DPP_HALF_MIRROR>(top));
+        top = fmaxf(top, dpp_f32<DPP_MIRROR>(top));
         // the largest element to 2^13..2^14 (rows of zeros and the ends of FP32's range: some power of two that does not overflow)
         const int e = min(max(int((__float_as_uint(top) >> 23) & 255), 40), 240);
         const float up = __uint_as_float(uint32_t(127 + 13 + 127 - e) << 23);
-        kq[n] = a.scale * 1.44269504088896341f * __uint_as_float(uint32_t(e - 13) << 23);
+        if (pc == 0) kqs[n * 16 + (tid >> 4)] = a.scale * 1.44269504088896341f * __uint_as_float(uint32_t(e - 13) << 23);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) {
-            if (QL && (b & 3) != wave && NB >= 4) continue;  // (each wave a quarter of the blocks)
-            constexpr int order[8] = {0, 2, 1, 3, 4, 6, 5, 7};
-            u32x4 qh, qlo;
+        for (int i = 0; i < NP; ++i) {
+            const int piece = (pc + 16 * i) & (HD / 4 - 1), to = (piece & 3) * 16 + (tid >> 4);  // 8 block + 4 half + g
+            u32x2 hi2, lo2;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                uint32_t hi2, lo2;
-                split2(x[b][order[2 * i]] * up, x[b][order[2 * i + 1]] * up, hi2, lo2, k4);
-                qh[i] = hi2;
-                qlo[i] = lo2;
+            for (int k = 0; k < 2; ++k) {
+                uint32_t hw, lw;
+                split2(x[i][k] * up, x[i][k + 2] * up, hw, lw, k4);
+                hi2[k] = hw;
+                lo2[k] = lw;
             }
-            if constexpr (QL) {
-                ql[(n * NB + b) * 2][lane] = qh;
-                ql[(n * NB + b) * 2 + 1][lane] = qlo;
-            } else {
-                q[n][b][0] = qh;
-                q[n][b][1] = qlo;
-            }
+            u32x4 * dst = ql[(n * NB + (piece >> 3)) * 2];
+            *reinterpret_cast<u32x2 *>(reinterpret_cast<uint8_t *>(dst + to) + (piece & 4) * 2) = hi2;
+            *reinterpret_cast<u32x2 *>(reinterpret_cast<uint8_t *>(dst + 64 + to) + (piece & 4) * 2) = lo2;
         }
+    }
+    __syncthreads();
+    u32x4 q[QL ? 1 : NQ][QL ? 1 : NB][2];
+    float kq[NQ];  // what brings the products back: scale * log2(e) over the row's power of two
+    int my_lo[NQ], my_hi[NQ];
+    f32x4 o[NQ][NB][2];
+    float c[NQ], l[NQ];
+#pragma unroll
+    for (int n = 0; n < NQ; ++n) {
+        const int t = int(unsigned(row0 + n * 16 + col) / unsigned(G));
+        const bool ok = t >= t_lo && t <= t_hi;
+        my_hi[n] = ok ? p0 + t : -1;
+        my_lo[n] = ok && a.window ? p0 + t - a.window + 1 : 0;
+        kq[n] = kqs[n * 16 + col];
         c[n] = KV4_LOW;
         l[n] = 0.0f;
 #pragma unroll
-        for (int b = 0; b < NB; ++b) o[n][b][0] = o[n][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int b = 0; b < NB; ++b) {
+            o[n][b][0] = o[n][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (!QL) {
+                q[n][b][0] = ql[(n * NB + b) * 2][lane];
+                q[n][b][1] = ql[(n * NB + b) * 2 + 1][lane];
+            }
+        }
     }
-    if constexpr (QL) __syncthreads();
+    bool sums = false;  // o holds something
     int e = 15;  // the value scales' exponent: the largest so far times 2^e is below 2^10 (scales below 2^-5 keep 2^15)
     for (; at <= last; at += 4) {
         const uint8_t * ahead = head + size_t(min(at + 4, last)) * kv4_record(HD);  // (the last one again where there is none)
@@ -452,13 +515,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
             const int e2 = 9 + 15 - top;
             const float f = __uint_as_float(uint32_t(127 + e2 - e) << 23);
             e = e2;
+            if (sums)
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
+                for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    o[n][b][0] *= f;
-                    o[n][b][1] *= f;
-                }
+                    for (int b = 0; b < NB; ++b) {
+                        o[n][b][0] *= f;
+                        o[n][b][1] *= f;
+                    }
         }
         {
             const _Float16 f = lane < 32 ? _Float16(1.0f) : _Float16(__uint_as_float(uint32_t(127 + e) << 23));
@@ -513,13 +577,15 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
                 const float c2 = fmaxf(m - 7.0f, c[n]), f = __builtin_amdgcn_exp2f(c[n] - c2);
                 c[n] = c2;
                 l[n] *= f;
+                if (sums)
 #pragma unroll
-                for (int b = 0; b < NB; ++b) {
-                    o[n][b][0] *= f;
-                    o[n][b][1] *= f;
-                }
+                    for (int b = 0; b < NB; ++b) {
+                        o[n][b][0] *= f;
+                        o[n][b][1] *= f;
+                    }
             }
         }
+        sums = true;
         u32x4 ph[NQ], pl[NQ];
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -560,7 +626,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
         tile.load_values(ahead, lane);
         wave_sync();  // the scales have been read
     }
-    // ---- the waves' sums joined, a block of 32 elements after another ----
+    // ---- the waves' sums joined ----
     const float down = __uint_as_float(uint32_t(127 - e) << 23);
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
@@ -571,35 +637,43 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
             ls[wave][n * 16 + col] = l[n];
         }
     }
+    const int rj = tid / JT, row = row0 + rj, tj = int(unsigned(row) / unsigned(G)), hq = h * G + row - tj * G;
+    const bool mine = tj >= t_lo && tj <= t_hi;
+    const size_t orow = size_t(s) * a.t.n_tok + tj;
+    float f[4] = {0.0f, 0.0f, 0.0f, 0.0f}, C = KV4_LOW, L = 0.0f;
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-        if (b) __syncthreads();
+    for (int b0 = 0; b0 < NB; b0 += JB) {
+        __syncthreads();  // (the queries, or the blocks before, have been read)
 #pragma unroll
         for (int n = 0; n < NQ; ++n)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) *reinterpret_cast<f32x4 *>(&part[wave][n * 16 + col][u * 16 + 4 * g]) = o[n][b][u] * down;
-        __syncthreads();
+            for (int b = 0; b < JB; ++b)
 #pragma unroll
-        for (int i = 0; i < (ROWS + 31) / 32; ++i) {
-            const int rj = (tid >> 3) + i * 32, ej = (tid & 7) * 4;  // this thread's row and elements of the block
-            const int row = row0 + rj, tj = row / G, hq = h * G + row % G;
-            if (rj >= ROWS || tj < t_lo || tj > t_hi) continue;
-            const float C = fmaxf(fmaxf(cs[0][rj], cs[1][rj]), fmaxf(cs[2][rj], cs[3][rj]));
-            f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-            float L = 0.0f;
+                for (int u = 0; u < 2; ++u)
+                    *reinterpret_cast<f32x4 *>(&part[wave][n * 16 + col][b * 32 + u * 16 + 4 * g]) = o[n][b0 + b][u] * down;
+        __syncthreads();
+        if (b0 == 0) {
+#pragma unroll
+            for (int w = 0; w < 4; ++w) C = fmaxf(C, cs[w][rj]);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                const float f = __builtin_amdgcn_exp2f(cs[w][rj] - C);
-                L += ls[w][rj] * f;
-                y += *reinterpret_cast<const f32x4 *>(&part[w][rj][ej]) * f;
+                f[w] = __builtin_amdgcn_exp2f(cs[w][rj] - C);
+                L += ls[w][rj] * f[w];
             }
-            const size_t orow = size_t(s) * a.t.n_tok + tj;
-            if (split == 1) {
-                kv4_out<HD>(a, orow, hq, b * 32 + ej, y, L);
+        }
+        if (!mine) continue;
+#pragma unroll 1
+        for (int ej = tid % JT * 4; ej < 32 * JB; ej += 4 * JT) {
+            f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < 4; ++w) y += *reinterpret_cast<const f32x4 *>(&part[w][rj][ej]) * f[w];
+            const int el = b0 * 32 + ej;
+            if (alone) {
+                kv4_out<HD>(a, orow, hq, el, y, L);
             } else {  // this range's set: [range][token][head][HD + 4], C and L behind the sums
                 float * w = a.work + ((size_t(range) * a.t.n_tok + tj) * a.n_head + hq) * (HD + 4);
-                *reinterpret_cast<f32x4 *>(w + b * 32 + ej) = y;
-                if (b == 0 && ej == 0) {
+                *reinterpret_cast<f32x4 *>(w + el) = y;
+                if (el == 0) {
                     w[HD] = C;
                     w[HD + 1] = L;
                 }
@@ -672,7 +746,8 @@ hipError_t by_dim(int hd, F f) {
 hipError_t launch_kv4_store(const Kv4RowsArgs & a, hipStream_t s) {
     const unsigned span = unsigned((a.t.n_tok + KV4_TILE - 2) / KV4_TILE + 1);  // records that n_tok positions can touch
     return by_dim(a.c.head_dim, [&](auto hd) {
-        GQ_LAUNCH(kv4_store_kernel<hd.value>, dim3(span, a.c.n_head_kv, a.t.n_seq), dim3(256), 0, s, a);
+        constexpr unsigned parts = 2 * (hd.value < 128 ? 1 : hd.value / 128);
+        GQ_LAUNCH(kv4_store_kernel<hd.value>, dim3(span * parts, a.c.n_head_kv, a.t.n_seq), dim3(KV4_STORE), 0, s, a);
     });
 }
 
@@ -685,7 +760,7 @@ hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s) {
 // Groups of 16 rows that a workgroup takes: as many as there are, up to what the registers hold.
 static int kv4_nq(int hd, int n_tok, int per_kv) {
     const long long rows = n_tok * (long long)per_kv;
-    return rows <= 16 ? 1 : rows <= 32 || hd == 256 ? 2 : 4;
+    return rows <= 16 || hd == 256 ? 1 : rows <= 32 || hd == 128 ? 2 : 4;
 }
 
 // How many ranges a call's records are dealt to: about KV4_GROUPS workgroups in all, but at least one range a sequence and no more
@@ -706,11 +781,14 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
     Kv4AttnArgs a = args;
     const int per_kv = a.n_head / a.c.n_head_kv, nq = kv4_nq(a.c.head_dim, a.t.n_tok, per_kv);
     a.ranges = kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head);
-    const dim3 grid(unsigned((a.t.n_tok * (long long)per_kv + 16 * nq - 1) / (16 * nq) * a.c.n_head_kv), unsigned(a.ranges));
+    a.group = per_kv;
+    const dim3 grid(unsigned((a.t.n_tok * (long long)per_kv + 16 * nq - 1) / (16 * nq)), unsigned(a.c.n_head_kv), unsigned(a.ranges));
     return by_dim(a.c.head_dim, [&](auto hd) {
         if (nq == 1) GQ_LAUNCH((kv4_attn_kernel<hd.value, 1>), grid, dim3(256), 0, s, a);
-        else if (nq == 2) GQ_LAUNCH((kv4_attn_kernel<hd.value, 2>), grid, dim3(256), 0, s, a);
-        else if constexpr (hd.value < 256) GQ_LAUNCH((kv4_attn_kernel<hd.value, 4>), grid, dim3(256), 0, s, a);
+        if constexpr (hd.value < 256)
+            if (nq == 2) GQ_LAUNCH((kv4_attn_kernel<hd.value, 2>), grid, dim3(256), 0, s, a);
+        if constexpr (hd.value < 128)
+            if (nq == 4) GQ_LAUNCH((kv4_attn_kernel<hd.value, 4>), grid, dim3(256), 0, s, a);
         if (a.ranges > a.t.n_seq)
             GQ_LAUNCH(kv4_join_kernel<hd.value>, dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
     });

@@ -73,7 +73,10 @@ struct Kv4AttnArgs {
     int group;           // set at launch: n_head / n_head_kv
 };
 
-constexpr int KV4_GROUPS = 1024;  // workgroups that a call's records are dealt to, where they are enough
+// Workgroups that a call's records are dealt to, where they are enough. Heads of 256: as many as are resident (two a CU), each with few
+// records; the others: two rounds of what is resident, which evens out (us at 512 / 1024 / 1536 / 2048, stores included: one sequence of
+// 32768, 16/4 heads of 256, 21.5 / 26.2 / 26.4 / 26.2; 32 sequences of up to 8192, 32/8 heads of 128, 78 / 58 / 55 / 56).
+constexpr int KV4_GROUPS = 1536, KV4_GROUPS_256 = 512;
 constexpr int KV4_LEAST = 4;      // records of a range at least: one a wave
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head);
 

@@ -297,9 +297,8 @@ struct Kv4Range {
     long long p0;
 };
 
-// Records that the tokens of a sequence see: from the first token's first position to the last one's own.
-__device__ __forceinline__ void kv4_seen(const Kv4AttnArgs & a, int s, Kv4Range & r) {
-    kv4_span(a.t, s, r.p0, r.n);
+// Records that the tokens of a sequence see (r.p0 and r.n are set): from the first token's first position to the last one's own.
+__device__ __forceinline__ void kv4_seen(const Kv4AttnArgs & a, Kv4Range & r) {
     const long long lo = r.p0 < 0 ? 0 : r.p0, hi = r.p0 + r.n < a.c.n_ctx ? r.p0 + r.n : a.c.n_ctx;  // positions of live tokens
     if (lo >= hi) {
         r.first = r.tiles = 0;
@@ -319,13 +318,29 @@ __device__ __forceinline__ int kv4_per(long long records, int ranges, int n_seq,
     return per > KV4_LEAST ? per : KV4_LEAST;
 }
 
-// All sequences' records (a wave's lanes scan them together): the ranges' length.
-__device__ __forceinline__ int kv4_length(const Kv4AttnArgs & a) {
+// The sequence that range number `range` belongs to (BY_RANGE), or sequence s itself, with its ranges; false: no such range. A wave's
+// lanes look at the sequences together, 64 at a time: first at all records, for the ranges' length, then at each sequence's ranges.
+template <bool BY_RANGE>
+__device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int & s, Kv4Range & r) {
+    if (a.t.n_seq == 1) {
+        s = 0;
+        kv4_span(a.t, 0, r.p0, r.n);
+        kv4_seen(a, r);
+        r.per = kv4_per(r.tiles, a.ranges, 1, r.tiles);
+        r.slot = 0;
+        return (long long)(BY_RANGE ? range : 0) * r.per < r.tiles;
+    }
+    const int lane = threadIdx.x & 63;
+    Kv4Range x;  // the lane's sequence
+    const auto look = [&](int i) {
+        x.p0 = x.n = 0;
+        if (i < a.t.n_seq) kv4_span(a.t, i, x.p0, x.n);
+        kv4_seen(a, x);
+    };
     long long sum = 0;
     int most = 0;
-    Kv4Range x;
-    for (int i = threadIdx.x & 63; i < a.t.n_seq; i += 64) {
-        kv4_seen(a, i, x);
+    for (int i0 = 0; i0 < a.t.n_seq; i0 += 64) {
+        look(i0 + lane);
         sum += x.tiles;
         most = max(most, x.tiles);
     }
@@ -334,26 +349,11 @@ __device__ __forceinline__ int kv4_length(const Kv4AttnArgs & a) {
         sum += __shfl_xor(sum, d, WAVE);
         most = max(most, __shfl_xor(most, d, WAVE));
     }
-    return kv4_per(sum, a.ranges, a.t.n_seq, most);
-}
-
-// The sequence that range number `range` belongs to (BY_RANGE), or sequence s itself, with its ranges; false: no such range.
-template <bool BY_RANGE>
-__device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int & s, Kv4Range & r) {
-    if (a.t.n_seq == 1) {
-        s = 0;
-        kv4_seen(a, 0, r);
-        r.per = kv4_per(r.tiles, a.ranges, 1, r.tiles);
-        r.slot = 0;
-        return (long long)(BY_RANGE ? range : 0) * r.per < r.tiles;
-    }
-    const int lane = threadIdx.x & 63, per = kv4_length(a);
+    const int per = kv4_per(sum, a.ranges, a.t.n_seq, most);
     int before = 0;
     for (int i0 = 0; i0 < a.t.n_seq; i0 += 64) {
-        Kv4Range x;
-        x.tiles = 0;
-        if (i0 + lane < a.t.n_seq) kv4_seen(a, i0 + lane, x);
-        const int mine = (x.tiles + per - 1) / per;
+        if (a.t.n_seq > 64) look(i0 + lane);  // (up to 64 sequences: as they are)
+        const int mine = int(unsigned(x.tiles + per - 1) / unsigned(per));
         int upto = before + mine;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -365,7 +365,10 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int &
             const int l = BY_RANGE ? __ffsll(__ballot(upto > range)) - 1 : s - i0;
             s = i0 + l;
             r.slot = __shfl(upto - mine, l, WAVE);
-            kv4_seen(a, s, r);
+            r.first = __shfl(x.first, l, WAVE);
+            r.tiles = __shfl(x.tiles, l, WAVE);
+            r.p0 = __shfl(int(x.p0), l, WAVE);
+            r.n = __shfl(x.n, l, WAVE);
             r.per = per;
             return r.tiles > 0;
         }
@@ -682,14 +685,14 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     }
 }
 
-// Workgroup (q head, token, sequence): the sets of a sequence with several ranges. The factors of all sets first, then HD / 4 threads
-// a set, 1024 / HD sets at a time.
-template <int HD>
+// Workgroup (q head and EL of its elements, token, sequence): the sets of a sequence with several ranges. The factors of all sets first,
+// then EL / 4 threads a set, 1024 / EL sets at a time.
+template <int HD, int EL>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
-    constexpr int PER = HD / 4, SETS = 256 / PER;
+    constexpr int PER = EL / 4, SETS = 256 / PER;
     __shared__ float f[KV4_GROUPS], red[2][4];
-    __shared__ __align__(16) float part[SETS][HD];
-    const int hq = blockIdx.x, t = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    __shared__ __align__(16) float part[SETS][EL];
+    const int hq = blockIdx.x / (HD / EL), e0 = blockIdx.x % (HD / EL) * EL, t = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int s = blockIdx.z;
     Kv4Range r;
     if (!kv4_find<false>(a, 0, s, r)) return;
@@ -720,13 +723,13 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
     const int e = tid % PER * 4;
 #pragma unroll 8
-    for (int j = tid / PER; j < n; j += SETS) y += *reinterpret_cast<const f32x4 *>(w + j * step + e) * f[j];
+    for (int j = tid / PER; j < n; j += SETS) y += *reinterpret_cast<const f32x4 *>(w + j * step + e0 + e) * f[j];
     *reinterpret_cast<f32x4 *>(&part[tid / PER][e]) = y;
     __syncthreads();
     if (tid >= PER) return;
 #pragma unroll
     for (int i = 1; i < SETS; ++i) y += *reinterpret_cast<const f32x4 *>(&part[i][e]);
-    kv4_out<HD>(a, size_t(s) * a.t.n_tok + t, hq, e, y, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
+    kv4_out<HD>(a, size_t(s) * a.t.n_tok + t, hq, e0 + e, y, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
 }
 
 template <typename F>
@@ -763,13 +766,13 @@ static int kv4_nq(int hd, int n_tok, int per_kv) {
     return rows <= 16 || hd == 256 ? 1 : rows <= 32 || hd == 128 ? 2 : 4;
 }
 
-// How many ranges a call's records are dealt to: about KV4_GROUPS workgroups in all, but at least one range a sequence and no more
-// than KV4_LEAST records each give.
+// How many ranges a call's records are dealt to: as many as give KV4_GROUPS workgroups in all (KV4_GROUPS_256 for heads of 256), but at
+// least one range a sequence, and no more than KV4_LEAST records each give.
 int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     const int per_kv = n_head / c.n_head_kv, rows = 16 * kv4_nq(c.head_dim, n_tok, per_kv);
     const long long units = (n_tok * (long long)per_kv + rows - 1) / rows * c.n_head_kv;
     const long long most = (long long)n_seq * ((c.tiles + KV4_LEAST - 1) / KV4_LEAST);
-    return int(std::min<long long>(std::max<long long>(n_seq, std::min(KV4_GROUPS / units, most)), 65535));
+    return int(std::min<long long>(std::max<long long>(n_seq, std::min((c.head_dim == 256 ? KV4_GROUPS_256 : KV4_GROUPS) / units, most)), 65535));
 }
 
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
@@ -789,8 +792,13 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
             if (nq == 2) GQ_LAUNCH((kv4_attn_kernel<hd.value, 2>), grid, dim3(256), 0, s, a);
         if constexpr (hd.value < 128)
             if (nq == 4) GQ_LAUNCH((kv4_attn_kernel<hd.value, 4>), grid, dim3(256), 0, s, a);
-        if (a.ranges > a.t.n_seq)
-            GQ_LAUNCH(kv4_join_kernel<hd.value>, dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
+        if (a.ranges <= a.t.n_seq) return;
+        // one sequence's sets may be many: then more, narrower workgroups
+        constexpr int narrow = hd.value < 64 ? 32 : 64;
+        if (a.t.n_seq * (long long)a.t.n_tok * a.n_head <= 256)
+            GQ_LAUNCH((kv4_join_kernel<hd.value, narrow>), dim3(a.n_head * (hd.value / narrow), a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
+        else
+            GQ_LAUNCH((kv4_join_kernel<hd.value, hd.value>), dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
     });
 }
 

@@ -3,8 +3,10 @@
 // buffers, are staged here in `scratch`, a fixed device array of this file (one copy per device, held until the
 // process ends). Nothing here allocates: the array's address on a device is looked up once, on the first call on
 // that device, and kept.
-// The 4-bit KV cache on caller-owned memory (gemvq_kv4_*_static): its arguments' checks and launches.
+// The 4-bit KV cache (gemvq_kv4_*_static) and the beam search's step (gemvq_beam_*_static) on caller-owned memory: their arguments'
+// checks and launches.
 #include "gemvq_hip.h"
+#include "gq_beam.h"
 #include "gq_kernels.h"
 #include "gq_kv4.h"
 
@@ -178,6 +180,98 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
     a.work = static_cast<float *>(work);
     const hipError_t e = launch_kv4_attn(a, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : -int(e);
+}
+
+}  // extern "C"
+
+static_assert(GEMVQ_BEAM_MAX == BEAM_MAX && GEMVQ_BEAM_MAX_VOCAB == BEAM_MAX_VOCAB, "limits in the header");
+
+namespace {
+bool beam_rows_ok(int n_group, int n_beam) {
+    return n_beam >= 1 && n_beam <= BEAM_MAX && n_group >= 1 && int64_t(n_group) * n_beam <= GRID_MAX;
+}
+}  // namespace
+
+extern "C" {
+
+uint64_t gemvq_beam_work(int n_group, int n_beam, int n_vocab) {
+    if (!beam_rows_ok(n_group, n_beam) || n_vocab < 1 || n_vocab > BEAM_MAX_VOCAB) return 0;
+    return beam_work(n_group, n_beam, n_vocab);
+}
+
+int gemvq_beam_select_static(const float * logits, int64_t row_stride, int n_vocab, int n_group, int n_beam, const float * score,
+                             const int32_t * last, int eos, float * score_out, int32_t * token, int32_t * parent, void * work,
+                             uint64_t work_bytes, void * stream) {
+    const uint64_t need = gemvq_beam_work(n_group, n_beam, n_vocab);
+    if (!need || !logits || row_stride < n_vocab || row_stride > (int64_t(1) << 40) || !score || !score_out || !token || !parent ||
+        !work || work_bytes < need)
+        return GEMVQ_EINVAL;
+    if (!aligned(logits, 4) || !aligned(score, 4) || !aligned(last, 4) || !aligned(score_out, 4) || !aligned(token, 4) ||
+        !aligned(parent, 4) || !aligned(work, 16))
+        return GEMVQ_EINVAL;
+    BeamSelectArgs a{};
+    a.x = logits;
+    a.stride = row_stride;
+    a.n_vocab = n_vocab;
+    a.n_group = n_group;
+    a.n_beam = n_beam;
+    a.eos = eos;
+    a.score = score;
+    a.last = last;
+    a.score_out = score_out;
+    a.token = token;
+    a.parent = parent;
+    a.work = work;
+    const hipError_t e = launch_beam_select(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : -int(e);
+}
+
+int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, const int32_t * parent, int n_group, int n_beam,
+                              void * stream) {
+    if (!arrays || n_arrays < 1 || !parent || !aligned(parent, 4) || !beam_rows_ok(n_group, n_beam)) return GEMVQ_EINVAL;
+    const uint64_t rows = uint64_t(n_group) * uint64_t(n_beam), most = uint64_t(1) << 46;  // (sums below stay below 2^63)
+    for (int i = 0; i < n_arrays; ++i) {
+        const gemvq_beam_array & x = arrays[i];
+        const uint64_t size = uint64_t(x.count) * x.unit_bytes;
+        if (!x.data || !aligned(x.data, 4) || x.n_part < 1 || x.n_part > uint32_t(GRID_MAX) || x.first > x.count || x.unit_bytes < 4 ||
+            x.unit_bytes % 4 || x.row_stride % 4 || x.part_stride % 4 || x.row_stride > most || x.part_stride > most || size > most)
+            return GEMVQ_EINVAL;
+        if (x.used && (!aligned(x.used, 4) || x.unit_len < 1 || x.used_stride < 1)) return GEMVQ_EINVAL;
+        // rows apart, and parts apart: all rows of a part before the next part, or all parts of a row before the next row
+        if (rows > 1 && x.row_stride < size) return GEMVQ_EINVAL;
+        if (x.n_part > 1 && x.part_stride < (rows - 1) * x.row_stride + size &&
+            (x.part_stride < size || (rows > 1 && x.row_stride < (x.n_part - 1) * x.part_stride + size)))
+            return GEMVQ_EINVAL;
+        if (((size - uint64_t(x.first) * x.unit_bytes) / BEAM_TILE + 1) * x.n_part > 0x7fffffffu / BEAM_MOVES) return GEMVQ_EINVAL;
+    }
+    for (int i = 0; i < n_arrays;) {
+        BeamReorderArgs a{};
+        a.parent = parent;
+        a.n_group = n_group;
+        a.n_beam = n_beam;
+        uint32_t end = 0;
+        for (; i < n_arrays && a.n < BEAM_MOVES; ++i) {
+            const gemvq_beam_array & x = arrays[i];
+            if (x.first == x.count) continue;
+            BeamMove & m = a.m[a.n++];
+            m.data = static_cast<uint8_t *>(x.data);
+            m.row_stride = x.row_stride;
+            m.part_stride = x.part_stride;
+            m.lo = uint64_t(x.first) * x.unit_bytes;
+            m.hi = uint64_t(x.count) * x.unit_bytes;
+            m.used = x.used;
+            m.unit_bytes = x.unit_bytes;
+            m.unit_len = x.unit_len;
+            m.used_stride = x.used_stride;
+            m.wide = aligned(x.data, 16) && x.unit_bytes % 16 == 0 && x.row_stride % 16 == 0 && (x.n_part == 1 || x.part_stride % 16 == 0);
+            m.tiles = uint32_t((m.hi - m.lo + BEAM_TILE - 1) / BEAM_TILE);
+            m.end = end += m.tiles * x.n_part;
+        }
+        if (!a.n) break;
+        const hipError_t e = launch_beam_reorder(a, static_cast<hipStream_t>(stream));
+        if (e != hipSuccess) return -int(e);
+    }
+    return 0;
 }
 
 }  // extern "C"

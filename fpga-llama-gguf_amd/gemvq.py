@@ -142,6 +142,13 @@ class Kv4(C.Structure):  # gemvq_kv4
     _fields_ = [("data", C.c_void_p)] + [(n, C.c_int32) for n in ("n_seq", "n_ctx", "n_head_kv", "head_dim")]
 
 
+class BeamArray(C.Structure):  # gemvq_beam_array
+    """An array whose rows follow the beams: its address, strides and units in bytes (gemvq_hip.h)."""
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_uint64), ("part_stride", C.c_uint64), ("n_part", C.c_uint32),
+                ("first", C.c_uint32), ("count", C.c_uint32), ("unit_bytes", C.c_uint32), ("unit_len", C.c_uint32),
+                ("used", C.c_void_p), ("used_stride", C.c_int32)]
+
+
 class LaunchStat(C.Structure):  # gemvq_launch_stat
     _fields_ = [("name", C.c_char * 40), ("first_cmd", C.c_int32), ("n_cmds", C.c_int32), ("bytes", C.c_uint64),
                 ("us", C.c_double)]
@@ -200,6 +207,9 @@ def hip_lib() -> C.CDLL:
             _c_fn(lib, name, i, kvp, vp, vp, i64, i, vp, vp, vp)
         _c_fn(lib, "gemvq_kv4_attn_work", u64, kvp, i, i)
         _c_fn(lib, "gemvq_kv4_attn_static", i, kvp, vp, i64, i64, vp, i64, i, i, vp, vp, i, C.c_float, vp, u64, vp)
+        _c_fn(lib, "gemvq_beam_work", u64, i, i, i)
+        _c_fn(lib, "gemvq_beam_select_static", i, vp, i64, i, i, i, vp, vp, i, vp, vp, vp, vp, u64, vp)
+        _c_fn(lib, "gemvq_beam_reorder_static", i, C.POINTER(BeamArray), i, vp, i, i, vp)
         _hip = lib
     return _hip
 
@@ -314,6 +324,23 @@ def kv4_attn_static(kv: Kv4, q: int, q_stride: int, q_head_stride: int, y: int, 
     """Attention of the tokens at positions pos[s] + t over the cache (their own keys and values stored before)."""
     _ok(hip_lib().gemvq_kv4_attn_static(kv, q, q_stride, q_head_stride, y, y_stride, n_tok, n_head, pos, num, window, scale,
                                         work, work_bytes, stream), "kv4 attention")
+
+
+def beam_work(n_group: int, n_beam: int, n_vocab: int) -> int:
+    """Bytes of workspace of beam_select_static (0: sizes that are not served)."""
+    return hip_lib().gemvq_beam_work(n_group, n_beam, n_vocab)
+
+
+def beam_select_static(logits: int, row_stride: int, n_vocab: int, n_group: int, n_beam: int, score: int, last: int, eos: int,
+                       score_out: int, token: int, parent: int, work: int, work_bytes: int, stream: int = 0) -> None:
+    """The n_beam best continuations of each group's beams: score, token and parent beam, in descending order."""
+    _ok(hip_lib().gemvq_beam_select_static(logits, row_stride, n_vocab, n_group, n_beam, score, last, eos, score_out, token,
+                                           parent, work, work_bytes, stream), "beam selection")
+
+
+def beam_reorder_static(arrays, parent: int, n_group: int, n_beam: int, stream: int = 0) -> None:
+    """In each of the arrays (a ctypes array of BeamArray), row i of every group becomes a copy of its row parent[i]."""
+    _ok(hip_lib().gemvq_beam_reorder_static(arrays, len(arrays), parent, n_group, n_beam, stream), "beam reordering")
 
 
 class Context:

@@ -323,6 +323,36 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
                           int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,
                           float scale, void * work, uint64_t work_bytes, void * stream);
 
+/* No counterpart in the reference: one step of a beam search over n_group independent groups of n_beam (1 .. GEMVQ_BEAM_MAX)
+ * beams, rows g * n_beam + b, at most 65535 rows; on caller-owned device memory, under the rules of the calls above.
+ * Selection: candidate v of beam b has the value score[b] + logit[b][v] - log(sum of e^logit[b]), formed in 64 bits; the n_beam best
+ * candidates of a group, in descending order: score_out (rounded to FP32), token, and parent (the beam in the group it
+ * continues); of equal ones the lower b * n_vocab + v first (among one beam's logits, the larger logit first). A beam whose last token (last[row], or
+ * last NULL) is eos has ended: it has the one candidate eos, at its score, and its logits are not read; eos outside the vocabulary: none ends.
+ * A beam with score -inf (the beams after the first, at a search's start) has no candidates before all others'. NaN logits and scores count as -inf, +inf logits
+ * as the largest finite number. logits: FP32 rows row_stride >= n_vocab floats apart, 1 <= n_vocab <= GEMVQ_BEAM_MAX_VOCAB, 4-byte
+ * aligned. score_out may be score, token may be last. work: gemvq_beam_work() bytes, 16-byte aligned, contents do not matter. */
+#define GEMVQ_BEAM_MAX 32
+#define GEMVQ_BEAM_MAX_VOCAB (1 << 20)
+uint64_t gemvq_beam_work(int n_group, int n_beam, int n_vocab);
+int gemvq_beam_select_static(const float * logits, int64_t row_stride, int n_vocab, int n_group, int n_beam, const float * score,
+                             const int32_t * last, int eos, float * score_out, int32_t * token, int32_t * parent, void * work,
+                             uint64_t work_bytes, void * stream);
+/* Reordering: what the beams keep follows the selection, in place: in each of the arrays, row i of every group becomes what row parent[i] of
+ * the group was (a value outside 0 .. n_beam - 1: the row stays). An array's row r has n_part parts, at data + r * row_stride + p *
+ * part_stride, of `count` units of unit_bytes each; units first .. count - 1 move (a prefix that all beams share need not). With
+ * used (int32 in device memory, for row r at used[r * used_stride]), only the source row's units below ceil(used / unit_len) move, and
+ * what the target has behind them stays. Addresses and sizes are multiples of 4 bytes (of 16 for full speed); rows and parts, arrays, used and parent lie apart from one another. */
+typedef struct {
+    void * data;
+    uint64_t row_stride, part_stride;
+    uint32_t n_part, first, count, unit_bytes, unit_len;
+    const int32_t * used;
+    int32_t used_stride;
+} gemvq_beam_array;
+int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, const int32_t * parent, int n_group, int n_beam,
+                              void * stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,11 +14,18 @@ struct BeamSelectArgs {
     const float * x;  // row r at x + r * stride
     long long stride;
     int n_vocab, n_group, n_beam, eos;
-    const float * score;   // [rows]
-    const int32_t * last;  // [rows] or NULL: no beam has ended
-    float * score_out;     // [rows], may be score
-    int32_t * token;       // [rows], may be last
-    int32_t * parent;      // [rows], beams of the group
+    const float * score;   // row r's at score[r * slot], and so the others
+    const int32_t * last;  // or NULL: no beam has ended
+    float * score_out;     // may be score
+    int32_t * token;       // may be last
+    int32_t * parent;      // beams of the group
+    int slot;
+    // With pos: row r is at position pos[r * slot] of its prompt (n_prompt[r * slot] ids, at most cap, at prompt + r * cap). While the prompt has
+    // a next id, that is its token, parent and score stay; a beam has ended only behind its prompt.
+    const int32_t * pos;
+    const int32_t * n_prompt;
+    const int32_t * prompt;
+    int cap;
     void * work;
     int per;               // set at launch: logits a thread takes in the first kernel
     int chunks;            // set at launch: workgroups a row there
@@ -29,12 +36,12 @@ hipError_t launch_beam_select(const BeamSelectArgs & a, hipStream_t s);
 // What each beam keeps, moved along with it: row i of a group becomes a copy of row parent[i], in place. Of every part p of a row (at
 // data + row * row_stride + p * part_stride) the bytes lo .. hi - 1 move; with used, hi is also at most the source row's
 // ceil(used / unit_len) units.
-struct BeamMove {
+struct BeamMove {  // hi: used[...] + used_more units of the source row
     uint8_t * data;
     unsigned long long row_stride, part_stride, lo, hi;
     const int32_t * used;
     uint32_t unit_bytes, unit_len;
-    int used_stride;
+    int used_stride, used_more;
     uint32_t tiles;  // workgroups of a part
     uint32_t end;    // workgroups of this array and those before it
     uint32_t wide;   // every address is a multiple of 16
@@ -43,9 +50,32 @@ constexpr int BEAM_MOVES = 24;      // arrays of one launch
 constexpr uint32_t BEAM_TILE = 4096;  // bytes of a part that a workgroup moves
 struct BeamReorderArgs {
     BeamMove m[BEAM_MOVES];
-    const int32_t * parent;  // [n_group * n_beam], values outside 0 .. n_beam - 1: the row stays
-    int n, n_group, n_beam;
+    const int32_t * parent;  // row r's at parent[r * parent_stride], values outside 0 .. n_beam - 1: the row stays
+    int n, n_group, n_beam, parent_stride;
 };
+// Rows apart, and parts apart: all rows of a part before the next part, or all parts of a row before the next row (the sizes in any unit,
+// below 2^46).
+inline bool beam_rows_apart(uint64_t rows, uint64_t size, uint64_t row_stride, uint64_t part_stride, uint64_t n_part) {
+    if (rows > 1 && row_stride < size) return false;
+    if (n_part <= 1) return true;
+    return part_stride >= (rows - 1) * row_stride + size ||
+           (part_stride >= size && (rows == 1 || row_stride >= (n_part - 1) * part_stride + size));
+}
+// The workgroups of an array whose addresses are set, behind those of `end`, and whether it moves in pieces of 16 bytes.
+inline void beam_move_shape(BeamMove & m, uint32_t n_part, uint32_t & end) {
+    m.wide = (reinterpret_cast<uintptr_t>(m.data) | m.row_stride | (n_part > 1 ? m.part_stride : 0) | m.lo | m.unit_bytes) % 16 == 0;
+    m.tiles = uint32_t((m.hi - m.lo + BEAM_TILE - 1) / BEAM_TILE);
+    m.end = end += m.tiles * n_part;
+}
+
+// The beams' new tokens into their id lists, and on to the next position: out[s * cap + pos + 1] = tok, pos += 1, for slots 16 apart.
+struct BeamNextArgs {
+    const int32_t * tok;
+    int32_t * pos;
+    int32_t * out;
+    int cap, n_seq;
+};
+hipError_t launch_beam_next(const BeamNextArgs & a, hipStream_t s);
 hipError_t launch_beam_reorder(const BeamReorderArgs & a, hipStream_t s);
 
 }  // namespace gq

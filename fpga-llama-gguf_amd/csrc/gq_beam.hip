@@ -51,8 +51,15 @@ __device__ __forceinline__ unsigned long long * beam_lists(const BeamSelectArgs 
 
 // A row that takes no logits: a beam that has ended (its one candidate), or one without a score (none).
 __device__ __forceinline__ bool beam_closed(const BeamSelectArgs & a, int row, bool & ended) {
-    ended = a.last && a.last[row] == a.eos && a.eos >= 0 && a.eos < a.n_vocab;
-    return ended || !(a.score[row] > -__builtin_inff());
+    const size_t at = size_t(row) * a.slot;
+    ended = a.last && a.last[at] == a.eos && a.eos >= 0 && a.eos < a.n_vocab && !(a.pos && a.pos[at] < a.n_prompt[at]);
+    return ended || !(a.score[at] > -__builtin_inff());
+}
+// Whether the row's prompt has a next id; its place in the prompt.
+__device__ __forceinline__ bool beam_prompted(const BeamSelectArgs & a, int row, int & next) {
+    if (!a.pos) return false;
+    next = a.pos[size_t(row) * a.slot] + 1;
+    return next >= 0 && next < min(a.n_prompt[size_t(row) * a.slot], a.cap);
 }
 
 template <int PER>
@@ -67,6 +74,8 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     const size_t at = size_t(row) * a.chunks + chunk;
     unsigned long long * out = beam_lists(a) + at * k;
     bool ended;
+    int next;
+    if (beam_prompted(a, row - row % k, next)) return;  // the group reads its prompt (its first beam says so, here and below)
     if (beam_closed(a, row, ended)) {
         // the first chunk lists the tokens in order at -inf, an ended beam's eos before them at 0 (of sum 1)
         for (int i = tid; i < k; i += 256) {
@@ -211,6 +220,14 @@ __global__ __launch_bounds__(T) void beam_pick_kernel(BeamSelectArgs a) {
     __shared__ uint32_t besti[2][W];
     const int g = blockIdx.x, k = a.n_beam, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lists = k * a.chunks;
     const size_t first = size_t(g) * k * a.chunks;
+    int ahead;
+    if (beam_prompted(a, g * k, ahead)) {  // the group's beams read their prompt
+        if (tid < k && beam_prompted(a, g * k + tid, ahead)) {
+            a.token[(g * k + tid) * a.slot] = a.prompt[size_t(g * k + tid) * a.cap + ahead];
+            a.parent[(g * k + tid) * a.slot] = tid;
+        }
+        return;
+    }
     const BeamStat * st = beam_stats(a) + first;
     const unsigned long long * li = beam_lists(a) + first * k;
     // the lists' first two entries, while the rows' sums are joined
@@ -234,7 +251,7 @@ __global__ __launch_bounds__(T) void beam_pick_kernel(BeamSelectArgs a) {
 #pragma unroll
         for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, WAVE);
         if (lane == 0) {
-            const float sc = a.score[g * k + b];
+            const float sc = a.score[(g * k + b) * a.slot];
             top[b] = m;
             logsum[b] = log(s);
             scores[b] = sc == sc ? double(sc) : -__builtin_inf();
@@ -287,9 +304,10 @@ __global__ __launch_bounds__(T) void beam_pick_kernel(BeamSelectArgs a) {
             }
         if (tid == 0) {
             const uint32_t b = bi / uint32_t(a.n_vocab);
-            a.score_out[g * k + j] = float(bv);
-            a.token[g * k + j] = int32_t(bi - b * uint32_t(a.n_vocab));
-            a.parent[g * k + j] = int32_t(b);
+            const int to = (g * k + j) * a.slot;
+            a.score_out[to] = float(bv);
+            a.token[to] = int32_t(bi - b * uint32_t(a.n_vocab));
+            a.parent[to] = int32_t(b);
         }
 #pragma unroll
         for (int i = 0; i < OWN; ++i)
@@ -308,7 +326,8 @@ __global__ __launch_bounds__(T) void beam_pick_kernel(BeamSelectArgs a) {
 // every row that changes, then the writes: in place, each moved byte read from HBM and written once (a source with several heirs is read again from
 // the caches). Rows that stay cost nothing.
 template <int NB, typename V>
-__device__ __forceinline__ void beam_move(const BeamMove & m, const int32_t * parent, uint8_t * part, unsigned long long from, int n_beam, int row0) {
+__device__ __forceinline__ void beam_move(const BeamMove & m, const int32_t * parent, int slot, uint8_t * part, unsigned long long from, int n_beam,
+                                          int row0) {
     constexpr int STEP = 256 * sizeof(V), N = BEAM_TILE / STEP;
     for (int it = 0; it < N; ++it) {
         const unsigned long long off = from + it * STEP + threadIdx.x * sizeof(V);
@@ -318,11 +337,11 @@ __device__ __forceinline__ void beam_move(const BeamMove & m, const int32_t * pa
         for (int i = 0; i < NB; ++i) {
             moved[i] = false;
             if (i >= n_beam) continue;
-            const int p = parent[row0 + i];
+            const int p = parent[size_t(row0 + i) * slot];
             if (p == i || p < 0 || p >= n_beam) continue;
             unsigned long long hi = m.hi;
             if (m.used) {
-                const int u = m.used[size_t(row0 + p) * m.used_stride];
+                const long long u = (long long)m.used[size_t(row0 + p) * m.used_stride] + m.used_more;
                 const unsigned long long units = u > 0 ? ((unsigned long long)u + m.unit_len - 1) / m.unit_len : 0;
                 hi = min(hi, units * m.unit_bytes);
             }
@@ -345,8 +364,16 @@ __global__ __launch_bounds__(256) void beam_reorder_kernel(BeamReorderArgs a) {
     uint8_t * part = m.data + row0 * m.row_stride + p * m.part_stride;
     const unsigned long long from = m.lo + (unsigned long long)(t - p * m.tiles) * BEAM_TILE;
     typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
-    if (m.wide) beam_move<NB, u32x4>(m, a.parent, part, from, a.n_beam, row0);
-    else beam_move<NB, uint32_t>(m, a.parent, part, from, a.n_beam, row0);
+    if (m.wide) beam_move<NB, u32x4>(m, a.parent, a.parent_stride, part, from, a.n_beam, row0);
+    else beam_move<NB, uint32_t>(m, a.parent, a.parent_stride, part, from, a.n_beam, row0);
+}
+
+__global__ void beam_next_kernel(BeamNextArgs a) {
+    const int s = threadIdx.x;
+    if (s >= a.n_seq) return;
+    const int p = a.pos[16 * s] + 1;
+    if (p >= 0 && p < a.cap) a.out[size_t(s) * a.cap + p] = a.tok[16 * s];
+    a.pos[16 * s] = p;
 }
 
 // Logits a thread of the first kernel takes: 32, or 8 where that gives too few workgroups to read at the memory's rate.
@@ -375,6 +402,11 @@ hipError_t launch_beam_select(const BeamSelectArgs & args, hipStream_t s) {
     if (e != hipSuccess) return e;
     if (a.n_beam * a.chunks <= 1024) GQ_LAUNCH(beam_pick_kernel<256>, dim3(unsigned(a.n_group)), dim3(256), 0, s, a);
     else GQ_LAUNCH(beam_pick_kernel<1024>, dim3(unsigned(a.n_group)), dim3(1024), 0, s, a);
+    return hipGetLastError();
+}
+
+hipError_t launch_beam_next(const BeamNextArgs & a, hipStream_t s) {
+    GQ_LAUNCH(beam_next_kernel, dim3(1), dim3(64), 0, s, a);
     return hipGetLastError();
 }
 

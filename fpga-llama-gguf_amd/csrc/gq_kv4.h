@@ -29,13 +29,13 @@ template <int HD>
 struct Kv4Layout {
     static constexpr int NB = HD / 32, KB = NB < 4 ? NB : 4, VB = NB < 2 ? NB : 2;
     static constexpr int VQ = 16 * HD, KD = 32 * HD, VD = 34 * HD, RECORD = 36 * HD;
-    __device__ static int kq(int p, int blk, int e) {
+    __host__ __device__ static int kq(int p, int blk, int e) {
         return (p >> 4) * 8 * HD + (blk / KB) * 256 * KB + ((e >> 2) * 16 + (p & 15)) * 4 * KB + (blk % KB) * 4 + (e & 3);
     }
-    __device__ static int vq(int p, int blk, int e) {
+    __host__ __device__ static int vq(int p, int blk, int e) {
         return VQ + (blk / VB) * 512 * VB + (((p & 15) >> 2) * 16 + e) * 8 * VB + (blk % VB) * 8 + (p >> 4) * 4 + (p & 3);
     }
-    __device__ static int scale(int p, int blk) { return ((((p & 15) >> 2) * NB + blk) * 8 + (p >> 4) * 4 + (p & 3)) * 2; }
+    __host__ __device__ static int scale(int p, int blk) { return ((((p & 15) >> 2) * NB + blk) * 8 + (p >> 4) * 4 + (p & 3)) * 2; }
 };
 
 // Tokens t < num[s] (num NULL: n_tok) of sequence s are at positions pos[s * pos_stride] + t; the ones outside 0 .. n_ctx - 1 are
@@ -46,9 +46,10 @@ struct Kv4Tokens {
     int pos_stride, n_tok, n_seq;
 };
 
-struct Kv4Cache {
+struct Kv4Cache {  // the records of sequence s and KV head h start at record s * seq + h * head
     uint8_t * data;
-    int n_ctx, tiles, n_head_kv, head_dim;  // tiles: records of a sequence and KV head
+    int n_ctx, n_head_kv, head_dim;  // n_ctx: positions of a sequence
+    long long seq, head;
 };
 
 struct Kv4RowsArgs {  // store or load: row (s * n_tok + t) of k and v at row_stride floats, KV heads packed
@@ -67,8 +68,9 @@ struct Kv4AttnArgs {
     long long q_row, q_head, y_row;
     int n_head, window;  // window 0: every position up to the token's own
     float scale;
-    const float * gate;  // NULL, or gate rows as q's (the output times sigmoid(gate))
-    float * work;        // kv4_work_floats
+    const float * gate;  // NULL, or gate rows (the output times sigmoid(gate)), g_row and g_head floats apart
+    long long g_row, g_head;
+    float * work;        // kv4_work_floats; NULL: one range a sequence
     int ranges;          // set at launch: ranges of records that the grid has workgroups for
     int group;           // set at launch: n_head / n_head_kv
 };
@@ -78,8 +80,26 @@ struct Kv4AttnArgs {
 // 32768, 16/4 heads of 256, 21.5 / 26.2 / 26.4 / 26.2; 32 sequences of up to 8192, 32/8 heads of 128, 78 / 58 / 55 / 56).
 constexpr int KV4_GROUPS = 1536, KV4_GROUPS_256 = 512;
 constexpr int KV4_LEAST = 4;      // records of a range at least: one a wave
+bool kv4_joins(const Kv4AttnArgs & a);  // the launch is followed by that of kv4_join_kernel
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head);
 
+// The ATTN command's part before the attention: every q head and new key normalized and rotated (gq_kernels.h, AttnArgs; q stays FP32 in
+// qr), the keys and values stored. Tokens as t says.
+struct Kv4AppendArgs {
+    Kv4Cache c;
+    Kv4Tokens t;
+    const float * q;   // row (s * n_tok + t) at n_head * q_stride floats
+    const float * k;   // rows of n_head_kv * head_dim floats
+    const float * v;
+    const float * qn;
+    const float * kn;
+    const float * cs;  // n_rot floats a position
+    float * qr;        // rows of n_head * head_dim floats
+    int n_head, n_rot, q_stride;
+    float eps;
+};
+
+hipError_t launch_kv4_append(const Kv4AppendArgs & a, hipStream_t s);
 hipError_t launch_kv4_store(const Kv4RowsArgs & a, hipStream_t s);
 hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s);
 hipError_t launch_kv4_attn(const Kv4AttnArgs & a, hipStream_t s);

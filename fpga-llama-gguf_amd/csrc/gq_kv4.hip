@@ -45,7 +45,7 @@ __device__ __forceinline__ void kv4_span(const Kv4Tokens & t, int s, long long &
 }
 
 __device__ __forceinline__ uint8_t * kv4_rec(const Kv4Cache & c, int s, int h, int tile) {
-    return c.data + ((size_t(s) * c.n_head_kv + h) * c.tiles + tile) * kv4_record(c.head_dim);
+    return c.data + size_t(s * c.seq + h * c.head + tile) * kv4_record(c.head_dim);
 }
 
 // Workgroup (record of the tokens' span; keys or values; four blocks | KV head | sequence): 8 lanes a block. A record that the tokens
@@ -110,6 +110,61 @@ __global__ __launch_bounds__(KV4_STORE) void kv4_store_kernel(Kv4RowsArgs a) {
     }
     for (int i = tid; i < 4 * BG; i += KV4_STORE)
         *reinterpret_cast<uint4 *>(rec + (val ? L::VD : L::KD) + (i / BG * L::NB + bg * BG + i % BG) * 16) = *reinterpret_cast<const uint4 *>(img + QB + i * 16);
+}
+
+// Workgroup (q head, or KV head behind them | token | sequence): the ATTN command's norm and rotation of one vector, in the order of
+// the F16 cache's kernels; a q head's goes to qr, a key's into the cache with its value, 8 lanes a block.
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
+    using L = Kv4Layout<HD>;
+    __shared__ __align__(16) float xs[HD], rot[HD];
+    __shared__ float red[4];
+    const int t = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    long long p0;
+    int n;
+    kv4_span(a.t, s, p0, n);
+    const long long pl = p0 + t;
+    if (t >= n || pl < 0 || pl >= a.c.n_ctx) return;
+    const int pos = int(pl), half = a.n_rot / 2;
+    const bool isq = int(blockIdx.x) < a.n_head;
+    const int h = isq ? blockIdx.x : blockIdx.x - a.n_head;
+    const size_t row = size_t(s) * a.t.n_tok + t;
+    const bool el = tid < HD;
+    const int e = el ? tid : 0;
+    const float x = !el ? 0.0f : isq ? a.q[(row * a.n_head + h) * size_t(a.q_stride) + e] : a.k[(row * a.c.n_head_kv + h) * HD + e];
+    const float w = isq ? a.qn[e] : a.kn[e];
+    const int pi = e < half ? e : e - half;
+    const bool turn = e < a.n_rot;
+    const float cs0 = turn ? a.cs[size_t(pos) * a.n_rot + 2 * pi] : 0.0f, cs1 = turn ? a.cs[size_t(pos) * a.n_rot + 2 * pi + 1] : 0.0f;
+    float sq[1] = {x * x};
+    pair_sum_lanes_n<64, 1>(sq);
+    if (lane == 0) red[wave] = sq[0];
+    __syncthreads();
+    const float sc = 1.0f / sqrtf(((red[0] + red[1]) + (red[2] + red[3])) / float(HD) + a.eps);
+    if (el) xs[e] = (x * sc) * w;
+    __syncthreads();
+    if (el) {
+        const float x0 = xs[pi], x1 = turn ? xs[pi + half] : 0.0f;
+        const float r = e < half ? x0 * cs0 - x1 * cs1 : turn ? x0 * cs1 + x1 * cs0 : xs[e];
+        if (isq) a.qr[(row * a.n_head + h) * HD + e] = r;
+        else rot[e] = r;
+    }
+    if (isq) return;
+    __syncthreads();
+    if (tid >= HD / 2) return;  // HD / 4 threads the key, as many the value
+    const bool val = tid >= HD / 4;
+    const int u = val ? tid - HD / 4 : tid, blk = u >> 3, j = u & 7, p = pos % KV4_TILE;
+    const float * src = val ? a.v + (row * a.c.n_head_kv + h) * HD + 4 * u : rot + 4 * u;
+    const float y[4] = {src[0], src[1], src[2], src[3]};
+    uint32_t d;
+    const uint32_t q = kv4_quantize(y, d), bytes = q | uint32_t(dpp_i32<0x104>(int(q))) << 4;
+    uint8_t * rec = kv4_rec(a.c, s, h, pos / KV4_TILE);
+    if (j < 4) {
+        uint8_t * to = rec + (val ? L::vq(p, blk, 4 * j) : L::kq(p, blk, 4 * j));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i * (val ? 8 * L::VB : 1)] = uint8_t(bytes >> (8 * i));
+    }
+    if (j == 0) *reinterpret_cast<uint16_t *>(rec + (val ? L::VD : L::KD) + L::scale(p, blk)) = uint16_t(d);
 }
 
 template <int HD>
@@ -381,7 +436,7 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int &
 template <int HD>
 __device__ __forceinline__ void kv4_out(const Kv4AttnArgs & a, size_t row, int hq, int e, f32x4 y, float l) {
     if (a.gate) {
-        const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + row * size_t(a.q_row) + size_t(hq) * size_t(a.q_head) + e);
+        const f32x4 g = *reinterpret_cast<const f32x4 *>(a.gate + row * size_t(a.g_row) + size_t(hq) * size_t(a.g_head) + e);
 #pragma unroll
         for (int i = 0; i < 4; ++i) y[i] = sigmoid_(g[i]) * (y[i] / l);
     } else {
@@ -421,7 +476,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     const int first = __builtin_amdgcn_readfirstlane(max(r.first + j * r.per, lo / KV4_TILE));
     const int last = __builtin_amdgcn_readfirstlane(min(r.first + min((j + 1) * r.per, r.tiles) - 1, hi / KV4_TILE));
     if (first > last) return;  // none of the range's positions are seen
-    const uint8_t * head = a.c.data + (size_t(s) * a.c.n_head_kv + h) * size_t(a.c.tiles) * kv4_record(HD);
+    const uint8_t * head = kv4_rec(a.c, s, h, 0);
     const Kv4Const k4;
 
     Kv4Tile<HD> tile;
@@ -746,6 +801,12 @@ hipError_t by_dim(int hd, F f) {
 
 }  // namespace
 
+hipError_t launch_kv4_append(const Kv4AppendArgs & a, hipStream_t s) {
+    return by_dim(a.c.head_dim, [&](auto hd) {
+        GQ_LAUNCH(kv4_append_kernel<hd.value>, dim3(a.n_head + a.c.n_head_kv, a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
+    });
+}
+
 hipError_t launch_kv4_store(const Kv4RowsArgs & a, hipStream_t s) {
     const unsigned span = unsigned((a.t.n_tok + KV4_TILE - 2) / KV4_TILE + 1);  // records that n_tok positions can touch
     return by_dim(a.c.head_dim, [&](auto hd) {
@@ -771,7 +832,7 @@ static int kv4_nq(int hd, int n_tok, int per_kv) {
 int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     const int per_kv = n_head / c.n_head_kv, rows = 16 * kv4_nq(c.head_dim, n_tok, per_kv);
     const long long units = (n_tok * (long long)per_kv + rows - 1) / rows * c.n_head_kv;
-    const long long most = (long long)n_seq * ((c.tiles + KV4_LEAST - 1) / KV4_LEAST);
+    const long long most = (long long)n_seq * ((kv4_tiles(c.n_ctx) + KV4_LEAST - 1) / KV4_LEAST);
     return int(std::min<long long>(std::max<long long>(n_seq, std::min((c.head_dim == 256 ? KV4_GROUPS_256 : KV4_GROUPS) / units, most)), 65535));
 }
 
@@ -780,10 +841,12 @@ size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     return ranges > n_seq ? size_t(ranges) * n_tok * n_head * (c.head_dim + 4) : 0;
 }
 
+bool kv4_joins(const Kv4AttnArgs & a) { return a.work && kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head) > a.t.n_seq; }
+
 hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
     Kv4AttnArgs a = args;
     const int per_kv = a.n_head / a.c.n_head_kv, nq = kv4_nq(a.c.head_dim, a.t.n_tok, per_kv);
-    a.ranges = kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head);
+    a.ranges = a.work ? kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head) : a.t.n_seq;
     a.group = per_kv;
     const dim3 grid(unsigned((a.t.n_tok * (long long)per_kv + 16 * nq - 1) / (16 * nq)), unsigned(a.c.n_head_kv), unsigned(a.ranges));
     return by_dim(a.c.head_dim, [&](auto hd) {

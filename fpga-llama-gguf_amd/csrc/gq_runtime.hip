@@ -3,7 +3,9 @@
 // fpga/src/gemvqc16.cpp:552-958, moved to the host because a GPU launch sequence can be captured once), and the
 // hipGraph capture and replay of per-token lists. C ABI in include/gemvq_hip.h.
 #include "gemvq_hip.h"
+#include "gq_beam.h"
 #include "gq_kernels.h"
+#include "gq_kv4.h"
 #include "gq_ref.h"
 #include "gq_refmath.h"
 
@@ -97,6 +99,9 @@ float weight_bound(int type, int rows, int cols, const uint8_t * gguf) {
 struct KvBuf {
     uint16_t * k = nullptr;
     uint16_t * v = nullptr;
+    uint8_t * q4 = nullptr;       // a 4-bit buffer's records (gq_kv4.h): KV head h's from record h * q4_records on; k and v are then NULL
+    size_t q4_records = 0;
+    int region = 0;               // its positions of a sequence in the last list compiled for it (n_ctx at first)
     float * part = nullptr;       // attention partials and counters: one set per token of a GEMM_MAX_TOK batch
     unsigned * counter = nullptr;
     float * qr = nullptr;         // a batch's rotated queries [GEMM_MAX_TOK][ATTN_MAXG * n_head_kv][head_dim]
@@ -119,9 +124,13 @@ struct LArgmax { const float * x; int n; unsigned long long * key; int rows, str
 struct LNext { NextTokenArgs a; };
 struct LGemmQ { GemmQuantArgs a; };
 struct LGemm { GemmArgs a; int type; };
+struct LAttn4 { Kv4AppendArgs p; Kv4AttnArgs a; };
+struct LBeam { BeamSelectArgs a; };
+struct LBeamMove { BeamReorderArgs a; };
+struct LBeamNext { BeamNextArgs a; };
 struct LTok { TokArgs a; int type; uint32_t x_off, x_len; };  // x_off, x_len: the token rows read (activation floats)
 using Launch = std::variant<LGemv, LNorm, LEw, LConv, LRope, LGdn, LGated, LAttn, LRows, LArgmax, LNext, LGemmQ, LGemm,
-                            LGdnOut, LTok>;
+                            LGdnOut, LTok, LAttn4, LBeam, LBeamMove, LBeamNext>;
 
 }  // namespace
 
@@ -167,6 +176,14 @@ struct gemvq_ctx {
     float * attn_wide = nullptr;  // attention partials and queries of a prompt chunk's batch (gq_attn_tokens), likewise
     size_t attn_wide_n = 0;
     std::vector<float *> attn_wide_old;
+    // Grown as lists need them, the smaller ones kept for graphs captured with them: the partial sums of 4-bit attention, the beam
+    // selection's workspace.
+    struct Scratch {
+        void * p = nullptr;
+        size_t n = 0;
+        std::vector<void *> old;
+    } kv4_work, beam_work;
+    int kv_type = GEMVQ_KV_F16;   // of the KV buffers created from now on
     size_t scratch_max = ~size_t(0);  // largest allocation for scratch that a launch can do without (set at creation)
     int max_tok = GEMM_MAX_TOK;   // tokens a command of the list being compiled may hold (gq_wide_lists)
     float * ref_x = nullptr;      // the reference arithmetic's copy of a GEMM's token rows and norm weight
@@ -259,6 +276,18 @@ void * optional_scratch(gemvq_ctx * c, size_t bytes) {
     if (hipMalloc(&p, bytes) == hipSuccess) return p;
     (void)hipGetLastError();
     return nullptr;
+}
+
+// At least `bytes` of s (growing at least twofold), NULL without memory for it.
+void * grown_scratch(gemvq_ctx * c, gemvq_ctx::Scratch & s, size_t bytes) {
+    if (s.n >= bytes) return s.p;
+    const size_t n = std::max(bytes, 2 * s.n);
+    void * p = optional_scratch(c, n);
+    if (!p) return nullptr;
+    if (s.p) s.old.push_back(s.p);
+    s.p = p;
+    s.n = n;
+    return p;
 }
 
 int einval(gemvq_ctx * c, const std::string & what) {
@@ -488,6 +517,23 @@ struct Compiler {
                 wr.push_back({k[6], ns > 1 ? k[6] + uint64_t(k[7] >> 8) * ns : c->act_floats});
                 break;
             }
+            case GEMVQ_OP_BEAM: {
+                const uint64_t sl = 16ull * std::max<uint64_t>(uint64_t(k[4] & 0xffu) * (k[4] >> 8), 1) - 15;
+                for (const uint32_t o : {k[6], k[7], k2 ? k2[0] : k[7]}) wr.push_back({o, o + sl});
+                step = 2;
+                break;
+            }
+            case GEMVQ_OP_BEAM_MOVE:
+                if ((k[1] & 0xffu) == GEMVQ_BEAM_ACT) {
+                    const uint64_t rows = uint64_t(k[7] & 0xffu) * (k[7] >> 8), parts = k[1] >> 8;
+                    wr.push_back({k[2], k[2] + rows * k[3] + parts * k[4] + k[5]});
+                }
+                step = 2;
+                break;
+            case GEMVQ_OP_BEAM_NEXT:
+                wr.push_back({k[2], k[2] + 16ull * k[5]});
+                wr.push_back({k[3], k[3] + uint64_t(k[4]) * k[5]});
+                break;
             case GEMVQ_OP_GEMM:
                 if (k2) wr.push_back({k[7], k[7] + uint64_t(k2[2]) * (k2[0] ? k2[0] - 1 : 0) + k[2]});
                 step = 2;
@@ -604,6 +650,7 @@ struct Compiler {
             const uint32_t * k = cmds + size_t(i) * GEMVQ_CMD_WORDS;
             const uint32_t op = k[0];
             if (op != GEMVQ_OP_GEMM) lastq.on = tok_open = false;
+            if (op != GEMVQ_OP_BEAM_MOVE) moves.open = false;
             switch (op) {
             case GEMVQ_OP_GEMV: {
                 unsigned used = 0;
@@ -843,6 +890,7 @@ struct Compiler {
                     hd < 16 || (hd & (hd - 1)) || nrot > hd || nrot % 2)
                     return reject(i, "ATTN shape");
                 const uint32_t qstride = (flags & 1) ? 2 * hd : hd, ntok = tokens16(flags);
+                if (b.q4) return attn4(i, k, k2, nh, nkv, hd, nrot, qstride, ntok);
                 // the cache's sets of partials and rotated queries serve GEMM_MAX_TOK tokens of ATTN_MAXG q heads per KV head;
                 // the model driver's lists use them for more tokens of fewer heads, or the context's (gq_attn_tokens)
                 const bool wide = c->max_tok > GEMM_MAX_TOK;
@@ -963,6 +1011,19 @@ struct Compiler {
                     spans.push_back({int(i), 1});
                 break;
             }
+            case GEMVQ_OP_BEAM: return beam(n, i, k);
+            case GEMVQ_OP_BEAM_MOVE: return beam_move(n, i, k);
+            case GEMVQ_OP_BEAM_NEXT: {
+                const uint32_t ns = k[5];
+                if (ns == 0 || ns > GEMVQ_GEMM_MAX_TOK || k[4] == 0 || !range(k[1], 16ull * (ns - 1) + 1) ||
+                    !range(k[2], 16ull * (ns - 1) + 1) || !range(k[3], uint64_t(k[4]) * ns))
+                    return reject(i, "BEAM_NEXT range");
+                BeamNextArgs a{reinterpret_cast<const int32_t *>(A(k[1])), reinterpret_cast<int32_t *>(A(k[2])),
+                               reinterpret_cast<int32_t *>(A(k[3])), int(k[4]), int(ns)};
+                out.push_back(LBeamNext{a});
+                spans.push_back({int(i), 1});
+                break;
+            }
             case GEMVQ_OP_FILL: {
                 if (k[1] == 0 || !range(k[2], k[1])) return reject(i, "FILL range");
                 EwArgs a{nullptr, nullptr, A(k[2]), int(k[1]), 0, 0, EW_FILL, bits_f(k[3])};
@@ -975,6 +1036,199 @@ struct Compiler {
             }
             ++i;
         }
+        return true;
+    }
+
+    // ATTN on a 4-bit KV buffer: the new keys, values and queries in one launch, then the attention over the records. The partial sums'
+    // scratch is shared by the context's buffers; without memory for it every sequence is one range.
+    bool attn4(unsigned & i, const uint32_t * k, const uint32_t * k2, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t nrot,
+               uint32_t qstride, uint32_t ntok) {
+        KvBuf & b = c->kvs[k[3]];
+        if (ref()) return reject(i, "ATTN on a 4-bit KV buffer in the reference arithmetic");
+        const uint32_t flags = k[7], sets = ATTN_MAXG * nkv * GEMM_MAX_TOK / std::max(nh, 1u);
+        const bool wide = c->max_tok > GEMM_MAX_TOK, own = wide && ntok > sets;
+        if (ntok > uint32_t(wide ? c->max_tok : GEMM_MAX_TOK) || (own && size_t(ntok) * nh * hd > c->attn_wide_n)) return reject(i, "ATTN tokens");
+        const bool seqs = (flags & GEMVQ_ATTN_SEQS) && ntok > 1;
+        if (seqs && (b.n_ctx % int(ntok) || !range(k[6], 16ull * (ntok - 1) + 1))) return reject(i, "ATTN sequences");
+        const int cap = seqs ? b.n_ctx / int(ntok) : b.n_ctx;
+        const uint64_t qt = uint64_t(nh) * qstride * (ntok - 1), kvt = uint64_t(nkv) * hd * ntok;
+        if (!range(k[2], qt + uint64_t(qstride) * (nh - 1) + hd) || !range(k[4], uint64_t(nh) * hd * ntok) || !range(k[6], 1) ||
+            !range(k2[0], kvt) || !range(k2[1], kvt) || !range(k2[4], hd) || !range(k2[5], hd) ||
+            k2[6] + uint64_t(cap) * nrot > c->act_floats)
+            return reject(i, "ATTN range");
+        if ((flags & 1) && !range(k2[7], qt + uint64_t(2 * hd) * (nh - 1) + hd)) return reject(i, "ATTN gate range");
+        LAttn4 l{};
+        const Kv4Cache cache{b.q4, cap, int(nkv), int(hd), kv4_tiles(cap), (long long)b.q4_records};
+        const Kv4Tokens t{reinterpret_cast<const int32_t *>(A(k[6])), nullptr, seqs ? 16 : 1, seqs ? 1 : int(ntok), seqs ? int(ntok) : 1};
+        b.region = cap;
+        l.p.c = l.a.c = cache;
+        l.p.t = l.a.t = t;
+        l.p.q = A(k[2]);
+        l.p.k = A(k2[0]);
+        l.p.v = A(k2[1]);
+        l.p.qn = A(k2[4]);
+        l.p.kn = A(k2[5]);
+        l.p.cs = A(k2[6]);
+        l.p.qr = own ? c->attn_wide : b.qr;
+        l.p.n_head = int(nh);
+        l.p.n_rot = int(nrot);
+        l.p.q_stride = int(qstride);
+        l.p.eps = bits_f(k2[3]);
+        l.a.q = l.p.qr;
+        l.a.q_row = (long long)nh * hd;
+        l.a.q_head = hd;
+        l.a.y = A(k[4]);
+        l.a.y_row = (long long)nh * hd;
+        l.a.n_head = int(nh);
+        l.a.scale = bits_f(k2[2]);
+        l.a.gate = (flags & 1) ? A(k2[7]) : nullptr;
+        l.a.g_row = (long long)nh * qstride;
+        l.a.g_head = qstride;
+        if (const size_t work = kv4_work_floats(cache, t.n_seq, t.n_tok, int(nh)))
+            l.a.work = static_cast<float *>(grown_scratch(c, c->kv4_work, work * sizeof(float)));
+        out.push_back(l);
+        spans.push_back({int(i), 2});
+        i += 2;
+        return true;
+    }
+
+    // One step of a beam search over the rows of logits (gq_beam.h).
+    bool beam(unsigned n, unsigned & i, const uint32_t * k) {
+        if (i + 1 >= n) return reject(i, "BEAM needs its second slot");
+        const uint32_t * k2 = k + GEMVQ_CMD_WORDS;
+        const uint32_t v = k[1], stride = k[3], nb = k[4] & 0xffu, ng = k[4] >> 8, cap = k2[4];
+        const uint64_t rows = uint64_t(nb) * ng, sl = 16 * (rows - 1) + 1;
+        if (nb == 0 || nb > uint32_t(BEAM_MAX) || ng == 0 || rows > GEMVQ_GEMM_MAX_TOK || v == 0 || v > uint32_t(BEAM_MAX_VOCAB))
+            return reject(i, "BEAM shape");
+        if (stride < v || stride % 16 || !range(k[2], uint64_t(stride) * (rows - 1) + v) || !range(k[6], sl) || !range(k[7], sl) ||
+            !range(k2[0], sl))
+            return reject(i, "BEAM range");
+        if (k2[2] && (!range(k2[1], sl) || !range(k2[2], sl) || cap == 0 || !range(k2[3], cap * rows))) return reject(i, "BEAM prompt");
+        BeamSelectArgs a{};
+        a.x = A(k[2]);
+        a.stride = stride;
+        a.n_vocab = int(v);
+        a.n_group = int(ng);
+        a.n_beam = int(nb);
+        a.eos = int32_t(k[5]);
+        a.score = a.score_out = A(k[6]);
+        a.token = reinterpret_cast<int32_t *>(A(k2[0]));
+        a.last = a.token;
+        a.parent = reinterpret_cast<int32_t *>(A(k[7]));
+        a.slot = 16;
+        if (k2[2]) {
+            a.pos = reinterpret_cast<const int32_t *>(A(k2[1]));
+            a.n_prompt = reinterpret_cast<const int32_t *>(A(k2[2]));
+            a.prompt = reinterpret_cast<const int32_t *>(A(k2[3]));
+            a.cap = int(cap);
+        }
+        a.work = grown_scratch(c, c->beam_work, beam_work(a.n_group, a.n_beam, a.n_vocab));
+        if (!a.work) return reject(i, "BEAM: no memory for its workspace");
+        out.push_back(LBeam{a});
+        spans.push_back({int(i), 2});
+        i += 2;
+        return true;
+    }
+
+    // The open launch of beam moves: what its arrays write and read (act floats; state rows; KV buffers).
+    struct Moves { bool open = false; std::vector<Rng> wr, rd, state; std::vector<uint32_t> kv; } moves;
+
+    // An array that follows the beams. Consecutive commands with the same parents become one launch while their arrays lie apart.
+    bool beam_move(unsigned n, unsigned & i, const uint32_t * k) {
+        if (i + 1 >= n) return reject(i, "BEAM_MOVE needs its second slot");
+        const uint32_t * k2 = k + GEMVQ_CMD_WORDS;
+        const uint32_t kind = k[1] & 0xffu, parts = std::max(k[1] >> 8, 1u), nb = k[7] & 0xffu, ng = k[7] >> 8, first = k2[1];
+        const uint64_t rows = uint64_t(nb) * ng, sl = 16 * (rows - 1) + 1, rs = k[3], ps = k[4], len = k[5];
+        if (nb == 0 || nb > uint32_t(BEAM_MAX) || ng == 0 || rows > GEMVQ_GEMM_MAX_TOK) return reject(i, "BEAM_MOVE shape");
+        if (!range(k[6], sl) || (k2[0] && !range(k2[0], sl))) return reject(i, "BEAM_MOVE range");
+        BeamMove m[2] = {};
+        uint32_t part_n[2] = {parts, 1};
+        int nm = 1;
+        Moves io;
+        io.rd = {{k[6], k[6] + sl}};
+        if (k2[0]) io.rd.push_back({k2[0], k2[0] + sl});
+        m[0].used = k2[0] ? reinterpret_cast<const int32_t *>(A(k2[0])) : nullptr;
+        m[0].used_stride = 16;
+        m[0].used_more = 1;
+        m[0].unit_len = 1;
+        if (kind == GEMVQ_BEAM_ACT || kind == GEMVQ_BEAM_STATE) {
+            const bool act = kind == GEMVQ_BEAM_ACT;
+            const uint64_t end = k[2] + rs * (rows - 1) + ps * (parts - 1) + len, unit = act ? 4 : 512;
+            if (len == 0 || first > len || parts > 65535u || !beam_rows_apart(rows, len, rs, ps, parts)) return reject(i, "BEAM_MOVE rows");
+            if (act ? (!range(k[2], 0) || end > c->act_floats) : end > c->state_rows) return reject(i, "BEAM_MOVE range");
+            m[0].data = reinterpret_cast<uint8_t *>(act ? A(k[2]) : c->state + size_t(k[2]) * 128);
+            m[0].row_stride = rs * unit;
+            m[0].part_stride = ps * unit;
+            m[0].unit_bytes = uint32_t(unit);
+            m[0].lo = first * unit;
+            m[0].hi = len * unit;
+            (act ? io.wr : io.state).push_back({k[2], end});
+            if (meet_any(io.wr, io.rd)) return reject(i, "BEAM_MOVE of its own parents or positions");
+        } else if (kind == GEMVQ_BEAM_KV) {
+            if (k[2] >= c->kvs.size() || c->kvs[k[2]].n_ctx % int(rows) || !k2[0]) return reject(i, "BEAM_MOVE kv buffer");
+            KvBuf & b = c->kvs[k[2]];
+            const int cap = b.n_ctx / int(rows);
+            if (first > uint32_t(cap)) return reject(i, "BEAM_MOVE kv buffer");
+            if (b.q4) {
+                const size_t rec = kv4_record(b.head_dim);
+                m[0].data = b.q4;
+                m[0].row_stride = size_t(kv4_tiles(cap)) * rec;
+                m[0].part_stride = b.q4_records * rec;
+                part_n[0] = uint32_t(b.n_head_kv);
+                m[0].unit_bytes = uint32_t(rec);
+                m[0].unit_len = KV4_TILE;
+                m[0].lo = first / KV4_TILE * rec;
+                m[0].hi = size_t(kv4_tiles(cap)) * rec;
+                b.region = cap;
+            } else {
+                const size_t row = size_t(b.n_head_kv) * b.head_dim * 2;
+                part_n[0] = 1;
+                m[0].data = reinterpret_cast<uint8_t *>(b.k);
+                m[0].row_stride = size_t(cap) * row;
+                m[0].unit_bytes = uint32_t(row);
+                m[0].lo = first * row;
+                m[0].hi = size_t(cap) * row;
+                m[1] = m[0];
+                m[1].data = reinterpret_cast<uint8_t *>(b.v);
+                nm = 2;
+            }
+            io.kv.push_back(k[2]);
+        } else {
+            return reject(i, "BEAM_MOVE kind");
+        }
+        for (int j = 0; j < nm; ++j)
+            if ((m[j].hi - m[j].lo) / BEAM_TILE + 1 > 0x7fffffffull / BEAM_MOVES / part_n[j]) return reject(i, "BEAM_MOVE size");
+        // joins the launch before it: same parents, nothing of either met by the other
+        const int32_t * parent = reinterpret_cast<const int32_t *>(A(k[6]));
+        LBeamMove * l = moves.open ? std::get_if<LBeamMove>(&out.back()) : nullptr;
+        if (l && (l->a.parent != parent || l->a.n_beam != int(nb) || l->a.n_group != int(ng) || l->a.n + nm > BEAM_MOVES ||
+                  meet_any(io.wr, moves.wr) || meet_any(io.wr, moves.rd) || meet_any(io.rd, moves.wr) || meet_any(io.state, moves.state) ||
+                  (!io.kv.empty() && std::find(moves.kv.begin(), moves.kv.end(), io.kv[0]) != moves.kv.end())))
+            l = nullptr;
+        if (!l) {
+            LBeamMove fresh{};
+            fresh.a.parent = parent;
+            fresh.a.parent_stride = 16;
+            fresh.a.n_group = int(ng);
+            fresh.a.n_beam = int(nb);
+            out.push_back(fresh);
+            spans.push_back({int(i), 0});
+            l = std::get_if<LBeamMove>(&out.back());
+            moves = {};
+            moves.open = true;
+        }
+        for (int j = 0; j < nm; ++j) {
+            if (m[j].lo >= m[j].hi) continue;
+            uint32_t end = l->a.n ? l->a.m[l->a.n - 1].end : 0;
+            beam_move_shape(m[j], part_n[j], end);
+            l->a.m[l->a.n++] = m[j];
+        }
+        moves.wr.insert(moves.wr.end(), io.wr.begin(), io.wr.end());
+        moves.rd.insert(moves.rd.end(), io.rd.begin(), io.rd.end());
+        moves.state.insert(moves.state.end(), io.state.begin(), io.state.end());
+        moves.kv.insert(moves.kv.end(), io.kv.begin(), io.kv.end());
+        spans.back().second += 2;
+        i += 2;
         return true;
     }
 
@@ -1507,6 +1761,21 @@ std::pair<std::string, uint64_t> describe(const Launch & l, int pos) {
         const uint64_t act = uint64_t(a.n_tok) * a.cols * 4 + (a.norm_w ? uint64_t(a.cols) * 4 : 0);
         return {"gemv_tok_kernel<" + std::to_string(x->type) + "," + std::to_string(a.n_tok) + ">", w + act + out};
     }
+    if (auto * x = std::get_if<LAttn4>(&l)) {
+        const Kv4AttnArgs & a = x->a;
+        const uint64_t rows = uint64_t(a.t.n_seq) * a.t.n_tok, nt = uint64_t(a.t.n_tok);  // a sequence's records are read once for its tokens
+        const uint64_t kv = uint64_t(a.t.n_seq) * (uint64_t(pos) + nt) * a.c.n_head_kv * a.c.head_dim * 9 / 8;
+        return {"kv4_attn_kernel", kv + (uint64_t(a.n_head) * a.c.head_dim * 4 * (a.gate ? 3 : 2) + uint64_t(a.c.n_head_kv) * a.c.head_dim * 8) * rows};
+    }
+    if (auto * x = std::get_if<LBeam>(&l))
+        return {"beam_scan_kernel", uint64_t(x->a.n_group) * x->a.n_beam * uint64_t(x->a.n_vocab) * 4};
+    if (auto * x = std::get_if<LBeamMove>(&l)) {  // every row moved: its bytes read and written
+        uint64_t b = 0;
+        for (int i = 0; i < x->a.n; ++i)
+            b += (x->a.m[i].hi - x->a.m[i].lo) * ((x->a.m[i].end - (i ? x->a.m[i - 1].end : 0)) / x->a.m[i].tiles) * 2;
+        return {"beam_reorder_kernel", b * uint64_t(x->a.n_group) * x->a.n_beam};
+    }
+    if (std::get_if<LBeamNext>(&l)) return {"beam_next_kernel", 32};
     return {"next_token_kernel", 32};
 }
 
@@ -1514,6 +1783,9 @@ std::pair<std::string, uint64_t> describe(const Launch & l, int pos) {
 int kernels_of(const Launch & l) {
     if (auto * x = std::get_if<LAttn>(&l)) return x->ref ? 2 : x->a.n_tok <= 1 ? 1 : attn_tiled(x->a) ? 3 : 2;
     if (auto * x = std::get_if<LGdn>(&l)) return !x->ref && gdn_ahead(x->a) ? 2 : 1;
+    if (auto * x = std::get_if<LAttn4>(&l)) return kv4_joins(x->a) ? 3 : 2;
+    if (std::get_if<LBeam>(&l)) return 2;
+    if (auto * x = std::get_if<LBeamMove>(&l)) return x->a.n ? 1 : 0;
     return 1;
 }
 
@@ -1551,9 +1823,62 @@ hipError_t issue(const std::vector<Launch> & ls, hipStream_t s) {
         else if (auto * x = std::get_if<LGemm>(&l)) e = launch_gemm(x->a, x->type, s);
         else if (auto * x = std::get_if<LGdnOut>(&l)) e = launch_gdn_out(x->a, x->type, s);
         else if (auto * x = std::get_if<LTok>(&l)) e = launch_gemv_tok(x->a, x->type, s);
+        else if (auto * x = std::get_if<LAttn4>(&l)) {
+            e = launch_kv4_append(x->p, s);
+            if (e == hipSuccess) e = launch_kv4_attn(x->a, s);
+        } else if (auto * x = std::get_if<LBeam>(&l)) e = launch_beam_select(x->a, s);
+        else if (auto * x = std::get_if<LBeamMove>(&l)) e = x->a.n ? launch_beam_reorder(x->a, s) : hipSuccess;
+        else if (auto * x = std::get_if<LBeamNext>(&l)) e = launch_beam_next(x->a, s);
         if (e != hipSuccess) return e;
     }
     return hipSuccess;
+}
+
+// Positions pos0 .. pos0 + npos - 1 of a 4-bit buffer, as fp16 (the values rounded). Position p is position p % region of region
+// p / region; a region's records start at a whole record.
+template <int HD>
+void kv4_unpack(const std::vector<uint8_t> & rec, size_t rec0, const KvBuf & b, int h, int pos0, int npos, uint16_t * k, uint16_t * v) {
+    using L = Kv4Layout<HD>;
+    const size_t per = size_t(kv4_tiles(b.region));
+    for (int i = 0; i < npos; ++i) {
+        const int r = (pos0 + i) / b.region, q = (pos0 + i) % b.region, p = q % KV4_TILE;
+        const uint8_t * x = rec.data() + (r * per + size_t(q / KV4_TILE) - rec0) * L::RECORD;
+        for (int e = 0; e < HD; ++e) {
+            const int blk = e / 32, up = (e & 16) ? 4 : 0;
+            const size_t to = (size_t(i) * b.n_head_kv + h) * HD + e;
+            const auto half = [&](int at, int byte) {
+                uint16_t d;
+                std::memcpy(&d, x + at, 2);
+                const _Float16 f = _Float16(half_to_float_host(d) * float(int((x[byte] >> up) & 15) - 8));
+                uint16_t u;
+                std::memcpy(&u, &f, 2);
+                return u;
+            };
+            if (k) k[to] = half(L::KD + L::scale(p, blk), L::kq(p, blk, e & 15));
+            if (v) v[to] = half(L::VD + L::scale(p, blk), L::vq(p, blk, e & 15));
+        }
+    }
+}
+
+int kv4_read(gemvq_ctx * c, const KvBuf & b, int pos0, int npos, uint16_t * k, uint16_t * v) {
+    if (npos == 0) return 0;
+    const size_t per = size_t(kv4_tiles(b.region)), rec = kv4_record(b.head_dim);
+    const auto at = [&](int p) { return size_t(p / b.region) * per + size_t(p % b.region) / KV4_TILE; };
+    const size_t r0 = at(pos0), r1 = at(pos0 + npos - 1) + 1;
+    std::vector<uint8_t> buf((r1 - r0) * rec);
+    for (int h = 0; h < b.n_head_kv; ++h) {
+        if (const int w = drain(c, "kv read")) return w;
+        c->busy = true;
+        const hipError_t e = hipMemcpyAsync(buf.data(), b.q4 + (h * b.q4_records + r0) * rec, buf.size(), hipMemcpyDeviceToHost, c->stream);
+        if (const int w = e == hipSuccess ? wait_stream(c, "kv read") : fail(c, e, "kv read")) return w;
+        switch (b.head_dim) {
+        case 32: kv4_unpack<32>(buf, r0, b, h, pos0, npos, k, v); break;
+        case 64: kv4_unpack<64>(buf, r0, b, h, pos0, npos, k, v); break;
+        case 128: kv4_unpack<128>(buf, r0, b, h, pos0, npos, k, v); break;
+        default: kv4_unpack<256>(buf, r0, b, h, pos0, npos, k, v); break;
+        }
+    }
+    return 0;
 }
 
 int compile_list(gemvq_ctx * c, const uint32_t * cmds, unsigned n, std::vector<Launch> & out,
@@ -1660,9 +1985,14 @@ void gemvq_ctx_destroy(gemvq_ctx * c) {
     for (auto & b : c->kvs) {
         hipFree(b.k);
         hipFree(b.v);
+        hipFree(b.q4);
         hipFree(b.part);
         hipFree(b.counter);
         hipFree(b.qr);
+    }
+    for (auto * s : {&c->kv4_work, &c->beam_work}) {
+        hipFree(s->p);
+        for (void * p : s->old) hipFree(p);
     }
     hipFree(c->act);
     hipFree(c->warena);
@@ -1816,15 +2146,37 @@ int gemvq_state_clear(gemvq_ctx * c) {
     return e == hipSuccess ? wait_stream(c, "state clear") : fail(c, e, "state clear");
 }
 
+int gemvq_set_kv_type(gemvq_ctx * c, int type) {
+    if (!c || (type != GEMVQ_KV_F16 && type != GEMVQ_KV_Q4_0)) return einval(c, "gemvq_set_kv_type: type");
+    c->kv_type = type;
+    return 0;
+}
+
 int gemvq_kv_create(gemvq_ctx * c, int n_ctx, int n_head_kv, int head_dim) {
     if (!c || n_ctx <= 0 || n_head_kv <= 0 || head_dim <= 0 || head_dim > 256 || head_dim % 16)
         return einval(c, "gemvq_kv_create: shape");
     if (!c->usable) return unusable(c);
     hipSetDevice(c->device);
     KvBuf b;
-    b.n_ctx = n_ctx;
+    b.n_ctx = b.region = n_ctx;
     b.n_head_kv = n_head_kv;
     b.head_dim = head_dim;
+    if (c->kv_type == GEMVQ_KV_Q4_0) {
+        if (!kv4_dim_ok(head_dim)) return einval(c, "gemvq_kv_create: a 4-bit buffer takes heads of 32, 64, 128 or 256");
+        // whole records for each of up to GEMM_MAX_TOK sequences' regions
+        b.q4_records = size_t(kv4_tiles(n_ctx)) + GEMM_MAX_TOK;
+        const size_t bytes = b.q4_records * n_head_kv * kv4_record(head_dim);
+        hipError_t e = hipMalloc(&b.q4, bytes);
+        if (e == hipSuccess) e = hipMalloc(&b.qr, size_t(ATTN_MAXG) * n_head_kv * GEMM_MAX_TOK * head_dim * 4);
+        if (e == hipSuccess) e = hipMemset(b.q4, 0, bytes);
+        if (e != hipSuccess) {
+            hipFree(b.q4);
+            hipFree(b.qr);
+            return fail(c, e, "kv create");
+        }
+        c->kvs.push_back(b);
+        return int(c->kvs.size()) - 1;
+    }
     const size_t kvn = size_t(n_ctx) * n_head_kv * head_dim;
     const size_t nch = size_t(n_ctx + ATTN_CHUNK - 1) / ATTN_CHUNK;
     const size_t heads = size_t(ATTN_MAXG) * n_head_kv * GEMM_MAX_TOK;  // (token, q head) sets of a batch
@@ -1855,6 +2207,7 @@ int gemvq_kv_read(gemvq_ctx * c, int kv, int pos0, int npos, uint16_t * k, uint1
     const KvBuf & b = c->kvs[kv];
     if (pos0 < 0 || npos < 0 || pos0 + npos > b.n_ctx) return einval(c, "gemvq_kv_read: range");
     hipSetDevice(c->device);
+    if (b.q4) return kv4_read(c, b, pos0, npos, k, v);
     const size_t row = size_t(b.n_head_kv) * b.head_dim, off = size_t(pos0) * row, n = size_t(npos) * row;
     if (const int w = drain(c, "kv read")) return w;
     c->busy = true;
@@ -1871,6 +2224,10 @@ int gemvq_kv_clear(gemvq_ctx * c) {
     hipError_t e = hipSuccess;
     c->busy = true;
     for (auto & b : c->kvs) {
+        if (b.q4) {
+            if (e == hipSuccess) e = hipMemsetAsync(b.q4, 0, b.q4_records * b.n_head_kv * kv4_record(b.head_dim), c->stream);
+            continue;
+        }
         const size_t kvn = size_t(b.n_ctx) * b.n_head_kv * b.head_dim;
         if (e == hipSuccess) e = hipMemsetAsync(b.k, 0, kvn * 2, c->stream);
         if (e == hipSuccess) e = hipMemsetAsync(b.v, 0, kvn * 2, c->stream);
@@ -1929,6 +2286,19 @@ __attribute__((visibility("hidden"))) int gq_attn_tokens(gemvq_ctx * c, int kv, 
     if (!c || kv < 0 || size_t(kv) >= c->kvs.size() || n_head < 1) return GEMVQ_EINVAL;
     const KvBuf & b = c->kvs[size_t(kv)];
     most = std::min(most, GEMM_WIDE_TOK) & ~31;
+    if (b.q4) {  // the rotated queries alone
+        const size_t n = size_t(most) * n_head * b.head_dim;
+        const int own = std::max(std::min(most, (ATTN_MAXG * b.n_head_kv * GEMM_MAX_TOK / n_head) & ~31), 32);
+        if (most <= own || !c->usable) return own;
+        if (c->attn_wide_n < n) {
+            float * p = static_cast<float *>(optional_scratch(c, n * sizeof(float)));
+            if (!p) return own;
+            if (c->attn_wide) c->attn_wide_old.push_back(c->attn_wide);
+            c->attn_wide = p;
+            c->attn_wide_n = n;
+        }
+        return most;
+    }
     const int sets = std::min(most, (ATTN_MAXG * b.n_head_kv * GEMM_MAX_TOK / n_head) & ~31);
     if (b.head_dim < ATTN_TILE_HD || !c->usable) return std::max(sets, 32);
     int tok = most;
@@ -2100,10 +2470,14 @@ int gemvq_profile(gemvq_ctx * c, const uint32_t * cmds, unsigned n, int reps, ge
     int pos = 0;
     if (const int w = drain(c, "profile")) return w;
     for (const Launch & l : ls)
-        if (auto * x = std::get_if<LAttn>(&l)) {
-            hipMemcpy(&pos, x->a.pos, 4, hipMemcpyDeviceToHost);
+    {
+        const auto * x = std::get_if<LAttn>(&l);
+        const auto * x4 = std::get_if<LAttn4>(&l);
+        if (x || x4) {
+            hipMemcpy(&pos, x ? x->a.pos : x4->a.t.pos, 4, hipMemcpyDeviceToHost);
             break;
         }
+    }
     const size_t L = ls.size();
     std::vector<LaunchTimer> timers(L);
     std::vector<std::vector<float>> ms_of(L);  // per launch, one duration (the sum over its kernels) per repetition

@@ -58,7 +58,8 @@ bool kv4_sizes_ok(const gemvq_kv4 * c) {
 bool kv4_ok(const gemvq_kv4 * c) { return kv4_sizes_ok(c) && c->data && aligned(c->data, 256); }
 
 Kv4Cache kv4_cache(const gemvq_kv4 * c) {
-    return {static_cast<uint8_t *>(c->data), c->n_ctx, kv4_tiles(c->n_ctx), c->n_head_kv, c->head_dim};
+    const long long tiles = kv4_tiles(c->n_ctx);
+    return {static_cast<uint8_t *>(c->data), c->n_ctx, c->n_head_kv, c->head_dim, tiles * c->n_head_kv, tiles};
 }
 
 bool kv4_tokens(const gemvq_kv4 * c, int n_tok, const int32_t * pos, const int32_t * num, Kv4Tokens & t) {
@@ -177,7 +178,7 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
     a.n_head = n_head;
     a.window = window;
     a.scale = scale;
-    a.work = static_cast<float *>(work);
+    a.work = need ? static_cast<float *>(work) : nullptr;
     const hipError_t e = launch_kv4_attn(a, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : -int(e);
 }
@@ -221,6 +222,7 @@ int gemvq_beam_select_static(const float * logits, int64_t row_stride, int n_voc
     a.score_out = score_out;
     a.token = token;
     a.parent = parent;
+    a.slot = 1;
     a.work = work;
     const hipError_t e = launch_beam_select(a, static_cast<hipStream_t>(stream));
     return e == hipSuccess ? 0 : -int(e);
@@ -237,11 +239,7 @@ int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, con
             x.unit_bytes % 4 || x.row_stride % 4 || x.part_stride % 4 || x.row_stride > most || x.part_stride > most || size > most)
             return GEMVQ_EINVAL;
         if (x.used && (!aligned(x.used, 4) || x.unit_len < 1 || x.used_stride < 1)) return GEMVQ_EINVAL;
-        // rows apart, and parts apart: all rows of a part before the next part, or all parts of a row before the next row
-        if (rows > 1 && x.row_stride < size) return GEMVQ_EINVAL;
-        if (x.n_part > 1 && x.part_stride < (rows - 1) * x.row_stride + size &&
-            (x.part_stride < size || (rows > 1 && x.row_stride < (x.n_part - 1) * x.part_stride + size)))
-            return GEMVQ_EINVAL;
+        if (!beam_rows_apart(rows, size, x.row_stride, x.part_stride, x.n_part)) return GEMVQ_EINVAL;
         if (((size - uint64_t(x.first) * x.unit_bytes) / BEAM_TILE + 1) * x.n_part > 0x7fffffffu / BEAM_MOVES) return GEMVQ_EINVAL;
     }
     for (int i = 0; i < n_arrays;) {
@@ -249,6 +247,7 @@ int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, con
         a.parent = parent;
         a.n_group = n_group;
         a.n_beam = n_beam;
+        a.parent_stride = 1;
         uint32_t end = 0;
         for (; i < n_arrays && a.n < BEAM_MOVES; ++i) {
             const gemvq_beam_array & x = arrays[i];
@@ -263,9 +262,7 @@ int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, con
             m.unit_bytes = x.unit_bytes;
             m.unit_len = x.unit_len;
             m.used_stride = x.used_stride;
-            m.wide = aligned(x.data, 16) && x.unit_bytes % 16 == 0 && x.row_stride % 16 == 0 && (x.n_part == 1 || x.part_stride % 16 == 0);
-            m.tiles = uint32_t((m.hi - m.lo + BEAM_TILE - 1) / BEAM_TILE);
-            m.end = end += m.tiles * x.n_part;
+            beam_move_shape(m, x.n_part, end);
         }
         if (!a.n) break;
         const hipError_t e = launch_beam_reorder(a, static_cast<hipStream_t>(stream));

@@ -71,6 +71,10 @@ struct gemvq_qwen35 {
     // (n_vocab) floats; its conv windows, DeltaNet state rows and KV region follow those of the sequence before
     int n_seq = 1;
     uint32_t skey = 0, spos = 0, slen = 0, sprompt = 0, sout = 0, slogits = 0;
+    // beam search (gemvq_qwen35_batch_set_beam): beams of a group (0: greedy), the eos id, the positions that a group's beams share (the
+    // shortest prompt's), and per sequence its score and parent slots
+    int n_beam = 0, eos = -1, shared = 0;
+    uint32_t sscore = 0, sparent = 0;
 };
 
 namespace {
@@ -148,6 +152,8 @@ size_t layout(gemvq_qwen35 & m, const gemvq_tensor_desc * tab, int n) {
         m.sprompt = take(ns * size_t(c.n_ctx));
         m.sout = take(ns * size_t(c.n_ctx));
         m.slogits = take(ns * size_t(c.n_vocab));
+        m.sscore = take(ns * 16);
+        m.sparent = take(ns * 16);
     }
     return off;
 }
@@ -257,6 +263,34 @@ bool build_chunk(const gemvq_qwen35 & m, uint32_t ntok, std::vector<uint32_t> & 
     return true;
 }
 
+// The end of a beam search's step: the selection, then everything a sequence keeps follows its parent: state rows, conv windows, keys
+// and values behind the shared prompt, token ids; then the new tokens join their lists.
+void build_beam_step(const gemvq_qwen35 & m, Emit & e) {
+    const gemvq_qw_config & c = m.c;
+    const uint32_t ns = uint32_t(m.n_seq), nb = uint32_t(m.n_beam), who = nb | ((ns / nb) << 8), cap = uint32_t(c.n_ctx);
+    const uint32_t rows = uint32_t(c.ssm_v_heads) * 128u, win = 3u * uint32_t(conv_ch(c));
+    e.cmd({GEMVQ_OP_BEAM, uint32_t(c.n_vocab), m.slogits, uint32_t(c.n_vocab), who, uint32_t(m.eos), m.sscore, m.sparent});
+    e.cmd({m.bid, m.spos, m.slen, m.sprompt, cap});
+    uint32_t gdn = 0;
+    for (int il = 0; il < c.n_layer; ++il) gdn += !is_attn(c, il);
+    if (gdn) {  // a layer's rows of all sequences after another
+        e.cmd({GEMVQ_OP_BEAM_MOVE, GEMVQ_BEAM_STATE | (gdn << 8), 0, rows, ns * rows, rows, m.sparent, who});
+        e.cmd({0, 0});
+    }
+    for (int il = 0; il < c.n_layer; ++il) {
+        if (is_attn(c, il)) {
+            e.cmd({GEMVQ_OP_BEAM_MOVE, GEMVQ_BEAM_KV, uint32_t(m.kv[il]), 0, 0, 0, m.sparent, who});
+            e.cmd({m.spos, uint32_t(m.shared)});
+        } else {
+            e.cmd({GEMVQ_OP_BEAM_MOVE, GEMVQ_BEAM_ACT, m.conv_state[il], win, 0, win, m.sparent, who});
+            e.cmd({0, 0});
+        }
+    }
+    e.cmd({GEMVQ_OP_BEAM_MOVE, GEMVQ_BEAM_ACT, m.sout, cap, 0, cap, m.sparent, who});
+    e.cmd({m.spos, uint32_t(m.shared)});
+    e.cmd({GEMVQ_OP_BEAM_NEXT, m.bid, m.spos, m.sout, cap, ns});
+}
+
 // One lockstep step of n_seq sequences, token t of sequence t: the chunk's GEMM projections over the n_seq token
 // rows; CONV, the DeltaNet step and attention in their sequences forms (each token on its own sequence's conv
 // window, state rows, KV region and position); the output norm and head per sequence; the argmax of every
@@ -301,6 +335,10 @@ bool build_batch(gemvq_qwen35 & m, std::string & err) {
             e.cmd({GEMVQ_OP_RMSNORM, E, m.bh + t * E, onorm.act_off, m.xn, fb(c.eps), 1, GEMVQ_NORM_DEFER});
             e.gemv(head, m.xn, m.slogits + t * V);
         }
+    }
+    if (m.n_beam) {
+        build_beam_step(m, e);
+        return true;
     }
     e.cmd({GEMVQ_OP_ARGMAX, V, m.slogits, m.skey, B, V});
     e.cmd({GEMVQ_OP_NEXT_TOKEN, m.skey, m.bid, m.spos, m.sprompt, m.slen, m.sout, B | (uint32_t(c.n_ctx) << 8)});
@@ -406,6 +444,15 @@ namespace {
 int set_err(gemvq_ctx * ctx, const std::string & what) {
     gq_set_error(ctx, what.c_str());
     return GEMVQ_EINVAL;
+}
+
+// The batch model's command list again; its graph is captured by the next step.
+int rebuild_batch(gemvq_qwen35 * m) {
+    std::string err;
+    m->cmds.clear();
+    if (m->graph >= 0) gemvq_graph_destroy(m->ctx, m->graph);
+    m->graph = -1;
+    return build_batch(*m, err) ? 0 : set_err(m->ctx, err);
 }
 }  // namespace
 
@@ -642,6 +689,13 @@ int gemvq_qwen35_batch_reset(gemvq_qwen35 * m, const int32_t * prompts, const in
     for (int s = 0; s < ns; ++s)
         if (offsets[s + 1] - offsets[s] < 1 || offsets[s + 1] - offsets[s] > cap) return GEMVQ_EINVAL;
     gemvq_ctx * ctx = m->ctx;
+    int shared = cap;
+    for (int s = 0; m->n_beam && s < ns; ++s) {  // the beams of a group start from one prompt
+        const int n = offsets[s + 1] - offsets[s], f = s / m->n_beam * m->n_beam;
+        if (offsets[f + 1] - offsets[f] != n || std::memcmp(prompts + offsets[f], prompts + offsets[s], size_t(n) * 4))
+            return set_err(ctx, "gemvq_qwen35_batch_reset: the beams of a group need the same prompt");
+        shared = std::min(shared, n);
+    }
     int st = gemvq_sync(ctx);
     if (!st) st = gemvq_state_clear(ctx);
     if (!st) st = gemvq_kv_clear(ctx);
@@ -663,6 +717,34 @@ int gemvq_qwen35_batch_reset(gemvq_qwen35 * m, const int32_t * prompts, const in
     if (!st) st = gemvq_act_write(ctx, m->spos, slots.data(), slots.size());  // every position 0
     if (!st) st = gemvq_act_write(ctx, m->skey, slots.data(), slots.size());
     if (!st) st = gemvq_act_write(ctx, m->bid, ids.data(), ids.size());
+    if (m->n_beam && !st) {  // a group's first beam starts alone
+        std::vector<float> score(size_t(ns) * 16, 0.0f);
+        for (int s = 0; s < ns; ++s)
+            if (s % m->n_beam) score[size_t(s) * 16] = -INFINITY;
+        st = gemvq_act_write(ctx, m->sscore, score.data(), score.size());
+        if (shared != m->shared) {  // the moves' first position is in their commands
+            m->shared = shared;
+            st = st ? st : rebuild_batch(m);
+        }
+    }
+    return st;
+}
+
+int gemvq_qwen35_batch_set_beam(gemvq_qwen35 * m, int n_beam, int eos) {
+    if (!m || m->n_seq < 2) return GEMVQ_EINVAL;
+    if (n_beam < 0 || (n_beam && m->n_seq % n_beam)) return set_err(m->ctx, "gemvq_qwen35_batch_set_beam: the sequences are no whole groups of n_beam");
+    if (n_beam && m->c.n_vocab > GEMVQ_BEAM_MAX_VOCAB) return set_err(m->ctx, "gemvq_qwen35_batch_set_beam: vocabulary");
+    m->n_beam = n_beam;
+    m->eos = eos;
+    m->shared = 0;
+    return rebuild_batch(m);
+}
+
+int gemvq_qwen35_batch_scores(gemvq_qwen35 * m, float * out) {
+    if (!m || !out || !m->n_beam) return GEMVQ_EINVAL;
+    std::vector<float> slots(size_t(m->n_seq) * 16);
+    const int st = gemvq_act_read(m->ctx, m->sscore, slots.data(), slots.size());
+    for (int s = 0; s < m->n_seq && !st; ++s) out[s] = slots[size_t(s) * 16];
     return st;
 }
 

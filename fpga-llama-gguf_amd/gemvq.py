@@ -22,6 +22,9 @@ Q4_0, Q4_1, Q8_0, Q5_K, Q6_K = 2, 3, 8, 13, 14
 # opcodes (gemvqc16.h:100-111 plus the opcodes of this backend)
 OP_GEMV, OP_RMSNORM, OP_ADD, OP_SILU_MUL, OP_MUL, OP_UNARY, OP_GDN, OP_CONV, OP_STATE_LOAD, OP_ROPE, OP_TRACE = range(1, 12)
 OP_ATTN, OP_GET_ROWS, OP_ARGMAX, OP_NEXT_TOKEN, OP_FILL, OP_GEMM = 12, 13, 14, 15, 16, 17
+OP_BEAM, OP_BEAM_MOVE, OP_BEAM_NEXT = 18, 19, 20
+BEAM_ACT, BEAM_STATE, BEAM_KV = 0, 1, 2
+KV_F16, KV_Q4_0 = 1, 2
 GEMM_MAX_TOK = 32
 GEMV_SWIGLU, GEMV_CONV, GEMV_ADD, GEMV_ARGMAX, GEMV_SILU = 0x100, 0x200, 0x400, 0x800, 0x1000
 GDN_WITH_GEMV, GDN_L2_QK, GDN_GATED, GDN_GATES, GDN_WITH_OUT, GDN_Z_SILU, GDN_SEQS = 1, 2, 4, 8, 16, 32, 64
@@ -118,6 +121,22 @@ def next_token(key: int, tok: int, pos: int, prompt: int, n_prompt: int, out: in
     return cmd(OP_NEXT_TOKEN, key, tok, pos, prompt, n_prompt, out)
 
 
+def beam(n_vocab: int, x: int, row_stride: int, n_beam: int, n_group: int, eos: int, score: int, parent: int, tok: int,
+         pos: int = 0, plen: int = 0, prompt: int = 0, cap: int = 0) -> list[int]:
+    """One step of a beam search over n_group groups of n_beam sequences; slots 16 floats apart."""
+    return cmd(OP_BEAM, n_vocab, x, row_stride, n_beam | (n_group << 8), eos, score, parent) + cmd(tok, pos, plen, prompt, cap)
+
+
+def beam_move(kind: int, off: int, row_stride: int, n: int, parent: int, n_beam: int, n_group: int, n_part: int = 1,
+              part_stride: int = 0, pos: int = 0, first: int = 0) -> list[int]:
+    """An array whose rows follow the beams (BEAM_ACT, BEAM_STATE, BEAM_KV)."""
+    return cmd(OP_BEAM_MOVE, kind | (n_part << 8), off, row_stride, part_stride, n, parent, n_beam | (n_group << 8)) + cmd(pos, first)
+
+
+def beam_next(tok: int, pos: int, out: int, cap: int, n_seq: int) -> list[int]:
+    return cmd(OP_BEAM_NEXT, tok, pos, out, cap, n_seq)
+
+
 def fill(n: int, y: int, value: float) -> list[int]:
     return cmd(OP_FILL, n, y, fbits(value))
 
@@ -182,6 +201,7 @@ def hip_lib() -> C.CDLL:
         _c_fn(lib, "gemvq_state_write", C.c_int, vp, C.c_size_t, vp, C.c_size_t)
         _c_fn(lib, "gemvq_state_read", C.c_int, vp, C.c_size_t, vp, C.c_size_t)
         _c_fn(lib, "gemvq_state_clear", C.c_int, vp)
+        _c_fn(lib, "gemvq_set_kv_type", C.c_int, vp, C.c_int)
         _c_fn(lib, "gemvq_kv_create", C.c_int, vp, C.c_int, C.c_int, C.c_int)
         _c_fn(lib, "gemvq_kv_read", C.c_int, vp, C.c_int, C.c_int, C.c_int, vp, vp)
         _c_fn(lib, "gemvq_kv_clear", C.c_int, vp)
@@ -409,6 +429,10 @@ class Context:
         out = np.empty(rows * 128, dtype=np.float32)
         self._check(self.lib.gemvq_state_read(self.h, row, _ptr(out), rows), "state read")
         return out
+
+    def set_kv_type(self, kind: int) -> None:
+        """KV_F16 (default) or KV_Q4_0: what the KV buffers created from now on hold."""
+        self._check(self.lib.gemvq_set_kv_type(self.h, kind), "set kv type")
 
     def kv_create(self, n_ctx: int, n_head_kv: int, head_dim: int) -> int:
         return self._check(self.lib.gemvq_kv_create(self.h, n_ctx, n_head_kv, head_dim), "kv create")

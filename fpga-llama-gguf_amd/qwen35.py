@@ -201,15 +201,17 @@ def _lib():
         gq._c_fn(lib, "gemvq_qwen35_batch_reset", C.c_int, vp, vp, vp)
         gq._c_fn(lib, "gemvq_qwen35_batch_tokens", C.c_int, vp, C.c_int, vp, C.c_int)
         gq._c_fn(lib, "gemvq_qwen35_batch_logits", C.c_int, vp, C.c_int, vp)
+        gq._c_fn(lib, "gemvq_qwen35_batch_set_beam", C.c_int, vp, C.c_int, C.c_int)
+        gq._c_fn(lib, "gemvq_qwen35_batch_scores", C.c_int, vp, vp)
         _fns = True
     return lib
 
 
 class Model:
     """The model on the GPU: one context sized for it, the weights uploaded, the per-token command list built (its
-    graph is captured by the first `step`)."""
+    graph is captured by the first `step`). kv_type gq.KV_Q4_0: its KV caches hold 4 bits a value."""
 
-    def __init__(self, blob: Blob, device: int = 0):
+    def __init__(self, blob: Blob, device: int = 0, kv_type: int = gq.KV_F16):
         self.lib = _lib()
         self.cfg = blob.cfg
         self.cc = config_c(blob.cfg)
@@ -217,6 +219,7 @@ class Model:
         if self.lib.gemvq_qwen35_sizes(C.byref(self.cc), blob.table, blob.n, C.byref(act), C.byref(wb), C.byref(st)):
             raise gq.GemvqError("qwen35 sizes")
         self.ctx = gq.Context(act_floats=act.value, weight_bytes=wb.value, state_rows=st.value, device=device)
+        self.ctx.set_kv_type(kv_type)
         self.h = self.lib.gemvq_qwen35_create(self.ctx.h, C.byref(self.cc), blob.table, blob.n, blob.data.ctypes.data)
         if not self.h:
             raise gq.GemvqError("qwen35 create: " + self.ctx.error())
@@ -304,7 +307,7 @@ class BatchModel:
     """n_seq sequences decoded in lockstep on the GPU (include/gemvq_qwen35.h gemvq_qwen35_batch_*): one step
     advances every sequence by one position, the layer projections reading each weight row once for all of them."""
 
-    def __init__(self, blob: Blob, n_seq: int, device: int = 0):
+    def __init__(self, blob: Blob, n_seq: int, device: int = 0, kv_type: int = gq.KV_F16):
         self.lib = _lib()
         self.cfg = blob.cfg
         self.n_seq = n_seq
@@ -314,6 +317,7 @@ class BatchModel:
                                              C.byref(st)):
             raise gq.GemvqError("qwen35 batch sizes")
         self.ctx = gq.Context(act_floats=act.value, weight_bytes=wb.value, state_rows=st.value, device=device)
+        self.ctx.set_kv_type(kv_type)
         self.h = self.lib.gemvq_qwen35_batch_create(self.ctx.h, C.byref(self.cc), blob.table, blob.n,
                                                     blob.data.ctypes.data, n_seq)
         if not self.h:
@@ -346,6 +350,16 @@ class BatchModel:
 
     def step(self, n: int = 1) -> None:
         self._ok(self.lib.gemvq_qwen35_step(self.h, n), "batch step")
+
+    def set_beam(self, n_beam: int, eos: int = -1) -> None:
+        """Beam search in groups of n_beam sequences, from the next reset on (0: greedy); gemvq_qwen35_batch_set_beam."""
+        self._ok(self.lib.gemvq_qwen35_batch_set_beam(self.h, n_beam, eos), "batch set beam")
+
+    def scores(self) -> np.ndarray:
+        """The beams' sums of log probabilities."""
+        out = np.empty(self.n_seq, np.float32)
+        self._ok(self.lib.gemvq_qwen35_batch_scores(self.h, out.ctypes.data), "batch scores")
+        return out
 
     def set_arith(self, arith: int) -> None:
         """gq.ARITH_REFERENCE: the following steps in the reference's CPU arithmetic (gemvq_qwen35_set_arith)."""

@@ -84,6 +84,23 @@
  *             and position at key_off, tok_off, pos_off + 16 s, its prompt length at act_i32[n_prompt + 16 s] (word
  *             5 is then an offset), its prompt at prompt_off + s * cap and its token ids at out_off + s * cap.
  *   FILL      [16, n, y_off, value bits, 0, 0, 0, 0]  y = value.
+ *   BEAM      [18, n_vocab, x_off, row_stride, n_beam | n_group << 8, eos, score_off, parent_off]
+ *             + [tok_off, pos_off, len_off, prompt_off, cap, 0, 0, 0]
+ *             One step of a beam search over n_group groups of n_beam sequences in lockstep (at most GEMVQ_GEMM_MAX_TOK in all; no
+ *             counterpart in the reference): gemvq_beam_select_static on the logits rows at x_off + s * row_stride. Sequence s's
+ *             score (FP32), token and parent (int32) are at act[score_off, tok_off, parent_off + 16 s]; the tokens there are the last ones, and the
+ *             new ones replace them. With len_off, a group whose first sequence is at position p = act_i32[pos_off + 16 s] with p + 1 <
+ *             act_i32[len_off + 16 s] reads its prompt instead: token = act_i32[prompt_off + s * cap + p + 1], the parent is the
+ *             sequence itself, the score stays; and eos ends a beam only behind its prompt.
+ *   BEAM_MOVE [19, kind | n_part << 8, off, row_stride, part_stride, n, parent_off, n_beam | n_group << 8]
+ *             + [pos_off, first, 0, 0, 0, 0, 0, 0]
+ *             gemvq_beam_reorder_static on one array: its row s becomes what row act_i32[parent_off + 16 s] of the group was. kind 0: rows of
+ *             n floats of the activation buffer from off on, kind 1: of n state rows (strides in floats, state rows; n_part 0: one
+ *             part); with pos_off only elements first .. pos move. kind 2: KV buffer off's regions as ATTN's sequences have them, positions
+ *             first .. pos (whole records of 32 in a 4-bit buffer). pos = act_i32[pos_off + 16 s] of the parent. Consecutive ones
+ *             with the same parents become one launch where their arrays lie apart.
+ *   BEAM_NEXT [20, tok_off, pos_off, out_off, cap, n_seq, 0, 0]  act_i32[out_off + s * cap + pos + 1] = tok (while that is below cap), pos += 1,
+ *             tok and pos at 16 s.
  *   GEMM      [17, format | flags, rows, cols, w_off lo, w_off hi, x_off, y_off]
  *             + [n_tok, x_stride, y_stride, res_off, res_stride, norm_w_off, eps bits, norm_flags]
  *             The batched GEMV (the reference's planned batched path, ROADMAP.md:78-96; no counterpart in its
@@ -130,6 +147,12 @@ extern "C" {
 #define GEMVQ_OP_NEXT_TOKEN 15u
 #define GEMVQ_OP_FILL 16u
 #define GEMVQ_OP_GEMM 17u
+#define GEMVQ_OP_BEAM 18u
+#define GEMVQ_OP_BEAM_MOVE 19u
+#define GEMVQ_OP_BEAM_NEXT 20u
+#define GEMVQ_BEAM_ACT 0u
+#define GEMVQ_BEAM_STATE 1u
+#define GEMVQ_BEAM_KV 2u
 #define GEMVQ_GEMM_MAX_TOK 32u
 #define GEMVQ_GEMV_SWIGLU 0x100u
 #define GEMVQ_GEMV_CONV 0x200u
@@ -154,8 +177,8 @@ extern "C" {
 #define GEMVQ_MAX_CMDS 4096u
 /* Feature words (gemvqc16.h:126-134 layout, marker 0x6B51 / 0x6B52). */
 #define GEMVQ_FEATURES 0x6B51FFFFu /* every format bit of the first word, Q4_1 (bit 2) included */
-#define GEMVQ_FEATURES2 0x6B52000Fu /* bit0 SILU_MUL sigmoid + strided g, bit1 ATTN/GET_ROWS/ARGMAX/NEXT_TOKEN,
-                                       bit2 GEMM, bit3 ATTN and GET_ROWS n_tok */
+#define GEMVQ_FEATURES2 0x6B52003Fu /* bit0 SILU_MUL sigmoid + strided g, bit1 ATTN/GET_ROWS/ARGMAX/NEXT_TOKEN,
+                                       bit2 GEMM, bit3 ATTN and GET_ROWS n_tok, bit4 4-bit KV buffers, bit5 BEAM* */
 
 typedef struct gemvq_ctx gemvq_ctx;
 
@@ -201,8 +224,17 @@ int gemvq_state_write(gemvq_ctx * ctx, size_t row, const float * src, size_t row
 int gemvq_state_read(gemvq_ctx * ctx, size_t row, float * dst, size_t rows);
 int gemvq_state_clear(gemvq_ctx * ctx);
 
-/* KV buffer for ATTN: n_ctx positions of n_head_kv x head_dim fp16 keys and values. Returns its id (>= 0). */
+/* What the KV buffers created from now on hold (no counterpart in the reference): fp16 (default), or 4 bits a value (Q4_0 blocks of 32, 4.5
+ * bits with their scales; heads of 32, 64, 128 or 256). ATTN on a 4-bit buffer has the meaning it has on an fp16 one, but for what its
+ * numbers are rounded to: keys and values as gemvq_kv4_store_static does, q not at all; and a batch's results agree with those of one-token commands to
+ * FP32 rounding, not bit for bit. GEMVQ_ARITH_REFERENCE rejects it. A sequence's region (GEMVQ_ATTN_SEQS) starts at a whole record of 32
+ * positions: where n_ctx / n_tok is no multiple of 32, a buffer keeps one number of sequences until gemvq_kv_clear. */
+#define GEMVQ_KV_F16 1
+#define GEMVQ_KV_Q4_0 2
+int gemvq_set_kv_type(gemvq_ctx * ctx, int type);
+/* KV buffer for ATTN: n_ctx positions of n_head_kv x head_dim keys and values. Returns its id (>= 0). */
 int gemvq_kv_create(gemvq_ctx * ctx, int n_ctx, int n_head_kv, int head_dim);
+/* fp16 values (a 4-bit buffer's rounded to it; its positions as the last list compiled for it has them). */
 int gemvq_kv_read(gemvq_ctx * ctx, int kv, int pos0, int npos, uint16_t * k, uint16_t * v);
 int gemvq_kv_clear(gemvq_ctx * ctx);
 

@@ -37,7 +37,8 @@ typedef struct gemvq_qwen35 gemvq_qwen35;
 /* Context sizes a model needs (activation floats, weight bytes, GDN state rows). */
 int gemvq_qwen35_sizes(const gemvq_qw_config * cfg, const gemvq_tensor_desc * table, int n_tensors,
                        size_t * act_floats, size_t * weight_bytes, size_t * state_rows);
-/* Uploads the weights into ctx, allocates KV buffers, lays out the activation buffer and builds the per-token
+/* Uploads the weights into ctx, allocates KV buffers (of the type gemvq_set_kv_type set on ctx; a prompt's chunks and lockstep sequences
+ * on 4-bit ones agree with single steps to rounding, not bit for bit), lays out the activation buffer and builds the per-token
  * command list. Returns NULL on failure (gemvq_last_error(ctx) says why). */
 gemvq_qwen35 * gemvq_qwen35_create(gemvq_ctx * ctx, const gemvq_qw_config * cfg, const gemvq_tensor_desc * table,
                                    int n_tensors, const uint8_t * blob);
@@ -89,6 +90,14 @@ int gemvq_qwen35_batch_reset(gemvq_qwen35 * m, const int32_t * prompts, const in
 /* Sequence seq's token ids at positions 0 .. n - 1; its logits of the last step (n_vocab floats); synchronize. */
 int gemvq_qwen35_batch_tokens(gemvq_qwen35 * m, int seq, int32_t * out, int n);
 int gemvq_qwen35_batch_logits(gemvq_qwen35 * m, int seq, float * out);
+/* Beam search over a batch model (no counterpart in the reference): its sequences become n_seq / n_beam groups of n_beam beams
+ * (sequences g * n_beam + b) from the next gemvq_qwen35_batch_reset on, which then takes the same prompt for all beams of a group. Steps
+ * read the prompt as before, and behind it select the n_beam best continuations of each group (BEAM), let states, conv windows, caches
+ * and ids follow their parents (BEAM_MOVE) and append the new tokens, all in the step's graph. Beams are in descending order of their scores
+ * (sums of the tokens' log probabilities); one whose last token is eos (outside the vocabulary: none) keeps its score, and eos as its next tokens. n_beam 0:
+ * greedy again. gemvq_qwen35_batch_tokens, _logits and _step apply; _scores gives the n_seq scores. 0 or GEMVQ_EINVAL. */
+int gemvq_qwen35_batch_set_beam(gemvq_qwen35 * m, int n_beam, int eos);
+int gemvq_qwen35_batch_scores(gemvq_qwen35 * m, float * out);
 /* The per-token command list gemvq_qwen35_create would build, without a device: weights placed as
  * gemvq_upload_weight places them in table order, KV buffers numbered in layer order. Returns the number of commands
  * (words copied when n_words is large enough), or GEMVQ_EINVAL. */

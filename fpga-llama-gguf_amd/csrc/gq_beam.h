@@ -29,6 +29,7 @@ struct BeamSelectArgs {
     void * work;
     int per;               // set at launch: logits a thread takes in the first kernel
     int chunks;            // set at launch: workgroups a row there
+    unsigned chunk_mul;    // set at launch: list / chunks = the high word of list * chunk_mul (lists below 2^13); 0: one chunk
 };
 size_t beam_work(int n_group, int n_beam, int n_vocab);
 hipError_t launch_beam_select(const BeamSelectArgs & a, hipStream_t s);

@@ -3,6 +3,7 @@
 #include "gq_device.h"
 
 #include <cfloat>
+#include <type_traits>
 
 namespace gq {
 namespace {
@@ -10,9 +11,10 @@ namespace {
 // ---- selection ----
 // Two launches. The first reads every logit once: workgroup (256 * PER logits of a row) forms their maximum m and sum of e^(x - m),
 // and their n_beam best in order. The second, a workgroup per group, joins the rows' sums, and takes the best candidate off the
-// sorted lists n_beam times. Values are 64-bit from the logits on (candidates of two beams may lie next to each other): e^(x - m) as
-// 2^n times a polynomial of degree 9, with an error below 1e-11.
+// sorted lists n_beam times. Values are 64-bit from the logits on (candidates of two beams may lie next to each other).
 // A list entry is one word that orders as the candidates of one row do: the logit's bits made monotone, above the token inverted.
+// 8 groups of 8 beams of 151936 logits (39 MB): 17.9 us (2.2 TB/s, of which 7 us are a workgroup's own way: read, reduce, rank) and 8.8 us, of
+// which n_beam steps of about 0.4 us that wait for one another; one group of 4: 7.4 and 6.4 us, both latency.
 constexpr int BEAM_SLACK = 8;
 
 __device__ __forceinline__ uint32_t order_of(float x) {  // monotone in x, > 0 for every number
@@ -21,21 +23,73 @@ __device__ __forceinline__ uint32_t order_of(float x) {  // monotone in x, > 0 f
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
-// e^t for t <= 0 (t = -inf and below the range: 0).
-__device__ __forceinline__ double beam_exp(double t) {
-    t = fmax(t * 1.4426950408889634, -1100.0);
-    const double n = __builtin_rint(t), r = (t - n) * 0.6931471805599453;
-    double p = 1.0 / 362880;
-    p = __builtin_fma(p, r, 1.0 / 40320);
-    p = __builtin_fma(p, r, 1.0 / 5040);
-    p = __builtin_fma(p, r, 1.0 / 720);
-    p = __builtin_fma(p, r, 1.0 / 120);
-    p = __builtin_fma(p, r, 1.0 / 24);
-    p = __builtin_fma(p, r, 1.0 / 6);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    return __builtin_ldexp(p, int(n));
+// 2^t for -1020 <= t <= 0: t = n + f with |f| <= 1/2, 1 + f q(f) with q interpolating (2^f - 1) / f at 7 Chebyshev points (off by at most
+// 1.2e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of t + 1.5 * 2^52 as its low word.
+__device__ __forceinline__ double beam_exp2(double t) {
+    const double magic = 6755399441055744.0, u = t + magic, f = t - (u - magic);
+    double p = 1.5297323765018243e-05;
+    p = __builtin_fma(p, f, 0.00015461444698569867);
+    p = __builtin_fma(p, f, 0.001333350238614389);
+    p = __builtin_fma(p, f, 0.009618056678524634);
+    p = __builtin_fma(p, f, 0.05550410883909642);
+    p = __builtin_fma(p, f, 0.24022650922288757);
+    p = __builtin_fma(p, f, 0.6931471805599453);
+    p = __builtin_fma(p, f, 1.0);
+    return __hiloint2double(__double2hiint(p) + (__double2loint(u) << 20), __double2loint(p));
+}
+// e^(x - m) for x <= m and m finite; 2^-1010 below that.
+__device__ __forceinline__ double beam_term(float x, float m) {
+    return beam_exp2(fmax((double(x) - double(m)) * 1.4426950408889634, -1010.0));
+}
+
+// log x for 1 <= x < 2^64: the hardware's FP32 logarithm y, and one step from it: x e^-y = 1 + r with r below 1e-6.
+__device__ __forceinline__ double beam_log(double x) {
+    const double y = double(__builtin_amdgcn_logf(float(x))), r = x * beam_exp2(-y) - 1.0;
+    return y * 0.6931471805599453 + r * (1.0 - 0.5 * r);
+}
+
+// Over a wave: by DPP within rows of 16, then across them.
+template <typename F>
+__device__ __forceinline__ uint32_t wave_u32(uint32_t x, F f) {
+    x = f(x, uint32_t(dpp_i32<DPP_XOR1>(int(x))));
+    x = f(x, uint32_t(dpp_i32<DPP_XOR2>(int(x))));
+    x = f(x, uint32_t(dpp_i32<DPP_HALF_MIRROR>(int(x))));
+    x = f(x, uint32_t(dpp_i32<DPP_MIRROR>(int(x))));
+    x = f(x, uint32_t(__shfl_xor(int(x), 16, WAVE)));
+    return f(x, uint32_t(__shfl_xor(int(x), 32, WAVE)));
+}
+template <typename F>
+__device__ __forceinline__ double wave_f64(double x, F f) {
+    const auto step = [&](auto ctrl) { x = f(x, __longlong_as_double(dpp_i64<ctrl.value>(__double_as_longlong(x)))); };
+    step(std::integral_constant<int, DPP_XOR1>());
+    step(std::integral_constant<int, DPP_XOR2>());
+    step(std::integral_constant<int, DPP_HALF_MIRROR>());
+    step(std::integral_constant<int, DPP_MIRROR>());
+    x = f(x, __shfl_xor(x, 16, WAVE));
+    return f(x, __shfl_xor(x, 32, WAVE));
+}
+__device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t min_u(uint32_t a, uint32_t b) { return a < b ? a : b; }
+__device__ __forceinline__ double sum_d(double a, double b) { return a + b; }
+
+// A bound on the wave's monotone words (0: none; low: the smallest, high: the largest): at least k of them are >= it, and no more than k +
+// BEAM_SLACK if equal ones do not forbid that; with fewer than k words: 1. n: how many pass.
+__device__ __forceinline__ uint32_t beam_bound(uint32_t x, int k, uint32_t low, uint32_t high, int & n) {
+    uint32_t lo = 1, hi = high + 1;  // at least k (or all) are >= lo, fewer than k are >= hi
+    n = __popcll(__ballot(x >= 1));
+    if (n <= k + BEAM_SLACK) return lo;
+    if (low) lo = low;
+    while (hi - lo > 1 && n > k + BEAM_SLACK) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const int c = __popcll(__ballot(x >= mid));
+        if (c >= k) {
+            lo = mid;
+            n = c;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
 }
 
 struct BeamStat {
@@ -73,6 +127,22 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), v0 = chunk * CH, cap = (k + BEAM_SLACK) * PER;
     const size_t at = size_t(row) * a.chunks + chunk;
     unsigned long long * out = beam_lists(a) + at * k;
+    const float * x = a.x + size_t(row) * size_t(a.stride);
+    // elements 4 (256 i + tid) + e from the chunk's start; rows start anywhere, so the pieces are brought to 16 bytes. Read before it is
+    // known whether the row takes logits at all, which is a microsecond later
+    const int skew = int((reinterpret_cast<uintptr_t>(x + v0) >> 2) & 3);
+    typedef float f32x4 __attribute__((ext_vector_type(4)));
+    float v[PER];
+#pragma unroll
+    for (int i = 0; i < PER / 4; ++i) {
+        const int t = v0 - skew + 4 * (256 * i + tid);
+        if (t >= v0 && t + 4 <= a.n_vocab) {
+            *reinterpret_cast<f32x4 *>(v + 4 * i) = *reinterpret_cast<const f32x4 *>(x + t);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[4 * i + e] = t + e >= v0 && t + e < a.n_vocab ? x[t + e] : -__builtin_inff();
+        }
+    }
     bool ended;
     int next;
     if (beam_prompted(a, row - row % k, next)) return;  // the group reads its prompt (its first beam says so, here and below)
@@ -86,104 +156,78 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         if (tid == 0) beam_stats(a)[at] = {ended && chunk == 0 ? 0.0f : -__builtin_inff(), 0, ended && chunk == 0 ? 1.0 : 0.0};
         return;
     }
-    const float * x = a.x + size_t(row) * size_t(a.stride);
-    // elements 4 (256 i + tid) + e from the chunk's start; rows start anywhere, so the pieces are brought to 16 bytes
-    const int skew = int((reinterpret_cast<uintptr_t>(x + v0) >> 2) & 3);
-    typedef float f32x4 __attribute__((ext_vector_type(4)));
-    float v[PER];
-#pragma unroll
-    for (int i = 0; i < PER / 4; ++i) {
-        const int t = v0 - skew + 4 * (256 * i + tid);
-        if (t >= v0 && t + 4 <= a.n_vocab) {
-            *reinterpret_cast<f32x4 *>(v + 4 * i) = *reinterpret_cast<const f32x4 *>(x + t);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * i + e] = t + e >= v0 && t + e < a.n_vocab ? x[t + e] : 0.0f;
-        }
-    }
     const auto token_of = [&](int j) { return v0 - skew + 4 * (256 * (j >> 2) + tid) + (j & 3); };
+    const auto real = [&](int j) { return token_of(j) >= v0 && token_of(j) < a.n_vocab; };
     // the last `skew` elements of the chunk are the pieces' overhang: one more each in the first threads
-    float extra = 0.0f;
     const int xt = v0 + CH - skew + tid;
     const bool more = tid < skew && xt < a.n_vocab;
-    if (more) extra = x[xt];
-    uint32_t o[PER];  // monotone bits, 0: no element
-    uint32_t top = 0;
+    float extra = more ? x[xt] : -__builtin_inff();
+    const auto clean = [](float y) { return y == y ? fminf(y, FLT_MAX) : -__builtin_inff(); };
+    float tv = extra = clean(extra);
 #pragma unroll
     for (int j = 0; j < PER; ++j) {
-        const int t = token_of(j);
-        const float y = v[j] == v[j] ? fminf(v[j], FLT_MAX) : -__builtin_inff();
-        v[j] = y;
-        o[j] = t >= v0 && t < a.n_vocab ? order_of(y) : 0;
-        top = max(top, o[j]);
+        v[j] = clean(v[j]);
+        tv = fmaxf(tv, v[j]);
     }
-    extra = extra == extra ? fminf(extra, FLT_MAX) : -__builtin_inff();
-    const uint32_t oe = more ? order_of(extra) : 0;
-    top = max(top, oe);
+    // the lane's best; 0: it has none (its first piece's last three elements may be the first of the chunk)
+    const bool any = max(token_of(0), v0) < a.n_vocab || more;
+    const uint32_t top = any ? order_of(tv) : 0;
     // ---- maximum and sum ----
-    uint32_t wtop = top, wlow = top;
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) {
-        wtop = max(wtop, uint32_t(__shfl_xor(int(wtop), d, WAVE)));
-        wlow = min(wlow, uint32_t(__shfl_xor(int(wlow), d, WAVE)));
-    }
-    wtop = __builtin_amdgcn_readfirstlane(wtop);
-    wlow = __builtin_amdgcn_readfirstlane(wlow);
+    const uint32_t wtop = __builtin_amdgcn_readfirstlane(wave_u32(top, max_u)), wlow = __builtin_amdgcn_readfirstlane(wave_u32(top, min_u));
     const float wm = wtop ? value_of(wtop) : -__builtin_inff();  // each wave's sum is relative to its own maximum
     double sum = 0.0;
     if (wm > -__builtin_inff()) {
 #pragma unroll
-        for (int j = 0; j < PER; ++j) sum += o[j] ? beam_exp(double(v[j]) - double(wm)) : 0.0;
-        if (oe) sum += beam_exp(double(extra) - double(wm));
+        for (int j = 0; j < PER; ++j) sum += beam_term(v[j], wm);
+        if (skew) sum += beam_term(extra, wm);
     }
-#pragma unroll
-    for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, WAVE);
-    // ---- the wave's candidates: a bound that at least k lanes' best pass, and not many more ----
-    uint32_t lo = 1, hi = wtop + 1;  // at least k lanes' best are >= lo (if so many lanes have any), fewer than k are >= hi
-    int n = __popcll(__ballot(top >= 1));
-    if (n > k + BEAM_SLACK) {
-        if (wlow) lo = wlow;
-        while (hi - lo > 1 && n > k + BEAM_SLACK) {
-            const uint32_t mid = lo + (hi - lo) / 2;
-            const int c = __popcll(__ballot(top >= mid));
-            if (c >= k) {
-                lo = mid;
-                n = c;
-            } else {
-                hi = mid;
-            }
-        }
-    }
-    int until = INT_MAX;  // of the elements at the bound itself, the tokens up to this one
-    if (n > k + BEAM_SLACK) {  // many lanes' best are equal: the ones with the lowest tokens
-        int mine = INT_MAX;
-        if (top == lo) {
-            if (oe == lo) mine = xt;
-#pragma unroll
-            for (int j = PER - 1; j >= 0; --j)
-                if (o[j] == lo) mine = token_of(j);
-        }
-        const int above = __popcll(__ballot(top > lo));
-        int l = v0 - 1, h = v0 + CH;  // fewer than k with tokens <= l, at least k with <= h
-        while (h - l > 1) {
-            const int mid = l + (h - l) / 2;
-            if (above + __popcll(__ballot(mine <= mid)) >= k) h = mid;
-            else l = mid;
-        }
-        until = h;
-    }
+    sum = wave_f64(sum, sum_d);
+    // ---- the wave's candidates: those that pass a bound on the lanes' best ----
+    int n;
+    const uint32_t lo = beam_bound(top, k, wlow, wtop, n);
     unsigned long long * mylist = list + wave * cap;
     int have = 0;
-    const auto put = [&](uint32_t ord, int t) {
-        const bool in = ord > lo || (ord == lo && t <= until);
+    const auto put = [&](bool in, float y, int t) {
         const unsigned long long who = __ballot(in);
         if (!who) return;
-        if (in) mylist[have + __popcll(who & ((1ull << lane) - 1))] = (unsigned long long)ord << 32 | uint32_t(~t);
+        if (in) mylist[have + __popcll(who & ((1ull << lane) - 1))] = (unsigned long long)order_of(y) << 32 | uint32_t(~t);
         have += __popcll(who);
     };
+    const uint32_t bottom = order_of(-__builtin_inff());
+    if (n <= k + BEAM_SLACK && lo > bottom) {
+        const float bound = value_of(lo);
 #pragma unroll
-    for (int j = 0; j < PER; ++j) put(o[j], token_of(j));
-    put(oe, xt);
+        for (int j = 0; j < PER; ++j) put(v[j] >= bound, v[j], token_of(j));
+        if (skew) put(extra >= bound, extra, xt);
+    } else {
+        // every element counts, or many lanes' best are equal: of the elements at the bound itself, the tokens up to `until`
+        int until = INT_MAX;
+        if (n > k + BEAM_SLACK) {
+            int mine = INT_MAX;
+            if (top == lo) {
+                if (more && order_of(extra) == lo) mine = xt;
+#pragma unroll
+                for (int j = PER - 1; j >= 0; --j)
+                    if (real(j) && order_of(v[j]) == lo) mine = token_of(j);
+            }
+            const int above = __popcll(__ballot(top > lo));
+            int l = v0 - 1, h = v0 + CH;  // fewer than k with tokens <= l, at least k with <= h
+            while (h - l > 1) {
+                const int mid = l + (h - l) / 2;
+                if (above + __popcll(__ballot(mine <= mid)) >= k) h = mid;
+                else l = mid;
+            }
+            until = h;
+        }
+        const auto passes = [&](float y, int t) { return order_of(y) > lo || (order_of(y) == lo && t <= until); };
+#pragma unroll
+        for (int j = 0; j < PER; ++j) put(real(j) && passes(v[j], token_of(j)), v[j], token_of(j));
+        put(more && passes(extra, xt), extra, xt);
+    }
+    if (lane < 8) {  // up to whole eights of entries
+        const int i = have + lane;
+        if (i < (have + 7) / 8 * 8) mylist[i] = 0;
+    }
     if (lane == 0) {
         red[wave] = wm;
         sums[wave] = sum;
@@ -198,7 +242,13 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         const unsigned long long key = mylist[i];
         int place = 0;
         for (int w = 0; w < 4; ++w)
-            for (int j = 0, c = count[w]; j < c; ++j) place += list[w * cap + j] > key;
+            for (int j = 0, c = count[w]; j < c; j += 8) {
+                unsigned long long y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = list[w * cap + j + e];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) place += y[e] > key;
+            }
         if (place < k) out[place] = key;
     }
     for (int i = all + tid; i < k; i += 256) out[i] = 0;
@@ -206,119 +256,289 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         const float m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         double s = 0.0;
         for (int w = 0; w < 4; ++w)
-            if (red[w] > -__builtin_inff()) s += sums[w] * beam_exp(double(red[w]) - double(m));
+            if (red[w] > -__builtin_inff()) s += sums[w] * beam_term(red[w], m);
         beam_stats(a)[at] = {m, 0, s};
     }
 }
 
-// Workgroup per group. A thread holds the heads of up to 4 of the group's lists.
-template <int T>
-__global__ __launch_bounds__(T) void beam_pick_kernel(BeamSelectArgs a) {
-    constexpr int OWN = 4, W = T / 64;
-    __shared__ double top[BEAM_MAX], logsum[BEAM_MAX], scores[BEAM_MAX];
-    __shared__ double bestv[2][W];
-    __shared__ uint32_t besti[2][W];
-    const int g = blockIdx.x, k = a.n_beam, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lists = k * a.chunks;
-    const size_t first = size_t(g) * k * a.chunks;
+// The second launch's beginning: the rows' maxima, the logarithms of their sums and their scores, 8 to 64 lanes a row. What is read of score
+// and last is read here (score_out and token may be the same memory). False: the group reads its prompt.
+template <int W>
+__device__ __forceinline__ bool beam_rows(const BeamSelectArgs & a, int g, double * top, double * logsum, double * scores) {
+    const int k = a.n_beam, tid = threadIdx.x, lane = tid & 63;
     int ahead;
     if (beam_prompted(a, g * k, ahead)) {  // the group's beams read their prompt
         if (tid < k && beam_prompted(a, g * k + tid, ahead)) {
             a.token[(g * k + tid) * a.slot] = a.prompt[size_t(g * k + tid) * a.cap + ahead];
             a.parent[(g * k + tid) * a.slot] = tid;
         }
-        return;
+        return false;
     }
-    const BeamStat * st = beam_stats(a) + first;
-    const unsigned long long * li = beam_lists(a) + first * k;
-    // the lists' first two entries, while the rows' sums are joined
-    unsigned long long next[OWN], head[OWN];
-    int taken[OWN];
-#pragma unroll
-    for (int i = 0; i < OWN; ++i) {
-        const int l = tid + i * T;
-        head[i] = l < lists ? li[size_t(l) * k] : 0;
-        next[i] = l < lists && k > 1 ? li[size_t(l) * k + 1] : 0;
-        taken[i] = 2;
-    }
-    for (int b = wave; b < k; b += W) {
+    const BeamStat * st = beam_stats(a) + size_t(g) * k * a.chunks;
+    const int sh = a.chunks > 32 ? 6 : a.chunks > 16 ? 5 : a.chunks > 8 ? 4 : 3, each = 64 >> sh;
+    const auto over = [&](auto x, auto f, auto get) {  // over a row's lanes
+        x = f(x, get(x, std::integral_constant<int, DPP_XOR1>()));
+        x = f(x, get(x, std::integral_constant<int, DPP_XOR2>()));
+        x = f(x, get(x, std::integral_constant<int, DPP_HALF_MIRROR>()));
+        if (sh > 3) x = f(x, get(x, std::integral_constant<int, DPP_MIRROR>()));
+        if (sh > 4) x = f(x, __shfl_xor(x, 16, WAVE));
+        if (sh > 5) x = f(x, __shfl_xor(x, 32, WAVE));
+        return x;
+    };
+    for (int b0 = 0; b0 < k; b0 += W * each) {
+        const int b = b0 + (tid >> 6) * each + (lane >> sh), c1 = lane & ((1 << sh) - 1);
+        const float sc = b < k ? a.score[(g * k + b) * a.slot] : 0.0f;
+        BeamStat x[2];
         float m = -__builtin_inff();
-        for (int c = lane; c < a.chunks; c += 64) m = fmaxf(m, st[b * a.chunks + c].m);
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) m = fmaxf(m, __shfl_xor(m, d, WAVE));
         double s = 0.0;
-        if (m > -__builtin_inff())
-            for (int c = lane; c < a.chunks; c += 64) s += st[b * a.chunks + c].sum * beam_exp(double(st[b * a.chunks + c].m) - double(m));
+        for (int c0 = c1; c0 < a.chunks + c1; c0 += 2 << sh) {  // (once but for more than 128 chunks)
 #pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) s += __shfl_xor(s, d, WAVE);
-        if (lane == 0) {
-            const float sc = a.score[(g * k + b) * a.slot];
-            top[b] = m;
-            logsum[b] = log(s);
+            for (int i = 0; i < 2; ++i) {
+                const int c = c0 + (i << sh);
+                x[i] = b < k && c < a.chunks ? st[b * a.chunks + c] : BeamStat{-__builtin_inff(), 0, 0.0};
+            }
+            const float m1 = fmaxf(m, fmaxf(x[0].m, x[1].m));
+            if (m1 > -__builtin_inff()) s = (m > -__builtin_inff() ? s * beam_term(m, m1) : 0.0) + x[0].sum * beam_term(x[0].m, m1) + x[1].sum * beam_term(x[1].m, m1);
+            m = m1;
+        }
+        const float wm = over(m, [](float y, float z) { return fmaxf(y, z); }, [](float y, auto c) { return dpp_f32<c.value>(y); });
+        s = over(m > -__builtin_inff() ? s * beam_term(m, wm) : 0.0, sum_d,
+                 [](double y, auto c) { return __longlong_as_double(dpp_i64<c.value>(__double_as_longlong(y))); });
+        if (c1 == 0 && b < k) {
+            top[b] = wm;
+            logsum[b] = beam_log(s);
             scores[b] = sc == sc ? double(sc) : -__builtin_inf();
         }
     }
-    __syncthreads();  // (score_out and token may be score and last: everything of them has been read)
-    const auto value = [&](unsigned long long e, int b) {
-        const float x = value_of(uint32_t(e >> 32));
-        return x > -__builtin_inff() && scores[b] > -__builtin_inf() ? scores[b] + ((double(x) - top[b]) - logsum[b]) : -__builtin_inf();
-    };
-    double v[OWN];
-    uint32_t id[OWN];  // beam * n_vocab + token; all ones: the list is empty
-    const auto show = [&](int i, int b) {
-        v[i] = value(head[i], b);
-        id[i] = head[i] ? uint32_t(b) * uint32_t(a.n_vocab) + ~uint32_t(head[i]) : 0xffffffffu;
-    };
-#pragma unroll
-    for (int i = 0; i < OWN; ++i) show(i, (tid + i * T) / a.chunks < k ? (tid + i * T) / a.chunks : 0);
-    for (int j = 0; j < k; ++j) {
-        double bv = v[0];
-        uint32_t bi = id[0];
-        const auto better = [](double v2, uint32_t i2, double v1, uint32_t i1) { return i2 != 0xffffffffu && (i1 == 0xffffffffu || v2 > v1 || (v2 == v1 && i2 < i1)); };
-#pragma unroll
-        for (int i = 1; i < OWN; ++i)
-            if (better(v[i], id[i], bv, bi)) {
-                bv = v[i];
-                bi = id[i];
-            }
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) {
-            const double v2 = __shfl_xor(bv, d, WAVE);
-            const uint32_t i2 = uint32_t(__shfl_xor(int(bi), d, WAVE));
-            if (better(v2, i2, bv, bi)) {
-                bv = v2;
-                bi = i2;
-            }
+    __syncthreads();
+    return true;
+}
+
+// The beam of a list.
+__device__ __forceinline__ int beam_of(const BeamSelectArgs & a, int list) {
+    return min(a.chunk_mul ? int(__umulhi(unsigned(list), a.chunk_mul)) : list, a.n_beam - 1);
+}
+
+// A list entry's value.
+__device__ __forceinline__ double beam_value(unsigned long long e, int b, const double * top, const double * logsum, const double * scores) {
+    const float x = value_of(uint32_t(e >> 32));
+    return x > -__builtin_inff() && scores[b] > -__builtin_inf() ? scores[b] + ((double(x) - top[b]) - logsum[b]) : -__builtin_inf();
+}
+constexpr uint32_t BEAM_NONE = 0xffffffffu;  // beam * n_vocab + token of an empty list's head
+
+// The lists' first `depth` entries in LDS as values and indexes, formed by all threads at once. Lists of which more is taken are read
+// further from memory (a microsecond each).
+constexpr int BEAM_LDS = 4096;  // entries: one at least of each list
+struct BeamLists {
+    const unsigned long long * li;
+    double * v;
+    uint32_t * id;
+    const double * top, * logsum, * scores;
+    int k, depth;
+
+    __device__ __forceinline__ void form(const BeamSelectArgs & a, unsigned long long e, int l, double & value, uint32_t & index) const {
+        const int b = beam_of(a, l);
+        value = e ? beam_value(e, b, top, logsum, scores) : -__builtin_inf();
+        index = e ? uint32_t(b) * uint32_t(a.n_vocab) + ~uint32_t(e) : BEAM_NONE;
+    }
+    __device__ __forceinline__ void at(const BeamSelectArgs & a, int l, int i, double & value, uint32_t & index) const {
+        if (i < depth) {
+            value = v[l * depth + i];
+            index = id[l * depth + i];
+        } else {
+            form(a, i < k ? li[size_t(l) * k + i] : 0, l, value, index);
         }
+    }
+};
+struct BeamShared {
+    double v[BEAM_LDS], top[BEAM_MAX], logsum[BEAM_MAX], scores[BEAM_MAX], won[BEAM_MAX];
+    uint32_t id[BEAM_LDS], taken[BEAM_MAX];
+};
+// False: the group reads its prompt.
+template <int T>
+__device__ __forceinline__ bool beam_fetch(const BeamSelectArgs & a, int g, BeamShared & sh, BeamLists & out) {
+    const int k = a.n_beam, lists = k * a.chunks, depth = min(k, BEAM_LDS / lists), n = lists * depth;
+    const unsigned long long * li = beam_lists(a) + size_t(g) * lists * k;
+    out = {li, sh.v, sh.id, sh.top, sh.logsum, sh.scores, k, depth};
+    constexpr int AHEAD = BEAM_LDS / T < 8 ? BEAM_LDS / T : 8;  // reads in flight a thread, beside the rows' sums
+    unsigned long long x[AHEAD];
+    const auto where = [&](int i) { return depth == k ? i : i / depth * k + i % depth; };
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+        const int i = threadIdx.x + e * T;
+        x[e] = i < n ? li[where(i)] : 0;
+    }
+    if (!beam_rows<T / 64>(a, g, sh.top, sh.logsum, sh.scores)) return false;
+#pragma unroll
+    for (int e = 0; e < AHEAD; ++e) {
+        const int i = threadIdx.x + e * T;
+        if (i < n) out.form(a, x[e], i / depth, sh.v[i], sh.id[i]);
+    }
+    for (int i = threadIdx.x + AHEAD * T; i < n; i += T) out.form(a, li[where(i)], i / depth, sh.v[i], sh.id[i]);
+    __syncthreads();
+    return true;
+}
+
+// The winners, written at the end (a store in a step would be waited for in the next one's reads).
+__device__ __forceinline__ void beam_write(const BeamSelectArgs & a, int g, const BeamShared & sh, int j) {
+    const uint32_t b = sh.taken[j] / uint32_t(a.n_vocab);
+    const int to = (g * a.n_beam + j) * a.slot;
+    a.score_out[to] = float(sh.won[j]);
+    a.token[to] = int32_t(sh.taken[j] - b * uint32_t(a.n_vocab));
+    a.parent[to] = int32_t(b);
+}
+
+__device__ __forceinline__ bool beam_better(double v2, uint32_t i2, double v1, uint32_t i1) { return v2 > v1 || (v2 == v1 && i2 < i1); }
+
+// The best of N heads, as a tree.
+template <int N>
+__device__ __forceinline__ void beam_best(const double * v, const uint32_t * id, double & bv, uint32_t & bi) {
+    if constexpr (N == 1) {
+        bv = v[0];
+        bi = id[0];
+    } else {
+        double v2;
+        uint32_t i2;
+        beam_best<N / 2>(v, id, bv, bi);
+        beam_best<N - N / 2>(v + N / 2, id + N / 2, v2, i2);
+        const bool other = beam_better(v2, i2, bv, bi);
+        bv = other ? v2 : bv;
+        bi = other ? i2 : bi;
+    }
+}
+
+// The wave's largest value, in every lane (by DPP alone: the rows of 16 upwards, then row 15 into the next and 31 into the upper half).
+__device__ __forceinline__ double wave_best(double x) {
+    const auto step = [&](auto ctrl, auto rows) {
+        const long long y = __double_as_longlong(x);
+        const int lo = __builtin_amdgcn_update_dpp(int(y), int(y), ctrl.value, rows.value, 0xf, false);
+        const int hi = __builtin_amdgcn_update_dpp(int(y >> 32), int(y >> 32), ctrl.value, rows.value, 0xf, false);
+        x = fmax(x, __hiloint2double(hi, lo));
+    };
+    using std::integral_constant;
+    step(integral_constant<int, 0x111>(), integral_constant<int, 0xf>());  // row_shr:1, 2, 4, 8
+    step(integral_constant<int, 0x112>(), integral_constant<int, 0xf>());
+    step(integral_constant<int, 0x114>(), integral_constant<int, 0xf>());
+    step(integral_constant<int, 0x118>(), integral_constant<int, 0xf>());
+    step(integral_constant<int, 0x142>(), integral_constant<int, 0xa>());  // row_bcast:15 into rows 1 and 3
+    step(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());  // row_bcast:31 into rows 2 and 3
+    const long long y = __double_as_longlong(x);
+    return __hiloint2double(__builtin_amdgcn_readlane(int(y >> 32), 63), __builtin_amdgcn_readlane(int(y), 63));
+}
+
+// Orders a wave's LDS writes before its other lanes' reads (a wave's LDS operations are carried out in order).
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// Workgroup per group of up to 64 * OWN lists: after the rows' sums its first wave alone, one winner a step. A lane holds the heads of OWN
+// lists, the best of them and, read ahead, what follows it in its list.
+template <int OWN>
+__global__ __launch_bounds__(256) void beam_pick_wave_kernel(BeamSelectArgs a) {
+    __shared__ BeamShared sh;
+    const int g = blockIdx.x, k = a.n_beam, tid = threadIdx.x, lists = k * a.chunks;
+    BeamLists li;
+    if (!beam_fetch<256>(a, g, sh, li) || tid >= 64) return;
+    double v[OWN], bv, nv;
+    uint32_t id[OWN], bi, ni;
+    int taken[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+        taken[i] = 0;
+        v[i] = -__builtin_inf();
+        id[i] = BEAM_NONE;
+        if (tid + 64 * i < lists) li.at(a, tid + 64 * i, 0, v[i], id[i]);
+    }
+    const auto best = [&] {
+        beam_best<OWN>(v, id, bv, bi);
+        int l = 0, t = 0;
+#pragma unroll
+        for (int i = 0; i < OWN; ++i)
+            if (id[i] == bi) {
+                l = tid + 64 * i;
+                t = taken[i];
+            }
+        nv = -__builtin_inf();
+        ni = BEAM_NONE;
+        if (bi != BEAM_NONE) li.at(a, l, t + 1, nv, ni);
+    };
+    best();
+    for (int j = 0; j < k; ++j) {
+        const double wv = wave_best(bv);
+        const unsigned long long who = __ballot(bv == wv);
+        uint32_t wi;
+        if (__popcll(who) == 1) {
+            wi = uint32_t(__builtin_amdgcn_readlane(int(bi), __ffsll(who) - 1));
+        } else {  // equal values: the lowest index
+            wi = __builtin_amdgcn_readfirstlane(wave_u32(bv == wv ? bi : BEAM_NONE, min_u));
+        }
+        if (bi == wi) {
+            sh.won[j] = wv;
+            sh.taken[j] = wi;
+#pragma unroll
+            for (int i = 0; i < OWN; ++i)
+                if (id[i] == wi) {
+                    ++taken[i];
+                    v[i] = nv;
+                    id[i] = ni;
+                }
+            best();
+        }
+    }
+    wave_lds();
+    if (tid < k) beam_write(a, g, sh, tid);
+}
+
+// More lists: sixteen waves, a thread the heads of up to 4 lists.
+__global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelectArgs a) {
+    constexpr int OWN = 4, T = 1024, W = T / 64;
+    __shared__ BeamShared sh;
+    __shared__ double bestv[2][W];
+    __shared__ uint32_t besti[2][W];
+    const int g = blockIdx.x, k = a.n_beam, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lists = k * a.chunks;
+    BeamLists li;
+    if (!beam_fetch<T>(a, g, sh, li)) return;
+    double v[OWN];
+    uint32_t id[OWN];
+    int taken[OWN];
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+        taken[i] = 0;
+        v[i] = -__builtin_inf();
+        id[i] = BEAM_NONE;
+        if (tid + i * T < lists) li.at(a, tid + i * T, 0, v[i], id[i]);
+    }
+    for (int j = 0; j < k; ++j) {
+        double bv;
+        uint32_t bi;
+        beam_best<OWN>(v, id, bv, bi);
+        const double wv = wave_best(bv);
+        const uint32_t wi = wave_u32(bv == wv ? bi : BEAM_NONE, min_u);
         if (lane == 0) {
-            bestv[j & 1][wave] = bv;
-            besti[j & 1][wave] = bi;
+            bestv[j & 1][wave] = wv;
+            besti[j & 1][wave] = wi;
         }
         __syncthreads();
         bv = bestv[j & 1][0];
         bi = besti[j & 1][0];
 #pragma unroll
         for (int w = 1; w < W; ++w)
-            if (better(bestv[j & 1][w], besti[j & 1][w], bv, bi)) {
+            if (beam_better(bestv[j & 1][w], besti[j & 1][w], bv, bi)) {
                 bv = bestv[j & 1][w];
                 bi = besti[j & 1][w];
             }
         if (tid == 0) {
-            const uint32_t b = bi / uint32_t(a.n_vocab);
-            const int to = (g * k + j) * a.slot;
-            a.score_out[to] = float(bv);
-            a.token[to] = int32_t(bi - b * uint32_t(a.n_vocab));
-            a.parent[to] = int32_t(b);
+            sh.won[j] = bv;
+            sh.taken[j] = bi;
         }
 #pragma unroll
         for (int i = 0; i < OWN; ++i)
-            if (id[i] == bi) {  // taken: the list's next entry becomes its head
-                const int l = tid + i * T;
-                head[i] = next[i];
-                next[i] = taken[i] < k ? li[size_t(l) * k + taken[i]] : 0;
-                ++taken[i];
-                show(i, l / a.chunks);
-            }
+            if (id[i] == bi) li.at(a, tid + i * T, ++taken[i], v[i], id[i]);  // the list's next entry becomes its head
     }
+    __syncthreads();
+    if (tid < k) beam_write(a, g, sh, tid);
 }
 
 // ---- reordering ----
@@ -376,32 +596,45 @@ __global__ void beam_next_kernel(BeamNextArgs a) {
     a.pos[16 * s] = p;
 }
 
-// Logits a thread of the first kernel takes: 32, or 8 where that gives too few workgroups to read at the memory's rate.
-int beam_per(int rows, int n_vocab) { return (long long)rows * ((n_vocab + 8191) / 8192) >= 512 ? 32 : 8; }
 // (a chunk's first piece may start up to 3 elements before it, so 256 * per elements and 3 more are read by a workgroup)
 int beam_chunks(int n_vocab, int per) { return (n_vocab + 256 * per - 1) / (256 * per); }
+// Logits a thread of the first kernel takes: 8, the shorter way through one workgroup, or 32 where those would give the second kernel 192
+// lists a group or the first more workgroups than the device holds at once. Both kernels with 8 and 32: 10.2 and 11.6 us at one group of 4 of
+// 32000, 10.5 and 11.3 at one of 2 of 151936, 15.4 and 18.0 at 70 of 8 of 4000; 12.8 and 12.2 at one of 4 of 151936, 17.8 and 15.6 at one of 12
+// of 32000, 17.0 and 14.9 at 20 of 5 of 32003, 41.4 and 26.4 at 8 of 8 of 151936.
+int beam_per(int n_group, int n_beam, int n_vocab) {
+    const int lists = n_beam * beam_chunks(n_vocab, 8);
+    return lists >= 192 || (long long)n_group * lists >= 1536 ? 32 : 8;
+}
 
 }  // namespace
 
 size_t beam_work(int n_group, int n_beam, int n_vocab) {
     const long long rows = (long long)n_group * n_beam;
-    const int per = beam_per(int(rows), n_vocab);
+    const int per = beam_per(n_group, n_beam, n_vocab);
     return size_t(rows) * beam_chunks(n_vocab, per) * (sizeof(BeamStat) + 8 * size_t(n_beam));
 }
 
 hipError_t launch_beam_select(const BeamSelectArgs & args, hipStream_t s) {
     BeamSelectArgs a = args;
     const int rows = a.n_group * a.n_beam;
-    a.per = beam_per(rows, a.n_vocab);
+    a.per = beam_per(a.n_group, a.n_beam, a.n_vocab);
     a.chunks = beam_chunks(a.n_vocab, a.per);
+    a.chunk_mul = a.chunks > 1 ? unsigned((0x100000000ull + unsigned(a.chunks) - 1) / unsigned(a.chunks)) : 0;
     const unsigned lds = unsigned((a.n_beam + BEAM_SLACK) * a.per * 4 * sizeof(unsigned long long));
     const dim3 grid(unsigned(a.chunks), unsigned(rows));
     if (a.per == 32) GQ_LAUNCH(beam_scan_kernel<32>, grid, dim3(256), lds, s, a);
     else GQ_LAUNCH(beam_scan_kernel<8>, grid, dim3(256), lds, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (a.n_beam * a.chunks <= 1024) GQ_LAUNCH(beam_pick_kernel<256>, dim3(unsigned(a.n_group)), dim3(256), 0, s, a);
-    else GQ_LAUNCH(beam_pick_kernel<1024>, dim3(unsigned(a.n_group)), dim3(1024), 0, s, a);
+    // lists of a group: at most 32 * 128. A second kernel for up to 128, 320 and 640 lists and for more, us with the next one in its place: 12.5 and
+    // 13.9 at 128 lists of 8 winners, 12.8 and 14.3 at 300 of 4, 56 and 74 at 608 of 32.
+    const int lists = a.n_beam * a.chunks;
+    const dim3 groups(unsigned(a.n_group));
+    if (lists <= 64 * 2) GQ_LAUNCH(beam_pick_wave_kernel<2>, groups, dim3(256), 0, s, a);
+    else if (lists <= 64 * 5) GQ_LAUNCH(beam_pick_wave_kernel<5>, groups, dim3(256), 0, s, a);
+    else if (lists <= 64 * 10) GQ_LAUNCH(beam_pick_wave_kernel<10>, groups, dim3(256), 0, s, a);
+    else GQ_LAUNCH(beam_pick_kernel, groups, dim3(1024), 0, s, a);
     return hipGetLastError();
 }
 

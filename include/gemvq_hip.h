@@ -360,7 +360,7 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
  * Selection: candidate v of beam b has the value score[b] + logit[b][v] - log(sum of e^logit[b]), formed in 64 bits; the n_beam best
  * candidates of a group, in descending order: score_out (rounded to FP32), token, and parent (the beam in the group it
  * continues); of equal ones the lower b * n_vocab + v first (among one beam's logits, the larger logit first). A beam whose last token (last[row], or
- * last NULL) is eos has ended: it has the one candidate eos, at its score, and its logits are not read; eos outside the vocabulary: none ends.
+ * last NULL) is eos has ended: it has the one candidate eos, at its score, whatever its logits (which are there all the same); eos outside the vocabulary: none ends.
  * A beam with score -inf (the beams after the first, at a search's start) has no candidates before all others'. NaN logits and scores count as -inf, +inf logits
  * as the largest finite number. logits: FP32 rows row_stride >= n_vocab floats apart, 1 <= n_vocab <= GEMVQ_BEAM_MAX_VOCAB, 4-byte
  * aligned. score_out may be score, token may be last. work: gemvq_beam_work() bytes, 16-byte aligned, contents do not matter. */

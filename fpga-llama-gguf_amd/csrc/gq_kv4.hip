@@ -199,9 +199,10 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 
 // ---- attention ----
 // A wave takes the rows (token, q head) of one KV head 16 at a time (NQ such groups) and records of 32 positions one after another:
-//   S^T = K Q^T   16x16x32 fp16 matrix instructions, a block of 32 elements each: the quants minus 8 are whole numbers, exact in fp16;
-//                 the query, scaled to its row's largest element, is the sum of two fp16 numbers (22 bits). Each block's sums are
-//                 multiplied by its scales in FP32.
+//   S^T = K Q^T   16x16x32 fp16 matrix instructions, a block of 32 elements each: the quants' bits as they are, 2^-24 n (2^-20 n in high
+//                 nibbles) as fp16, exact; the accumulator begins at -8 times the sum of the block's query elements. The query, scaled
+//                 to its row's largest element, is the sum of two fp16 numbers (22 bits). Each block's sums are multiplied by its
+//                 scales in FP32.
 //   P = 2^(S - c) in FP32, c = m - 7 with m the query's running maximum, taken anew only when a score passes it by 8 (so P < 2^15).
 //                 P is the sum of two fp16 numbers, whole multiples of 2^-24 (2^-31 of the largest weight). Lane 16 g + q holds
 //                 query q's weights of the 8 positions that it feeds to
@@ -323,7 +324,12 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t & hi, uint32_t
     lo = pack2(__builtin_fmaf(half_of(hi, 0), k.minus, a), __builtin_fmaf(half_of(hi, 1), k.minus, b));
 }
 
-// The 8 nibbles of four bytes minus 8, as fp16: low nibbles of bytes 0, 2, 1, 3, then the high ones.
+// The 8 nibbles of four bytes as fp16: low nibbles of bytes 0, 2, 1, 3 times 2^-24, then the high ones times 2^-20.
+__device__ __forceinline__ u32x4 nibbles_raw(uint32_t w, const Kv4Const & k) {
+    const uint32_t x = w >> 8;
+    return {w & k.m0, x & k.m0, w & k.m1, x & k.m1};
+}
+// The 8 nibbles minus 8, in the same order.
 __device__ __forceinline__ u32x4 nibbles(uint32_t w, const Kv4Const & k) {
     const half2 c0 = {_Float16(-1032.0f), _Float16(-1032.0f)}, c1 = {_Float16(-72.0f), _Float16(-72.0f)};
     const uint32_t x = w >> 8;
@@ -446,8 +452,9 @@ __device__ __forceinline__ void kv4_out(const Kv4AttnArgs & a, size_t row, int h
     *reinterpret_cast<f32x4 *>(a.y + row * size_t(a.y_row) + size_t(hq) * HD + e) = y;
 }
 
+// (three waves a SIMD where the registers can be kept to that: 32 sequences of up to 8192, 32/8 heads of 128, 52 us, 58 with two)
 template <int HD, int NQ>
-__global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(256, HD * NQ <= 128 ? 3 : 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     constexpr int NB = HD / 32, ROWS = 16 * NQ;
     // Blocks of 32 elements that the waves' sums are joined in at a time; threads of a row there.
     constexpr int JB = NQ == 1 ? NB : 1, PAD = 32 * JB + 4, JT = 256 / ROWS;
@@ -456,11 +463,13 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     u32x4(*ql)[64] = reinterpret_cast<u32x4(*)[64]>(both);              // the queries' parts
     float(*part)[ROWS][PAD] = reinterpret_cast<float(*)[ROWS][PAD]>(both);  // later the waves' sums
     constexpr bool QL = HD * NQ > 128;  // the queries stay in LDS where registers would not leave room for two waves a SIMD
-    __shared__ float kqs[ROWS], cs[4][ROWS], ls[4][ROWS];
+    __shared__ float kqs[ROWS], qsum[NB][ROWS], cs[4][ROWS], ls[4][ROWS];
     __shared__ __align__(16) uint32_t scales[4][HD];  // a wave's record's key scales, then its value scales: [g][block][8] each
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
-    const int G = a.group, h = blockIdx.y, row0 = blockIdx.x * ROWS;  // rows of the KV head: token row / G, q head row % G
-    const int range = blockIdx.z;
+    // Workgroup (KV head, group of rows behind it | range): the groups of one KV head, which read the same records, stay on an XCD or
+    // a few. Rows of the KV head: token row / G, q head row % G
+    const int G = a.group, h = int(unsigned(blockIdx.x) % unsigned(a.c.n_head_kv)), row0 = int(unsigned(blockIdx.x) / unsigned(a.c.n_head_kv)) * ROWS;
+    const int range = blockIdx.y;
     int s = 0;
     Kv4Range r;
     if (!kv4_find<true>(a, range, s, r)) return;
@@ -512,11 +521,17 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int piece = (pc + 16 * i) & (HD / 4 - 1), to = (piece & 3) * 16 + (tid >> 4);  // 8 block + 4 half + g
+            float sum = (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
+            sum += dpp_f32<DPP_XOR1>(sum);
+            sum += dpp_f32<DPP_XOR2>(sum);
+            sum += dpp_f32<DPP_HALF_MIRROR>(sum);
+            if ((piece & 7) == 0) qsum[piece >> 3][n * 16 + (tid >> 4)] = sum * up * -0x1p-21f;
+            const float up2 = piece & 4 ? up * 0.0625f : up;  // high nibbles are 16 times theirs
             u32x2 hi2, lo2;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 uint32_t hw, lw;
-                split2(x[i][k] * up, x[i][k + 2] * up, hw, lw, k4);
+                split2(x[i][k] * up2, x[i][k + 2] * up2, hw, lw, k4);
                 hi2[k] = hw;
                 lo2[k] = lw;
             }
@@ -528,6 +543,7 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
     __syncthreads();
     u32x4 q[QL ? 1 : NQ][QL ? 1 : NB][2];
     float kq[NQ];  // what brings the products back: scale * log2(e) over the row's power of two
+    f32x4 s0[NQ][NB];  // -8 times the sums of the query's blocks
     int my_lo[NQ], my_hi[NQ];
     f32x4 o[NQ][NB][2];
     float c[NQ], l[NQ];
@@ -537,12 +553,15 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
         const bool ok = t >= t_lo && t <= t_hi;
         my_hi[n] = ok ? p0 + t : -1;
         my_lo[n] = ok && a.window ? p0 + t - a.window + 1 : 0;
-        kq[n] = kqs[n * 16 + col];
+        kq[n] = kqs[n * 16 + col] * 0x1p24f;
         c[n] = KV4_LOW;
         l[n] = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             o[n][b][0] = o[n][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            const float y = qsum[b][n * 16 + col];
+            s0[n][b] = f32x4{y, y, y, y};
+            __asm__("" : "+v"(s0[n][b]));  // (four registers, not four copies in every record)
             if constexpr (!QL) {
                 q[n][b][0] = ql[(n * NB + b) * 2][lane];
                 q[n][b][1] = ql[(n * NB + b) * 2 + 1][lane];
@@ -598,10 +617,10 @@ __global__ __launch_bounds__(256, 2) void kv4_attn_kernel(Kv4AttnArgs a) {
                 const u32x4 kd = *reinterpret_cast<const u32x4 *>(&scales[wave][(g * NB + b) * 4]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const u32x4 kk = nibbles(tile.k[u][b], k4);
+                    const u32x4 kk = nibbles_raw(tile.k[u][b], k4);
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
-                        f32x4 x = mfma(kk, QL ? ql[(n * NB + b) * 2][lane] : q[QL ? 0 : n][QL ? 0 : b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                        f32x4 x = mfma(kk, QL ? ql[(n * NB + b) * 2][lane] : q[QL ? 0 : n][QL ? 0 : b][0], s0[n][b]);
                         x = mfma(kk, QL ? ql[(n * NB + b) * 2 + 1][lane] : q[QL ? 0 : n][QL ? 0 : b][1], x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[n][u][i] = __builtin_fmaf(x[i], half_of(kd[2 * u + (i & 1)], i >> 1), acc[n][u][i]);
@@ -848,7 +867,7 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
     const int per_kv = a.n_head / a.c.n_head_kv, nq = kv4_nq(a.c.head_dim, a.t.n_tok, per_kv);
     a.ranges = a.work ? kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head) : a.t.n_seq;
     a.group = per_kv;
-    const dim3 grid(unsigned((a.t.n_tok * (long long)per_kv + 16 * nq - 1) / (16 * nq)), unsigned(a.c.n_head_kv), unsigned(a.ranges));
+    const dim3 grid(unsigned((a.t.n_tok * (long long)per_kv + 16 * nq - 1) / (16 * nq) * a.c.n_head_kv), unsigned(a.ranges));
     return by_dim(a.c.head_dim, [&](auto hd) {
         if (nq == 1) GQ_LAUNCH((kv4_attn_kernel<hd.value, 1>), grid, dim3(256), 0, s, a);
         if constexpr (hd.value < 256)

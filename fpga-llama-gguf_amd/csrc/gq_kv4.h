@@ -80,6 +80,11 @@ struct Kv4AttnArgs {
 // 32768, 16/4 heads of 256, 21.5 / 26.2 / 26.4 / 26.2; 32 sequences of up to 8192, 32/8 heads of 128, 78 / 58 / 55 / 56).
 constexpr int KV4_GROUPS = 1536, KV4_GROUPS_256 = 512;
 constexpr int KV4_LEAST = 4;      // records of a range at least: one a wave
+// Records times head_dim up to which a cache's sequences are not split, which needs no second launch: its waves' few records more take less than
+// joining. Half as many where the cache is longer, but no sequence in it (us whole, whole with the second launch, and split: one sequence of
+// 320, 16/4 heads of 256, 12.7 / 14.2 / 12.8; 4 of 1500 19.7 / - / 13.8; 32 of 256, 32/8 heads of 128, 10.2 / 13.3 / 16.6; 7 of 5 tokens in a window
+// of 1000, 8 heads of 64, - / 14.3 / 13.3).
+constexpr int KV4_ALONE = 2048;
 bool kv4_joins(const Kv4AttnArgs & a);  // the launch is followed by that of kv4_join_kernel
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head);
 

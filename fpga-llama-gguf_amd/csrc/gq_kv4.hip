@@ -369,10 +369,11 @@ __device__ __forceinline__ void kv4_seen(const Kv4AttnArgs & a, Kv4Range & r) {
     r.tiles = int((hi - 1) / KV4_TILE) - r.first + 1;
 }
 
-// The ranges' length: all records over the ranges that the grid has room for, a sequence's last one being short.
-__device__ __forceinline__ int kv4_per(long long records, int ranges, int n_seq, int most) {
+// The ranges' length: all records over the ranges that the grid has room for, a sequence's last one being short. `most`: the longest
+// sequence's records; up to half of KV4_ALONE, each sequence stays one range.
+__device__ __forceinline__ int kv4_per(long long records, int ranges, int n_seq, int most, int hd) {
     int per = most;
-    if (ranges > n_seq) {
+    if (ranges > n_seq && most > KV4_ALONE / 2 / hd) {
         if (n_seq == 1) per = int((unsigned(records) + unsigned(ranges) - 1u) / unsigned(ranges));
         else per = int(ceil(double(records) / double(ranges - n_seq)));  // (quotients below 2^27 with fractions of at least 2^-16)
     }
@@ -387,7 +388,7 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int &
         s = 0;
         kv4_span(a.t, 0, r.p0, r.n);
         kv4_seen(a, r);
-        r.per = kv4_per(r.tiles, a.ranges, 1, r.tiles);
+        r.per = kv4_per(r.tiles, a.ranges, 1, r.tiles, a.c.head_dim);
         r.slot = 0;
         return (long long)(BY_RANGE ? range : 0) * r.per < r.tiles;
     }
@@ -410,7 +411,7 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int &
         sum += __shfl_xor(sum, d, WAVE);
         most = max(most, __shfl_xor(most, d, WAVE));
     }
-    const int per = kv4_per(sum, a.ranges, a.t.n_seq, most);
+    const int per = kv4_per(sum, a.ranges, a.t.n_seq, most, a.c.head_dim);
     int before = 0;
     for (int i0 = 0; i0 < a.t.n_seq; i0 += 64) {
         if (a.t.n_seq > 64) look(i0 + lane);  // (up to 64 sequences: as they are)
@@ -847,8 +848,9 @@ static int kv4_nq(int hd, int n_tok, int per_kv) {
 }
 
 // How many ranges a call's records are dealt to: as many as give KV4_GROUPS workgroups in all (KV4_GROUPS_256 for heads of 256), but at
-// least one range a sequence, and no more than KV4_LEAST records each give.
+// least one range a sequence, and no more than KV4_LEAST records each give; one a sequence where no position needs more.
 int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
+    if (kv4_tiles(c.n_ctx) <= KV4_ALONE / c.head_dim) return n_seq;
     const int per_kv = n_head / c.n_head_kv, rows = 16 * kv4_nq(c.head_dim, n_tok, per_kv);
     const long long units = (n_tok * (long long)per_kv + rows - 1) / rows * c.n_head_kv;
     const long long most = (long long)n_seq * ((kv4_tiles(c.n_ctx) + KV4_LEAST - 1) / KV4_LEAST);

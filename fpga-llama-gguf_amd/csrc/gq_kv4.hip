@@ -199,10 +199,11 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 
 // ---- attention ----
 // A wave takes the rows (token, q head) of one KV head 16 at a time (NQ such groups) and records of 32 positions one after another:
-//   S^T = K Q^T   16x16x32 fp16 matrix instructions, a block of 32 elements each: the quants' bits as they are, 2^-24 n (2^-20 n in high
-//                 nibbles) as fp16, exact; the accumulator begins at -8 times the sum of the block's query elements. The query, scaled
-//                 to its row's largest element, is the sum of two fp16 numbers (22 bits). Each block's sums are multiplied by its
-//                 scales in FP32.
+//   S^T = K Q^T   16x16x32 fp16 matrix instructions, a block of 32 elements each: the quants minus 8 are whole numbers, exact in fp16;
+//                 the query, scaled to its row's largest element, is the sum of two fp16 numbers (22 bits). Each block's sums are
+//                 multiplied by its scales in FP32. (The quants' bits as they are, 2^-24 n, with the 8 taken off through the
+//                 accumulator's start, are a tenth fewer vector instructions, but the instruction's sums of such small factors keep
+//                 several bits less: results are off by 5e-6 in place of 3e-7.)
 //   P = 2^(S - c) in FP32, c = m - 7 with m the query's running maximum, taken anew only when a score passes it by 8 (so P < 2^15).
 //                 P is the sum of two fp16 numbers, whole multiples of 2^-24 (2^-31 of the largest weight). Lane 16 g + q holds
 //                 query q's weights of the 8 positions that it feeds to
@@ -324,12 +325,7 @@ __device__ __forceinline__ void split2(float a, float b, uint32_t & hi, uint32_t
     lo = pack2(__builtin_fmaf(half_of(hi, 0), k.minus, a), __builtin_fmaf(half_of(hi, 1), k.minus, b));
 }
 
-// The 8 nibbles of four bytes as fp16: low nibbles of bytes 0, 2, 1, 3 times 2^-24, then the high ones times 2^-20.
-__device__ __forceinline__ u32x4 nibbles_raw(uint32_t w, const Kv4Const & k) {
-    const uint32_t x = w >> 8;
-    return {w & k.m0, x & k.m0, w & k.m1, x & k.m1};
-}
-// The 8 nibbles minus 8, in the same order.
+// The 8 nibbles of four bytes minus 8, as fp16: low nibbles of bytes 0, 2, 1, 3, then the high ones.
 __device__ __forceinline__ u32x4 nibbles(uint32_t w, const Kv4Const & k) {
     const half2 c0 = {_Float16(-1032.0f), _Float16(-1032.0f)}, c1 = {_Float16(-72.0f), _Float16(-72.0f)};
     const uint32_t x = w >> 8;
@@ -464,7 +460,7 @@ __global__ __launch_bounds__(256, HD * NQ <= 128 ? 3 : 2) void kv4_attn_kernel(K
     u32x4(*ql)[64] = reinterpret_cast<u32x4(*)[64]>(both);              // the queries' parts
     float(*part)[ROWS][PAD] = reinterpret_cast<float(*)[ROWS][PAD]>(both);  // later the waves' sums
     constexpr bool QL = HD * NQ > 128;  // the queries stay in LDS where registers would not leave room for two waves a SIMD
-    __shared__ float kqs[ROWS], qsum[NB][ROWS], cs[4][ROWS], ls[4][ROWS];
+    __shared__ float kqs[ROWS], cs[4][ROWS], ls[4][ROWS];
     __shared__ __align__(16) uint32_t scales[4][HD];  // a wave's record's key scales, then its value scales: [g][block][8] each
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
     // Workgroup (KV head, group of rows behind it | range): the groups of one KV head, which read the same records, stay on an XCD or
@@ -522,17 +518,11 @@ __global__ __launch_bounds__(256, HD * NQ <= 128 ? 3 : 2) void kv4_attn_kernel(K
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int piece = (pc + 16 * i) & (HD / 4 - 1), to = (piece & 3) * 16 + (tid >> 4);  // 8 block + 4 half + g
-            float sum = (x[i][0] + x[i][1]) + (x[i][2] + x[i][3]);
-            sum += dpp_f32<DPP_XOR1>(sum);
-            sum += dpp_f32<DPP_XOR2>(sum);
-            sum += dpp_f32<DPP_HALF_MIRROR>(sum);
-            if ((piece & 7) == 0) qsum[piece >> 3][n * 16 + (tid >> 4)] = sum * up * -0x1p-21f;
-            const float up2 = piece & 4 ? up * 0.0625f : up;  // high nibbles are 16 times theirs
             u32x2 hi2, lo2;
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
                 uint32_t hw, lw;
-                split2(x[i][k] * up2, x[i][k + 2] * up2, hw, lw, k4);
+                split2(x[i][k] * up, x[i][k + 2] * up, hw, lw, k4);
                 hi2[k] = hw;
                 lo2[k] = lw;
             }
@@ -544,7 +534,6 @@ __global__ __launch_bounds__(256, HD * NQ <= 128 ? 3 : 2) void kv4_attn_kernel(K
     __syncthreads();
     u32x4 q[QL ? 1 : NQ][QL ? 1 : NB][2];
     float kq[NQ];  // what brings the products back: scale * log2(e) over the row's power of two
-    f32x4 s0[NQ][NB];  // -8 times the sums of the query's blocks
     int my_lo[NQ], my_hi[NQ];
     f32x4 o[NQ][NB][2];
     float c[NQ], l[NQ];
@@ -554,15 +543,12 @@ __global__ __launch_bounds__(256, HD * NQ <= 128 ? 3 : 2) void kv4_attn_kernel(K
         const bool ok = t >= t_lo && t <= t_hi;
         my_hi[n] = ok ? p0 + t : -1;
         my_lo[n] = ok && a.window ? p0 + t - a.window + 1 : 0;
-        kq[n] = kqs[n * 16 + col] * 0x1p24f;
+        kq[n] = kqs[n * 16 + col];
         c[n] = KV4_LOW;
         l[n] = 0.0f;
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             o[n][b][0] = o[n][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            const float y = qsum[b][n * 16 + col];
-            s0[n][b] = f32x4{y, y, y, y};
-            __asm__("" : "+v"(s0[n][b]));  // (four registers, not four copies in every record)
             if constexpr (!QL) {
                 q[n][b][0] = ql[(n * NB + b) * 2][lane];
                 q[n][b][1] = ql[(n * NB + b) * 2 + 1][lane];
@@ -618,10 +604,10 @@ __global__ __launch_bounds__(256, HD * NQ <= 128 ? 3 : 2) void kv4_attn_kernel(K
                 const u32x4 kd = *reinterpret_cast<const u32x4 *>(&scales[wave][(g * NB + b) * 4]);
 #pragma unroll
                 for (int u = 0; u < 2; ++u) {
-                    const u32x4 kk = nibbles_raw(tile.k[u][b], k4);
+                    const u32x4 kk = nibbles(tile.k[u][b], k4);
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
-                        f32x4 x = mfma(kk, QL ? ql[(n * NB + b) * 2][lane] : q[QL ? 0 : n][QL ? 0 : b][0], s0[n][b]);
+                        f32x4 x = mfma(kk, QL ? ql[(n * NB + b) * 2][lane] : q[QL ? 0 : n][QL ? 0 : b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
                         x = mfma(kk, QL ? ql[(n * NB + b) * 2 + 1][lane] : q[QL ? 0 : n][QL ? 0 : b][1], x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[n][u][i] = __builtin_fmaf(x[i], half_of(kd[2 * u + (i & 1)], i >> 1), acc[n][u][i]);

@@ -124,7 +124,7 @@ def test_attention(gq, hip, nh, nkv, hd, n_tok, first, window):
 
 
 @pytest.mark.gpu
-@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("nh,nkv,hd", [(8, 2, 128), (4, 1, 256), (6, 3, 64), (4, 2, 32)])
 def test_attention_long_and_ragged(gq, hip, nh, nkv, hd):
     """Sequences of very unlike lengths in one call, one not in use, one past its end, one with a single position."""
     n_ctx, n_tok = 9000, 3
@@ -155,6 +155,22 @@ def test_attention_ranges(gq, hip, what):
         v *= np.float32(50000)
     else:
         v[0, 17] *= np.float32(10000)
+    kv, _ = _cache(gq, hip, 1, n, nkv, hd)
+    _store(gq, hip, kv, k, v, [0])
+    y = _attend(gq, hip, kv, q, [n - 1], None, 0, hd ** -0.5)
+    _check(q, ref.values(k), ref.values(v), y, [n - 1], [1], 0, hd ** -0.5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd", [64, 256])
+def test_keys_with_an_outlier_channel(gq, hip, hd):
+    """One key channel far above the others of its block, which become zeros, and small in the queries."""
+    nh, nkv, n = 4, 2, 200
+    rng = np.random.default_rng(16)
+    k, v = _data(rng, 1, n, nkv, hd)
+    q = rng.standard_normal((1, 1, nh, hd)).astype(np.float32)
+    k[..., 5::32] *= 100
+    q[..., 5::32] *= np.float32(0.01)
     kv, _ = _cache(gq, hip, 1, n, nkv, hd)
     _store(gq, hip, kv, k, v, [0])
     y = _attend(gq, hip, kv, q, [n - 1], None, 0, hd ** -0.5)
@@ -249,6 +265,12 @@ def test_refusals(gq):
         bad += [dict(work=0), dict(work=P + 8), dict(nw=lib.gemvq_kv4_attn_work(kv(), 4, 4) - 1)]
     for b in bad:
         a = {**attn, **b}
+        assert lib.gemvq_kv4_attn_static(*[a[n] for n in attn], 0) == gq.EINVAL, b
+    long = dict(attn, kv=kv(n_ctx=4096))
+    need = lib.gemvq_kv4_attn_work(long["kv"], 4, 4)
+    assert need > 0 and lib.gemvq_kv4_attn_work(kv(), 4, 4) == 0  # 64 positions: one range a sequence
+    for b in (dict(work=0), dict(work=P + 8), dict(nw=need - 1)):
+        a = {**long, **b}
         assert lib.gemvq_kv4_attn_static(*[a[n] for n in attn], 0) == gq.EINVAL, b
     with pytest.raises(gq.GemvqError):
         gq.kv4_store_static(kv(), P, P, 100, 1, P)

@@ -472,7 +472,8 @@ __global__ __launch_bounds__(256, HD * NQ <= 128 ? 3 : 2) void kv4_attn_kernel(K
     if (!kv4_find<true>(a, range, s, r)) return;
     s = __builtin_amdgcn_readfirstlane(s);
     const int p0 = __builtin_amdgcn_readfirstlane(int(r.p0));
-    const int live = min(__builtin_amdgcn_readfirstlane(r.n), a.c.n_ctx - p0);  // tokens -p0 (where p0 < 0) .. live - 1 have positions
+    // tokens -p0 (where p0 < 0) .. live - 1 have positions
+    const int live = int(min((long long)__builtin_amdgcn_readfirstlane(r.n), (long long)a.c.n_ctx - p0));
     const int t_lo = max(int(unsigned(row0) / unsigned(G)), -p0), t_hi = min(int(unsigned(row0 + ROWS - 1) / unsigned(G)), live - 1);
     if (t_lo > t_hi) return;
     // the group's positions: lo .. hi, the rows' own ranges within them

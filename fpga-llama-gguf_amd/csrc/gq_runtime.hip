@@ -17,6 +17,8 @@
 #include <cstdlib>
 #include <cstring>
 #include <map>
+#include <memory>
+#include <new>
 #include <string>
 #include <thread>
 #include <variant>
@@ -1837,12 +1839,12 @@ hipError_t issue(const std::vector<Launch> & ls, hipStream_t s) {
 // Positions pos0 .. pos0 + npos - 1 of a 4-bit buffer, as fp16 (the values rounded). Position p is position p % region of region
 // p / region; a region's records start at a whole record.
 template <int HD>
-void kv4_unpack(const std::vector<uint8_t> & rec, size_t rec0, const KvBuf & b, int h, int pos0, int npos, uint16_t * k, uint16_t * v) {
+void kv4_unpack(const uint8_t * rec, size_t rec0, const KvBuf & b, int h, int pos0, int npos, uint16_t * k, uint16_t * v) {
     using L = Kv4Layout<HD>;
     const size_t per = size_t(kv4_tiles(b.region));
     for (int i = 0; i < npos; ++i) {
         const int r = (pos0 + i) / b.region, q = (pos0 + i) % b.region, p = q % KV4_TILE;
-        const uint8_t * x = rec.data() + (r * per + size_t(q / KV4_TILE) - rec0) * L::RECORD;
+        const uint8_t * x = rec + (r * per + size_t(q / KV4_TILE) - rec0) * L::RECORD;
         for (int e = 0; e < HD; ++e) {
             const int blk = e / 32, up = (e & 16) ? 4 : 0;
             const size_t to = (size_t(i) * b.n_head_kv + h) * HD + e;
@@ -1865,11 +1867,17 @@ int kv4_read(gemvq_ctx * c, const KvBuf & b, int pos0, int npos, uint16_t * k, u
     const size_t per = size_t(kv4_tiles(b.region)), rec = kv4_record(b.head_dim);
     const auto at = [&](int p) { return size_t(p / b.region) * per + size_t(p % b.region) / KV4_TILE; };
     const size_t r0 = at(pos0), r1 = at(pos0 + npos - 1) + 1;
-    std::vector<uint8_t> buf((r1 - r0) * rec);
+    const size_t bytes = (r1 - r0) * rec;
+    const std::unique_ptr<uint8_t[]> mem(new (std::nothrow) uint8_t[bytes]);
+    uint8_t * buf = mem.get();
+    if (!buf) {
+        c->err = "gemvq_kv_read: no host memory";
+        return -int(hipErrorOutOfMemory);
+    }
     for (int h = 0; h < b.n_head_kv; ++h) {
         if (const int w = drain(c, "kv read")) return w;
         c->busy = true;
-        const hipError_t e = hipMemcpyAsync(buf.data(), b.q4 + (h * b.q4_records + r0) * rec, buf.size(), hipMemcpyDeviceToHost, c->stream);
+        const hipError_t e = hipMemcpyAsync(buf, b.q4 + (h * b.q4_records + r0) * rec, bytes, hipMemcpyDeviceToHost, c->stream);
         if (const int w = e == hipSuccess ? wait_stream(c, "kv read") : fail(c, e, "kv read")) return w;
         switch (b.head_dim) {
         case 32: kv4_unpack<32>(buf, r0, b, h, pos0, npos, k, v); break;
@@ -2469,8 +2477,7 @@ int gemvq_profile(gemvq_ctx * c, const uint32_t * cmds, unsigned n, int reps, ge
     // the token position (attention bytes depend on it): the first ATTN's pos operand
     int pos = 0;
     if (const int w = drain(c, "profile")) return w;
-    for (const Launch & l : ls)
-    {
+    for (const Launch & l : ls) {
         const auto * x = std::get_if<LAttn>(&l);
         const auto * x4 = std::get_if<LAttn4>(&l);
         if (x || x4) {

@@ -55,6 +55,11 @@ bool kv4_sizes_ok(const gemvq_kv4 * c) {
     return c && c->n_seq > 0 && c->n_seq <= GRID_MAX && c->n_ctx > 0 && c->n_head_kv > 0 && c->n_head_kv <= GRID_MAX &&
            kv4_dim_ok(c->head_dim);
 }
+// Query rows of a sequence: their workgroups fit a grid.
+bool kv4_heads_ok(const gemvq_kv4 * c, int n_tok, int n_head) {
+    return n_tok >= 1 && n_tok <= GEMVQ_KV4_MAX_TOK && n_head >= 1 && n_head <= GRID_MAX && n_head % c->n_head_kv == 0 &&
+           int64_t(n_tok) * n_head <= GEMVQ_KV4_MAX_ROWS;
+}
 bool kv4_ok(const gemvq_kv4 * c) { return kv4_sizes_ok(c) && c->data && aligned(c->data, 256); }
 
 Kv4Cache kv4_cache(const gemvq_kv4 * c) {
@@ -152,8 +157,7 @@ int gemvq_kv4_load_static(const gemvq_kv4 * kv, float * k, float * v, int64_t ro
 }
 
 uint64_t gemvq_kv4_attn_work(const gemvq_kv4 * kv, int n_tok, int n_head) {
-    if (!kv4_sizes_ok(kv) || n_tok < 1 || n_tok > GEMVQ_KV4_MAX_TOK || n_head < 1 || n_head > GRID_MAX || n_head % kv->n_head_kv)
-        return 0;
+    if (!kv4_sizes_ok(kv) || !kv4_heads_ok(kv, n_tok, n_head)) return 0;
     return kv4_work_floats(kv4_cache(kv), kv->n_seq, n_tok, n_head) * sizeof(float);
 }
 
@@ -162,7 +166,7 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
                           float scale, void * work, uint64_t work_bytes, void * stream) {
     Kv4AttnArgs a{};
     if (!kv4_ok(kv) || !kv4_tokens(kv, n_tok, pos, num, a.t)) return GEMVQ_EINVAL;
-    if (n_head < 1 || n_head > GRID_MAX || n_head % kv->n_head_kv || window < 0) return GEMVQ_EINVAL;
+    if (!kv4_heads_ok(kv, n_tok, n_head) || window < 0) return GEMVQ_EINVAL;
     const uint64_t need = gemvq_kv4_attn_work(kv, n_tok, n_head);
     if (work_bytes < need || (need && (!work || !aligned(work, 16)))) return GEMVQ_EINVAL;
     const int64_t hd = kv->head_dim;

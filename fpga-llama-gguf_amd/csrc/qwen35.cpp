@@ -74,6 +74,7 @@ struct gemvq_qwen35 {
     // beam search (gemvq_qwen35_batch_set_beam): beams of a group (0: greedy), the eos id, the positions that a group's beams share (the
     // shortest prompt's), and per sequence its score and parent slots
     int n_beam = 0, eos = -1, shared = 0;
+    bool beams_changed = false;  // since the last reset, which the steps then wait for
     uint32_t sscore = 0, sparent = 0;
 };
 
@@ -660,6 +661,7 @@ int gemvq_qwen35_prefill(gemvq_qwen35 * m, int n) {
 
 int gemvq_qwen35_step(gemvq_qwen35 * m, int n) {
     if (!m) return GEMVQ_EINVAL;
+    if (m->beams_changed) return set_err(m->ctx, "gemvq_qwen35_step: gemvq_qwen35_batch_set_beam takes a reset first");
     if (m->graph < 0) {
         const int st = gemvq_graph_create(m->ctx, m->cmds.data(), unsigned(m->cmds.size() / GEMVQ_CMD_WORDS), &m->graph);
         if (st) return st;
@@ -727,6 +729,7 @@ int gemvq_qwen35_batch_reset(gemvq_qwen35 * m, const int32_t * prompts, const in
             st = st ? st : rebuild_batch(m);
         }
     }
+    if (!st) m->beams_changed = false;
     return st;
 }
 
@@ -737,6 +740,7 @@ int gemvq_qwen35_batch_set_beam(gemvq_qwen35 * m, int n_beam, int eos) {
     m->n_beam = n_beam;
     m->eos = eos;
     m->shared = 0;
+    m->beams_changed = true;
     return rebuild_batch(m);
 }
 

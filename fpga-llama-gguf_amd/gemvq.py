@@ -359,7 +359,9 @@ def beam_select_static(logits: int, row_stride: int, n_vocab: int, n_group: int,
 
 
 def beam_reorder_static(arrays, parent: int, n_group: int, n_beam: int, stream: int = 0) -> None:
-    """In each of the arrays (a ctypes array of BeamArray), row i of every group becomes a copy of its row parent[i]."""
+    """In each of the arrays (BeamArray), row i of every group becomes a copy of its row parent[i]."""
+    if not isinstance(arrays, C.Array):
+        arrays = (BeamArray * len(arrays))(*arrays)
     _ok(hip_lib().gemvq_beam_reorder_static(arrays, len(arrays), parent, n_group, n_beam, stream), "beam reordering")
 
 

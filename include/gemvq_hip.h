@@ -332,6 +332,7 @@ int gemvq_gemm_static(int type, int rows, int cols, const void * w, const float 
  * multiples of 4 and no smaller than a row. Outputs do not overlap inputs.
  * Status: 0, GEMVQ_EINVAL (nothing launched) or a negated HIP error. */
 #define GEMVQ_KV4_MAX_TOK 65535
+#define GEMVQ_KV4_MAX_ROWS (1 << 27) /* n_tok * n_head of an attention */
 typedef struct {
     void * data;
     int32_t n_seq, n_ctx, n_head_kv, head_dim;
@@ -361,7 +362,7 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
  * candidates of a group, in descending order: score_out (rounded to FP32), token, and parent (the beam in the group it
  * continues); of equal ones the lower b * n_vocab + v first (among one beam's logits, the larger logit first). A beam whose last token (last[row], or
  * last NULL) is eos has ended: it has the one candidate eos, at its score, whatever its logits (which are there all the same); eos outside the vocabulary: none ends.
- * A beam with score -inf (the beams after the first, at a search's start) has no candidates before all others'. NaN logits and scores count as -inf, +inf logits
+ * The candidates of a beam with score -inf (the beams after the first, at a search's start) come after all others. NaN logits and scores count as -inf, +inf logits
  * as the largest finite number. logits: FP32 rows row_stride >= n_vocab floats apart, 1 <= n_vocab <= GEMVQ_BEAM_MAX_VOCAB, 4-byte
  * aligned. score_out may be score, token may be last. work: gemvq_beam_work() bytes, 16-byte aligned, contents do not matter. */
 #define GEMVQ_BEAM_MAX 32

@@ -361,8 +361,12 @@ def test_beam_refusals_of_the_model(gq, q35):
             with pytest.raises(gq.GemvqError):
                 bm.set_beam(n)
         bm.set_beam(2)
+        with pytest.raises(gq.GemvqError, match="reset first"):
+            bm.step(1)
         with pytest.raises(gq.GemvqError, match="same prompt"):
             bm.reset([[1, 2], [1, 3], [4], [4]])
+        with pytest.raises(gq.GemvqError, match="reset first"):
+            bm.step(1)
         bm.reset([[1, 2], [1, 2], [4], [4]])
         bm.step(3)
         bm.set_beam(0)  # greedy again

@@ -140,6 +140,23 @@ def test_attention_long_and_ragged(gq, hip, nh, nkv, hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n_seq,n_ctx", [(64, 600), (65, 90), (150, 600)])
+def test_attention_of_many_sequences(gq, hip, n_seq, n_ctx):
+    """More sequences than a wave looks at in one go, some without tokens, with one range or several each."""
+    nh, nkv, hd = 4, 2, 128
+    rng = np.random.default_rng(n_seq)
+    k, v = _data(rng, n_seq, n_ctx, nkv, hd)
+    q = rng.standard_normal((n_seq, 2, nh, hd)).astype(np.float32)
+    kv, _ = _cache(gq, hip, n_seq, n_ctx, nkv, hd)
+    _store(gq, hip, kv, k, v, [0] * n_seq)
+    for most in (n_ctx, 40):
+        pos = [int(p) for p in rng.integers(-1, most, n_seq)]
+        num = [int(n) for n in rng.integers(0, 3, n_seq)]
+        y = _attend(gq, hip, kv, q, pos, num, 0, hd ** -0.5)
+        _check(q, ref.values(k), ref.values(v), y, pos, num, 0, hd ** -0.5)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("what", ["large scores", "tiny values", "huge values", "one value block far above"])
 def test_attention_ranges(gq, hip, what):
     """Scores of hundreds, value scales at both ends of fp16's range, and one position whose values dwarf the others'."""
@@ -266,6 +283,8 @@ def test_refusals(gq):
     for b in bad:
         a = {**attn, **b}
         assert lib.gemvq_kv4_attn_static(*[a[n] for n in attn], 0) == gq.EINVAL, b
+    a = dict(attn, n_tok=1 << 15, nh=1 << 13, ys=64 << 13)  # 2^28 query rows
+    assert lib.gemvq_kv4_attn_static(*[a[n] for n in attn], 0) == gq.EINVAL
     long = dict(attn, kv=kv(n_ctx=4096))
     need = lib.gemvq_kv4_attn_work(long["kv"], 4, 4)
     assert need > 0 and lib.gemvq_kv4_attn_work(kv(), 4, 4) == 0  # 64 positions: one range a sequence

@@ -32,7 +32,8 @@ def reference(x, score, last, eos, groups, beams):
     out = []
     for g in range(groups):
         flat = c[g * beams:(g + 1) * beams].ravel()
-        out.append(np.argsort(-flat, kind="stable")[:beams])
+        some = np.flatnonzero(flat >= np.partition(flat, -beams)[-beams])
+        out.append(some[np.argsort(-flat[some], kind="stable")[:beams]])
     flat = np.stack(out)
     val = np.take_along_axis(c.reshape(groups, -1), flat, 1)
     return val, flat % v, flat // v
@@ -66,7 +67,7 @@ def check(got, want):
 @pytest.mark.gpu
 @pytest.mark.parametrize("groups,beams,v", [(1, 1, 1), (1, 1, 7), (2, 3, 5), (1, 4, 2047), (1, 4, 2048), (2, 4, 2049), (3, 5, 8193),
                                             (1, 32, 40), (2, 32, 5000), (16, 8, 40001), (600, 1, 300), (1, 2, 1 << 20),
-                                            (1, 32, 151936)])
+                                            (1, 32, 151936), (1, 32, 300001), (2, 8, 1 << 20), (1, 32, 1 << 20)])
 @pytest.mark.parametrize("skew", [0, 1, 3])
 def test_selection(gq, hip, groups, beams, v, skew):
     print(f"[beam selection] {groups} x {beams} of {v}, skew {skew}", flush=True)
@@ -83,7 +84,7 @@ def test_selection(gq, hip, groups, beams, v, skew):
 @pytest.mark.gpu
 @pytest.mark.parametrize("what", ["equal", "few values", "ascending", "descending", "masked", "all masked", "one left", "start",
                                   "dead", "all ended", "nan", "inf", "extremes", "spikes"])
-@pytest.mark.parametrize("beams,v", [(4, 5000), (32, 9000), (1, 100)])
+@pytest.mark.parametrize("beams,v", [(4, 5000), (32, 9000), (1, 100), (8, 60000), (24, 230000)])
 def test_selection_at_the_edges(gq, hip, what, beams, v):
     """The groups' beams share their logits, so equal candidates are equal bits and their order is that of the indexes."""
     print(f"[beam selection] {what}, {beams} of {v}", flush=True)

@@ -13,8 +13,9 @@ namespace {
 // and their n_beam best in order. The second, a workgroup per group, joins the rows' sums, and takes the best candidate off the
 // sorted lists n_beam times. Values are 64-bit from the logits on (candidates of two beams may lie next to each other).
 // A list entry is one word that orders as the candidates of one row do: the logit's bits made monotone, above the token inverted.
-// 8 groups of 8 beams of 151936 logits (39 MB): 17.9 us (2.2 TB/s, of which 7 us are a workgroup's own way: read, reduce, rank) and 8.8 us, of
-// which n_beam steps of about 0.4 us that wait for one another; one group of 4: 7.4 and 6.4 us, both latency.
+// 8 groups of 8 beams of 151936 logits (39 MB): 17.0 us (2.3 TB/s: a workgroup's own way of read, reduce and rank is 7 us, the 64-bit
+// exponentials another 5, partly behind the reads) and 8.5 us, of which n_beam steps of about 0.4 us that wait for one another; one group
+// of 4: 7.4 and 4.7 us, both latency.
 constexpr int BEAM_SLACK = 8;
 
 __device__ __forceinline__ uint32_t order_of(float x) {  // monotone in x, > 0 for every number
@@ -24,9 +25,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {  // monotone in x, > 0 f
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
 // 2^t for -1020 <= t <= 0: t = n + f with |f| <= 1/2, 1 + f q(f) with q interpolating (2^f - 1) / f at 7 Chebyshev points (off by at most
-// 1.2e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of t + 1.5 * 2^52 as its low word.
-__device__ __forceinline__ double beam_exp2(double t) {
-    const double magic = 6755399441055744.0, u = t + magic, f = t - (u - magic);
+// 1.2e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of u = t + 1.5 * 2^52 as its low word.
+__device__ __forceinline__ double beam_poly(double f, double u) {
     double p = 1.5297323765018243e-05;
     p = __builtin_fma(p, f, 0.00015461444698569867);
     p = __builtin_fma(p, f, 0.001333350238614389);
@@ -37,10 +37,17 @@ __device__ __forceinline__ double beam_exp2(double t) {
     p = __builtin_fma(p, f, 1.0);
     return __hiloint2double(__double2hiint(p) + (__double2loint(u) << 20), __double2loint(p));
 }
-// e^(x - m) for x <= m and m finite; 2^-1010 below that.
-__device__ __forceinline__ double beam_term(float x, float m) {
-    return beam_exp2(fmax((double(x) - double(m)) * 1.4426950408889634, -1010.0));
+__device__ __forceinline__ double beam_exp2(double t) {
+    const double magic = 6755399441055744.0, u = t + magic;
+    return beam_poly(t - (u - magic), u);
 }
+// e^(x - m) for x <= m and m finite; below m - 700, and for NaN, e^-700. As beam_exp2, with the multiplication by log2(e) in both of its sums.
+__device__ __forceinline__ double beam_term(float x, double m, double low) {
+    constexpr double magic = 6755399441055744.0, log2e = 1.4426950408889634;
+    const double d = fmax(double(x) - m, low), u = __builtin_fma(d, log2e, magic);
+    return beam_poly(__builtin_fma(d, log2e, magic - u), u);
+}
+__device__ __forceinline__ double beam_term(float x, float m) { return beam_term(x, double(m), -700.0); }
 
 // log x for 1 <= x < 2^64: the hardware's FP32 logarithm y, and one step from it: x e^-y = 1 + r with r below 1e-6.
 __device__ __forceinline__ double beam_log(double x) {
@@ -163,12 +170,20 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     const bool more = tid < skew && xt < a.n_vocab;
     float extra = more ? x[xt] : -__builtin_inff();
     const auto clean = [](float y) { return y == y ? fminf(y, FLT_MAX) : -__builtin_inff(); };
-    float tv = extra = clean(extra);
+    float tv = extra;
 #pragma unroll
-    for (int j = 0; j < PER; ++j) {
-        v[j] = clean(v[j]);
-        tv = fmaxf(tv, v[j]);
+    for (int j = 0; j < PER; ++j) tv = fmaxf(tv, v[j]);
+    const auto clean_all = [&] {
+        __asm__ volatile("");  // (a branch of its own: not done ahead of it and selected)
+        extra = clean(extra);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = clean(v[j]);
+    };
+    if (__any(tv == __builtin_inff())) {
+        clean_all();
+        tv = fminf(tv, FLT_MAX);
     }
+    tv = clean(tv);  // (NaN: the lane has no number; the others pass maxima and terms by)
     // the lane's best; 0: it has none (its first piece's last three elements may be the first of the chunk)
     const bool any = max(token_of(0), v0) < a.n_vocab || more;
     const uint32_t top = any ? order_of(tv) : 0;
@@ -200,6 +215,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         for (int j = 0; j < PER; ++j) put(v[j] >= bound, v[j], token_of(j));
         if (skew) put(extra >= bound, extra, xt);
     } else {
+        clean_all();
         // every element counts, or many lanes' best are equal: of the elements at the bound itself, the tokens up to `until`
         int until = INT_MAX;
         if (n > k + BEAM_SLACK) {

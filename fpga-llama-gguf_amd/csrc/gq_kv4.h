@@ -75,10 +75,12 @@ struct Kv4AttnArgs {
     int group;           // set at launch: n_head / n_head_kv
 };
 
-// Workgroups that a call's records are dealt to, where they are enough. Heads of 256: as many as are resident (two a CU), each with few
-// records; the others: two rounds of what is resident, which evens out (us at 512 / 1024 / 1536 / 2048, stores included: one sequence of
-// 32768, 16/4 heads of 256, 21.5 / 26.2 / 26.4 / 26.2; 32 sequences of up to 8192, 32/8 heads of 128, 78 / 58 / 55 / 56).
-constexpr int KV4_GROUPS = 1536, KV4_GROUPS_256 = 512;
+// Workgroups of the attention a CU holds at once (nq groups of 16 query rows each): three where the registers can be kept to that (32 sequences of
+// up to 8192, 32/8 heads of 128: 52 us, 58 with two). A call's records are dealt to as many as the device holds, each with its share: twice as
+// many, each with half of it, are 21.6 us in place of 19.9 (4 sequences of 8192, 32/8 heads of 128), 27.7 and 23.3 (8 of 5 tokens at 8000,
+// 32/8 heads of 64), 30.7 and 24.7 (8 of 8 tokens, 16/4 heads of 128); 26.2 and 21.5 (one of 32768, 16/4 heads of 256).
+__host__ __device__ constexpr int kv4_resident(int hd, int nq) { return hd * nq <= 128 ? 3 : 2; }
+constexpr int KV4_GROUPS = 768;   // at most
 constexpr int KV4_LEAST = 4;      // records of a range at least: one a wave
 // Records times head_dim up to which a cache's sequences are not split, which needs no second launch: its waves' few records more take less than
 // joining. Half as many where the cache is longer, but no sequence in it (us whole, whole with the second launch, and split: one sequence of

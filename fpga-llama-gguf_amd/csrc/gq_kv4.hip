@@ -365,6 +365,17 @@ __device__ __forceinline__ void kv4_seen(const Kv4AttnArgs & a, Kv4Range & r) {
     r.tiles = int((hi - 1) / KV4_TILE) - r.first + 1;
 }
 
+// A wave's sum (DPP: the rows of 16 upwards, then row 15 into the next and 31 into the upper half).
+__device__ __forceinline__ int wave_total(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);  // row_shr:1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast:15 into rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast:31 into rows 2 and 3
+    return __builtin_amdgcn_readlane(x, 63);
+}
+
 // The ranges' length: all records over the ranges that the grid has room for, a sequence's last one being short. `most`: the longest
 // sequence's records; up to half of KV4_ALONE, each sequence stays one range.
 __device__ __forceinline__ int kv4_per(long long records, int ranges, int n_seq, int most, int hd) {
@@ -407,7 +418,17 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int &
         sum += __shfl_xor(sum, d, WAVE);
         most = max(most, __shfl_xor(most, d, WAVE));
     }
-    const int per = kv4_per(sum, a.ranges, a.t.n_seq, most, a.c.head_dim);
+    int per = kv4_per(sum, a.ranges, a.t.n_seq, most, a.c.head_dim);
+    // That leaves room for a short range of every sequence; less will do. Worth its 0.3 us where the sequences are many (32 of up to 8192,
+    // 32/8 heads of 128: 53.0 and 58.2 us).
+    if (a.t.n_seq <= 64 && 8 * a.t.n_seq > a.ranges && per < most) {
+        int low = max(int((sum + a.ranges - 1) / a.ranges), KV4_LEAST);
+        for (int i = 0; i < 4 && low < per; ++i) {
+            const int mid = (low + per) >> 1;
+            if (wave_total(int(unsigned(x.tiles + mid - 1) / unsigned(mid))) <= a.ranges) per = mid;
+            else low = mid + 1;
+        }
+    }
     int before = 0;
     for (int i0 = 0; i0 < a.t.n_seq; i0 += 64) {
         if (a.t.n_seq > 64) look(i0 + lane);  // (up to 64 sequences: as they are)
@@ -449,9 +470,8 @@ __device__ __forceinline__ void kv4_out(const Kv4AttnArgs & a, size_t row, int h
     *reinterpret_cast<f32x4 *>(a.y + row * size_t(a.y_row) + size_t(hq) * HD + e) = y;
 }
 
-// (three waves a SIMD where the registers can be kept to that: 32 sequences of up to 8192, 32/8 heads of 128, 52 us, 58 with two)
 template <int HD, int NQ>
-__global__ __launch_bounds__(256, HD * NQ <= 128 ? 3 : 2) void kv4_attn_kernel(Kv4AttnArgs a) {
+__global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4AttnArgs a) {
     constexpr int NB = HD / 32, ROWS = 16 * NQ;
     // Blocks of 32 elements that the waves' sums are joined in at a time; threads of a row there.
     constexpr int JB = NQ == 1 ? NB : 1, PAD = 32 * JB + 4, JT = 256 / ROWS;
@@ -834,14 +854,15 @@ static int kv4_nq(int hd, int n_tok, int per_kv) {
     return rows <= 16 || hd == 256 ? 1 : rows <= 32 || hd == 128 ? 2 : 4;
 }
 
-// How many ranges a call's records are dealt to: as many as give KV4_GROUPS workgroups in all (KV4_GROUPS_256 for heads of 256), but at
-// least one range a sequence, and no more than KV4_LEAST records each give; one a sequence where no position needs more.
+// How many ranges a call's records are dealt to: as many as give the workgroups that are resident together, but at least one range a sequence,
+// and no more than KV4_LEAST records each give; one a sequence where no position needs more.
 int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     if (kv4_tiles(c.n_ctx) <= KV4_ALONE / c.head_dim) return n_seq;
-    const int per_kv = n_head / c.n_head_kv, rows = 16 * kv4_nq(c.head_dim, n_tok, per_kv);
+    const int per_kv = n_head / c.n_head_kv, nq = kv4_nq(c.head_dim, n_tok, per_kv), rows = 16 * nq;
+    const int groups = 256 * kv4_resident(c.head_dim, nq);
     const long long units = (n_tok * (long long)per_kv + rows - 1) / rows * c.n_head_kv;
     const long long most = (long long)n_seq * ((kv4_tiles(c.n_ctx) + KV4_LEAST - 1) / KV4_LEAST);
-    return int(std::min<long long>(std::max<long long>(n_seq, std::min((c.head_dim == 256 ? KV4_GROUPS_256 : KV4_GROUPS) / units, most)), 65535));
+    return int(std::min<long long>(std::max<long long>(n_seq, std::min(groups / units, most)), 65535));
 }
 
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {

@@ -221,7 +221,7 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 // registers for more than 16 rows to share that. What bounds it, by the counters:
 //   512 tokens at 7680, 16/4 heads of 256: 206 us, 320 TFLOP/s of the formula's 66.6 GFLOP (2.5 times that in parts). Vector instructions are
 //     issued in 61 % of the cycles and matrix instructions run in 33 %, on the same SIMDs with little overlap.
-//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 42 us, 3.6 TB/s; vector instructions in 54 %, matrix instructions in 20 %, the rest
+//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 42 us, 3.6 TB/s; vector instructions in 48 %, matrix instructions in 19 %, the rest
 //     the beginnings and ends of workgroups that have some ten records a wave.
 //   one sequence of 32768, 16/4 heads of 256 (38 MB): 14.8 us, 2.5 TB/s, two records a wave: the chain of position, record, sums and joining
 //     is half of it; of 640: 7.3 us, that chain alone.

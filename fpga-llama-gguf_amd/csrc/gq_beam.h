@@ -20,8 +20,8 @@ struct BeamSelectArgs {
     int32_t * token;       // may be last
     int32_t * parent;      // beams of the group
     int slot;
-    // With pos: row r is at position pos[r * slot] of its prompt (n_prompt[r * slot] ids, at most cap, at prompt + r * cap). While the prompt has
-    // a next id, that is its token, parent and score stay; a beam has ended only behind its prompt.
+    // With pos: row r is at position pos[r * slot] of its prompt (n_prompt[r * slot] ids, at most cap, at prompt + r * cap). While the
+    // prompt has a next id, that is its token, parent and score stay; a beam has ended only behind its prompt.
     const int32_t * pos;
     const int32_t * n_prompt;
     const int32_t * prompt;
@@ -54,8 +54,8 @@ struct BeamReorderArgs {
     const int32_t * parent;  // row r's at parent[r * parent_stride], values outside 0 .. n_beam - 1: the row stays
     int n, n_group, n_beam, parent_stride;
 };
-// Rows apart, and parts apart: all rows of a part before the next part, or all parts of a row before the next row (the sizes in any unit,
-// below 2^46).
+// Rows apart, and parts apart: all rows of a part before the next part, or all parts of a row before the next row (the sizes in any
+// unit, below 2^46).
 inline bool beam_rows_apart(uint64_t rows, uint64_t size, uint64_t row_stride, uint64_t part_stride, uint64_t n_part) {
     if (rows > 1 && row_stride < size) return false;
     if (n_part <= 1) return true;

@@ -9,13 +9,14 @@ namespace gq {
 namespace {
 
 // ---- selection ----
-// Two launches. The first reads every logit once: workgroup (256 * PER logits of a row) forms their maximum m and sum of e^(x - m),
-// and their n_beam best in order. The second, a workgroup per group, joins the rows' sums, and takes the best candidate off the
-// sorted lists n_beam times. Values are 64-bit from the logits on (candidates of two beams may lie next to each other).
-// A list entry is one word that orders as the candidates of one row do: the logit's bits made monotone, above the token inverted.
-// 8 groups of 8 beams of 151936 logits (39 MB): 17.0 us (2.3 TB/s: a workgroup's own way of read, reduce and rank is 7 us, the 64-bit
-// exponentials another 5, partly behind the reads) and 8.5 us, of which n_beam steps of about 0.4 us that wait for one another; one group
-// of 4: 7.4 and 4.7 us, both latency.
+// Two launches. The first reads every logit once: workgroup (256 * PER logits of a row) forms their maximum m and
+// sum of e^(x - m), and their n_beam best in order. The second, a workgroup per group, joins the rows' sums, and takes the best
+// candidate off the sorted lists n_beam times. Values are 64-bit from the logits on (candidates of two beams may lie next to each
+// other). A list entry is one word that orders as the candidates of one row do: the logit's bits made monotone, above the token
+// inverted.
+// 8 groups of 8 beams of 151936 logits (39 MB): 17.0 us (2.3 TB/s: a workgroup's own way of read, reduce and rank is 7 us,
+// the 64-bit exponentials another 5, partly behind the reads) and 8.5 us, of which n_beam steps of about 0.4 us that wait for one
+// another; one group of 4: 7.4 and 4.7 us, both latency.
 constexpr int BEAM_SLACK = 8;
 
 __device__ __forceinline__ uint32_t order_of(float x) {  // monotone in x, > 0 for every number
@@ -24,8 +25,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {  // monotone in x, > 0 f
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
-// 2^t for -1020 <= t <= 0: t = n + f with |f| <= 1/2, 1 + f q(f) with q interpolating (2^f - 1) / f at 7 Chebyshev points (off by at most
-// 1.2e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of u = t + 1.5 * 2^52 as its low word.
+// 2^t for -1020 <= t <= 0: t = n + f with |f| <= 1/2, 1 + f q(f) with q interpolating (2^f - 1) / f at 7 Chebyshev points (off by at
+// most 1.2e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of u = t + 1.5 * 2^52 as its low word.
 __device__ __forceinline__ double beam_poly(double f, double u) {
     double p = 1.5297323765018243e-05;
     p = __builtin_fma(p, f, 0.00015461444698569867);
@@ -41,7 +42,8 @@ __device__ __forceinline__ double beam_exp2(double t) {
     const double magic = 6755399441055744.0, u = t + magic;
     return beam_poly(t - (u - magic), u);
 }
-// e^(x - m) for x <= m and m finite; below m - 700, and for NaN, e^-700. As beam_exp2, with the multiplication by log2(e) in both of its sums.
+// e^(x - m) for x <= m and m finite; below m - 700, and for NaN, e^-700. As beam_exp2, with the multiplication by log2(e) in both of
+// its sums.
 __device__ __forceinline__ double beam_term(float x, double m, double low) {
     constexpr double magic = 6755399441055744.0, log2e = 1.4426950408889634;
     const double d = fmax(double(x) - m, low), u = __builtin_fma(d, log2e, magic);
@@ -79,8 +81,8 @@ __device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return a > b
 __device__ __forceinline__ uint32_t min_u(uint32_t a, uint32_t b) { return a < b ? a : b; }
 __device__ __forceinline__ double sum_d(double a, double b) { return a + b; }
 
-// A bound on the wave's monotone words (0: none; low: the smallest, high: the largest): at least k of them are >= it, and no more than k +
-// BEAM_SLACK if equal ones do not forbid that; with fewer than k words: 1. n: how many pass.
+// A bound on the wave's monotone words (0: none; low: the smallest, high: the largest): at least k of them are >= it, and no more than
+// k + BEAM_SLACK if equal ones do not forbid that; with fewer than k words: 1. n: how many pass.
 __device__ __forceinline__ uint32_t beam_bound(uint32_t x, int k, uint32_t low, uint32_t high, int & n) {
     uint32_t lo = 1, hi = high + 1;  // at least k (or all) are >= lo, fewer than k are >= hi
     n = __popcll(__ballot(x >= 1));
@@ -135,8 +137,8 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     const size_t at = size_t(row) * a.chunks + chunk;
     unsigned long long * out = beam_lists(a) + at * k;
     const float * x = a.x + size_t(row) * size_t(a.stride);
-    // elements 4 (256 i + tid) + e from the chunk's start; rows start anywhere, so the pieces are brought to 16 bytes. Read before it is
-    // known whether the row takes logits at all, which is a microsecond later
+    // elements 4 (256 i + tid) + e from the chunk's start; rows start anywhere, so the pieces are brought to 16 bytes. Read before it
+    // is known whether the row takes logits at all, which is a microsecond later
     const int skew = int((reinterpret_cast<uintptr_t>(x + v0) >> 2) & 3);
     typedef float f32x4 __attribute__((ext_vector_type(4)));
     float v[PER];
@@ -277,8 +279,8 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     }
 }
 
-// The second launch's beginning: the rows' maxima, the logarithms of their sums and their scores, 8 to 64 lanes a row. What is read of score
-// and last is read here (score_out and token may be the same memory). False: the group reads its prompt.
+// The second launch's beginning: the rows' maxima, the logarithms of their sums and their scores, 8 to 64 lanes a row. What is read of
+// score and last is read here (score_out and token may be the same memory). False: the group reads its prompt.
 template <int W>
 __device__ __forceinline__ bool beam_rows(const BeamSelectArgs & a, int g, double * top, double * logsum, double * scores) {
     const int k = a.n_beam, tid = threadIdx.x, lane = tid & 63;
@@ -449,8 +451,8 @@ __device__ __forceinline__ void wave_lds() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-// Workgroup per group of up to 64 * OWN lists: after the rows' sums its first wave alone, one winner a step. A lane holds the heads of OWN
-// lists, the best of them and, read ahead, what follows it in its list.
+// Workgroup per group of up to 64 * OWN lists: after the rows' sums its first wave alone, one winner a step. A lane holds the heads of
+// OWN lists, the best of them and, read ahead, what follows it in its list.
 template <int OWN>
 __global__ __launch_bounds__(256) void beam_pick_wave_kernel(BeamSelectArgs a) {
     __shared__ BeamShared sh;
@@ -558,10 +560,10 @@ __global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelectArgs a) {
 }
 
 // ---- reordering ----
-// Workgroup (4 KB of one part of an array, group): a thread takes the same 16 bytes of all the group's rows, first the sources of
-// every row that changes, then the writes: in place, each moved byte read from HBM and written once (a source with several heirs is read again from
-// the caches). Rows that stay cost nothing. Bound by the memory: 4 groups of 8, 8 caches of 2000 positions (2.3 GB read and written): 438 us, 5.3
-// TB/s; one group of 4 with 24 layers of states (327 MB): 65 us, 5.0 TB/s.
+// Workgroup (4 KB of one part of an array, group): a thread takes the same 16 bytes of all the group's rows, first
+// the sources of every row that changes, then the writes: in place, each moved byte read from HBM and written once (a source with
+// several heirs is read again from the caches). Rows that stay cost nothing. Bound by the memory: 4 groups of 8, 8 caches of 2000
+// positions (2.3 GB read and written): 438 us, 5.3 TB/s; one group of 4 with 24 layers of states (327 MB): 65 us, 5.0 TB/s.
 template <int NB, typename V>
 __device__ __forceinline__ void beam_move(const BeamMove & m, const int32_t * parent, int slot, uint8_t * part, unsigned long long from, int n_beam,
                                           int row0) {
@@ -616,10 +618,10 @@ __global__ void beam_next_kernel(BeamNextArgs a) {
 
 // (a chunk's first piece may start up to 3 elements before it, so 256 * per elements and 3 more are read by a workgroup)
 int beam_chunks(int n_vocab, int per) { return (n_vocab + 256 * per - 1) / (256 * per); }
-// Logits a thread of the first kernel takes: 8, the shorter way through one workgroup, or 32 where those would give the second kernel 192
-// lists a group or the first more workgroups than the device holds at once. Both kernels with 8 and 32: 10.2 and 11.6 us at one group of 4 of
-// 32000, 10.5 and 11.3 at one of 2 of 151936, 15.4 and 18.0 at 70 of 8 of 4000; 12.8 and 12.2 at one of 4 of 151936, 17.8 and 15.6 at one of 12
-// of 32000, 17.0 and 14.9 at 20 of 5 of 32003, 41.4 and 26.4 at 8 of 8 of 151936.
+// Logits a thread of the first kernel takes: 8, the shorter way through one workgroup, or 32 where those would give the second kernel
+// 192 lists a group or the first more workgroups than the device holds at once. Both kernels with 8 and 32: 10.2 and 11.6 us at one
+// group of 4 of 32000, 10.5 and 11.3 at one of 2 of 151936, 15.4 and 18.0 at 70 of 8 of 4000; 12.8 and 12.2 at one of 4 of 151936, 17.8
+// and 15.6 at one of 12 of 32000, 17.0 and 14.9 at 20 of 5 of 32003, 41.4 and 26.4 at 8 of 8 of 151936.
 int beam_per(int n_group, int n_beam, int n_vocab) {
     const int lists = n_beam * beam_chunks(n_vocab, 8);
     return lists >= 192 || (long long)n_group * lists >= 1536 ? 32 : 8;
@@ -645,8 +647,8 @@ hipError_t launch_beam_select(const BeamSelectArgs & args, hipStream_t s) {
     else GQ_LAUNCH(beam_scan_kernel<8>, grid, dim3(256), lds, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // lists of a group: at most 32 * 128. A second kernel for up to 128, 320 and 640 lists and for more, us with the next one in its place: 12.5 and
-    // 13.9 at 128 lists of 8 winners, 12.8 and 14.3 at 300 of 4, 56 and 74 at 608 of 32.
+    // lists of a group: at most 32 * 128. A second kernel for up to 128, 320 and 640 lists and for more, us with the next one in its
+    // place: 12.5 and 13.9 at 128 lists of 8 winners, 12.8 and 14.3 at 300 of 4, 56 and 74 at 608 of 32.
     const int lists = a.n_beam * a.chunks;
     const dim3 groups(unsigned(a.n_group));
     if (lists <= 64 * 2) GQ_LAUNCH(beam_pick_wave_kernel<2>, groups, dim3(256), 0, s, a);

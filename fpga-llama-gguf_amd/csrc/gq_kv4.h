@@ -75,23 +75,24 @@ struct Kv4AttnArgs {
     int group;           // set at launch: n_head / n_head_kv
 };
 
-// Workgroups of the attention a CU holds at once (nq groups of 16 query rows each): three where the registers can be kept to that (32 sequences of
-// up to 8192, 32/8 heads of 128: 52 us, 58 with two). A call's records are dealt to as many as the device holds, each with its share: twice as
-// many, each with half of it, are 21.6 us in place of 19.9 (4 sequences of 8192, 32/8 heads of 128), 27.7 and 23.3 (8 of 5 tokens at 8000,
-// 32/8 heads of 64), 30.7 and 24.7 (8 of 8 tokens, 16/4 heads of 128); 26.2 and 21.5 (one of 32768, 16/4 heads of 256).
+// Workgroups of the attention a CU holds at once (nq groups of 16 query rows each): three where the registers can be kept to that (32
+// sequences of up to 8192, 32/8 heads of 128: 52 us, 58 with two). A call's records are dealt to as many as the device holds, each with
+// its share: twice as many, each with half of it, are 21.6 us in place of 19.9 (4 sequences of 8192, 32/8 heads of 128), 27.7 and 23.3
+// (8 of 5 tokens at 8000, 32/8 heads of 64), 30.7 and 24.7 (8 of 8 tokens, 16/4 heads of 128); 26.2 and 21.5 (one of 32768, 16/4 heads
+// of 256).
 __host__ __device__ constexpr int kv4_resident(int hd, int nq) { return hd * nq <= 128 ? 3 : 2; }
 constexpr int KV4_GROUPS = 768;   // at most
 constexpr int KV4_LEAST = 4;      // records of a range at least: one a wave
-// Records times head_dim up to which a cache's sequences are not split, which needs no second launch: its waves' few records more take less than
-// joining. Half as many where the cache is longer, but no sequence in it (us whole, whole with the second launch, and split: one sequence of
-// 320, 16/4 heads of 256, 12.7 / 14.2 / 12.8; 4 of 1500 19.7 / - / 13.8; 32 of 256, 32/8 heads of 128, 10.2 / 13.3 / 16.6; 7 of 5 tokens in a window
-// of 1000, 8 heads of 64, - / 14.3 / 13.3).
+// Records times head_dim up to which a cache's sequences are not split, which needs no second launch: its waves' few records more take
+// less than joining. Half as many where the cache is longer, but no sequence in it (us whole, whole with the second launch, and split:
+// one sequence of 320, 16/4 heads of 256, 12.7 / 14.2 / 12.8; 4 of 1500 19.7 / - / 13.8; 32 of 256, 32/8 heads of 128, 10.2 / 13.3 /
+// 16.6; 7 of 5 tokens in a window of 1000, 8 heads of 64, - / 14.3 / 13.3).
 constexpr int KV4_ALONE = 2048;
 bool kv4_joins(const Kv4AttnArgs & a);  // the launch is followed by that of kv4_join_kernel
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head);
 
-// The ATTN command's part before the attention: every q head and new key normalized and rotated (gq_kernels.h, AttnArgs; q stays FP32 in
-// qr), the keys and values stored. Tokens as t says.
+// The ATTN command's part before the attention: every q head and new key normalized and rotated (gq_kernels.h, AttnArgs; q stays FP32
+// in qr), the keys and values stored. Tokens as t says.
 struct Kv4AppendArgs {
     Kv4Cache c;
     Kv4Tokens t;

@@ -49,10 +49,11 @@ __device__ __forceinline__ uint8_t * kv4_rec(const Kv4Cache & c, int s, int h, i
 }
 
 // Workgroup (record of the tokens' span; keys or values; four blocks | KV head | sequence): 8 lanes a block. A record that the tokens
-// fill is put together in LDS and written in 16-byte pieces; of the others only the tokens' own bytes are written. So small a share
-// of a record (2.3 KB) that a prompt of 512 tokens still has a few hundred workgroups, each with its 8 reads in flight together.
-// 1983 tokens of 4 heads of 256 (18.5 MB): 9.3 us, 2.0 TB/s; 512 of them 6.4 us; one token of each of 32 sequences, 8 heads of 128, 4 us. The
-// launch and one trip to memory are 3 to 4 us of each; behind them the largest is bound by the shuffles and conversions of its blocks.
+// fill is put together in LDS and written in 16-byte pieces; of the others only the tokens' own bytes are written. So small a share of
+// a record (2.3 KB) that a prompt of 512 tokens still has a few hundred workgroups, each with its 8 reads in flight together.
+// 1983 tokens of 4 heads of 256 (18.5 MB): 9.3 us, 2.0 TB/s; 512 of them 6.4 us; one token of each of 32 sequences, 8 heads of 128, 4 us.
+// The launch and one trip to memory are 3 to 4 us of each; behind them the largest is bound by the shuffles and conversions of its
+// blocks.
 constexpr int KV4_STORE = 128;  // threads
 template <int HD>
 __global__ __launch_bounds__(KV4_STORE) void kv4_store_kernel(Kv4RowsArgs a) {
@@ -115,8 +116,8 @@ __global__ __launch_bounds__(KV4_STORE) void kv4_store_kernel(Kv4RowsArgs a) {
 }
 
 // Workgroup (q head, or KV head behind them | token | sequence): the ATTN command's norm and rotation of one vector, in the order of
-// the F16 cache's kernels; a q head's goes to qr, a key's into the cache with its value, 8 lanes a block. One vector a workgroup: a decode
-// step has few, each a chain of two sums and two trips to memory (4 us).
+// the F16 cache's kernels; a q head's goes to qr, a key's into the cache with its value, 8 lanes a block. One vector a workgroup: a
+// decode step has few, each a chain of two sums and two trips to memory (4 us).
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_append_kernel(Kv4AppendArgs a) {
     using L = Kv4Layout<HD>;
@@ -183,8 +184,8 @@ __device__ __forceinline__ float kv4_value(const uint8_t * rec, int p, int e) {
     return h2f(*reinterpret_cast<const uint16_t *>(rec + L::VD + L::scale(p, blk))) * float(q - 8);
 }
 
-// Workgroup (token, KV head, sequence), a thread an element: the writes, 7 times what is read, are whole lines (1983 tokens of 4 heads of 256,
-// 18.5 MB: 9.4 us, 2.0 TB/s).
+// Workgroup (token, KV head, sequence), a thread an element: the writes, 7 times what is read, are whole lines (1983 tokens of 4 heads
+// of 256, 18.5 MB: 9.4 us, 2.0 TB/s).
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
     const int h = blockIdx.y, s = blockIdx.z, t = blockIdx.x;
@@ -215,19 +216,19 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 //                 fused multiply-add, what is missing). The scales are brought up by a power of two 2^e common to the wave, the
 //                 largest so far to 2^9..2^10, so that the second number is a multiple of 2^-24 too. Three of the four products of
 //                 parts are summed (the fourth is below 2^-22 of the first).
-// The accumulators stay with the query's lanes and nothing crosses lanes in the loop. The four waves of a workgroup take the
-// records of its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
-// A record and 16 rows, heads of 256, are 80 matrix instructions and about 600 others, half of them unpacking; wider heads than 128 leave no
-// registers for more than 16 rows to share that. What bounds it, by the counters:
-//   512 tokens at 7680, 16/4 heads of 256: 206 us, 320 TFLOP/s of the formula's 66.6 GFLOP (2.5 times that in parts). Vector instructions are
-//     issued in 61 % of the cycles and matrix instructions run in 33 %, on the same SIMDs with little overlap.
-//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 42 us, 3.6 TB/s; vector instructions in 48 %, matrix instructions in 19 %, the rest
-//     the beginnings and ends of workgroups that have some ten records a wave.
-//   one sequence of 32768, 16/4 heads of 256 (38 MB): 14.8 us, 2.5 TB/s, two records a wave: the chain of position, record, sums and joining
-//     is half of it; of 640: 7.3 us, that chain alone.
-// Tried and taken back: workgroups whose waves share one record's unpacking for 64 rows through LDS (two barriers a record; 190 us and 16 us of
-// joining for the 512 tokens), 32 rows a wave at heads of 256 with one wave a SIMD (244 us), matrix instructions at a raised wave priority (188 us in place
-// of 191 there, 52.6 in place of 51.9 for the 32 sequences).
+// The accumulators stay with the query's lanes and nothing crosses lanes in the loop. The four waves of a workgroup take the records of
+// its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
+// A record and 16 rows, heads of 256, are 80 matrix instructions and about 600 others, half of them unpacking; wider heads than 128
+// leave no registers for more than 16 rows to share that. What bounds it, by the counters:
+//   512 tokens at 7680, 16/4 heads of 256: 206 us, 320 TFLOP/s of the formula's 66.6 GFLOP (2.5 times that in parts). Vector instructions
+//     are issued in 61 % of the cycles and matrix instructions run in 33 %, on the same SIMDs with little overlap.
+//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 42 us, 3.6 TB/s; vector instructions in 48 %, matrix instructions in 19 %, the
+//     rest the beginnings and ends of workgroups that have some ten records a wave.
+//   one sequence of 32768, 16/4 heads of 256 (38 MB): 14.8 us, 2.5 TB/s, two records a wave: the chain of position, record, sums and
+//     joining is half of it; of 640: 7.3 us, that chain alone.
+// Tried and taken back: workgroups whose waves share one record's unpacking for 64 rows through LDS (two barriers a record; 190 us and
+// 16 us of joining for the 512 tokens), 32 rows a wave at heads of 256 with one wave a SIMD (244 us), matrix instructions at a raised
+// wave priority (188 us in place of 191 there, 52.6 in place of 51.9 for the 32 sequences).
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -434,8 +435,8 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int &
         most = max(most, __shfl_xor(most, d, WAVE));
     }
     int per = kv4_per(sum, a.ranges, a.t.n_seq, most, a.c.head_dim);
-    // That leaves room for a short range of every sequence; less will do. Worth its 0.3 us where the sequences are many (32 of up to 8192,
-    // 32/8 heads of 128: 53.0 and 58.2 us).
+    // That leaves room for a short range of every sequence; less will do. Worth its 0.3 us where the sequences are many (32 of up to
+    // 8192, 32/8 heads of 128: 53.0 and 58.2 us).
     if (a.t.n_seq <= 64 && 8 * a.t.n_seq > a.ranges && per < most) {
         int low = max(int((sum + a.ranges - 1) / a.ranges), KV4_LEAST);
         for (int i = 0; i < 4 && low < per; ++i) {
@@ -782,9 +783,9 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     }
 }
 
-// Workgroup (q head and EL of its elements, token, sequence): the sets of a sequence with several ranges. The factors of all sets first,
-// then EL / 4 threads a set, 1024 / EL sets at a time. 128 sets of 16 heads of 256 (2.1 MB): 4.4 us with 64 elements a workgroup, three trips to
-// memory in a row; 32 sequences' up to 96 sets of 32 heads of 128: 7.6 us.
+// Workgroup (q head and EL of its elements, token, sequence): the sets of a sequence with several ranges. The factors of all sets
+// first, then EL / 4 threads a set, 1024 / EL sets at a time. 128 sets of 16 heads of 256 (2.1 MB): 4.4 us with 64 elements a
+// workgroup, three trips to memory in a row; 32 sequences' up to 96 sets of 32 heads of 128: 7.6 us.
 template <int HD, int EL>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     constexpr int PER = EL / 4, SETS = 256 / PER;
@@ -870,8 +871,8 @@ static int kv4_nq(int hd, int n_tok, int per_kv) {
     return rows <= 16 || hd == 256 ? 1 : rows <= 32 || hd == 128 ? 2 : 4;
 }
 
-// How many ranges a call's records are dealt to: as many as give the workgroups that are resident together, but at least one range a sequence,
-// and no more than KV4_LEAST records each give; one a sequence where no position needs more.
+// How many ranges a call's records are dealt to: as many as give the workgroups that are resident together, but at least one range a
+// sequence, and no more than KV4_LEAST records each give; one a sequence where no position needs more.
 int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     if (kv4_tiles(c.n_ctx) <= KV4_ALONE / c.head_dim) return n_seq;
     const int per_kv = n_head / c.n_head_kv, nq = kv4_nq(c.head_dim, n_tok, per_kv), rows = 16 * nq;

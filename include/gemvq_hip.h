@@ -86,20 +86,22 @@
  *   FILL      [16, n, y_off, value bits, 0, 0, 0, 0]  y = value.
  *   BEAM      [18, n_vocab, x_off, row_stride, n_beam | n_group << 8, eos, score_off, parent_off]
  *             + [tok_off, pos_off, len_off, prompt_off, cap, 0, 0, 0]
- *             One step of a beam search over n_group groups of n_beam sequences in lockstep (at most GEMVQ_GEMM_MAX_TOK in all; no
- *             counterpart in the reference): gemvq_beam_select_static on the logits rows at x_off + s * row_stride. Sequence s's
- *             score (FP32), token and parent (int32) are at act[score_off, tok_off, parent_off + 16 s]; the tokens there are the last ones, and the
- *             new ones replace them. With len_off, a group whose first sequence is at position p = act_i32[pos_off + 16 s] with p + 1 <
- *             act_i32[len_off + 16 s] reads its prompt instead: token = act_i32[prompt_off + s * cap + p + 1], the parent is the
- *             sequence itself, the score stays; and eos ends a beam only behind its prompt.
+ *             One step of a beam search over n_group groups of n_beam sequences in lockstep (at most GEMVQ_GEMM_MAX_TOK in all;
+ *             no counterpart in the reference): gemvq_beam_select_static on the logits rows at x_off + s * row_stride. Sequence
+ *             s's score (FP32), token and parent (int32) are at act[score_off, tok_off, parent_off + 16 s]; the tokens there
+ *             are the last ones, and the new ones replace them. With len_off, a group whose first sequence is at position p =
+ *             act_i32[pos_off + 16 s] with p + 1 < act_i32[len_off + 16 s] reads its prompt instead: token = act_i32[prompt_off
+ *             + s * cap + p + 1], the parent is the sequence itself, the score stays; and eos ends a beam only behind its
+ *             prompt.
  *   BEAM_MOVE [19, kind | n_part << 8, off, row_stride, part_stride, n, parent_off, n_beam | n_group << 8]
  *             + [pos_off, first, 0, 0, 0, 0, 0, 0]
- *             gemvq_beam_reorder_static on one array: its row s becomes what row act_i32[parent_off + 16 s] of the group was. kind 0: rows of
- *             n floats of the activation buffer from off on, kind 1: of n state rows (strides in floats, state rows; n_part 0: one
- *             part); with pos_off only elements first .. pos move. kind 2: KV buffer off's regions as ATTN's sequences have them, positions
- *             first .. pos (whole records of 32 in a 4-bit buffer). pos = act_i32[pos_off + 16 s] of the parent. Consecutive ones
- *             with the same parents become one launch where their arrays lie apart.
- *   BEAM_NEXT [20, tok_off, pos_off, out_off, cap, n_seq, 0, 0]  act_i32[out_off + s * cap + pos + 1] = tok (while that is below cap), pos += 1,
+ *             gemvq_beam_reorder_static on one array: its row s becomes what row act_i32[parent_off + 16 s] of the group was.
+ *             kind 0: rows of n floats of the activation buffer from off on, kind 1: of n state rows (strides in floats, state
+ *             rows; n_part 0: one part); with pos_off only elements first .. pos move. kind 2: KV buffer off's regions as
+ *             ATTN's sequences have them, positions first .. pos (whole records of 32 in a 4-bit buffer). pos = act_i32[pos_off
+ *             + 16 s] of the parent. Consecutive ones with the same parents become one launch where their arrays lie apart.
+ *   BEAM_NEXT [20, tok_off, pos_off, out_off, cap, n_seq, 0, 0]
+ *             act_i32[out_off + s * cap + pos + 1] = tok (while that is below cap), pos += 1,
  *             tok and pos at 16 s.
  *   GEMM      [17, format | flags, rows, cols, w_off lo, w_off hi, x_off, y_off]
  *             + [n_tok, x_stride, y_stride, res_off, res_stride, norm_w_off, eps bits, norm_flags]
@@ -224,11 +226,12 @@ int gemvq_state_write(gemvq_ctx * ctx, size_t row, const float * src, size_t row
 int gemvq_state_read(gemvq_ctx * ctx, size_t row, float * dst, size_t rows);
 int gemvq_state_clear(gemvq_ctx * ctx);
 
-/* What the KV buffers created from now on hold (no counterpart in the reference): fp16 (default), or 4 bits a value (Q4_0 blocks of 32, 4.5
- * bits with their scales; heads of 32, 64, 128 or 256). ATTN on a 4-bit buffer has the meaning it has on an fp16 one, but for what its
- * numbers are rounded to: keys and values as gemvq_kv4_store_static does, q not at all; and a batch's results agree with those of one-token commands to
- * FP32 rounding, not bit for bit. GEMVQ_ARITH_REFERENCE rejects it. A sequence's region (GEMVQ_ATTN_SEQS) starts at a whole record of 32
- * positions: where n_ctx / n_tok is no multiple of 32, a buffer keeps one number of sequences until gemvq_kv_clear. */
+/* What the KV buffers created from now on hold (no counterpart in the reference): fp16 (default), or 4 bits a value (Q4_0
+ * blocks of 32, 4.5 bits with their scales; heads of 32, 64, 128 or 256). ATTN on a 4-bit buffer has the meaning it has on an fp16 one, but
+ * for what its numbers are rounded to: keys and values as gemvq_kv4_store_static does, q not at all; and a batch's results
+ * agree with those of one-token commands to FP32 rounding, not bit for bit. GEMVQ_ARITH_REFERENCE rejects it. A sequence's
+ * region (GEMVQ_ATTN_SEQS) starts at a whole record of 32 positions: where n_ctx / n_tok is no multiple of 32, a buffer
+ * keeps one number of sequences until gemvq_kv_clear. */
 #define GEMVQ_KV_F16 1
 #define GEMVQ_KV_Q4_0 2
 int gemvq_set_kv_type(gemvq_ctx * ctx, int type);
@@ -320,16 +323,18 @@ int gemvq_gemm_static(int type, int rows, int cols, const void * w, const float 
                       float * y, int y_stride, void * stream);
 
 /* No counterpart in the reference: a KV cache held in 4 bits (ggml's Q4_0 blocks of 32 along head_dim: 4.5 bits a value
- * against F16's 16), on caller-owned device memory. `data` holds gemvq_kv4_bytes() bytes, 256-byte aligned: n_ctx positions of
- * n_head_kv keys and values of head_dim (32, 64, 128 or 256) for each of n_seq sequences, in a layout of its own (records of 32
- * positions of one KV head, csrc/gq_kv4.h). Nothing needs clearing: positions that were not stored are not read.
- * All calls run on the current device, asynchronously on `stream` (a hipStream_t of that device; NULL for the null stream),
- * allocate nothing and keep nothing: they can be captured into a graph, and calls overlap freely where their memory is apart.
- * Tokens: row s * n_tok + t of k, v, q and y is token t of sequence s, at position pos[s] + t (pos: n_seq int32 in device
- * memory). num (n_seq int32 in device memory, or NULL for n_tok each) says how many tokens of a sequence there are: the others,
- * and tokens whose position is outside 0 .. n_ctx - 1, are neither stored nor read, and their rows of y, k and v are left as they
- * were. 1 <= n_tok <= GEMVQ_KV4_MAX_TOK. Rows start at multiples of 16 bytes: pointers 16-byte aligned, strides (in floats)
- * multiples of 4 and no smaller than a row. Outputs do not overlap inputs.
+ * against F16's 16), on caller-owned device memory. `data` holds gemvq_kv4_bytes() bytes, 256-byte aligned: n_ctx positions
+ * of n_head_kv keys and values of head_dim (32, 64, 128 or 256) for each of n_seq sequences, in a layout of its own
+ * (records of 32 positions of one KV head, csrc/gq_kv4.h). Nothing needs clearing: positions that were not stored are not
+ * read.
+ * All calls run on the current device, asynchronously on `stream` (a hipStream_t of that device; NULL for the null
+ * stream), allocate nothing and keep nothing: they can be captured into a graph, and calls overlap freely where their
+ * memory is apart.
+ * Tokens: row s * n_tok + t of k, v, q and y is token t of sequence s, at position pos[s] + t (pos: n_seq
+ * int32 in device memory). num (n_seq int32 in device memory, or NULL for n_tok each) says how many tokens of a sequence
+ * there are: the others, and tokens whose position is outside 0 .. n_ctx - 1, are neither stored nor read, and their rows
+ * of y, k and v are left as they were. 1 <= n_tok <= GEMVQ_KV4_MAX_TOK. Rows start at multiples of 16 bytes: pointers
+ * 16-byte aligned, strides (in floats) multiples of 4 and no smaller than a row. Outputs do not overlap inputs.
  * Status: 0, GEMVQ_EINVAL (nothing launched) or a negated HIP error. */
 #define GEMVQ_KV4_MAX_TOK 65535
 #define GEMVQ_KV4_MAX_ROWS (1 << 27) /* n_tok * n_head of an attention */
@@ -348,9 +353,9 @@ int gemvq_kv4_load_static(const gemvq_kv4 * kv, float * k, float * v, int64_t ro
                           const int32_t * num, void * stream);
 /* Attention: the token at position p gives y = sum_j softmax_j(scale * q . k_j) v_j over the positions j from 0, or from
  * max(0, p - window + 1) with window > 0, to p (store the tokens' own keys and values first). q head h of a row starts at
- * h * q_head_stride and reads KV head h / (n_head / n_head_kv); y's heads are packed. q enters as it is (no rounding to 16 bits);
- * products, softmax and sums in FP32. work: gemvq_kv4_attn_work() bytes of device memory, 16-byte aligned, whose contents do
- * not matter before or after; calls that may overlap need one each. */
+ * h * q_head_stride and reads KV head h / (n_head / n_head_kv); y's heads are packed. q enters as it is (no rounding to 16
+ * bits); products, softmax and sums in FP32. work: gemvq_kv4_attn_work() bytes of device memory, 16-byte aligned, whose
+ * contents do not matter before or after; calls that may overlap need one each. */
 uint64_t gemvq_kv4_attn_work(const gemvq_kv4 * kv, int n_tok, int n_head);
 int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
                           int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,
@@ -358,24 +363,27 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
 
 /* No counterpart in the reference: one step of a beam search over n_group independent groups of n_beam (1 .. GEMVQ_BEAM_MAX)
  * beams, rows g * n_beam + b, at most 65535 rows; on caller-owned device memory, under the rules of the calls above.
- * Selection: candidate v of beam b has the value score[b] + logit[b][v] - log(sum of e^logit[b]), formed in 64 bits; the n_beam best
- * candidates of a group, in descending order: score_out (rounded to FP32), token, and parent (the beam in the group it
- * continues); of equal ones the lower b * n_vocab + v first (among one beam's logits, the larger logit first). A beam whose last token (last[row], or
- * last NULL) is eos has ended: it has the one candidate eos, at its score, whatever its logits (which are there all the same); eos outside the vocabulary: none ends.
- * The candidates of a beam with score -inf (the beams after the first, at a search's start) come after all others. NaN logits and scores count as -inf, +inf logits
- * as the largest finite number. logits: FP32 rows row_stride >= n_vocab floats apart, 1 <= n_vocab <= GEMVQ_BEAM_MAX_VOCAB, 4-byte
- * aligned. score_out may be score, token may be last. work: gemvq_beam_work() bytes, 16-byte aligned, contents do not matter. */
+ * Selection: candidate v of beam b has the value score[b] + logit[b][v] - log(sum of e^logit[b]), formed in 64 bits; the
+ * n_beam best candidates of a group, in descending order: score_out (rounded to FP32), token, and parent (the beam in the
+ * group it continues); of equal ones the lower b * n_vocab + v first (among one beam's logits, the larger logit first). A
+ * beam whose last token (last[row], or last NULL) is eos has ended: it has the one candidate eos, at its score, whatever
+ * its logits (which are there all the same); eos outside the vocabulary: none ends. The candidates of a beam with score
+ * -inf (the beams after the first, at a search's start) come after all others. NaN logits and scores count as -inf, +inf
+ * logits as the largest finite number. logits: FP32 rows row_stride >= n_vocab floats apart, 1 <= n_vocab <=
+ * GEMVQ_BEAM_MAX_VOCAB, 4-byte aligned. score_out may be score, token may be last. work: gemvq_beam_work() bytes, 16-byte
+ * aligned, contents do not matter. */
 #define GEMVQ_BEAM_MAX 32
 #define GEMVQ_BEAM_MAX_VOCAB (1 << 20)
 uint64_t gemvq_beam_work(int n_group, int n_beam, int n_vocab);
 int gemvq_beam_select_static(const float * logits, int64_t row_stride, int n_vocab, int n_group, int n_beam, const float * score,
                              const int32_t * last, int eos, float * score_out, int32_t * token, int32_t * parent, void * work,
                              uint64_t work_bytes, void * stream);
-/* Reordering: what the beams keep follows the selection, in place: in each of the arrays, row i of every group becomes what row parent[i] of
- * the group was (a value outside 0 .. n_beam - 1: the row stays). An array's row r has n_part parts, at data + r * row_stride + p *
- * part_stride, of `count` units of unit_bytes each; units first .. count - 1 move (a prefix that all beams share need not). With
- * used (int32 in device memory, for row r at used[r * used_stride]), only the source row's units below ceil(used / unit_len) move, and
- * what the target has behind them stays. Addresses and sizes are multiples of 4 bytes (of 16 for full speed); rows and parts, arrays, used and parent lie apart from one another. */
+/* Reordering: what the beams keep follows the selection, in place: in each of the arrays, row i of every group becomes what
+ * row parent[i] of the group was (a value outside 0 .. n_beam - 1: the row stays). An array's row r has n_part parts, at data + r *
+ * row_stride + p * part_stride, of `count` units of unit_bytes each; units first .. count - 1 move (a prefix that all beams
+ * share need not). With used (int32 in device memory, for row r at used[r * used_stride]), only the source row's units
+ * below ceil(used / unit_len) move, and what the target has behind them stays. Addresses and sizes are multiples of 4 bytes
+ * (of 16 for full speed); rows and parts, arrays, used and parent lie apart from one another. */
 typedef struct {
     void * data;
     uint64_t row_stride, part_stride;

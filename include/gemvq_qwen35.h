@@ -38,8 +38,8 @@ typedef struct gemvq_qwen35 gemvq_qwen35;
 int gemvq_qwen35_sizes(const gemvq_qw_config * cfg, const gemvq_tensor_desc * table, int n_tensors,
                        size_t * act_floats, size_t * weight_bytes, size_t * state_rows);
 /* Uploads the weights into ctx, allocates KV buffers (of the type gemvq_set_kv_type set on ctx; a prompt's chunks and lockstep sequences
- * on 4-bit ones agree with single steps to rounding, not bit for bit), lays out the activation buffer and builds the per-token
- * command list. Returns NULL on failure (gemvq_last_error(ctx) says why). */
+ * on 4-bit ones agree with single steps to rounding, not bit for bit), lays out the activation buffer and builds the
+ * per-token command list. Returns NULL on failure (gemvq_last_error(ctx) says why). */
 gemvq_qwen35 * gemvq_qwen35_create(gemvq_ctx * ctx, const gemvq_qw_config * cfg, const gemvq_tensor_desc * table,
                                    int n_tensors, const uint8_t * blob);
 void gemvq_qwen35_destroy(gemvq_qwen35 * m);
@@ -49,10 +49,11 @@ int gemvq_qwen35_reset(gemvq_qwen35 * m, const int32_t * prompt, int n);
  * reset with a new prompt length); asynchronous. */
 int gemvq_qwen35_step(gemvq_qwen35 * m, int n);
 /* Runs the next n prompt positions (all before the last prompt token) in chunks of up to 512 tokens (as much
- * of them as n_ctx holds; GEMVQ_GEMM_MAX_TOK in the reference arithmetic) per weight read (GEMM commands; the reference plans this batched path, ROADMAP.md:78-96, and has no counterpart):
- * afterwards the model is where n decode steps would have left it (states, KV cache, position, token ids), bit for
- * bit, without the logits. GEMVQ_EINVAL when a projection has no batched form (Q4_0 / Q4_1 / Q8_0 with columns a
- * multiple of 512; decode steps then do the same work) or the positions pass the last prompt token but one; synchronizes. */
+ * of them as n_ctx holds; GEMVQ_GEMM_MAX_TOK in the reference arithmetic) per weight read (GEMM commands; the reference
+ * plans this batched path, ROADMAP.md:78-96, and has no counterpart): afterwards the model is where n decode steps
+ * would have left it (states, KV cache, position, token ids), bit for bit, without the logits. GEMVQ_EINVAL when a
+ * projection has no batched form (Q4_0 / Q4_1 / Q8_0 with columns a multiple of 512; decode steps then do the same
+ * work) or the positions pass the last prompt token but one; synchronizes. */
 int gemvq_qwen35_prefill(gemvq_qwen35 * m, int n);
 /* Token ids at positions 0 .. n - 1 (prompt tokens, then generated ones); synchronizes. */
 int gemvq_qwen35_tokens(gemvq_qwen35 * m, int32_t * out, int n);
@@ -91,11 +92,13 @@ int gemvq_qwen35_batch_reset(gemvq_qwen35 * m, const int32_t * prompts, const in
 int gemvq_qwen35_batch_tokens(gemvq_qwen35 * m, int seq, int32_t * out, int n);
 int gemvq_qwen35_batch_logits(gemvq_qwen35 * m, int seq, float * out);
 /* Beam search over a batch model (no counterpart in the reference): its sequences become n_seq / n_beam groups of n_beam beams
- * (sequences g * n_beam + b). It takes a gemvq_qwen35_batch_reset next (a step before it is refused), with the same prompt for all beams of a group. Steps
- * read the prompt as before, and behind it select the n_beam best continuations of each group (BEAM), let states, conv windows, caches
- * and ids follow their parents (BEAM_MOVE) and append the new tokens, all in the step's graph. Beams are in descending order of their scores
- * (sums of the tokens' log probabilities); one whose last token is eos (outside the vocabulary: none) keeps its score, and eos as its next tokens. n_beam 0:
- * greedy again. gemvq_qwen35_batch_tokens, _logits and _step apply; _scores gives the n_seq scores. 0 or GEMVQ_EINVAL. */
+ * (sequences g * n_beam + b). It takes a gemvq_qwen35_batch_reset next (a step before it is refused), with the same
+ * prompt for all beams of a group. Steps read the prompt as before, and behind it select the n_beam best continuations
+ * of each group (BEAM), let states, conv windows, caches and ids follow their parents (BEAM_MOVE) and append the new
+ * tokens, all in the step's graph. Beams are in descending order of their scores (sums of the tokens' log
+ * probabilities); one whose last token is eos (outside the vocabulary: none) keeps its score, and eos as its next
+ * tokens. n_beam 0: greedy again. gemvq_qwen35_batch_tokens, _logits and _step apply; _scores gives the n_seq scores. 0
+ * or GEMVQ_EINVAL. */
 int gemvq_qwen35_batch_set_beam(gemvq_qwen35 * m, int n_beam, int eos);
 int gemvq_qwen35_batch_scores(gemvq_qwen35 * m, float * out);
 /* The per-token command list gemvq_qwen35_create would build, without a device: weights placed as

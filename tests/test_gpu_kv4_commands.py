@@ -125,6 +125,15 @@ def test_attn_command_without_scratch(gq, monkeypatch):
     _attn_case(gq, 8, 2, 128, 32, False, [(0, 32), (32, 32), (64, 32), (96, 32), (128, 32), (160, 1)], 192)
 
 
+@pytest.mark.parametrize("scratch", [True, False])
+def test_attn_command_over_ranges(gq, monkeypatch, scratch):
+    """Buffers long enough to be split into ranges, with and without memory for their partial sums (unstored positions are zeros)."""
+    if not scratch:
+        monkeypatch.setenv("GEMVQ_SCRATCH_LIMIT", "0")
+    _attn_case(gq, 16, 4, 256, 64, True, [(0, 32), (500, 32), (890, 5), (899, 1), (310, 1)], 900)
+    _attn_case(gq, 8, 2, 128, 32, False, [([600, 3, 1199], 1), ([601, 4, 1200], 1), ([1198, 1198, 600], 1)], 1200, seqs=3)
+
+
 def test_attn_command_rejections(gq):
     with gq.Context(act_floats=1 << 16, weight_bytes=1 << 12) as ctx:
         with pytest.raises(gq.GemvqError):

@@ -303,6 +303,33 @@ def test_model_over_a_4_bit_cache(gq, q35):
         assert np.array_equal(got[gq.KV_Q4_0, "steps"][i], got["lockstep"][i])
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim", [(16, 2, 64), (4, 1, 256)])
+def test_long_prompt_over_a_4_bit_cache(gq, q35, monkeypatch, heads, kv_heads, dim):
+    """Prompt chunks of 512 tokens (their rotated queries in the context's scratch) and of as many as the buffers' own scratch holds: the first
+    attention layer's cache is the same bits. The second's depends on the first's attention, whose FP32 rounding differs by chunk; that turns
+    few activations' 8-bit roundings, each a 254th of its block's largest, so that few of 16 levels change, by one: 1 in 20 at most is
+    asked for, where a wrong row would change nearly all."""
+    cfg = q35.Config(n_layer=8, n_embd=1024, n_ff=2048, n_vocab=2048, n_head=heads, n_head_kv=kv_heads, head_dim=dim, n_rot=32,
+                     ssm_k_heads=2, ssm_v_heads=4, n_ctx=1100)
+    blob = q35.generate(cfg, seed=7)
+    ids = q35.prompt_ids(cfg, 1050, 5)
+    row, got = kv_heads * dim, []
+    for limit in (None, "0"):
+        if limit:
+            monkeypatch.setenv("GEMVQ_SCRATCH_LIMIT", limit)
+        with q35.Model(blob, kv_type=gq.KV_Q4_0) as m:
+            m.reset(ids)
+            assert m.prefill(1049)
+            m.step(20)
+            assert np.isfinite(m.logits()).all()
+            got.append([m.ctx.kv_read(layer, 0, 1049, row) for layer in (0, 1)])
+    for i in range(2):
+        assert np.array_equal(got[0][0][i], got[1][0][i])
+        a, b = (np.asarray(g[1][i]).view(np.float16).astype(np.float64).reshape(-1, 32) for g in got)
+        step = np.maximum(np.abs(a).max(1), np.abs(b).max(1))[:, None] / 8
+        assert (np.abs(a - b) > step / 2).mean() < 0.05
+
+
 @pytest.mark.parametrize("kind", ["f16", "q4_0"])
 @pytest.mark.parametrize("groups,beams,lens", [(2, 3, (9, 4)), (1, 4, (33,))])
 def test_beam_search_of_the_model(gq, q35, kind, groups, beams, lens):

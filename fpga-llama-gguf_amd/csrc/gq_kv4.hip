@@ -802,27 +802,39 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     const int n = (int(p / KV4_TILE) - r.first) / r.per - j0 + 1;
     const size_t step = size_t(a.t.n_tok) * a.n_head * (HD + 4);
     const float * w = a.work + (size_t(r.slot + j0) * a.t.n_tok + t) * a.n_head * (HD + 4) + size_t(hq) * (HD + 4);
+    // every first read before the first use: the sets' c and sums of weights, AHEAD sets of the thread's elements
+    constexpr int STATS = KV4_GROUPS / 256, AHEAD = 8;
+    static_assert(KV4_GROUPS % 256 == 0, "a thread's sets");
+    float2 cl[STATS];
+#pragma unroll
+    for (int i = 0; i < STATS; ++i) cl[i] = tid + 256 * i < n ? *reinterpret_cast<const float2 *>(w + (tid + 256 * i) * step + HD) : float2{KV4_LOW, 0.0f};
+    const int e = tid % PER * 4, j1 = tid / PER;
+    f32x4 x[AHEAD];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) x[i] = j1 + i * SETS < n ? *reinterpret_cast<const f32x4 *>(w + (j1 + i * SETS) * step + e0 + e) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     float C = KV4_LOW, L = 0.0f;
-    for (int j = tid; j < n; j += 256) {
-        f[j] = w[j * step + HD];
-        C = fmaxf(C, f[j]);
-    }
+#pragma unroll
+    for (int i = 0; i < STATS; ++i) C = fmaxf(C, cl[i].x);
     C = wave_max(C);
     if (lane == 0) red[0][wave] = C;
     __syncthreads();
     C = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-    for (int j = tid; j < n; j += 256) {
-        f[j] = __builtin_amdgcn_exp2f(f[j] - C);
-        L += w[j * step + HD + 1] * f[j];
+#pragma unroll
+    for (int i = 0; i < STATS; ++i) {
+        const float g = __builtin_amdgcn_exp2f(cl[i].x - C);
+        if (tid + 256 * i < n) f[tid + 256 * i] = g;
+        L += cl[i].y * g;
     }
 #pragma unroll
     for (int d = 32; d >= 1; d >>= 1) L += __shfl_xor(L, d, WAVE);
     if (lane == 0) red[1][wave] = L;
     __syncthreads();
     f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int e = tid % PER * 4;
-#pragma unroll 8
-    for (int j = tid / PER; j < n; j += SETS) y += *reinterpret_cast<const f32x4 *>(w + j * step + e0 + e) * f[j];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+        if (j1 + i * SETS < n) y += x[i] * f[j1 + i * SETS];
+#pragma unroll 4
+    for (int j = j1 + AHEAD * SETS; j < n; j += SETS) y += *reinterpret_cast<const f32x4 *>(w + j * step + e0 + e) * f[j];
     *reinterpret_cast<f32x4 *>(&part[tid / PER][e]) = y;
     __syncthreads();
     if (tid >= PER) return;

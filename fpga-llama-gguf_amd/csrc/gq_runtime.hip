@@ -1047,7 +1047,8 @@ struct Compiler {
                uint32_t qstride, uint32_t ntok) {
         KvBuf & b = c->kvs[k[3]];
         if (ref()) return reject(i, "ATTN on a 4-bit KV buffer in the reference arithmetic");
-        const uint32_t flags = k[7], sets = ATTN_MAXG * nkv * GEMM_MAX_TOK / std::max(nh, 1u);
+        if (nh == 0) return reject(i, "ATTN shape");
+        const uint32_t flags = k[7], sets = ATTN_MAXG * nkv * GEMM_MAX_TOK / nh;
         const bool wide = c->max_tok > GEMM_MAX_TOK, own = wide && ntok > sets;
         if (ntok > uint32_t(wide ? c->max_tok : GEMM_MAX_TOK) || (own && size_t(ntok) * nh * hd > c->attn_wide_n)) return reject(i, "ATTN tokens");
         const bool seqs = (flags & GEMVQ_ATTN_SEQS) && ntok > 1;

@@ -149,6 +149,7 @@ def test_attn_command_rejections(gq):
         assert ctx.run(c) == 1 and "4-bit" in ctx.error()
         ctx.set_arith(gq.ARITH_CANONICAL)
         assert ctx.run(gq.attn(4, 2, 64, kv, 1024, 64, 0, 32, 2048, 2304, 0.125, EPS, 4096, 4160, 4224, n_tok=33)) == 1
+        assert ctx.run(gq.attn(0, 2, 64, kv, 1024, 64, 0, 32, 2048, 2304, 0.125, EPS, 4096, 4160, 4224)) == 1
         ctx.set_kv_type(gq.KV_F16)  # buffers of both kinds side by side
         kv16 = ctx.kv_create(64, 2, 64)
         both = c + gq.attn(4, 2, 64, kv16, 1024, 64, 0, 32, 2048, 2304, 0.125, EPS, 4096, 4160, 4224)

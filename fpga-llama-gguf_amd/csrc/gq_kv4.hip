@@ -209,13 +209,13 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 //                 multiplied by its scales in FP32. (The quants' bits as they are, 2^-24 n, with the 8 taken off through the
 //                 accumulator's start, are a tenth fewer vector instructions, but the instruction's sums of such small factors keep
 //                 several bits less: results are off by 5e-6 in place of 3e-7.)
-//   P = 2^(S - c) in FP32, c = m - 7 with m the query's running maximum, taken anew only when a score passes it by 8 (so P < 2^15).
-//                 P is the sum of two fp16 numbers, whole multiples of 2^-24 (2^-31 of the largest weight). Lane 16 g + q holds
+//   P = 2^(S - c) in FP32, c = m - 4 with m the query's running maximum, taken anew only when a score passes it by 4 (so P < 2^8).
+//                 P is the sum of two fp16 numbers, whole multiples of 2^-24 (2^-28 of the largest weight). Lane 16 g + q holds
 //                 query q's weights of the 8 positions that it feeds to
-//   O^T += V^T P^T: a value, quant minus 8 times scale, has 15 bits: the sum of two fp16 numbers again (the rounded product and, by a
-//                 fused multiply-add, what is missing). The scales are brought up by a power of two 2^e common to the wave, the
-//                 largest so far to 2^9..2^10, so that the second number is a multiple of 2^-24 too. Three of the four products of
-//                 parts are summed (the fourth is below 2^-22 of the first).
+//   O^T += V^T P^T: the quants minus 8 again; a block's scales go to the weights, P d = h + l: h the rounded product of d and P's upper part, l, by
+//                 two fused multiply-adds, what that rounding left and the lower part's product (22 bits). The scales are
+//                 brought up by a power of two 2^e common to the wave, the largest so far to 2^6..2^7 (so P d < 2^15; a scale 2^21
+//                 below the largest is still a normal number).
 // The accumulators stay with the query's lanes and nothing crosses lanes in the loop. The four waves of a workgroup take the records of
 // its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
 // A record and 16 rows, heads of 256, are 80 matrix instructions and about 600 others, half of them unpacking; wider heads than 128
@@ -593,7 +593,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
         }
     }
     bool sums = false;  // o holds something
-    int e = 15;  // the value scales' exponent: the largest so far times 2^e is below 2^10 (scales below 2^-5 keep 2^15)
+    int e = 15;  // the value scales' exponent: the largest so far times 2^e is below 2^7 (scales below 2^-8 keep 2^15)
     for (; at <= last; at += 4) {
         const uint8_t * ahead = head + size_t(min(at + 4, last)) * kv4_record(HD);  // (the last one again where there is none)
         const int from = at * KV4_TILE;
@@ -609,11 +609,11 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 #pragma unroll
         for (int i = 0; i < Kv4Tile<HD>::NW; ++i) dtop = max(dtop, max(tile.d[i] & 0x7fffu, (tile.d[i] >> 16) & 0x7fffu));
         if (lane < 32) dtop = 0;
-        if (__any(int(dtop >> 10) - 15 + e >= 10)) {  // a larger value scale: bring it to 2^9
+        if (__any(int(dtop >> 10) - 15 + e >= 7)) {  // a larger value scale: bring it to 2^6
             int top = int(dtop >> 10);
 #pragma unroll
             for (int d = 32; d >= 1; d >>= 1) top = max(top, __shfl_xor(top, d, WAVE));
-            const int e2 = 9 + 15 - top;
+            const int e2 = 6 + 15 - top;
             const float f = __uint_as_float(uint32_t(127 + e2 - e) << 23);
             e = e2;
             if (sums)
@@ -668,14 +668,14 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
                     if (p < my_lo[n] || p > my_hi[n]) sc[n][i] = -__builtin_inff();
                 }
             top[n] = fmaxf(fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])), fmaxf(fmaxf(sc[n][4], sc[n][5]), fmaxf(sc[n][6], sc[n][7])));
-            again |= bool(__any(top[n] > c[n] + 15.0f));
+            again |= bool(__any(top[n] > c[n] + 8.0f));
         }
         if (again) {  // new maxima
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 float m = fmaxf(top[n], __shfl_xor(top[n], 16, WAVE));
                 m = fmaxf(m, __shfl_xor(m, 32, WAVE));
-                const float c2 = fmaxf(m - 7.0f, c[n]), f = __builtin_amdgcn_exp2f(c[n] - c2);
+                const float c2 = fmaxf(m - 4.0f, c[n]), f = __builtin_amdgcn_exp2f(c[n] - c2);
                 c[n] = c2;
                 l[n] *= f;
                 if (sums)
@@ -706,21 +706,23 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
         for (int b = 0; b < NB; ++b) {
             const u32x4 vd = *reinterpret_cast<const u32x4 *>(&scales[wave][HD / 2 + (g * NB + b) * 4]);
             const u32x4 v0 = nibbles(tile.v[b][0], k4), v1 = nibbles(tile.v[b][1], k4);  // positions 0, 2, 1, 3 and 4, 6, 5, 7 of the lane's 8
+            u32x4 dh[NQ], dl[NQ];
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {  // the lane's element, and the one 16 further
-                u32x4 vh, vl;
+            for (int n = 0; n < NQ; ++n)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const uint32_t w32 = i < 2 ? v0[2 * u + i] : v1[2 * u + i - 2], d32 = vd[i];
-                    const half2 w = __builtin_bit_cast(half2, w32), d = __builtin_bit_cast(half2, d32), p = w * d;
-                    vh[i] = __builtin_bit_cast(uint32_t, p);
-                    vl[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(w, d, -p));
+                    const uint32_t h32 = ph[n][i], l32 = pl[n][i], d32 = vd[i];
+                    const half2 h = __builtin_bit_cast(half2, h32), d = __builtin_bit_cast(half2, d32), x = h * d;
+                    dh[n][i] = __builtin_bit_cast(uint32_t, x);
+                    dl[n][i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(__builtin_bit_cast(half2, l32), d, __builtin_elementwise_fma(h, d, -x)));
                 }
 #pragma unroll
+            for (int u = 0; u < 2; ++u) {  // the lane's element, and the one 16 further
+                const u32x4 w = {v0[2 * u], v0[2 * u + 1], v1[2 * u], v1[2 * u + 1]};
+#pragma unroll
                 for (int n = 0; n < NQ; ++n) {
-                    o[n][b][u] = mfma(vh, ph[n], o[n][b][u]);
-                    o[n][b][u] = mfma(vh, pl[n], o[n][b][u]);
-                    o[n][b][u] = mfma(vl, ph[n], o[n][b][u]);
+                    o[n][b][u] = mfma(w, dh[n], o[n][b][u]);
+                    o[n][b][u] = mfma(w, dl[n], o[n][b][u]);
                 }
             }
         }

@@ -3,6 +3,7 @@
 #include "gq_kv4.h"
 
 #include <algorithm>
+#include <cfloat>
 #include <type_traits>
 
 namespace gq {
@@ -550,8 +551,9 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
         top = fmaxf(top, dpp_f32<DPP_MIRROR>(top));
         // the largest element to 2^13..2^14 (rows of zeros and the ends of FP32's range: some power of two that does not overflow)
         const int e = min(max(int((__float_as_uint(top) >> 23) & 255), 40), 240);
-        const float up = __uint_as_float(uint32_t(127 + 13 + 127 - e) << 23);
-        if (pc == 0) kqs[n * 16 + (tid >> 4)] = a.scale * 1.44269504088896341f * __uint_as_float(uint32_t(e - 13) << 23);
+        // (with the scale's sign: what brings the products back is positive then, if only just for a scale of 0)
+        const float up = __builtin_copysignf(__uint_as_float(uint32_t(127 + 13 + 127 - e) << 23), a.scale);
+        if (pc == 0) kqs[n * 16 + (tid >> 4)] = fmaxf(fabsf(a.scale) * 1.44269504088896341f * __uint_as_float(uint32_t(e - 13) << 23), FLT_MIN);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int piece = (pc + 16 * i) & (HD / 4 - 1), to = (piece & 3) * 16 + (tid >> 4);  // 8 block + 4 half + g
@@ -570,7 +572,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     }
     __syncthreads();
     u32x4 q[QL ? 1 : NQ][QL ? 1 : NB][2];
-    float kq[NQ];  // what brings the products back: scale * log2(e) over the row's power of two
+    float kq[NQ];  // what brings the products back: |scale| * log2(e) over the row's power of two
     int my_lo[NQ], my_hi[NQ];
     f32x4 o[NQ][NB][2];
     float c[NQ], l[NQ];
@@ -655,7 +657,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 #pragma unroll
             for (int n = 0; n < NQ; ++n)
 #pragma unroll
-                for (int i = 0; i < 8; ++i) sc[n][i] = acc[n][i >> 2][i & 3] * kq[n];
+                for (int i = 0; i < 8; ++i) sc[n][i] = acc[n][i >> 2][i & 3];
         }
         bool again = false;
         float top[NQ];
@@ -667,7 +669,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
                     const int p = from + (i >> 2) * 16 + 4 * g + (i & 3);
                     if (p < my_lo[n] || p > my_hi[n]) sc[n][i] = -__builtin_inff();
                 }
-            top[n] = fmaxf(fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])), fmaxf(fmaxf(sc[n][4], sc[n][5]), fmaxf(sc[n][6], sc[n][7])));
+            top[n] = fmaxf(fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])), fmaxf(fmaxf(sc[n][4], sc[n][5]), fmaxf(sc[n][6], sc[n][7]))) * kq[n];
             again |= bool(__any(top[n] > c[n] + 8.0f));
         }
         if (again) {  // new maxima
@@ -691,7 +693,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) sc[n][i] = __builtin_amdgcn_exp2f(sc[n][i] - c[n]);
+            for (int i = 0; i < 8; ++i) sc[n][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[n][i], kq[n], -c[n]));
             l[n] += ((sc[n][0] + sc[n][1]) + (sc[n][2] + sc[n][3])) + ((sc[n][4] + sc[n][5]) + (sc[n][6] + sc[n][7]));
 #pragma unroll
             for (int i = 0; i < 4; ++i) {

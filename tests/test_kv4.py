@@ -195,6 +195,27 @@ def test_keys_with_an_outlier_channel(gq, hip, hd):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("scale", [0.0, -0.0, -0.2, 1e-30, 30.0])
+def test_attention_scales(gq, hip, scale):
+    """A scale of either sign, none at all (the mean of the values), and ends of its range."""
+    nh, nkv, hd, n = 4, 2, 128, 210
+    rng = np.random.default_rng(17)
+    k, v = _data(rng, 1, n, nkv, hd)
+    q = rng.standard_normal((1, 3, nh, hd)).astype(np.float32)
+    q[0, 1] = 0
+    kv, _ = _cache(gq, hip, 1, n, nkv, hd)
+    _store(gq, hip, kv, k, v, [0])
+    y = _attend(gq, hip, kv, q, [n - 3], None, 0, scale)
+    scale = float(np.float32(scale))
+    for t in range(3):
+        for h in range(nh):
+            # the bound takes the scale's magnitude
+            want, tol = ref.attention(np.sign(scale) * q[0, t, h].astype(np.float64), ref.values(k)[0, :, h // 2], ref.values(v)[0, :, h // 2], n - 3 + t, 0,
+                                      abs(scale))
+            assert (np.abs(y[0, t, h] - want) <= tol).all(), (t, h)
+
+
+@pytest.mark.gpu
 def test_attention_strides(gq, hip):
     """Queries interleaved with gates, rows apart from one another; y rows apart, what is between them untouched."""
     nh, nkv, hd, n_tok, n = 4, 2, 64, 5, 130

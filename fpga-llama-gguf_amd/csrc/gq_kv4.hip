@@ -496,7 +496,9 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     __shared__ __align__(16) uint8_t both[QBYTES > JBYTES ? QBYTES : JBYTES];
     u32x4(*ql)[64] = reinterpret_cast<u32x4(*)[64]>(both);              // the queries' parts
     float(*part)[ROWS][PAD] = reinterpret_cast<float(*)[ROWS][PAD]>(both);  // later the waves' sums
-    constexpr bool QL = HD * NQ > 128;  // the queries stay in LDS where registers would not leave room for two waves a SIMD
+    // The queries' parts that stay in registers, as many as leave room for two waves a SIMD (512 tokens at 7680, us with two, one and none:
+    // 16/4 heads of 256 184.9 / 187.8 / 192.4, 32/8 of 128 no room / 172.1 / 176.5). The others are read from LDS for every record.
+    constexpr int QR = NQ == 1 || HD * NQ <= 128 ? 2 : 1;
     __shared__ float kqs[ROWS], cs[4][ROWS], ls[4][ROWS];
     __shared__ __align__(16) uint32_t scales[4][HD];  // a wave's record's key scales, then its value scales: [g][block][8] each
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
@@ -571,7 +573,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
         }
     }
     __syncthreads();
-    u32x4 q[QL ? 1 : NQ][QL ? 1 : NB][2];
+    u32x4 q[NQ][NB][QR];
     float kq[NQ];  // what brings the products back: |scale| * log2(e) over the row's power of two
     int my_lo[NQ], my_hi[NQ];
     f32x4 o[NQ][NB][2];
@@ -588,10 +590,8 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 #pragma unroll
         for (int b = 0; b < NB; ++b) {
             o[n][b][0] = o[n][b][1] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (!QL) {
-                q[n][b][0] = ql[(n * NB + b) * 2][lane];
-                q[n][b][1] = ql[(n * NB + b) * 2 + 1][lane];
-            }
+#pragma unroll
+            for (int i = 0; i < QR; ++i) q[n][b][i] = ql[(n * NB + b) * 2 + i][lane];
         }
     }
     bool sums = false;  // o holds something
@@ -646,8 +646,8 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
                     const u32x4 kk = nibbles(tile.k[u][b], k4);
 #pragma unroll
                     for (int n = 0; n < NQ; ++n) {
-                        f32x4 x = mfma(kk, QL ? ql[(n * NB + b) * 2][lane] : q[QL ? 0 : n][QL ? 0 : b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
-                        x = mfma(kk, QL ? ql[(n * NB + b) * 2 + 1][lane] : q[QL ? 0 : n][QL ? 0 : b][1], x);
+                        f32x4 x = mfma(kk, q[n][b][0], f32x4{0.0f, 0.0f, 0.0f, 0.0f});
+                        x = mfma(kk, QR == 2 ? q[n][b][QR - 1] : ql[(n * NB + b) * 2 + 1][lane], x);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) acc[n][u][i] = __builtin_fmaf(x[i], half_of(kd[2 * u + (i & 1)], i >> 1), acc[n][u][i]);
                     }

@@ -219,17 +219,18 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 //                 below the largest is still a normal number).
 // The accumulators stay with the query's lanes and nothing crosses lanes in the loop. The four waves of a workgroup take the records of
 // its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
-// A record and 16 rows, heads of 256, are 80 matrix instructions and about 600 others, half of them unpacking; wider heads than 128
+// A record and 16 rows, heads of 256, are 64 matrix instructions and about 540 others, half of them unpacking; wider heads than 128
 // leave no registers for more than 16 rows to share that. What bounds it, by the counters:
-//   512 tokens at 7680, 16/4 heads of 256: 206 us, 320 TFLOP/s of the formula's 66.6 GFLOP (2.5 times that in parts). Vector instructions
-//     are issued in 61 % of the cycles and matrix instructions run in 33 %, on the same SIMDs with little overlap.
-//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 42 us, 3.6 TB/s; vector instructions in 48 %, matrix instructions in 19 %, the
-//     rest the beginnings and ends of workgroups that have some ten records a wave.
-//   one sequence of 32768, 16/4 heads of 256 (38 MB): 14.8 us, 2.5 TB/s, two records a wave: the chain of position, record, sums and
-//     joining is half of it; of 640: 7.3 us, that chain alone.
-// Tried and taken back: workgroups whose waves share one record's unpacking for 64 rows through LDS (two barriers a record; 190 us and
-// 16 us of joining for the 512 tokens), 32 rows a wave at heads of 256 with one wave a SIMD (244 us), matrix instructions at a raised
-// wave priority (188 us in place of 191 there, 52.6 in place of 51.9 for the 32 sequences).
+//   512 tokens at 7680, 16/4 heads of 256: 180 us, 370 TFLOP/s of the formula's 66.6 GFLOP (twice that in parts). Vector instructions are
+//     issued in 64 % of the cycles, and without any matrix instruction it would still be 159 us: each hundred instructions less a
+//     record are 21 us.
+//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 41.6 us, 3.7 TB/s; vector instructions in 47 %, matrix instructions in 16 %,
+//     the rest the beginnings and ends of workgroups that have some ten records a wave.
+//   one sequence of 32768, 16/4 heads of 256 (38 MB): 14.5 us, 2.6 TB/s, two records a wave: the chain of position, record, sums and
+//     joining is half of it; of 640: 7.2 us, that chain alone.
+// Tried and taken back, for the 512 tokens, then at 202 us: workgroups whose waves share one record's unpacking for 64 rows through LDS
+// (two barriers a record; 190 us and 16 us of joining); 32 rows a wave at heads of 256 with one wave a SIMD (244 us). A raised wave
+// priority around the matrix instructions, and other orders of them, change less than 1 %.
 typedef _Float16 half2 __attribute__((ext_vector_type(2)));
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));

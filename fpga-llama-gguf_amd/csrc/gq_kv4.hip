@@ -213,10 +213,10 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 //   P = 2^(S - c) in FP32, c = m - 4 with m the query's running maximum, taken anew only when a score passes it by 4 (so P < 2^8).
 //                 P is the sum of two fp16 numbers, whole multiples of 2^-24 (2^-28 of the largest weight). Lane 16 g + q holds
 //                 query q's weights of the 8 positions that it feeds to
-//   O^T += V^T P^T: the quants minus 8 again; a block's scales go to the weights, P d = h + l: h the rounded product of d and P's upper part, l, by
-//                 two fused multiply-adds, what that rounding left and the lower part's product (22 bits). The scales are
-//                 brought up by a power of two 2^e common to the wave, the largest so far to 2^6..2^7 (so P d < 2^15; a scale 2^21
-//                 below the largest is still a normal number).
+//   O^T += V^T P^T: the quants minus 8 again; a block's scales go to the weights, P d = h + l: h the rounded product of d and P's upper
+//                 part, l, by two fused multiply-adds, what that rounding left and the lower part's product (22 bits). The scales
+//                 are brought up by a power of two 2^e common to the wave, the largest so far to 2^6..2^7 (so P d < 2^15; a scale
+//                 2^21 below the largest is still a normal number).
 // The accumulators stay with the query's lanes and nothing crosses lanes in the loop. The four waves of a workgroup take the records of
 // its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
 // A record and 16 rows, heads of 256, are 64 matrix instructions and about 540 others, half of them unpacking; wider heads than 128
@@ -790,7 +790,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 
 // Workgroup (q head and EL of its elements, token, sequence): the sets of a sequence with several ranges. The factors of all sets
 // first, then EL / 4 threads a set, 1024 / EL sets at a time. 128 sets of 16 heads of 256 (2.1 MB): 4.4 us with 64 elements a
-// workgroup, three trips to memory in a row; 32 sequences' up to 96 sets of 32 heads of 128: 7.6 us.
+// workgroup, two trips to memory in a row (positions, sets); 32 sequences' up to 96 sets of 32 heads of 128: 7.6 us.
 template <int HD, int EL>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     constexpr int PER = EL / 4, SETS = 256 / PER;

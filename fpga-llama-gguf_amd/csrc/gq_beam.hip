@@ -9,9 +9,9 @@ namespace gq {
 namespace {
 
 // ---- selection ----
-// Two launches. The first reads every logit once: workgroup (256 * PER logits of a row) forms their maximum m and
-// sum of e^(x - m), and their n_beam best in order. The second, a workgroup per group, joins the rows' sums, and takes the best
-// candidate off the sorted lists n_beam times. Values are 64-bit from the logits on (candidates of two beams may lie next to each
+// Two launches. The first reads every logit once: workgroup (256 * PER logits of a row) forms their maximum m and sum of e^(x - m), and
+// their n_beam best in order. The second, a workgroup per group, joins the rows' sums, and takes the best candidate off the sorted
+// lists n_beam times (or, of many, merges them). Values are 64-bit from the logits on (candidates of two beams may lie next to each
 // other). A list entry is one word that orders as the candidates of one row do: the logit's bits made monotone, above the token
 // inverted.
 // 8 groups of 8 beams of 151936 logits (39 MB): 17.0 us (2.3 TB/s: a workgroup's own way of read, reduce and rank is 7 us,
@@ -509,88 +509,106 @@ __global__ __launch_bounds__(256) void beam_pick_wave_kernel(BeamSelectArgs a) {
     if (tid < k) beam_write(a, g, sh, tid);
 }
 
-// More lists: sixteen waves, a thread the heads of up to 4 lists.
-__global__ __launch_bounds__(1024) void beam_pick_kernel(BeamSelectArgs a) {
-    constexpr int OWN = 4, T = 1024, W = T / 64;
+// A better candidate of the pair keeps the lane where `first`, the other one the lane's partner.
+__device__ __forceinline__ void beam_exchange(double & v, uint32_t & id, double v2, uint32_t i2, bool first) {
+    const bool take = beam_better(v2, i2, v, id) == first;
+    v = take ? v2 : v;
+    id = take ? i2 : id;
+}
+template <int XOR>
+__device__ __forceinline__ void beam_stage(double & v, uint32_t & id, int lane) {  // lanes XOR apart, in groups of 32
+    constexpr int PATTERN = XOR << 10 | 0x1f;
+    const long long x = __double_as_longlong(v);
+    const int lo = __builtin_amdgcn_ds_swizzle(int(x), PATTERN), hi = __builtin_amdgcn_ds_swizzle(int(x >> 32), PATTERN);
+    const uint32_t i2 = uint32_t(__builtin_amdgcn_ds_swizzle(int(id), PATTERN));
+    beam_exchange(v, id, __hiloint2double(hi, lo), i2, (lane & XOR) == 0);
+}
+// 32 lanes' candidates, in order, become the best 32 of them and of another 32 in order, whose number 31 - lane the lane brings.
+__device__ __forceinline__ void beam_merge(double & v, uint32_t & id, double v2, uint32_t i2, int lane) {
+    beam_exchange(v, id, v2, i2, true);  // the best 32, rising and then falling
+    beam_stage<16>(v, id, lane);
+    beam_stage<8>(v, id, lane);
+    beam_stage<4>(v, id, lane);
+    beam_stage<2>(v, id, lane);
+    beam_stage<1>(v, id, lane);
+}
+
+// Many winners, or many lists: halves of waves each merge their share of the lists into their best 32 in order (a list whose head is no
+// better than the k-th so far is passed by), and those then pairwise.
+__global__ __launch_bounds__(1024) void beam_pick_merge_kernel(BeamSelectArgs a) {
+    constexpr int T = 1024, H = T / 32;
     __shared__ BeamShared sh;
-    __shared__ double bestv[2][W];
-    __shared__ uint32_t besti[2][W];
-    const int g = blockIdx.x, k = a.n_beam, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lists = k * a.chunks;
+    __shared__ double bestv[H / 2][32];
+    __shared__ uint32_t besti[H / 2][32];
+    const int g = blockIdx.x, k = a.n_beam, tid = threadIdx.x, lane = tid & 31, half = tid >> 5, lists = k * a.chunks;
     BeamLists li;
     if (!beam_fetch<T>(a, g, sh, li)) return;
-    double v[OWN];
-    uint32_t id[OWN];
-    int taken[OWN];
-#pragma unroll
-    for (int i = 0; i < OWN; ++i) {
-        taken[i] = 0;
-        v[i] = -__builtin_inf();
-        id[i] = BEAM_NONE;
-        if (tid + i * T < lists) li.at(a, tid + i * T, 0, v[i], id[i]);
+    double v = -__builtin_inf();
+    uint32_t id = BEAM_NONE;
+    const int there = 31 - lane;
+    for (int l = half; l < lists; l += H) {
+        double hv, v2 = -__builtin_inf();
+        uint32_t hi, i2 = BEAM_NONE;
+        li.at(a, l, 0, hv, hi);
+        const bool worth = beam_better(hv, hi, __shfl(v, k - 1, 32), uint32_t(__shfl(int(id), k - 1, 32)));
+        if (!__any(worth)) continue;
+        if (worth && there < k) li.at(a, l, there, v2, i2);
+        beam_merge(v, id, v2, i2, lane);
     }
-    for (int j = 0; j < k; ++j) {
-        double bv;
-        uint32_t bi;
-        beam_best<OWN>(v, id, bv, bi);
-        const double wv = wave_best(bv);
-        const uint32_t wi = wave_u32(bv == wv ? bi : BEAM_NONE, min_u);
-        if (lane == 0) {
-            bestv[j & 1][wave] = wv;
-            besti[j & 1][wave] = wi;
+    for (int n = H / 2; n >= 1; n /= 2) {
+        if (half >= n && half < 2 * n) {
+            bestv[half - n][there] = v;
+            besti[half - n][there] = id;
         }
         __syncthreads();
-        bv = bestv[j & 1][0];
-        bi = besti[j & 1][0];
-#pragma unroll
-        for (int w = 1; w < W; ++w)
-            if (beam_better(bestv[j & 1][w], besti[j & 1][w], bv, bi)) {
-                bv = bestv[j & 1][w];
-                bi = besti[j & 1][w];
-            }
-        if (tid == 0) {
-            sh.won[j] = bv;
-            sh.taken[j] = bi;
-        }
-#pragma unroll
-        for (int i = 0; i < OWN; ++i)
-            if (id[i] == bi) li.at(a, tid + i * T, ++taken[i], v[i], id[i]);  // the list's next entry becomes its head
+        if (half < n) beam_merge(v, id, bestv[half][lane], besti[half][lane], lane);
+        __syncthreads();
     }
-    __syncthreads();
-    if (tid < k) beam_write(a, g, sh, tid);
+    if (tid < k) {
+        sh.won[tid] = v;
+        sh.taken[tid] = id;
+        beam_write(a, g, sh, tid);
+    }
 }
 
 // ---- reordering ----
 // Workgroup (4 KB of one part of an array, group): a thread takes the same 16 bytes of all the group's rows, first
 // the sources of every row that changes, then the writes: in place, each moved byte read from HBM and written once (a source with
 // several heirs is read again from the caches). Rows that stay cost nothing. Bound by the memory: 4 groups of 8, 8 caches of 2000
-// positions (2.3 GB read and written): 438 us, 5.3 TB/s; one group of 4 with 24 layers of states (327 MB): 65 us, 5.0 TB/s.
+// positions (2.3 GB read and written): 419 us, 5.5 TB/s; one group of 4 with 24 layers of states (327 MB): 66 us, 5.0 TB/s. Few and
+// short arrays: three trips to memory (one group of 15, 2.6 MB: 8.4 us).
+
+// The rows from I on at `at` in the tile: row I's source is read, the further rows' all follow, then row I is written. (A recursion:
+// with an array of 8 pieces the compiler keeps one value of 32 registers, and copies of it.)
+template <int I, int NB, typename V>
+__device__ __forceinline__ void beam_rows_move(uint8_t * at, int off, int bytes, int p, unsigned long long row_stride) {
+    if constexpr (I < NB) {
+        const bool on = off < __builtin_amdgcn_readlane(bytes, I);
+        V x = {};
+        if (on) x = *reinterpret_cast<const V *>(at + __builtin_amdgcn_readlane(p, I) * row_stride);
+        beam_rows_move<I + 1, NB, V>(at, off, bytes, p, row_stride);
+        if (on) *reinterpret_cast<V *>(at + I * row_stride) = x;
+    }
+}
+
+// Each wave's lanes look at a row each first: its parent and the bytes that move, which all lanes then take from there.
 template <int NB, typename V>
 __device__ __forceinline__ void beam_move(const BeamMove & m, const int32_t * parent, int slot, uint8_t * part, unsigned long long from, int n_beam,
                                           int row0) {
-    constexpr int STEP = 256 * sizeof(V), N = BEAM_TILE / STEP;
-    for (int it = 0; it < N; ++it) {
-        const unsigned long long off = from + it * STEP + threadIdx.x * sizeof(V);
-        V x[NB];
-        bool moved[NB];
-#pragma unroll
-        for (int i = 0; i < NB; ++i) {
-            moved[i] = false;
-            if (i >= n_beam) continue;
-            const int p = parent[size_t(row0 + i) * slot];
-            if (p == i || p < 0 || p >= n_beam) continue;
-            unsigned long long hi = m.hi;
-            if (m.used) {
-                const long long u = (long long)m.used[size_t(row0 + p) * m.used_stride] + m.used_more;
-                const unsigned long long units = u > 0 ? ((unsigned long long)u + m.unit_len - 1) / m.unit_len : 0;
-                hi = min(hi, units * m.unit_bytes);
-            }
-            moved[i] = off < hi;
-            if (moved[i]) x[i] = *reinterpret_cast<const V *>(part + p * m.row_stride + off);
-        }
-#pragma unroll
-        for (int i = 0; i < NB; ++i)
-            if (moved[i]) *reinterpret_cast<V *>(part + i * m.row_stride + off) = x[i];
+    const int lane = threadIdx.x & 63;
+    int p = lane < n_beam ? parent[size_t(row0 + lane) * slot] : -1;
+    if (p == lane || p >= n_beam) p = -1;
+    unsigned long long hi = p < 0 ? 0 : m.hi;
+    if (m.used && p >= 0) {
+        const long long u = (long long)m.used[size_t(row0 + p) * m.used_stride] + m.used_more;
+        const unsigned long long units = u > 0 ? ((unsigned long long)u + m.unit_len - 1) / m.unit_len : 0;
+        hi = min(hi, units * m.unit_bytes);
     }
+    const int bytes = hi > from ? int(min(hi - from, (unsigned long long)BEAM_TILE)) : 0;  // of this tile
+    if (!__any(bytes > 0)) return;
+#pragma unroll 1
+    for (int off = threadIdx.x * sizeof(V); off < int(BEAM_TILE); off += 256 * sizeof(V))
+        beam_rows_move<0, NB, V>(part + from + off, off, bytes, p, m.row_stride);
 }
 
 template <int NB>
@@ -635,6 +653,11 @@ size_t beam_work(int n_group, int n_beam, int n_vocab) {
     return size_t(rows) * beam_chunks(n_vocab, per) * (sizeof(BeamStat) + 8 * size_t(n_beam));
 }
 
+// Winners from which on the lists are merged; also where a group has more lists than a wave's registers take the heads of. Both
+// kernels, winners one by one and merged: 25.3 and 26.1 us at 8 groups of 8 of 151936, 18.4 and 17.5 at one of 10 of 151936, 29.2 and
+// 26.3 at 4 of 12, 57 and 38 at one of 32; 32.3 and 25.3 at 17 of 29 of 4687. One by one with 2 and 5 lists a lane: 12.5 and 13.9 us at
+// one of 8 of 32000.
+constexpr int BEAM_MANY = 10;
 hipError_t launch_beam_select(const BeamSelectArgs & args, hipStream_t s) {
     BeamSelectArgs a = args;
     const int rows = a.n_group * a.n_beam;
@@ -647,14 +670,12 @@ hipError_t launch_beam_select(const BeamSelectArgs & args, hipStream_t s) {
     else GQ_LAUNCH(beam_scan_kernel<8>, grid, dim3(256), lds, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    // lists of a group: at most 32 * 128. A second kernel for up to 128, 320 and 640 lists and for more, us with the next one in its
-    // place: 12.5 and 13.9 at 128 lists of 8 winners, 12.8 and 14.3 at 300 of 4, 56 and 74 at 608 of 32.
+    // lists of a group: at most 32 * 128
     const int lists = a.n_beam * a.chunks;
     const dim3 groups(unsigned(a.n_group));
-    if (lists <= 64 * 2) GQ_LAUNCH(beam_pick_wave_kernel<2>, groups, dim3(256), 0, s, a);
-    else if (lists <= 64 * 5) GQ_LAUNCH(beam_pick_wave_kernel<5>, groups, dim3(256), 0, s, a);
-    else if (lists <= 64 * 10) GQ_LAUNCH(beam_pick_wave_kernel<10>, groups, dim3(256), 0, s, a);
-    else GQ_LAUNCH(beam_pick_kernel, groups, dim3(1024), 0, s, a);
+    if (a.n_beam >= BEAM_MANY || lists > 64 * 5) GQ_LAUNCH(beam_pick_merge_kernel, groups, dim3(1024), 0, s, a);
+    else if (lists <= 64 * 2) GQ_LAUNCH(beam_pick_wave_kernel<2>, groups, dim3(256), 0, s, a);
+    else GQ_LAUNCH(beam_pick_wave_kernel<5>, groups, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

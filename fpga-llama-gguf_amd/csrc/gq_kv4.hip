@@ -790,7 +790,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 
 // Workgroup (q head and EL of its elements, token, sequence): the sets of a sequence with several ranges. The factors of all sets
 // first, then EL / 4 threads a set, 1024 / EL sets at a time. 128 sets of 16 heads of 256 (2.1 MB): 4.4 us with 64 elements a
-// workgroup, two trips to memory in a row (positions, sets); 32 sequences' up to 96 sets of 32 heads of 128: 7.6 us.
+// workgroup, two trips to memory in a row (positions, sets).
 template <int HD, int EL>
 __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     constexpr int PER = EL / 4, SETS = 256 / PER;
@@ -848,6 +848,55 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     kv4_out<HD>(a, size_t(s) * a.t.n_tok + t, hq, e0 + e, y, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
 }
 
+// The same for many rows (q heads of tokens): a wave `per_wave` of them one after another, its lanes HD / 4 to a set. What each workgroup does
+// before its first row (finding the sequence's ranges, 2 us) is shared by its rows. 3 sequences of 360 tokens of 8 heads of 64: 14 us.
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_join_rows_kernel(Kv4AttnArgs a, int per_wave) {
+    constexpr int PER = HD / 4, SETS = 64 / PER;
+    const int lane = threadIdx.x & 63, sub = lane / PER, e = lane % PER * 4;
+    int s = blockIdx.y;
+    Kv4Range r;
+    if (!kv4_find<false>(a, 0, s, r) || r.tiles <= r.per) return;
+    const int rows = a.t.n_tok * a.n_head, row0 = int(blockIdx.x * 4 + (threadIdx.x >> 6)) * per_wave;
+    const size_t step = size_t(a.t.n_tok) * a.n_head * (HD + 4);
+    for (int row = row0; row < min(row0 + per_wave, rows); ++row) {
+        const int t = int(unsigned(row) / unsigned(a.n_head)), hq = row - t * a.n_head;
+        const long long p = r.p0 + t;
+        if (t >= r.n || p < 0 || p >= a.c.n_ctx) continue;
+        const int k0 = ((a.window && p >= a.window ? int((p - a.window + 1) / KV4_TILE) : 0) - r.first) / r.per;
+        const int n = (int(p / KV4_TILE) - r.first) / r.per - k0 + 1;
+        const float * w = a.work + size_t(r.slot + k0) * step + size_t(row) * (HD + 4);
+        f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+        float C = KV4_LOW, L = 0.0f;
+        for (int b = 0; b < n; b += 64) {  // 64 sets (often all) at a time
+            const float2 cl = b + lane < n ? *reinterpret_cast<const float2 *>(w + (b + lane) * step + HD) : float2{KV4_LOW, 0.0f};
+            const float top = fmaxf(wave_max(cl.x), C), old = __builtin_amdgcn_exp2f(C - top), f = __builtin_amdgcn_exp2f(cl.x - top);
+            C = top;
+            L = L * old + cl.y * f;  // the lane's own sets'
+            y *= old;
+            const int m = min(n - b, 64);
+            for (int j0 = sub; j0 < m + sub; j0 += 4 * SETS) {  // (as often in every lane)
+                f32x4 x[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    x[i] = j0 + i * SETS < m ? *reinterpret_cast<const f32x4 *>(w + (b + j0 + i * SETS) * step + e) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float fj = __shfl(f, (j0 + i * SETS) & 63, WAVE);
+                    if (j0 + i * SETS < m) y += x[i] * fj;
+                }
+            }
+        }
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) L += __shfl_xor(L, d, WAVE);
+#pragma unroll
+        for (int d = 32; d >= PER; d >>= 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], d, WAVE);
+        if (sub == 0) kv4_out<HD>(a, size_t(s) * a.t.n_tok + t, hq, e, y, L);
+    }
+}
+
 template <typename F>
 hipError_t by_dim(int hd, F f) {
     switch (hd) {
@@ -895,8 +944,12 @@ int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     const int per_kv = n_head / c.n_head_kv, nq = kv4_nq(c.head_dim, n_tok, per_kv), rows = 16 * nq;
     const int groups = 256 * kv4_resident(c.head_dim, nq);
     const long long units = (n_tok * (long long)per_kv + rows - 1) / rows * c.n_head_kv;
-    const long long most = (long long)n_seq * ((kv4_tiles(c.n_ctx) + KV4_LEAST - 1) / KV4_LEAST);
-    return int(std::min<long long>(std::max<long long>(n_seq, std::min(groups / units, most)), 65535));
+    const long long records = (long long)n_seq * kv4_tiles(c.n_ctx), most = (long long)n_seq * ((kv4_tiles(c.n_ctx) + KV4_LEAST - 1) / KV4_LEAST);
+    long long ranges = std::max<long long>(n_seq, std::min(groups / units, most));
+    // Few long ranges for sequences of unlike lengths come out unlike themselves: twice as many (3 sequences of 96 tokens at up to 10776,
+    // 32/8 heads of 128: 58 and 79 us; one of 512 at 7680, 16/4 heads of 256, 192 and 185; 3 of 360 at 1451, 8 heads of 64, 49 and 42).
+    if (n_seq > 1 && records >= 128 * ranges) ranges = std::max<long long>(ranges, std::min<long long>(2 * ranges, KV4_GROUPS));
+    return int(std::min<long long>(ranges, 65535));
 }
 
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
@@ -906,6 +959,10 @@ size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
 
 bool kv4_joins(const Kv4AttnArgs & a) { return a.work && kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head) > a.t.n_seq; }
 
+// Rows (q heads of tokens) up to which each has workgroups of its own: several up to half as many. us with several, one, and a wave's share
+// of one: 26.7 / 24.7 / 25.3 at 320 rows, 30.8 / 30.4 / 32.2 at 352 (of 23 sets), 47.7 / 45.2 / 45.5 at 512, 55.6 / 51.4 / 49.7 at 1024,
+// - / 61.2 / 41.7 at 8640.
+constexpr int KV4_FEW = 512;
 hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
     Kv4AttnArgs a = args;
     const int per_kv = a.n_head / a.c.n_head_kv, nq = kv4_nq(a.c.head_dim, a.t.n_tok, per_kv);
@@ -919,12 +976,16 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
         if constexpr (hd.value < 128)
             if (nq == 4) GQ_LAUNCH((kv4_attn_kernel<hd.value, 4>), grid, dim3(256), 0, s, a);
         if (a.ranges <= a.t.n_seq) return;
-        // one sequence's sets may be many: then more, narrower workgroups
-        constexpr int narrow = hd.value < 64 ? 32 : 64;
-        if (a.t.n_seq * (long long)a.t.n_tok * a.n_head <= 256)
+        const long long rows = a.t.n_tok * (long long)a.n_head, all = a.t.n_seq * rows;
+        if (all <= KV4_FEW / 2) {
+            constexpr int narrow = hd.value < 64 ? 32 : 64;
             GQ_LAUNCH((kv4_join_kernel<hd.value, narrow>), dim3(a.n_head * (hd.value / narrow), a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
-        else
+        } else if (all <= KV4_FEW) {
             GQ_LAUNCH((kv4_join_kernel<hd.value, hd.value>), dim3(a.n_head, a.t.n_tok, a.t.n_seq), dim3(256), 0, s, a);
+        } else {
+            const int per_wave = int(std::min<long long>(std::max<long long>(all / 4096, 1), 16));
+            GQ_LAUNCH(kv4_join_rows_kernel<hd.value>, dim3(unsigned((rows + 4 * per_wave - 1) / (4 * per_wave)), a.t.n_seq), dim3(256), 0, s, a, per_wave);
+        }
     });
 }
 

@@ -221,10 +221,10 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 // its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
 // A record and 16 rows, heads of 256, are 64 matrix instructions and about 540 others, half of them unpacking; wider heads than 128
 // leave no registers for more than 16 rows to share that. What bounds it, by the counters:
-//   512 tokens at 7680, 16/4 heads of 256: 180 us, 370 TFLOP/s of the formula's 66.6 GFLOP (twice that in parts). Vector instructions are
+//   512 tokens at 7680, 16/4 heads of 256: 179 us, 370 TFLOP/s of the formula's 66.6 GFLOP (twice that in parts). Vector instructions are
 //     issued in 64 % of the cycles, and without any matrix instruction it would still be 159 us: each hundred instructions less a
 //     record are 21 us.
-//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 41.6 us, 3.7 TB/s; vector instructions in 47 %, matrix instructions in 16 %,
+//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 39 us, 3.9 TB/s; vector instructions in 47 %, matrix instructions in 16 %,
 //     the rest the beginnings and ends of workgroups that have some ten records a wave.
 //   one sequence of 32768, 16/4 heads of 256 (38 MB): 14.5 us, 2.6 TB/s, two records a wave: the chain of position, record, sums and
 //     joining is half of it; of 640: 7.2 us, that chain alone.

@@ -125,6 +125,13 @@ __device__ __forceinline__ bool beam_prompted(const BeamSelectArgs & a, int row,
     return next >= 0 && next < min(a.n_prompt[size_t(row) * a.slot], a.cap);
 }
 
+// Orders a wave's LDS writes before its other lanes' reads (a wave's LDS operations are carried out in order).
+__device__ __forceinline__ void wave_lds() {
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 template <int PER>
 __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     constexpr int CH = 256 * PER;
@@ -132,6 +139,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     __shared__ float red[4];
     __shared__ double sums[4];
     __shared__ int count[4];
+    __shared__ unsigned long long best[4][BEAM_MAX];
     const int row = blockIdx.y, chunk = blockIdx.x, k = a.n_beam, tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), v0 = chunk * CH, cap = (k + BEAM_SLACK) * PER;
     const size_t at = size_t(row) * a.chunks + chunk;
@@ -249,27 +257,38 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     if (lane == 0) {
         red[wave] = wm;
         sums[wave] = sum;
-        count[wave] = have;
+        count[wave] = min(have, k);
     }
-    __syncthreads();
-    // ---- the chunk's: each candidate's place is the number of better ones ----
-    int all = 0;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) all += count[w];
+    // ---- in order: the wave's, each candidate's place being the number of better ones; then the chunk's, a place further for every better
+    // one of the other waves ----
+    wave_lds();
+    if (lane < BEAM_MAX && lane >= have) best[wave][lane] = 0;
     for (int i = lane; i < have; i += 64) {
         const unsigned long long key = mylist[i];
         int place = 0;
-        for (int w = 0; w < 4; ++w)
-            for (int j = 0, c = count[w]; j < c; j += 8) {
-                unsigned long long y[8];
+        for (int j = 0; j < have; j += 8) {
+            unsigned long long y[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) y[e] = list[w * cap + j + e];
+            for (int e = 0; e < 8; ++e) y[e] = mylist[j + e];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) place += y[e] > key;
-            }
+            for (int e = 0; e < 8; ++e) place += y[e] > key;
+        }
+        if (place < BEAM_MAX) best[wave][place] = key;
+    }
+    __syncthreads();
+    if (lane < count[wave]) {
+        const unsigned long long key = best[wave][lane];
+        int before[3] = {0, 0, 0};
+#pragma unroll
+        for (int st = BEAM_MAX / 2; st >= 1; st /= 2)
+#pragma unroll
+            for (int w = 0; w < 3; ++w) before[w] += best[(wave + 1 + w) & 3][before[w] + st - 1] > key ? st : 0;
+        int place = lane;
+#pragma unroll
+        for (int w = 0; w < 3; ++w) place += before[w] + (best[(wave + 1 + w) & 3][before[w]] > key);
         if (place < k) out[place] = key;
     }
-    for (int i = all + tid; i < k; i += 256) out[i] = 0;
+    for (int i = count[0] + count[1] + count[2] + count[3] + tid; i < k; i += 256) out[i] = 0;
     if (tid == 0) {
         const float m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
         double s = 0.0;
@@ -442,13 +461,6 @@ __device__ __forceinline__ double wave_best(double x) {
     step(integral_constant<int, 0x143>(), integral_constant<int, 0xc>());  // row_bcast:31 into rows 2 and 3
     const long long y = __double_as_longlong(x);
     return __hiloint2double(__builtin_amdgcn_readlane(int(y >> 32), 63), __builtin_amdgcn_readlane(int(y), 63));
-}
-
-// Orders a wave's LDS writes before its other lanes' reads (a wave's LDS operations are carried out in order).
-__device__ __forceinline__ void wave_lds() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 // Workgroup per group of up to 64 * OWN lists: after the rows' sums its first wave alone, one winner a step. A lane holds the heads of

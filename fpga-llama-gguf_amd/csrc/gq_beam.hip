@@ -14,10 +14,10 @@ namespace {
 // lists n_beam times (or, of many, merges them). Values are 64-bit from the logits on (candidates of two beams may lie next to each
 // other). A list entry is one word that orders as the candidates of one row do: the logit's bits made monotone, above the token
 // inverted.
-// 8 groups of 8 beams of 151936 logits (39 MB): 17.0 us (2.3 TB/s: a workgroup's own way of read, reduce and rank is 7 us,
-// the 64-bit exponentials another 5, partly behind the reads) and 8.5 us, of which n_beam steps of about 0.4 us that wait for one
-// another; one group of 4: 7.4 and 4.7 us, both latency.
-constexpr int BEAM_SLACK = 8;
+// 8 groups of 8 beams of 151936 logits (39 MB): 16.3 us (2.4 TB/s: a workgroup's own way of read, reduce and rank is 7 us, the 64-bit
+// exponentials another 5, partly behind the reads) and 8.4 us, of which n_beam steps of about 0.4 us that wait for one another; one
+// group of 4: 7.0 and 4.7 us, both latency.
+constexpr int BEAM_SLACK = 4;  // lanes beyond n_beam that a bound may let pass (24.4, 24.6 and 25.1 us with 4, 8 and 16 there)
 
 __device__ __forceinline__ uint32_t order_of(float x) {  // monotone in x, > 0 for every number
     const uint32_t b = __float_as_uint(x);

@@ -259,8 +259,8 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         sums[wave] = sum;
         count[wave] = min(have, k);
     }
-    // ---- in order: the wave's, each candidate's place being the number of better ones; then the chunk's, a place further for every better
-    // one of the other waves ----
+    // ---- in order: the wave's, each candidate's place being the number of better ones; then the chunk's, a place further for every
+    // better one of the other waves ----
     wave_lds();
     if (lane < BEAM_MAX && lane >= have) best[wave][lane] = 0;
     for (int i = lane; i < have; i += 64) {

@@ -51,11 +51,11 @@ __device__ __forceinline__ uint8_t * kv4_rec(const Kv4Cache & c, int s, int h, i
 
 // Workgroup (record of the tokens' span; keys or values; four blocks | KV head | sequence): 8 lanes a block. A record that the tokens
 // fill is put together in LDS and written in 16-byte pieces; of the others only the tokens' own bytes are written. So small a share of
-// a record (2.3 KB) that a prompt of 512 tokens still has a few hundred workgroups, each with its 8 reads in flight together.
-// 1983 tokens of 4 heads of 256 (18.5 MB): 9.3 us, 2.0 TB/s; 512 of them 6.4 us; one token of each of 32 sequences, 8 heads of 128, 4 us.
+// a record (2.3 KB) that a prompt of 512 tokens still has a few hundred workgroups, each with its 4 reads in flight together.
+// 1983 tokens of 4 heads of 256 (18.5 MB): 8.0 us, 2.3 TB/s; 512 of them 4.9 us; one token of each of 32 sequences, 8 heads of 128, 3 us.
 // The launch and one trip to memory are 3 to 4 us of each; behind them the largest is bound by the shuffles and conversions of its
 // blocks.
-constexpr int KV4_STORE = 128;  // threads
+constexpr int KV4_STORE = 256;  // threads (1983 tokens as below with their reading back: 17.9, 15.7 and 14.6 us with 64, 128 and 256)
 template <int HD>
 __global__ __launch_bounds__(KV4_STORE) void kv4_store_kernel(Kv4RowsArgs a) {
     using L = Kv4Layout<HD>;
@@ -185,8 +185,8 @@ __device__ __forceinline__ float kv4_value(const uint8_t * rec, int p, int e) {
     return h2f(*reinterpret_cast<const uint16_t *>(rec + L::VD + L::scale(p, blk))) * float(q - 8);
 }
 
-// Workgroup (token, KV head, sequence), a thread an element: the writes, 7 times what is read, are whole lines (1983 tokens of 4 heads
-// of 256, 18.5 MB: 9.4 us, 2.0 TB/s).
+// Workgroup (token, KV head, sequence), a thread an element: the writes, 7 times what is read, are whole lines. Few tokens: a trip to
+// memory after the positions' one, 3 us.
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
     const int h = blockIdx.y, s = blockIdx.z, t = blockIdx.x;
@@ -200,6 +200,44 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
     for (int e = threadIdx.x; e < HD; e += 256) {
         a.k[row + e] = kv4_key<HD>(rec, int(p % KV4_TILE), e);
         a.v[row + e] = kv4_value<HD>(rec, int(p % KV4_TILE), e);
+    }
+}
+
+// Many tokens: workgroup (record of the tokens' span; keys or values | KV head | sequence) takes its half of the record to LDS in
+// 16-byte pieces and writes the rows in 16-byte pieces. 1983 tokens of 4 heads of 256 (18.5 MB): 7.1 us, 2.6 TB/s, 3 to 4 of them the
+// launch and two trips to memory.
+template <int HD>
+__global__ __launch_bounds__(256) void kv4_load_records_kernel(Kv4RowsArgs a) {
+    using L = Kv4Layout<HD>;
+    constexpr int QB = 16 * HD, ROW = HD / 4;  // bytes of the keys' or the values' quants; threads of a row
+    __shared__ __align__(16) uint8_t img[QB + 2 * HD];
+    const int h = blockIdx.y, s = blockIdx.z, tid = threadIdx.x, val = blockIdx.x & 1;
+    long long p0;
+    int n;
+    kv4_span(a.t, s, p0, n);
+    const long long lo = p0 < 0 ? 0 : p0, hi = p0 + n < a.c.n_ctx ? p0 + n : a.c.n_ctx;  // positions to read
+    const long long at = (lo / KV4_TILE + (blockIdx.x >> 1)) * KV4_TILE;                  // the record's first position
+    if (lo >= hi || at >= hi) return;
+    const int first = int(lo - at > 0 ? lo - at : 0), end = int(hi - at < KV4_TILE ? hi - at : KV4_TILE);
+    const uint8_t * rec = kv4_rec(a.c, s, h, int(at / KV4_TILE));
+    for (int i = tid; i < QB / 16; i += 256) reinterpret_cast<uint4 *>(img)[i] = reinterpret_cast<const uint4 *>(rec + (val ? L::VQ : 0))[i];
+    for (int i = tid; i < HD / 8; i += 256) reinterpret_cast<uint4 *>(img + QB)[i] = reinterpret_cast<const uint4 *>(rec + (val ? L::VD : L::KD))[i];
+    __syncthreads();
+    const int e = tid % ROW * 4, blk = e >> 5, up = e & 16 ? 4 : 0;
+    float * to = (val ? a.v : a.k) + ((long long)s * a.t.n_tok + (at - p0)) * a.row_stride + size_t(h) * HD + e;
+    for (int p = first + tid / ROW; p < end; p += 256 / ROW) {
+        const float d = h2f(*reinterpret_cast<const uint16_t *>(img + QB + L::scale(p, blk)));
+        typedef float f32x4 __attribute__((ext_vector_type(4)));
+        f32x4 y;
+        if (val) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = d * float((img[L::vq(p, blk, (e & 15) + i) - L::VQ] >> up & 15) - 8);
+        } else {
+            const uint32_t w = *reinterpret_cast<const uint32_t *>(img + L::kq(p, blk, e & 15));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = d * float(int(w >> (8 * i + up) & 15) - 8);
+        }
+        *reinterpret_cast<f32x4 *>(to + p * a.row_stride) = y;
     }
 }
 
@@ -221,8 +259,8 @@ __global__ __launch_bounds__(256) void kv4_load_kernel(Kv4RowsArgs a) {
 // its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
 // A record and 16 rows, heads of 256, are 64 matrix instructions and about 540 others, half of them unpacking; wider heads than 128
 // leave no registers for more than 16 rows to share that. What bounds it, by the counters:
-//   512 tokens at 7680, 16/4 heads of 256: 179 us, 370 TFLOP/s of the formula's 66.6 GFLOP (twice that in parts). Vector instructions are
-//     issued in 64 % of the cycles, and without any matrix instruction it would still be 159 us: each hundred instructions less a
+//   512 tokens at 7680, 16/4 heads of 256: 179 us, 370 TFLOP/s of the formula's 66.6 GFLOP (twice that in parts). Vector instructions
+//     are issued in 64 % of the cycles, and without any matrix instruction it would still be 159 us: each hundred instructions less a
 //     record are 21 us.
 //   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 39 us, 3.9 TB/s; vector instructions in 47 %, matrix instructions in 16 %,
 //     the rest the beginnings and ends of workgroups that have some ten records a wave.
@@ -497,8 +535,9 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     __shared__ __align__(16) uint8_t both[QBYTES > JBYTES ? QBYTES : JBYTES];
     u32x4(*ql)[64] = reinterpret_cast<u32x4(*)[64]>(both);              // the queries' parts
     float(*part)[ROWS][PAD] = reinterpret_cast<float(*)[ROWS][PAD]>(both);  // later the waves' sums
-    // The queries' parts that stay in registers, as many as leave room for two waves a SIMD (512 tokens at 7680, us with two, one and none:
-    // 16/4 heads of 256 184.9 / 187.8 / 192.4, 32/8 of 128 no room / 172.1 / 176.5). The others are read from LDS for every record.
+    // The queries' parts that stay in registers, as many as leave room for two waves a SIMD (512 tokens at 7680, us with two, one and
+    // none: 16/4 heads of 256 184.9 / 187.8 / 192.4, 32/8 of 128 no room / 172.1 / 176.5). The others are read from LDS for every
+    // record.
     constexpr int QR = NQ == 1 || HD * NQ <= 128 ? 2 : 1;
     __shared__ float kqs[ROWS], cs[4][ROWS], ls[4][ROWS];
     __shared__ __align__(16) uint32_t scales[4][HD];  // a wave's record's key scales, then its value scales: [g][block][8] each
@@ -848,8 +887,9 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
     kv4_out<HD>(a, size_t(s) * a.t.n_tok + t, hq, e0 + e, y, (red[1][0] + red[1][1]) + (red[1][2] + red[1][3]));
 }
 
-// The same for many rows (q heads of tokens): a wave `per_wave` of them one after another, its lanes HD / 4 to a set. What each workgroup does
-// before its first row (finding the sequence's ranges, 2 us) is shared by its rows. 3 sequences of 360 tokens of 8 heads of 64: 14 us.
+// The same for many rows (q heads of tokens): a wave `per_wave` of them one after another, its lanes HD / 4 to a set. What each
+// workgroup does before its first row (finding the sequence's ranges, 2 us) is shared by its rows. 3 sequences of 360 tokens of 8 heads
+// of 64: 14 us.
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_join_rows_kernel(Kv4AttnArgs a, int per_wave) {
     constexpr int PER = HD / 4, SETS = 64 / PER;
@@ -925,9 +965,15 @@ hipError_t launch_kv4_store(const Kv4RowsArgs & a, hipStream_t s) {
     });
 }
 
+// Rows (KV heads of tokens) from which on the records are read whole, where a sequence has tokens for half a record; us with single
+// rows and records, and the storing before: 8.1 and 9.3 at 400 rows, 10.5 and 10.6 at 2048, 10.2 and 8.9 at 4096, 18.2 and 15.5 at 7932.
+constexpr int KV4_RECORDS = 2048;
 hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s) {
+    const unsigned span = unsigned((a.t.n_tok + KV4_TILE - 2) / KV4_TILE + 1);  // records that n_tok positions can touch
     return by_dim(a.c.head_dim, [&](auto hd) {
-        GQ_LAUNCH(kv4_load_kernel<hd.value>, dim3(a.t.n_tok, a.c.n_head_kv, a.t.n_seq), dim3(256), 0, s, a);
+        if (a.t.n_tok >= KV4_TILE / 2 && (long long)a.t.n_seq * a.t.n_tok * a.c.n_head_kv >= KV4_RECORDS)
+            GQ_LAUNCH(kv4_load_records_kernel<hd.value>, dim3(2 * span, a.c.n_head_kv, a.t.n_seq), dim3(256), 0, s, a);
+        else GQ_LAUNCH(kv4_load_kernel<hd.value>, dim3(a.t.n_tok, a.c.n_head_kv, a.t.n_seq), dim3(256), 0, s, a);
     });
 }
 
@@ -946,8 +992,9 @@ int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     const long long units = (n_tok * (long long)per_kv + rows - 1) / rows * c.n_head_kv;
     const long long records = (long long)n_seq * kv4_tiles(c.n_ctx), most = (long long)n_seq * ((kv4_tiles(c.n_ctx) + KV4_LEAST - 1) / KV4_LEAST);
     long long ranges = std::max<long long>(n_seq, std::min(groups / units, most));
-    // Few long ranges for sequences of unlike lengths come out unlike themselves: twice as many (3 sequences of 96 tokens at up to 10776,
-    // 32/8 heads of 128: 58 and 79 us; one of 512 at 7680, 16/4 heads of 256, 192 and 185; 3 of 360 at 1451, 8 heads of 64, 49 and 42).
+    // Few long ranges for sequences of unlike lengths come out unlike themselves: twice as many (3 sequences of 96 tokens at up to
+    // 10776, 32/8 heads of 128: 58 and 79 us; one of 512 at 7680, 16/4 heads of 256, 192 and 185; 3 of 360 at 1451, 8 heads of 64, 49
+    // and 42).
     if (n_seq > 1 && records >= 128 * ranges) ranges = std::max<long long>(ranges, std::min<long long>(2 * ranges, KV4_GROUPS));
     return int(std::min<long long>(ranges, 65535));
 }
@@ -959,9 +1006,9 @@ size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
 
 bool kv4_joins(const Kv4AttnArgs & a) { return a.work && kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head) > a.t.n_seq; }
 
-// Rows (q heads of tokens) up to which each has workgroups of its own: several up to half as many. us with several, one, and a wave's share
-// of one: 26.7 / 24.7 / 25.3 at 320 rows, 30.8 / 30.4 / 32.2 at 352 (of 23 sets), 47.7 / 45.2 / 45.5 at 512, 55.6 / 51.4 / 49.7 at 1024,
-// - / 61.2 / 41.7 at 8640.
+// Rows (q heads of tokens) up to which each has workgroups of its own: several up to half as many. us with several, one, and a wave's
+// share of one: 26.7 / 24.7 / 25.3 at 320 rows, 30.8 / 30.4 / 32.2 at 352 (of 23 sets), 47.7 / 45.2 / 45.5 at 512, 55.6 / 51.4 / 49.7
+// at 1024, - / 61.2 / 41.7 at 8640.
 constexpr int KV4_FEW = 512;
 hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
     Kv4AttnArgs a = args;

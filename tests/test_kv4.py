@@ -85,8 +85,9 @@ def test_store_writes_its_bytes_alone(gq, hip, hd, n_tok, pos, num):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd", [32, 64, 128, 256])
-def test_load_gives_what_was_stored(gq, hip, hd):
-    n_seq, n_ctx, nkv, n_tok, pos, num = 2, 100, 3, 40, [2, 59], [40, 33]
+@pytest.mark.parametrize("n_ctx,n_tok,pos,num", [(100, 40, [2, 59], [40, 33]), (700, 400, [33, 299], [400, 395]), (400, 400, [0, 31], [400, 17])])
+def test_load_gives_what_was_stored(gq, hip, hd, n_ctx, n_tok, pos, num):
+    n_seq, nkv = 2, 3
     rng = np.random.default_rng(2)
     k, v = _data(rng, n_seq, n_tok, nkv, hd)
     kv, _ = _cache(gq, hip, n_seq, n_ctx, nkv, hd)

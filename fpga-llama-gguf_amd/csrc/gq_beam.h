@@ -31,6 +31,41 @@ struct BeamSelectArgs {
     int chunks;            // set at launch: workgroups a row there
     unsigned chunk_mul;    // set at launch: list / chunks = the high word of list * chunk_mul (lists below 2^13); 0: one chunk
 };
+
+// Logits as words that order as their values do, > 0 for every number. Both zeros are one word: a wave counts its candidates by the
+// words and takes them by the values, and equal logits go by their index.
+__host__ __device__ inline uint32_t beam_order(float x) {
+    const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);  // (-0 + 0 is +0)
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__host__ __device__ inline float beam_number(uint32_t o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o); }
+
+constexpr int BEAM_SLACK = 4;  // lanes beyond n_beam that a bound may let pass (24.4, 24.6 and 25.1 us with 4, 8 and 16 at 8 groups of 8 of 151936)
+
+// A bound on a wave's words, of which at_least(w) lanes' are w or more (0: none; low: the smallest, high: the largest): at least k of
+// them are >= it, and no more than k + BEAM_SLACK if equal ones do not forbid that; with fewer than k words: 1. n: how many pass.
+template <typename F>
+__host__ __device__ inline uint32_t beam_bound(F at_least, int k, uint32_t low, uint32_t high, int & n) {
+    uint32_t lo = 1, hi = high + 1;  // at least k (or all) are >= lo, fewer than k are >= hi
+    n = at_least(1u);
+    if (n <= k + BEAM_SLACK) return lo;
+    if (low) lo = low;
+    while (hi - lo > 1 && n > k + BEAM_SLACK) {
+        const uint32_t mid = lo + (hi - lo) / 2;
+        const int c = at_least(mid);
+        if (c >= k) {
+            lo = mid;
+            n = c;
+        } else {
+            hi = mid;
+        }
+    }
+    return lo;
+}
+
+// Entries of a wave's list of candidates, `per` logits a lane.
+constexpr int beam_list(int n_beam, int per) { return (n_beam + BEAM_SLACK) * per; }
+
 size_t beam_work(int n_group, int n_beam, int n_vocab);
 hipError_t launch_beam_select(const BeamSelectArgs & a, hipStream_t s);
 

@@ -17,13 +17,6 @@ namespace {
 // 8 groups of 8 beams of 151936 logits (39 MB): 16.3 us (2.4 TB/s: a workgroup's own way of read, reduce and rank is 7 us, the 64-bit
 // exponentials another 5, partly behind the reads) and 8.4 us, of which n_beam steps of about 0.4 us that wait for one another; one
 // group of 4: 7.0 and 4.7 us, both latency.
-constexpr int BEAM_SLACK = 4;  // lanes beyond n_beam that a bound may let pass (24.4, 24.6 and 25.1 us with 4, 8 and 16 there)
-
-__device__ __forceinline__ uint32_t order_of(float x) {  // monotone in x, > 0 for every number
-    const uint32_t b = __float_as_uint(x);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
-}
-__device__ __forceinline__ float value_of(uint32_t o) { return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
 // 2^t for -1020 <= t <= 0: t = n + f with |f| <= 1/2, 1 + f q(f) with q interpolating (2^f - 1) / f at 7 Chebyshev points (off by at
 // most 1.2e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of u = t + 1.5 * 2^52 as its low word.
@@ -81,26 +74,6 @@ __device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return a > b
 __device__ __forceinline__ uint32_t min_u(uint32_t a, uint32_t b) { return a < b ? a : b; }
 __device__ __forceinline__ double sum_d(double a, double b) { return a + b; }
 
-// A bound on the wave's monotone words (0: none; low: the smallest, high: the largest): at least k of them are >= it, and no more than
-// k + BEAM_SLACK if equal ones do not forbid that; with fewer than k words: 1. n: how many pass.
-__device__ __forceinline__ uint32_t beam_bound(uint32_t x, int k, uint32_t low, uint32_t high, int & n) {
-    uint32_t lo = 1, hi = high + 1;  // at least k (or all) are >= lo, fewer than k are >= hi
-    n = __popcll(__ballot(x >= 1));
-    if (n <= k + BEAM_SLACK) return lo;
-    if (low) lo = low;
-    while (hi - lo > 1 && n > k + BEAM_SLACK) {
-        const uint32_t mid = lo + (hi - lo) / 2;
-        const int c = __popcll(__ballot(x >= mid));
-        if (c >= k) {
-            lo = mid;
-            n = c;
-        } else {
-            hi = mid;
-        }
-    }
-    return lo;
-}
-
 struct BeamStat {
     float m;
     uint32_t pad;
@@ -135,13 +108,13 @@ __device__ __forceinline__ void wave_lds() {
 template <int PER>
 __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     constexpr int CH = 256 * PER;
-    extern __shared__ unsigned long long list[];  // the waves' candidates: (n_beam + BEAM_SLACK) * PER each
+    extern __shared__ unsigned long long list[];  // the waves' candidates: beam_list each
     __shared__ float red[4];
     __shared__ double sums[4];
     __shared__ int count[4];
     __shared__ unsigned long long best[4][BEAM_MAX];
     const int row = blockIdx.y, chunk = blockIdx.x, k = a.n_beam, tid = threadIdx.x, lane = tid & 63;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), v0 = chunk * CH, cap = (k + BEAM_SLACK) * PER;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), v0 = chunk * CH, cap = beam_list(k, PER);
     const size_t at = size_t(row) * a.chunks + chunk;
     unsigned long long * out = beam_lists(a) + at * k;
     const float * x = a.x + size_t(row) * size_t(a.stride);
@@ -168,7 +141,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         for (int i = tid; i < k; i += 256) {
             const int token = ended ? (i == 0 ? a.eos : i - 1 < a.eos ? i - 1 : i) : i;
             const float x = ended && i == 0 ? 0.0f : -__builtin_inff();
-            out[i] = chunk == 0 && token < a.n_vocab ? (unsigned long long)order_of(x) << 32 | uint32_t(~token) : 0ull;
+            out[i] = chunk == 0 && token < a.n_vocab ? (unsigned long long)beam_order(x) << 32 | uint32_t(~token) : 0ull;
         }
         if (tid == 0) beam_stats(a)[at] = {ended && chunk == 0 ? 0.0f : -__builtin_inff(), 0, ended && chunk == 0 ? 1.0 : 0.0};
         return;
@@ -196,10 +169,10 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     tv = clean(tv);  // (NaN: the lane has no number; the others pass maxima and terms by)
     // the lane's best; 0: it has none (its first piece's last three elements may be the first of the chunk)
     const bool any = max(token_of(0), v0) < a.n_vocab || more;
-    const uint32_t top = any ? order_of(tv) : 0;
+    const uint32_t top = any ? beam_order(tv) : 0;
     // ---- maximum and sum ----
     const uint32_t wtop = __builtin_amdgcn_readfirstlane(wave_u32(top, max_u)), wlow = __builtin_amdgcn_readfirstlane(wave_u32(top, min_u));
-    const float wm = wtop ? value_of(wtop) : -__builtin_inff();  // each wave's sum is relative to its own maximum
+    const float wm = wtop ? beam_number(wtop) : -__builtin_inff();  // each wave's sum is relative to its own maximum
     double sum = 0.0;
     if (wm > -__builtin_inff()) {
 #pragma unroll
@@ -209,18 +182,18 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     sum = wave_f64(sum, sum_d);
     // ---- the wave's candidates: those that pass a bound on the lanes' best ----
     int n;
-    const uint32_t lo = beam_bound(top, k, wlow, wtop, n);
+    const uint32_t lo = beam_bound([&](uint32_t w) { return __popcll(__ballot(top >= w)); }, k, wlow, wtop, n);
     unsigned long long * mylist = list + wave * cap;
     int have = 0;
     const auto put = [&](bool in, float y, int t) {
         const unsigned long long who = __ballot(in);
         if (!who) return;
-        if (in) mylist[have + __popcll(who & ((1ull << lane) - 1))] = (unsigned long long)order_of(y) << 32 | uint32_t(~t);
+        if (in) mylist[have + __popcll(who & ((1ull << lane) - 1))] = (unsigned long long)beam_order(y) << 32 | uint32_t(~t);
         have += __popcll(who);
     };
-    const uint32_t bottom = order_of(-__builtin_inff());
+    const uint32_t bottom = beam_order(-__builtin_inff());
     if (n <= k + BEAM_SLACK && lo > bottom) {
-        const float bound = value_of(lo);
+        const float bound = beam_number(lo);
 #pragma unroll
         for (int j = 0; j < PER; ++j) put(v[j] >= bound, v[j], token_of(j));
         if (skew) put(extra >= bound, extra, xt);
@@ -231,10 +204,10 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         if (n > k + BEAM_SLACK) {
             int mine = INT_MAX;
             if (top == lo) {
-                if (more && order_of(extra) == lo) mine = xt;
+                if (more && beam_order(extra) == lo) mine = xt;
 #pragma unroll
                 for (int j = PER - 1; j >= 0; --j)
-                    if (real(j) && order_of(v[j]) == lo) mine = token_of(j);
+                    if (real(j) && beam_order(v[j]) == lo) mine = token_of(j);
             }
             const int above = __popcll(__ballot(top > lo));
             int l = v0 - 1, h = v0 + CH;  // fewer than k with tokens <= l, at least k with <= h
@@ -245,7 +218,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
             }
             until = h;
         }
-        const auto passes = [&](float y, int t) { return order_of(y) > lo || (order_of(y) == lo && t <= until); };
+        const auto passes = [&](float y, int t) { return beam_order(y) > lo || (beam_order(y) == lo && t <= until); };
 #pragma unroll
         for (int j = 0; j < PER; ++j) put(real(j) && passes(v[j], token_of(j)), v[j], token_of(j));
         put(more && passes(extra, xt), extra, xt);
@@ -358,7 +331,7 @@ __device__ __forceinline__ int beam_of(const BeamSelectArgs & a, int list) {
 
 // A list entry's value.
 __device__ __forceinline__ double beam_value(unsigned long long e, int b, const double * top, const double * logsum, const double * scores) {
-    const float x = value_of(uint32_t(e >> 32));
+    const float x = beam_number(uint32_t(e >> 32));
     return x > -__builtin_inff() && scores[b] > -__builtin_inf() ? scores[b] + ((double(x) - top[b]) - logsum[b]) : -__builtin_inf();
 }
 constexpr uint32_t BEAM_NONE = 0xffffffffu;  // beam * n_vocab + token of an empty list's head
@@ -676,7 +649,7 @@ hipError_t launch_beam_select(const BeamSelectArgs & args, hipStream_t s) {
     a.per = beam_per(a.n_group, a.n_beam, a.n_vocab);
     a.chunks = beam_chunks(a.n_vocab, a.per);
     a.chunk_mul = a.chunks > 1 ? unsigned((0x100000000ull + unsigned(a.chunks) - 1) / unsigned(a.chunks)) : 0;
-    const unsigned lds = unsigned((a.n_beam + BEAM_SLACK) * a.per * 4 * sizeof(unsigned long long));
+    const unsigned lds = unsigned(beam_list(a.n_beam, a.per) * 4 * sizeof(unsigned long long));
     const dim3 grid(unsigned(a.chunks), unsigned(rows));
     if (a.per == 32) GQ_LAUNCH(beam_scan_kernel<32>, grid, dim3(256), lds, s, a);
     else GQ_LAUNCH(beam_scan_kernel<8>, grid, dim3(256), lds, s, a);

@@ -118,19 +118,20 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     const size_t at = size_t(row) * a.chunks + chunk;
     unsigned long long * out = beam_lists(a) + at * k;
     const float * x = a.x + size_t(row) * size_t(a.stride);
-    // elements 4 (256 i + tid) + e from the chunk's start; rows start anywhere, so the pieces are brought to 16 bytes. Read before it
-    // is known whether the row takes logits at all, which is a microsecond later
-    const int skew = int((reinterpret_cast<uintptr_t>(x + v0) >> 2) & 3);
+    // elements 4 (256 i + tid) + e of the chunk, wherever the row starts (a 16-byte load takes any multiple of 4): what a lane holds goes by
+    // the tokens alone, so beams with the same logits have the same sums and tie. Read before it is known whether the row takes
+    // logits at all, which is a microsecond later
     typedef float f32x4 __attribute__((ext_vector_type(4)));
+    typedef float f32x4_at_4 __attribute__((ext_vector_type(4), aligned(4)));
     float v[PER];
 #pragma unroll
     for (int i = 0; i < PER / 4; ++i) {
-        const int t = v0 - skew + 4 * (256 * i + tid);
-        if (t >= v0 && t + 4 <= a.n_vocab) {
-            *reinterpret_cast<f32x4 *>(v + 4 * i) = *reinterpret_cast<const f32x4 *>(x + t);
+        const int t = v0 + 4 * (256 * i + tid);
+        if (t + 4 <= a.n_vocab) {
+            *reinterpret_cast<f32x4 *>(v + 4 * i) = *reinterpret_cast<const f32x4_at_4 *>(x + t);
         } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * i + e] = t + e >= v0 && t + e < a.n_vocab ? x[t + e] : -__builtin_inff();
+            for (int e = 0; e < 4; ++e) v[4 * i + e] = t + e < a.n_vocab ? x[t + e] : -__builtin_inff();
         }
     }
     bool ended;
@@ -146,19 +147,14 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         if (tid == 0) beam_stats(a)[at] = {ended && chunk == 0 ? 0.0f : -__builtin_inff(), 0, ended && chunk == 0 ? 1.0 : 0.0};
         return;
     }
-    const auto token_of = [&](int j) { return v0 - skew + 4 * (256 * (j >> 2) + tid) + (j & 3); };
-    const auto real = [&](int j) { return token_of(j) >= v0 && token_of(j) < a.n_vocab; };
-    // the last `skew` elements of the chunk are the pieces' overhang: one more each in the first threads
-    const int xt = v0 + CH - skew + tid;
-    const bool more = tid < skew && xt < a.n_vocab;
-    float extra = more ? x[xt] : -__builtin_inff();
+    const auto token_of = [&](int j) { return v0 + 4 * (256 * (j >> 2) + tid) + (j & 3); };
+    const auto real = [&](int j) { return token_of(j) < a.n_vocab; };
     const auto clean = [](float y) { return y == y ? fminf(y, FLT_MAX) : -__builtin_inff(); };
-    float tv = extra;
+    float tv = v[0];
 #pragma unroll
-    for (int j = 0; j < PER; ++j) tv = fmaxf(tv, v[j]);
+    for (int j = 1; j < PER; ++j) tv = fmaxf(tv, v[j]);
     const auto clean_all = [&] {
         __asm__ volatile("");  // (a branch of its own: not done ahead of it and selected)
-        extra = clean(extra);
 #pragma unroll
         for (int j = 0; j < PER; ++j) v[j] = clean(v[j]);
     };
@@ -167,9 +163,7 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         tv = fminf(tv, FLT_MAX);
     }
     tv = clean(tv);  // (NaN: the lane has no number; the others pass maxima and terms by)
-    // the lane's best; 0: it has none (its first piece's last three elements may be the first of the chunk)
-    const bool any = max(token_of(0), v0) < a.n_vocab || more;
-    const uint32_t top = any ? beam_order(tv) : 0;
+    const uint32_t top = real(0) ? beam_order(tv) : 0;  // the lane's best; 0: it has none
     // ---- maximum and sum ----
     const uint32_t wtop = __builtin_amdgcn_readfirstlane(wave_u32(top, max_u)), wlow = __builtin_amdgcn_readfirstlane(wave_u32(top, min_u));
     const float wm = wtop ? beam_number(wtop) : -__builtin_inff();  // each wave's sum is relative to its own maximum
@@ -177,7 +171,6 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
     if (wm > -__builtin_inff()) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) sum += beam_term(v[j], wm);
-        if (skew) sum += beam_term(extra, wm);
     }
     sum = wave_f64(sum, sum_d);
     // ---- the wave's candidates: those that pass a bound on the lanes' best ----
@@ -196,7 +189,6 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         const float bound = beam_number(lo);
 #pragma unroll
         for (int j = 0; j < PER; ++j) put(v[j] >= bound, v[j], token_of(j));
-        if (skew) put(extra >= bound, extra, xt);
     } else {
         clean_all();
         // every element counts, or many lanes' best are equal: of the elements at the bound itself, the tokens up to `until`
@@ -204,7 +196,6 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         if (n > k + BEAM_SLACK) {
             int mine = INT_MAX;
             if (top == lo) {
-                if (more && beam_order(extra) == lo) mine = xt;
 #pragma unroll
                 for (int j = PER - 1; j >= 0; --j)
                     if (real(j) && beam_order(v[j]) == lo) mine = token_of(j);
@@ -221,7 +212,6 @@ __global__ __launch_bounds__(256) void beam_scan_kernel(BeamSelectArgs a) {
         const auto passes = [&](float y, int t) { return beam_order(y) > lo || (beam_order(y) == lo && t <= until); };
 #pragma unroll
         for (int j = 0; j < PER; ++j) put(real(j) && passes(v[j], token_of(j)), v[j], token_of(j));
-        put(more && passes(extra, xt), extra, xt);
     }
     if (lane < 8) {  // up to whole eights of entries
         const int i = have + lane;
@@ -619,7 +609,6 @@ __global__ void beam_next_kernel(BeamNextArgs a) {
     a.pos[16 * s] = p;
 }
 
-// (a chunk's first piece may start up to 3 elements before it, so 256 * per elements and 3 more are read by a workgroup)
 int beam_chunks(int n_vocab, int per) { return (n_vocab + 256 * per - 1) / (256 * per); }
 // Logits a thread of the first kernel takes: 8, the shorter way through one workgroup, or 32 where those would give the second kernel
 // 192 lists a group or the first more workgroups than the device holds at once. Both kernels with 8 and 32: 10.2 and 11.6 us at one

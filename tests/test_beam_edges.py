@@ -21,21 +21,20 @@ def hip(gq):
 
 @pytest.fixture(scope="module")
 def lists(tmp_path_factory):
-    """Per (logits a lane, beams, skew): the most entries of a wave, the list's size, whether the best were among them, the pattern."""
+    """Per (logits a lane, beams): the most entries of a wave, the list's size, whether the best were among them, the pattern."""
     exe = tmp_path_factory.mktemp("beam") / "beam_list_check"
     src = os.path.join(HERE, "..", "fpga-llama-gguf_amd", "csrc")
     subprocess.run([os.environ.get("HIPCC", "/opt/rocm/bin/hipcc"), "-x", "hip", "--offload-host-only", "-O2", "-std=c++17", "-ffp-contract=off", "-w",
                     "-I" + os.path.join(HERE, "..", "include"), "-I" + src, os.path.join(HERE, "beam_list_check.cpp"), "-o", str(exe)], check=True)
-    out = subprocess.run([str(exe), "3"], check=True, capture_output=True, text=True).stdout
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
     return np.array([[int(x) for x in line.split()] for line in out.splitlines()])
 
 
 def test_lists_hold_every_candidate(lists):
-    """Rows that start at 16 bytes, signed zeros among them: no wave lists more than its list holds, and the best are listed in order."""
-    rows = lists[lists[:, 2] == 0]
-    assert len(rows) == 2 * 32
-    assert (rows[:, 3] <= rows[:, 4]).all(), rows[rows[:, 3] > rows[:, 4]]
-    assert rows[:, 5].all(), rows[rows[:, 5] == 0]
+    """No wave lists more than its list holds, and the best are listed in order."""
+    assert len(lists) == 2 * 32
+    assert (lists[:, 2] <= lists[:, 3]).all(), lists[lists[:, 2] > lists[:, 3]]
+    assert lists[:, 4].all(), lists[lists[:, 4] == 0]
 
 
 @pytest.mark.gpu
@@ -59,3 +58,41 @@ def test_signed_zeros_are_equal(gq, hip, beams, v, what):
     x = np.repeat(x, beams, 0)
     score = -np.arange(groups * beams, dtype=np.float32) / 4
     check(select(gq, hip, x, score, None, -1, groups, beams), reference(x, score, None, -1, groups, beams))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("beams,v", [(1, 2048), (2, 2048), (4, 2048), (4, 300000), (8, 60000), (32, 9000)])
+@pytest.mark.parametrize("skew", [0, 1, 2, 3])
+@pytest.mark.parametrize("equal", [True, False])
+def test_lanes_full_of_candidates(gq, hip, beams, v, skew, equal):
+    """All logits of as many lanes of the first wave as may pass are above all others, in rows that all start `skew` floats past 16 bytes."""
+    v += -(v + skew) % 4
+    print(f"[beam selection] full lanes, {beams} of {v}, skew {skew}, equal {equal}", flush=True)
+    rng = np.random.default_rng(beams + v)
+    per = 32 if beams * -(-v // 2048) >= 192 else 8  # logits a lane
+    at = np.arange(min(v, 256 * per))
+    for first in range(4):
+        for lanes, lane in ((n, (at + back) // 4 % 256) for n in (beams, beams + 4, beams + 5) for back in (0, skew)):  # by tokens, by lines
+            x = (-5 - rng.random(v)).astype(np.float32)
+            high = at[(lane >= first) & (lane < first + lanes)]
+            x[high] = 2.0 if equal else (2 + rng.random(high.size)).astype(np.float32)
+            x = np.repeat(x[None], beams, 0)
+            score = -np.arange(beams, dtype=np.float32) / 4
+            check(select(gq, hip, x, score, None, -1, 1, beams, skew), reference(x, score, None, -1, 1, beams))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("what", ["equal", "few values", "ascending", "descending", "masked", "one left", "spikes", "zeros"])
+@pytest.mark.parametrize("beams,v", [(4, 5000), (32, 9001), (1, 101), (24, 230002)])
+@pytest.mark.parametrize("skew", [1, 2, 3])
+def test_structured_rows_off_their_lines(gq, hip, what, beams, v, skew):
+    """Rows with many equal or ordered logits, each at a place of its own in its lines: a group's beams share their logits, so they tie."""
+    print(f"[beam selection] {what}, {beams} of {v}, skew {skew}", flush=True)
+    rng = np.random.default_rng(3)
+    x = {"equal": np.full(v, 1.25), "few values": rng.integers(-1, 2, v), "ascending": np.arange(v) / 64, "descending": -np.arange(v) / 64,
+         "masked": np.where(rng.random(v) < 0.9, -np.inf, rng.standard_normal(v)), "one left": np.where(np.arange(v) == v - 1, 3.0, -np.inf),
+         "spikes": np.where(np.arange(v) % 1024 == 0, 50.0, rng.standard_normal(v)),
+         "zeros": np.where(rng.random(v) < 0.5, 0.0, -0.0)}[what].astype(np.float32)
+    x = np.repeat(x[None], 2 * beams, 0)
+    score = np.repeat(np.float32([-1.5, -2.25]), beams)
+    check(select(gq, hip, x, score, None, -1, 2, beams, skew), reference(x, score, None, -1, 2, beams))

@@ -85,11 +85,13 @@ __device__ __forceinline__ unsigned long long * beam_lists(const BeamSelectArgs 
     return reinterpret_cast<unsigned long long *>(beam_stats(a) + size_t(a.n_group) * a.n_beam * a.chunks);
 }
 
-// A row that takes no logits: a beam that has ended (its one candidate), or one without a score (none).
+// A row that takes no logits: a beam that has ended (its one candidate), or one without a score (none, also where its last token is eos:
+// its candidates are all at -inf, so their order is that of the tokens).
 __device__ __forceinline__ bool beam_closed(const BeamSelectArgs & a, int row, bool & ended) {
     const size_t at = size_t(row) * a.slot;
-    ended = a.last && a.last[at] == a.eos && a.eos >= 0 && a.eos < a.n_vocab && !(a.pos && a.pos[at] < a.n_prompt[at]);
-    return ended || !(a.score[at] > -__builtin_inff());
+    const bool scored = a.score[at] > -__builtin_inff();
+    ended = scored && a.last && a.last[at] == a.eos && a.eos >= 0 && a.eos < a.n_vocab && !(a.pos && a.pos[at] < a.n_prompt[at]);
+    return ended || !scored;
 }
 // Whether the row's prompt has a next id; its place in the prompt.
 __device__ __forceinline__ bool beam_prompted(const BeamSelectArgs & a, int row, int & next) {

@@ -96,3 +96,21 @@ def test_structured_rows_off_their_lines(gq, hip, what, beams, v, skew):
     x = np.repeat(x[None], 2 * beams, 0)
     score = np.repeat(np.float32([-1.5, -2.25]), beams)
     check(select(gq, hip, x, score, None, -1, 2, beams, skew), reference(x, score, None, -1, 2, beams))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("beams,v", [(1, 100), (4, 5000), (12, 9000), (32, 40)])
+@pytest.mark.parametrize("dead", ["first", "all", "nan"])
+def test_ended_beams_without_a_score(gq, hip, beams, v, dead):
+    """A beam whose last token is eos and whose score is -inf (or NaN): all its candidates are at -inf, ordered by their tokens."""
+    rng = np.random.default_rng(beams)
+    x = rng.standard_normal((2 * beams, v)).astype(np.float32)
+    score = -np.arange(2 * beams, dtype=np.float32) - 1
+    if dead == "first":
+        score[::beams] = -np.inf
+        x[1:beams] = -np.inf  # the first group has fewer candidates above -inf than winners
+    else:
+        score[:] = np.nan if dead == "nan" else -np.inf
+    last = np.full(2 * beams, 7, np.int32)
+    last[1:beams] = 3
+    check(select(gq, hip, x, score, last, 7, 2, beams), reference(x, score, last, 7, 2, beams))

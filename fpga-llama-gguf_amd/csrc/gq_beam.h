@@ -21,7 +21,8 @@ struct BeamSelectArgs {
     int32_t * parent;      // beams of the group
     int slot;
     // With pos: row r is at position pos[r * slot] of its prompt (n_prompt[r * slot] ids, at most cap, at prompt + r * cap). While the
-    // prompt has a next id, that is its token, parent and score stay; a beam has ended only behind its prompt.
+    // group's first row's prompt has a next id, the group reads prompts: each row's next id is its token (none left: the token stays), the
+    // row its own parent, the score stays; a beam has ended only behind its prompt.
     const int32_t * pos;
     const int32_t * n_prompt;
     const int32_t * prompt;

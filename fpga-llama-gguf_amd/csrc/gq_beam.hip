@@ -270,8 +270,8 @@ __device__ __forceinline__ bool beam_rows(const BeamSelectArgs & a, int g, doubl
     const int k = a.n_beam, tid = threadIdx.x, lane = tid & 63;
     int ahead;
     if (beam_prompted(a, g * k, ahead)) {  // the group's beams read their prompt
-        if (tid < k && beam_prompted(a, g * k + tid, ahead)) {
-            a.token[(g * k + tid) * a.slot] = a.prompt[size_t(g * k + tid) * a.cap + ahead];
+        if (tid < k) {
+            if (beam_prompted(a, g * k + tid, ahead)) a.token[(g * k + tid) * a.slot] = a.prompt[size_t(g * k + tid) * a.cap + ahead];
             a.parent[(g * k + tid) * a.slot] = tid;
         }
         return false;

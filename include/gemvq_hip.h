@@ -90,9 +90,9 @@
  *             no counterpart in the reference): gemvq_beam_select_static on the logits rows at x_off + s * row_stride. Sequence
  *             s's score (FP32), token and parent (int32) are at act[score_off, tok_off, parent_off + 16 s]; the tokens there
  *             are the last ones, and the new ones replace them. With len_off, a group whose first sequence is at position p =
- *             act_i32[pos_off + 16 s] with p + 1 < act_i32[len_off + 16 s] reads its prompt instead: token = act_i32[prompt_off
- *             + s * cap + p + 1], the parent is the sequence itself, the score stays; and eos ends a beam only behind its
- *             prompt.
+ *             act_i32[pos_off + 16 s] with p + 1 < act_i32[len_off + 16 s] reads its prompts instead: for each of its
+ *             sequences token = act_i32[prompt_off + s * cap + p + 1] (unchanged behind the sequence's own prompt), the parent
+ *             is the sequence itself, the score stays; and eos ends a beam only behind its prompt.
  *   BEAM_MOVE [19, kind | n_part << 8, off, row_stride, part_stride, n, parent_off, n_beam | n_group << 8]
  *             + [pos_off, first, 0, 0, 0, 0, 0, 0]
  *             gemvq_beam_reorder_static on one array: its row s becomes what row act_i32[parent_off + 16 s] of the group was.

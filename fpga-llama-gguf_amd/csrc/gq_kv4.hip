@@ -276,7 +276,7 @@ typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef uint16_t __attribute__((may_alias)) half_word;  // 16 bits of memory that is read as words
 
-constexpr float KV4_LOW = -1e30f;  // below every score: the maximum before the first one
+constexpr float KV4_LOW = -FLT_MAX;  // no score is below it: the maximum before the first one
 
 template <int N>
 __device__ __forceinline__ void load_words(const uint8_t * p, uint32_t * w) {
@@ -591,11 +591,12 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
         top = fmaxf(top, dpp_f32<DPP_XOR2>(top));
         top = fmaxf(top, dpp_f32<DPP_HALF_MIRROR>(top));
         top = fmaxf(top, dpp_f32<DPP_MIRROR>(top));
-        // the largest element to 2^13..2^14 (rows of zeros and the ends of FP32's range: some power of two that does not overflow)
-        const int e = min(max(int((__float_as_uint(top) >> 23) & 255), 40), 240);
-        // (with the scale's sign: what brings the products back is positive then, if only just for a scale of 0)
-        const float up = __builtin_copysignf(__uint_as_float(uint32_t(127 + 13 + 127 - e) << 23), a.scale);
-        if (pc == 0) kqs[n * 16 + (tid >> 4)] = fmaxf(fabsf(a.scale) * 1.44269504088896341f * __uint_as_float(uint32_t(e - 13) << 23), FLT_MIN);
+        // the largest element to 2^13..2^14 (rows of zeros: some power of two), times the mantissa and sign of the scale and log2(e), which
+        // leaves it below 2^15.6; what brings the products back is a power of two, so scores times it are exact at any size, and a
+        // row's largest score less itself is 0
+        const int e = min(max(int((__float_as_uint(top) >> 23) & 255), 40), 254);
+        const float up = __uint_as_float(uint32_t(127 + 13 + 127 - e) << 23) * (__builtin_amdgcn_frexp_mantf(a.scale) * 2.88539008177792681f);
+        if (pc == 0) kqs[n * 16 + (tid >> 4)] = __uint_as_float(uint32_t(min(max(e - 14 + __builtin_amdgcn_frexp_expf(a.scale), 1), 254)) << 23);
 #pragma unroll
         for (int i = 0; i < NP; ++i) {
             const int piece = (pc + 16 * i) & (HD / 4 - 1), to = (piece & 3) * 16 + (tid >> 4);  // 8 block + 4 half + g
@@ -614,7 +615,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     }
     __syncthreads();
     u32x4 q[NQ][NB][QR];
-    float kq[NQ];  // what brings the products back: |scale| * log2(e) over the row's power of two
+    float kq[NQ];  // what brings the products back: the scale's power of two over the row's
     int my_lo[NQ], my_hi[NQ];
     f32x4 o[NQ][NB][2];
     float c[NQ], l[NQ];
@@ -710,7 +711,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
                     if (p < my_lo[n] || p > my_hi[n]) sc[n][i] = -__builtin_inff();
                 }
             top[n] = fmaxf(fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])), fmaxf(fmaxf(sc[n][4], sc[n][5]), fmaxf(sc[n][6], sc[n][7]))) * kq[n];
-            again |= bool(__any(top[n] > c[n] + 8.0f));
+            again |= bool(__any(top[n] - c[n] > 8.0f));  // (not c + 8, which may round to the maximum)
         }
         if (again) {  // new maxima
 #pragma unroll

@@ -1,0 +1,55 @@
+"""Attention over the 4-bit cache at the ends of its numbers: scores of any finite size."""
+import numpy as np
+import pytest
+
+import kv4_ref as ref
+from hip_rt import Hip
+from test_kv4 import _attend, _cache, _data, _store
+
+U = ref.U
+
+
+@pytest.fixture
+def hip(gq):
+    h = Hip(gq)
+    yield h
+    h.close()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 32), (8, 2, 128), (4, 1, 256)])
+@pytest.mark.parametrize("size", [1e6, 3e8, 1e10, 1e15, 1e25, 1e33, 1e36, "one element"])
+@pytest.mark.parametrize("first,n_tok", [(0, 6), (700, 1)])
+def test_scores_of_any_size(gq, hip, nh, nkv, hd, size, first, n_tok):
+    """Scores so far apart that a token's output is the value of its best position, and so large that a rounding of one is many powers of e.
+    FP32 sums of hd products and the query in two parts leave a score off by (hd + 8) u times its products' magnitudes: heads whose two best
+    positions are not further apart than that are left out. The value comes back as a weight of 1 in two parts (22 bits) times quants
+    and scale, over the sum of weights: a few u."""
+    rng = np.random.default_rng(hd)
+    n = first + n_tok
+    k, v = _data(rng, 1, n, nkv, hd)
+    q = rng.standard_normal((1, n_tok, nh, hd)).astype(np.float32)
+    if size == "one element":  # up to the end of FP32's range
+        q *= 0
+        q[..., 3] = rng.uniform(1.1e38, 3.4e38, q.shape[:-1]) * rng.choice([-1, 1], q.shape[:-1])
+        k *= np.float32(1e-3)
+    else:
+        q *= np.float32(size)
+    kv, _ = _cache(gq, hip, 1, n, nkv, hd)
+    _store(gq, hip, kv, k, v, [0])
+    scale = hd ** -0.5
+    y = _attend(gq, hip, kv, q, [first], None, 0, scale)
+    kk, vv = ref.values(k)[0], ref.values(v)[0]
+    seen = 0
+    for t in range(n_tok):
+        for h in range(nh):
+            x = kk[:first + t + 1, h * nkv // nh]
+            s = x @ q[0, t, h].astype(np.float64) * scale
+            off = (hd + 8) * U * (np.abs(x) @ np.abs(q[0, t, h].astype(np.float64))).max() * scale
+            best = int(s.argmax())
+            if (np.delete(s, best) > s[best] - 2 * off - 30).any():
+                continue
+            seen += 1
+            want = vv[best, h * nkv // nh]
+            assert (np.abs(y[0, t, h] - want) <= 16 * U * np.abs(want)).all(), (t, h, y[0, t, h], want)
+    assert seen >= nh // 2

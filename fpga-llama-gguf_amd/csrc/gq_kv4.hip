@@ -248,13 +248,16 @@ __global__ __launch_bounds__(256) void kv4_load_records_kernel(Kv4RowsArgs a) {
 //                 multiplied by its scales in FP32. (The quants' bits as they are, 2^-24 n, with the 8 taken off through the
 //                 accumulator's start, are a tenth fewer vector instructions, but the instruction's sums of such small factors keep
 //                 several bits less: results are off by 5e-6 in place of 3e-7.)
-//   P = 2^(S - c) in FP32, c = m - 4 with m the query's running maximum, taken anew only when a score passes it by 4 (so P < 2^8).
-//                 P is the sum of two fp16 numbers, whole multiples of 2^-24 (2^-28 of the largest weight). Lane 16 g + q holds
-//                 query q's weights of the 8 positions that it feeds to
+//   P = 2^(S - c) in FP32, c = m - 7 with m the query's running maximum, taken anew when a score passes it by 2 (so P <= 2^9). P is the
+//                 sum of two fp16 numbers: 22 bits, but no finer than 2^-24, at most 2^-31 of the largest weight. (FP32 would keep 24
+//                 bits of the smallest ones too, in three parts: half as many matrix instructions again. The nearer P is to the end of
+//                 fp16's range, the less is lost, and the more often maxima are taken anew: 512 tokens at 7680, 16/4 heads of 256,
+//                 178.6 us with m - 4 and 4 more, 180.0 with m - 6 and 3, 180.8 so.) Lane 16 g + q holds query q's weights of the 8
+//                 positions that it feeds to
 //   O^T += V^T P^T: the quants minus 8 again; a block's scales go to the weights, P d = h + l: h the rounded product of d and P's upper
 //                 part, l, by two fused multiply-adds, what that rounding left and the lower part's product (22 bits). The scales
-//                 are brought up by a power of two 2^e common to the wave, the largest so far to 2^6..2^7 (so P d < 2^15; a scale
-//                 2^21 below the largest is still a normal number).
+//                 are brought up by a power of two 2^e common to the wave, the largest so far to 2^6..2^7, its 11 bits below 2^7, so
+//                 P d is at most 65504, fp16's largest number; a scale 2^20 below the largest is still a normal number.
 // The accumulators stay with the query's lanes and nothing crosses lanes in the loop. The four waves of a workgroup take the records of
 // its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
 // A record and 16 rows, heads of 256, are 64 matrix instructions and about 540 others, half of them unpacking; wider heads than 128
@@ -711,14 +714,14 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
                     if (p < my_lo[n] || p > my_hi[n]) sc[n][i] = -__builtin_inff();
                 }
             top[n] = fmaxf(fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])), fmaxf(fmaxf(sc[n][4], sc[n][5]), fmaxf(sc[n][6], sc[n][7]))) * kq[n];
-            again |= bool(__any(top[n] - c[n] > 8.0f));  // (not c + 8, which may round to the maximum)
+            again |= bool(__any(top[n] - c[n] > 9.0f));  // (not c + 9, which may round to the maximum)
         }
         if (again) {  // new maxima
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
                 float m = fmaxf(top[n], __shfl_xor(top[n], 16, WAVE));
                 m = fmaxf(m, __shfl_xor(m, 32, WAVE));
-                const float c2 = fmaxf(m - 4.0f, c[n]), f = __builtin_amdgcn_exp2f(c[n] - c2);
+                const float c2 = fmaxf(m - 7.0f, c[n]), f = __builtin_amdgcn_exp2f(c[n] - c2);
                 c[n] = c2;
                 l[n] *= f;
                 if (sums)

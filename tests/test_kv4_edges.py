@@ -1,4 +1,4 @@
-"""Attention over the 4-bit cache at the ends of its numbers: scores of any finite size."""
+"""Attention over the 4-bit cache at the ends of its numbers: scores of any finite size, weights far below the largest."""
 import numpy as np
 import pytest
 
@@ -53,3 +53,30 @@ def test_scores_of_any_size(gq, hip, nh, nkv, hd, size, first, n_tok):
             want = vv[best, h * nkv // nh]
             assert (np.abs(y[0, t, h] - want) <= 16 * U * np.abs(want)).all(), (t, h, y[0, t, h], want)
     assert seen >= nh // 2
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("hd,n_tok", [(32, 1), (64, 40), (128, 1), (128, 20), (256, 3)])
+def test_a_dominant_position_without_values(gq, hip, hd, n_tok):
+    """One position far above all others, whose values are zero: the output is made of the others' weights alone. All of them are equal, so
+    what rounding leaves of one adds up. A weight is held no finer than 2^-31 of the largest (off by half of that), a weight times a
+    value scale no finer than 2^-24 beside a largest product of at least 2^7 * 2^6 (8 quants of the largest scale: 2^-35 of the values)."""
+    nh, nkv, n = 8, 2, 700
+    rng = np.random.default_rng(hd)
+    first = n - n_tok
+    k = np.zeros((1, n, nkv, hd), np.float32)
+    v = rng.uniform(0.5, 1.5, (1, n, nkv, hd)).astype(np.float32)
+    k[0, 11, :, 3], v[0, 11] = 1, 0
+    q = rng.standard_normal((1, n_tok, nh, hd)).astype(np.float32)
+    q[..., 3] = np.linspace(9, 22, n_tok * nh).reshape(n_tok, nh)  # how far above, in nats
+    kv, _ = _cache(gq, hip, 1, n, nkv, hd)
+    _store(gq, hip, kv, k, v, [0])
+    y = _attend(gq, hip, kv, q, [first], None, 0, 1.0)
+    kk, vv = ref.values(k)[0], ref.values(v)[0]
+    for t in range(n_tok):
+        for h in range(nh):
+            g = h * nkv // nh
+            want, tol = ref.attention(q[0, t, h].astype(np.float64), kk[:, g], vv[:, g], first + t, 0, 1.0)
+            seen = vv[:first + t + 1, g]
+            tol = tol + 2.0 ** -32 * seen.sum(0) + 2.0 ** -35 * len(seen) * seen.max()
+            assert (np.abs(y[0, t, h] - want) <= tol).all(), (t, h, float((np.abs(y[0, t, h] - want) / tol).max()))

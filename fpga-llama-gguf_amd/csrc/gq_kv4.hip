@@ -12,22 +12,25 @@ namespace {
 // A block of 32 elements held by 8 lanes, lane j elements 4 j .. 4 j + 3: returns the lane's four quants as the low nibbles of four
 // bytes and, in d16, the block's fp16 scale.
 __device__ __forceinline__ uint32_t kv4_quantize(const float * x, uint32_t & d16) {
-    float am = fabsf(x[0]), m = x[0];
+    // magnitudes as words: a NaN is above all numbers and becomes the scale, so the block reads back as NaN
+    const auto size = [](float y) { return __float_as_uint(y) & 0x7fffffffu; };
+    uint32_t am = size(x[0]);
+    float m = x[0];
 #pragma unroll
     for (int i = 1; i < 4; ++i) {
-        const bool more = fabsf(x[i]) > am;
-        am = more ? fabsf(x[i]) : am;
+        const bool more = size(x[i]) > am;
+        am = more ? size(x[i]) : am;
         m = more ? x[i] : m;
     }
     const int lane = threadIdx.x;
-    const auto take = [&](float am2, float m2, bool later) {  // the other lanes' largest; of equal ones the first
-        const bool other = am2 > am || (later && am2 == am);
-        am = other ? am2 : am;
+    const auto take = [&](float m2, bool later) {  // the other lanes' largest; of equal ones the first
+        const bool other = size(m2) > am || (later && size(m2) == am);
+        am = other ? size(m2) : am;
         m = other ? m2 : m;
     };
-    take(dpp_f32<DPP_XOR1>(am), dpp_f32<DPP_XOR1>(m), lane & 1);
-    take(dpp_f32<DPP_XOR2>(am), dpp_f32<DPP_XOR2>(m), lane & 2);
-    take(dpp_f32<DPP_HALF_MIRROR>(am), dpp_f32<DPP_HALF_MIRROR>(m), lane & 4);
+    take(dpp_f32<DPP_XOR1>(m), lane & 1);
+    take(dpp_f32<DPP_XOR2>(m), lane & 2);
+    take(dpp_f32<DPP_HALF_MIRROR>(m), lane & 4);
     const float d = m / -8.0f, id = d != 0.0f ? 1.0f / d : 0.0f;
     d16 = f2h(d);
     uint32_t q = 0;

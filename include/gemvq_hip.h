@@ -345,7 +345,8 @@ typedef struct {
 /* 0 for sizes that are not served. */
 uint64_t gemvq_kv4_bytes(int n_seq, int n_ctx, int n_head_kv, int head_dim);
 /* Quantizes the tokens' keys and values (KV head h of a row at h * head_dim) into the cache, in FP32 as ggml does: d the
- * element of largest magnitude over -8, each value min(15, trunc(x * (1 / d) + 8.5)). */
+ * element of largest magnitude over -8, each value min(15, trunc(x * (1 / d) + 8.5)); a block with a NaN, or with more than fp16 holds as d, reads
+ * back as NaN and infinities. */
 int gemvq_kv4_store_static(const gemvq_kv4 * kv, const float * k, const float * v, int64_t row_stride, int n_tok,
                            const int32_t * pos, const int32_t * num, void * stream);
 /* The other way: what the cache holds at the tokens' positions, fp16(d) * (quant - 8). */

@@ -659,10 +659,42 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
         for (int i = 0; i < Kv4Tile<HD>::NW; ++i) dtop = max(dtop, max(tile.d[i] & 0x7fffu, (tile.d[i] >> 16) & 0x7fffu));
         if (lane < 32) dtop = 0;
         if (__any(int(dtop >> 10) - 15 + e >= 7)) {  // a larger value scale: bring it to 2^6
-            int top = int(dtop >> 10);
+            if (__any(dtop >= 0x7c00u)) {
+                // Infinities or NaN among the value scales: their blocks come out NaN in the rows that see the positions, and they become 0 (a
+                // weight of 0 times an infinity would be NaN in the other rows too)
+                tile.stage(scales[wave], lane, half2{_Float16(1.0f), _Float16(1.0f)});
+                wave_sync();
+#pragma unroll
+                for (int b = 0; b < NB; ++b) {
+                    const u32x4 vd = *reinterpret_cast<const u32x4 *>(&scales[wave][HD / 2 + (g * NB + b) * 4]);
+#pragma unroll
+                    for (int n = 0; n < NQ; ++n) {
+                        bool hit = false;
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {  // word i / 2: positions 0 and 2, 1 and 3 of the lane's four, and 16 further
+                            const int p = from + (i >> 2) * 16 + 4 * g + ((i >> 1) & 1) + 2 * (i & 1);
+                            hit |= p >= my_lo[n] && p <= my_hi[n] && (vd[i >> 1] >> 16 * (i & 1) & 0x7c00u) == 0x7c00u;
+                        }
+                        unsigned long long hits = __ballot(hit);
+                        hits |= hits >> 32;
+                        const float add = uint32_t(hits | hits >> 16) >> col & 1 ? __builtin_nanf("") : 0.0f;
+                        o[n][b][0] += add;
+                        o[n][b][1] += add;
+                    }
+                }
+                wave_sync();
+                dtop = 0;
+#pragma unroll
+                for (int i = 0; i < 2 * Kv4Tile<HD>::NW; ++i) {
+                    const uint32_t d = (tile.d[i >> 1] >> 16 * (i & 1)) & 0x7fffu;
+                    if (lane >= 32 && d >= 0x7c00u) tile.d[i >> 1] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+                    else if (lane >= 32) dtop = max(dtop, d);
+                }
+            }
+            int top = max(int(dtop >> 10), 6 + 15 - e);
 #pragma unroll
             for (int d = 32; d >= 1; d >>= 1) top = max(top, __shfl_xor(top, d, WAVE));
-            const int e2 = 6 + 15 - top;
+            const int e2 = 6 + 15 - top;  // (e where no finite scale asks for less)
             const float f = __uint_as_float(uint32_t(127 + e2 - e) << 23);
             e = e2;
             if (sums)

@@ -354,11 +354,13 @@ int gemvq_kv4_load_static(const gemvq_kv4 * kv, float * k, float * v, int64_t ro
                           const int32_t * num, void * stream);
 /* Attention: the token at position p gives y = sum_j softmax_j(scale * q . k_j) v_j over the positions j from 0, or from
  * max(0, p - window + 1) with window > 0, to p (store the tokens' own keys and values first). q head h of a row starts at
- * h * q_head_stride and reads KV head h / (n_head / n_head_kv); y's heads are packed. q enters as
- * it is (no rounding to 16 bits); scores, softmax statistics and sums are FP32. The matrix instructions' factors are sums of two
- * fp16 numbers: queries (22 bits of their row's largest element) and softmax weights times value scales (22 bits, but weights
- * no finer than 2^-31 of the row's largest, and scales no finer than 2^-30 of the largest among the positions read together). work: gemvq_kv4_attn_work() bytes of device memory, 16-byte aligned, whose
- * contents do not matter before or after; calls that may overlap need one each. */
+ * h * q_head_stride and reads KV head h / (n_head / n_head_kv); y's heads are packed. q enters as it is (no rounding to 16
+ * bits); scores, softmax statistics and sums are FP32. The matrix instructions' factors are sums of two fp16 numbers: queries
+ * (22 bits of their row's largest element) and softmax weights times value scales (22 bits, but weights no finer than 2^-31 of
+ * the row's largest, and scales no finer than 2^-30 of the largest among the positions read together). A block of values that
+ * has no finite scale comes out NaN in the rows that see its position; what other positions hold does not reach a row. work:
+ * gemvq_kv4_attn_work() bytes of device memory, 16-byte aligned, whose contents do not matter before or after; calls that may
+ * overlap need one each. */
 uint64_t gemvq_kv4_attn_work(const gemvq_kv4 * kv, int n_tok, int n_head);
 int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
                           int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,

@@ -1,4 +1,5 @@
-"""Attention over the 4-bit cache at the ends of its numbers: scores of any finite size, weights far below the largest."""
+"""Attention over the 4-bit cache at the ends of its numbers: scores of any finite size, weights far below the largest,
+infinities and NaN where a row does not look."""
 import numpy as np
 import pytest
 
@@ -80,3 +81,40 @@ def test_a_dominant_position_without_values(gq, hip, hd, n_tok):
             seen = vv[:first + t + 1, g]
             tol = tol + 2.0 ** -32 * seen.sum(0) + 2.0 ** -35 * len(seen) * seen.max()
             assert (np.abs(y[0, t, h] - want) <= tol).all(), (t, h, float((np.abs(y[0, t, h] - want) / tol).max()))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("nh,nkv,hd,n_tok", [(4, 2, 32, 70), (6, 2, 64, 33), (8, 2, 128, 20), (4, 1, 256, 9)])
+@pytest.mark.parametrize("first,window", [(0, 0), (45, 0), (0, 7), (600, 33), (9, 900)])
+def test_infinities_and_nan_out_of_sight(gq, hip, nh, nkv, hd, n_tok, first, window):
+    """Keys and values of later tokens, and of positions behind a token's window, that are infinite, NaN or too large for an fp16 scale: the
+    tokens that do not see them come out as if they were not there, the others not finite where they are."""
+    rng = np.random.default_rng(n_tok + first)
+    n = first + n_tok
+    k, v = _data(rng, 1, n, nkv, hd)
+    q = rng.standard_normal((1, n_tok, nh, hd)).astype(np.float32)
+    bad_v, bad_k = {first + n_tok // 2: (np.inf, 3), first + n_tok - 2: (np.nan, 31)}, {first + n_tok - 1: np.nan}
+    if window:
+        bad_v[max(first - 3, 0)] = (-3e6, 0)
+    kv, _ = _cache(gq, hip, 1, n, nkv, hd)
+    clean_k, clean_v = k.copy(), v.copy()
+    for p, (x, e) in bad_v.items():
+        v[0, p, :, e] = x
+    for p, x in bad_k.items():
+        k[0, p] = x
+    _store(gq, hip, kv, k, v, [0])
+    y = _attend(gq, hip, kv, q, [first], None, window, hd ** -0.5)[0]
+    kk, vv = ref.values(clean_k)[0], ref.values(clean_v)[0]
+    for t in range(n_tok):
+        p = first + t
+        seen = range(max(0, p - window + 1) if window else 0, p + 1)
+        for h in range(nh):
+            if any(x in seen for x in bad_k):
+                assert np.isnan(y[t, h]).all()
+                continue
+            want, tol = ref.attention(q[0, t, h].astype(np.float64), kk[:, h * nkv // nh], vv[:, h * nkv // nh], p, window, hd ** -0.5)
+            fine = np.ones(hd, bool)
+            if any(x in seen for x in bad_v):
+                fine[:32] = False
+                assert not np.isfinite(y[t, h, :32]).all()
+            assert (np.abs(y[t, h] - want) <= tol)[fine].all(), (t, h)

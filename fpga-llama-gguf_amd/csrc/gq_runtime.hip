@@ -128,11 +128,12 @@ struct LGemmQ { GemmQuantArgs a; };
 struct LGemm { GemmArgs a; int type; };
 struct LAttn4 { Kv4AppendArgs p; Kv4AttnArgs a; };
 struct LBeam { BeamSelectArgs a; };
-struct LBeamMove { BeamReorderArgs a; };
+struct LBeamMove { std::shared_ptr<BeamReorderArgs> a; };  // (2 KB: beside the launch, of which every command has one)
 struct LBeamNext { BeamNextArgs a; };
 struct LTok { TokArgs a; int type; uint32_t x_off, x_len; };  // x_off, x_len: the token rows read (activation floats)
 using Launch = std::variant<LGemv, LNorm, LEw, LConv, LRope, LGdn, LGated, LAttn, LRows, LArgmax, LNext, LGemmQ, LGemm,
                             LGdnOut, LTok, LAttn4, LBeam, LBeamMove, LBeamNext>;
+static_assert(sizeof(Launch) <= sizeof(LGemv) + 8, "a list's launches are compiled and copied one after another: no other is as large");
 
 }  // namespace
 
@@ -1203,28 +1204,28 @@ struct Compiler {
             if ((m[j].hi - m[j].lo) / BEAM_TILE + 1 > 0x7fffffffull / BEAM_MOVES / part_n[j]) return reject(i, "BEAM_MOVE size");
         // joins the launch before it: same parents, nothing of either met by the other
         const int32_t * parent = reinterpret_cast<const int32_t *>(A(k[6]));
-        LBeamMove * l = moves.open ? std::get_if<LBeamMove>(&out.back()) : nullptr;
-        if (l && (l->a.parent != parent || l->a.n_beam != int(nb) || l->a.n_group != int(ng) || l->a.n + nm > BEAM_MOVES ||
+        BeamReorderArgs * l = moves.open ? std::get<LBeamMove>(out.back()).a.get() : nullptr;
+        if (l && (l->parent != parent || l->n_beam != int(nb) || l->n_group != int(ng) || l->n + nm > BEAM_MOVES ||
                   meet_any(io.wr, moves.wr) || meet_any(io.wr, moves.rd) || meet_any(io.rd, moves.wr) || meet_any(io.state, moves.state) ||
                   (!io.kv.empty() && std::find(moves.kv.begin(), moves.kv.end(), io.kv[0]) != moves.kv.end())))
             l = nullptr;
         if (!l) {
-            LBeamMove fresh{};
-            fresh.a.parent = parent;
-            fresh.a.parent_stride = 16;
-            fresh.a.n_group = int(ng);
-            fresh.a.n_beam = int(nb);
-            out.push_back(fresh);
+            const auto fresh = std::make_shared<BeamReorderArgs>();
+            l = fresh.get();
+            l->parent = parent;
+            l->parent_stride = 16;
+            l->n_group = int(ng);
+            l->n_beam = int(nb);
+            out.push_back(LBeamMove{fresh});
             spans.push_back({int(i), 0});
-            l = std::get_if<LBeamMove>(&out.back());
             moves = {};
             moves.open = true;
         }
         for (int j = 0; j < nm; ++j) {
             if (m[j].lo >= m[j].hi) continue;
-            uint32_t end = l->a.n ? l->a.m[l->a.n - 1].end : 0;
+            uint32_t end = l->n ? l->m[l->n - 1].end : 0;
             beam_move_shape(m[j], part_n[j], end);
-            l->a.m[l->a.n++] = m[j];
+            l->m[l->n++] = m[j];
         }
         moves.wr.insert(moves.wr.end(), io.wr.begin(), io.wr.end());
         moves.rd.insert(moves.rd.end(), io.rd.begin(), io.rd.end());
@@ -1773,10 +1774,10 @@ std::pair<std::string, uint64_t> describe(const Launch & l, int pos) {
     if (auto * x = std::get_if<LBeam>(&l))
         return {"beam_scan_kernel", uint64_t(x->a.n_group) * x->a.n_beam * uint64_t(x->a.n_vocab) * 4};
     if (auto * x = std::get_if<LBeamMove>(&l)) {  // every row moved: its bytes read and written
+        const BeamReorderArgs & a = *x->a;
         uint64_t b = 0;
-        for (int i = 0; i < x->a.n; ++i)
-            b += (x->a.m[i].hi - x->a.m[i].lo) * ((x->a.m[i].end - (i ? x->a.m[i - 1].end : 0)) / x->a.m[i].tiles) * 2;
-        return {"beam_reorder_kernel", b * uint64_t(x->a.n_group) * x->a.n_beam};
+        for (int i = 0; i < a.n; ++i) b += (a.m[i].hi - a.m[i].lo) * ((a.m[i].end - (i ? a.m[i - 1].end : 0)) / a.m[i].tiles) * 2;
+        return {"beam_reorder_kernel", b * uint64_t(a.n_group) * a.n_beam};
     }
     if (std::get_if<LBeamNext>(&l)) return {"beam_next_kernel", 32};
     return {"next_token_kernel", 32};
@@ -1788,7 +1789,7 @@ int kernels_of(const Launch & l) {
     if (auto * x = std::get_if<LGdn>(&l)) return !x->ref && gdn_ahead(x->a) ? 2 : 1;
     if (auto * x = std::get_if<LAttn4>(&l)) return kv4_joins(x->a) ? 3 : 2;
     if (std::get_if<LBeam>(&l)) return 2;
-    if (auto * x = std::get_if<LBeamMove>(&l)) return x->a.n ? 1 : 0;
+    if (auto * x = std::get_if<LBeamMove>(&l)) return x->a->n ? 1 : 0;
     return 1;
 }
 
@@ -1830,7 +1831,7 @@ hipError_t issue(const std::vector<Launch> & ls, hipStream_t s) {
             e = launch_kv4_append(x->p, s);
             if (e == hipSuccess) e = launch_kv4_attn(x->a, s);
         } else if (auto * x = std::get_if<LBeam>(&l)) e = launch_beam_select(x->a, s);
-        else if (auto * x = std::get_if<LBeamMove>(&l)) e = x->a.n ? launch_beam_reorder(x->a, s) : hipSuccess;
+        else if (auto * x = std::get_if<LBeamMove>(&l)) e = x->a->n ? launch_beam_reorder(*x->a, s) : hipSuccess;
         else if (auto * x = std::get_if<LBeamNext>(&l)) e = launch_beam_next(x->a, s);
         if (e != hipSuccess) return e;
     }

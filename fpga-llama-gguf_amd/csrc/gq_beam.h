@@ -85,6 +85,7 @@ struct BeamMove {  // hi: used[...] + used_more units of the source row
 };
 constexpr int BEAM_MOVES = 24;      // arrays of one launch
 constexpr uint32_t BEAM_TILE = 4096;  // bytes of a part that a workgroup moves
+constexpr uint32_t BEAM_GRID = (1u << 24) - 1;  // workgroups of a launch: fewer than 2^32 threads
 struct BeamReorderArgs {
     BeamMove m[BEAM_MOVES];
     const int32_t * parent;  // row r's at parent[r * parent_stride], values outside 0 .. n_beam - 1: the row stays
@@ -98,6 +99,8 @@ inline bool beam_rows_apart(uint64_t rows, uint64_t size, uint64_t row_stride, u
     return part_stride >= (rows - 1) * row_stride + size ||
            (part_stride >= size && (rows == 1 || row_stride >= (n_part - 1) * part_stride + size));
 }
+// The workgroups of an array.
+inline uint64_t beam_move_groups(uint64_t lo, uint64_t hi, uint64_t n_part) { return (hi - lo + BEAM_TILE - 1) / BEAM_TILE * n_part; }
 // The workgroups of an array whose addresses are set, behind those of `end`, and whether it moves in pieces of 16 bytes.
 inline void beam_move_shape(BeamMove & m, uint32_t n_part, uint32_t & end) {
     m.wide = (reinterpret_cast<uintptr_t>(m.data) | m.row_stride | (n_part > 1 ? m.part_stride : 0) | m.lo | m.unit_bytes) % 16 == 0;

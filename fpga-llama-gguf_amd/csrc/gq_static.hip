@@ -244,7 +244,7 @@ int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, con
             return GEMVQ_EINVAL;
         if (x.used && (!aligned(x.used, 4) || x.unit_len < 1 || x.used_stride < 1)) return GEMVQ_EINVAL;
         if (!beam_rows_apart(rows, size, x.row_stride, x.part_stride, x.n_part)) return GEMVQ_EINVAL;
-        if (((size - uint64_t(x.first) * x.unit_bytes) / BEAM_TILE + 1) * x.n_part > 0x7fffffffu / BEAM_MOVES) return GEMVQ_EINVAL;
+        if (beam_move_groups(uint64_t(x.first) * x.unit_bytes, size, x.n_part) > BEAM_GRID) return GEMVQ_EINVAL;
     }
     for (int i = 0; i < n_arrays;) {
         BeamReorderArgs a{};
@@ -256,6 +256,7 @@ int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, con
         for (; i < n_arrays && a.n < BEAM_MOVES; ++i) {
             const gemvq_beam_array & x = arrays[i];
             if (x.first == x.count) continue;
+            if (end + beam_move_groups(uint64_t(x.first) * x.unit_bytes, uint64_t(x.count) * x.unit_bytes, x.n_part) > BEAM_GRID) break;
             BeamMove & m = a.m[a.n++];
             m.data = static_cast<uint8_t *>(x.data);
             m.row_stride = x.row_stride;

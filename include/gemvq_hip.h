@@ -388,7 +388,8 @@ int gemvq_beam_select_static(const float * logits, int64_t row_stride, int n_voc
  * row_stride + p * part_stride, of `count` units of unit_bytes each; units first .. count - 1 move (a prefix that all beams
  * share need not). With used (int32 in device memory, for row r at used[r * used_stride]), only the source row's units
  * below ceil(used / unit_len) move, and what the target has behind them stays. Addresses and sizes are multiples of 4 bytes
- * (of 16 for full speed); rows and parts, arrays, used and parent lie apart from one another. */
+ * (of 16 for full speed); rows and parts, arrays, used and parent lie apart from one another. A row's moved bytes, each part
+ * rounded up to 4 KB, are less than 64 GiB an array. */
 typedef struct {
     void * data;
     uint64_t row_stride, part_stride;

@@ -114,3 +114,44 @@ def test_ended_beams_without_a_score(gq, hip, beams, v, dead):
     last = np.full(2 * beams, 7, np.int32)
     last[1:beams] = 3
     check(select(gq, hip, x, score, last, 7, 2, beams), reference(x, score, last, 7, 2, beams))
+
+
+def _array(gq, data, **k):
+    d = dict(data=data, row_stride=64, part_stride=0, n_part=1, first=0, count=16, unit_bytes=4, unit_len=1, used=0, used_stride=1)
+    return gq.BeamArray(*{**d, **k}.values())
+
+
+def test_arrays_past_a_launch_are_refused(gq):
+    """Rows whose workgroups have 2^32 threads or more (no device is touched)."""
+    lib, P, g = gq.hip_lib(), 1 << 20, 1 << 30
+    for k in (dict(count=64, unit_bytes=g, row_stride=64 * g), dict(n_part=2, count=32, unit_bytes=g, row_stride=64 * g, part_stride=32 * g),
+              dict(n_part=65535, count=257, unit_bytes=4096, row_stride=257 << 12, part_stride=257 << 13)):
+        assert lib.gemvq_beam_reorder_static((gq.BeamArray * 1)(_array(gq, P, **k)), 1, P, 1, 2 if k.get("n_part") != 2 else 1, 0) == gq.EINVAL, k
+
+
+@pytest.mark.gpu
+def test_arrays_that_fill_several_launches(gq, hip):
+    """Two arrays of two rows of 33 GiB, whose workgroups do not fit one launch (of each the first 12288 bytes are in use), and small
+    ones before, between and behind them."""
+    rng = np.random.default_rng(2)
+    row, page = 33 << 30, 4096
+    try:
+        big = [hip.alloc(2 * row) for _ in range(2)]
+    except AssertionError:
+        pytest.skip("132 GiB of device memory are not free")
+    small = [rng.integers(0, 1 << 30, (2, 16)).astype(np.int32) for _ in range(3)]
+    large = [rng.integers(0, 256, (2, 4 * page)).astype(np.uint8) for _ in big]
+    for b, x in zip(big, large):
+        for i in range(2):
+            hip.write(b + i * row, x[i])
+    used = hip.upload(np.int32([3, 3]))
+    at = [hip.upload(x) for x in small]
+    arrays = [_array(gq, at[0])]
+    for b, p in zip(big, at[1:]):
+        arrays += [_array(gq, b, row_stride=row, count=row // page, unit_bytes=page, used=used), _array(gq, p)]
+    gq.beam_reorder_static(arrays, hip.upload(np.int32([1, 1])), 1, 2)
+    for x, p in zip(small, at):
+        assert np.array_equal(hip.download(p, x.shape, np.int32), x[[1, 1]])
+    for b, x in zip(big, large):
+        assert np.array_equal(hip.download(b, (4 * page,), np.uint8), np.concatenate([x[1, :3 * page], x[0, 3 * page:]]))
+        assert np.array_equal(hip.download(b + row, (4 * page,), np.uint8), x[1])

@@ -409,6 +409,7 @@ struct Compiler {
     std::vector<std::pair<int, int>> spans;  // per launch: first command, number of commands
     int bad = 0;  // 1-based index of the first invalid command
     std::string why;
+    std::vector<std::pair<uint32_t, int>> regions;  // 4-bit buffers of the list, with their positions of a sequence
 
     bool range(uint32_t off, uint64_t n) const { return off % 16 == 0 && uint64_t(off) + n <= c->act_floats; }
     // the list is compiled in the reference arithmetic (gq_ref.h): no fused forms whose arithmetic differs from it
@@ -1046,7 +1047,7 @@ struct Compiler {
     // scratch is shared by the context's buffers; without memory for it every sequence is one range.
     bool attn4(unsigned & i, const uint32_t * k, const uint32_t * k2, uint32_t nh, uint32_t nkv, uint32_t hd, uint32_t nrot,
                uint32_t qstride, uint32_t ntok) {
-        KvBuf & b = c->kvs[k[3]];
+        const KvBuf & b = c->kvs[k[3]];
         if (ref()) return reject(i, "ATTN on a 4-bit KV buffer in the reference arithmetic");
         if (nh == 0) return reject(i, "ATTN shape");
         const uint32_t flags = k[7], sets = ATTN_MAXG * nkv * GEMM_MAX_TOK / nh;
@@ -1064,7 +1065,7 @@ struct Compiler {
         LAttn4 l{};
         const Kv4Cache cache{b.q4, cap, int(nkv), int(hd), kv4_tiles(cap), (long long)b.q4_records};
         const Kv4Tokens t{reinterpret_cast<const int32_t *>(A(k[6])), nullptr, seqs ? 16 : 1, seqs ? 1 : int(ntok), seqs ? int(ntok) : 1};
-        b.region = cap;
+        regions.push_back({k[3], cap});
         l.p.c = l.a.c = cache;
         l.p.t = l.a.t = t;
         l.p.q = A(k[2]);
@@ -1170,7 +1171,7 @@ struct Compiler {
             if (meet_any(io.wr, io.rd)) return reject(i, "BEAM_MOVE of its own parents or positions");
         } else if (kind == GEMVQ_BEAM_KV) {
             if (k[2] >= c->kvs.size() || c->kvs[k[2]].n_ctx % int(rows) || !k2[0]) return reject(i, "BEAM_MOVE kv buffer");
-            KvBuf & b = c->kvs[k[2]];
+            const KvBuf & b = c->kvs[k[2]];
             const int cap = b.n_ctx / int(rows);
             if (first > uint32_t(cap)) return reject(i, "BEAM_MOVE kv buffer");
             if (b.q4) {
@@ -1183,7 +1184,7 @@ struct Compiler {
                 m[0].unit_len = KV4_TILE;
                 m[0].lo = first / KV4_TILE * rec;
                 m[0].hi = size_t(kv4_tiles(cap)) * rec;
-                b.region = cap;
+                regions.push_back({k[2], cap});
             } else {
                 const size_t row = size_t(b.n_head_kv) * b.head_dim * 2;
                 part_n[0] = 1;
@@ -1903,6 +1904,7 @@ int compile_list(gemvq_ctx * c, const uint32_t * cmds, unsigned n, std::vector<L
         c->err = cp.why;
         return cp.bad;
     }
+    for (const auto & [kv, cap] : cp.regions) c->kvs[kv].region = cap;
     out = std::move(cp.out);
     if (spans) *spans = std::move(cp.spans);
     c->last_launches = 0;

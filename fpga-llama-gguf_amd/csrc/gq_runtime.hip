@@ -281,16 +281,24 @@ void * optional_scratch(gemvq_ctx * c, size_t bytes) {
     return nullptr;
 }
 
-// At least `bytes` of s (growing at least twofold), NULL without memory for it.
-void * grown_scratch(gemvq_ctx * c, gemvq_ctx::Scratch & s, size_t bytes) {
+// At least `bytes` of s (growing twofold where there is memory for it), NULL without memory for them. needed: the launch cannot do
+// without, so the limit on scratch that it could do without does not hold.
+void * grown_scratch(gemvq_ctx * c, gemvq_ctx::Scratch & s, size_t bytes, bool needed) {
     if (s.n >= bytes) return s.p;
-    const size_t n = std::max(bytes, 2 * s.n);
-    void * p = optional_scratch(c, n);
-    if (!p) return nullptr;
-    if (s.p) s.old.push_back(s.p);
-    s.p = p;
-    s.n = n;
-    return p;
+    for (const size_t n : {std::max(bytes, 2 * s.n), bytes}) {
+        if (!c->usable || (!needed && n > c->scratch_max)) continue;
+        hipSetDevice(c->device);
+        void * p = nullptr;
+        if (hipMalloc(&p, n) != hipSuccess) {
+            (void)hipGetLastError();
+            continue;
+        }
+        if (s.p) s.old.push_back(s.p);
+        s.p = p;
+        s.n = n;
+        return p;
+    }
+    return nullptr;
 }
 
 int einval(gemvq_ctx * c, const std::string & what) {
@@ -1090,7 +1098,7 @@ struct Compiler {
         l.a.g_row = (long long)nh * qstride;
         l.a.g_head = qstride;
         if (const size_t work = kv4_work_floats(cache, t.n_seq, t.n_tok, int(nh)))
-            l.a.work = static_cast<float *>(grown_scratch(c, c->kv4_work, work * sizeof(float)));
+            l.a.work = static_cast<float *>(grown_scratch(c, c->kv4_work, work * sizeof(float), false));
         out.push_back(l);
         spans.push_back({int(i), 2});
         i += 2;
@@ -1127,7 +1135,7 @@ struct Compiler {
             a.prompt = reinterpret_cast<const int32_t *>(A(k2[3]));
             a.cap = int(cap);
         }
-        a.work = grown_scratch(c, c->beam_work, beam_work(a.n_group, a.n_beam, a.n_vocab));
+        a.work = grown_scratch(c, c->beam_work, beam_work(a.n_group, a.n_beam, a.n_vocab), true);
         if (!a.work) return reject(i, "BEAM: no memory for its workspace");
         out.push_back(LBeam{a});
         spans.push_back({int(i), 2});

@@ -40,3 +40,20 @@ def test_a_group_with_prompts_of_unlike_lengths(gq):
             assert np.array_equal(ctx.read(at["parent"], 16 * ns, np.int32)[::16], np.tile(np.arange(nb), ng)), p
             assert np.array_equal(ctx.read(at["score"], 16 * ns)[::16], score)
             assert np.array_equal(ctx.read(at["win"], rows.size).reshape(rows.shape), rows), p
+
+
+def test_beam_under_a_scratch_limit(gq, monkeypatch):
+    """The limit is on scratch that a launch can do without; the selection's workspace is none of it. Larger ones follow smaller ones."""
+    monkeypatch.setenv("GEMVQ_SCRATCH_LIMIT", "0")
+    rng = np.random.default_rng(2)
+    with gq.Context(act_floats=1 << 18, weight_bytes=1 << 12) as ctx:
+        ctx.write(64, slots(F([-1.0, -2.0])))
+        for v in (64, 512, 40000):
+            x = rng.standard_normal((2, v)).astype(F)
+            ctx.write(1024, x)
+            ctx.write(64, slots(F([-1.0, -2.0])))
+            assert ctx.run(gq.beam(v, 1024, v, 2, 1, -1, 64, 128, 192)) == 0, ctx.error()
+            lp = x - np.log(np.exp(x.astype(np.float64)).sum(1, keepdims=True)) + np.array([[-1.0], [-2.0]])
+            best = np.argsort(-lp.ravel(), kind="stable")[:2]
+            assert np.array_equal(ctx.read(192, 32, np.int32)[::16], best % v)
+            assert np.array_equal(ctx.read(128, 32, np.int32)[::16], best // v)

@@ -19,7 +19,7 @@ namespace {
 // group of 4: 7.0 and 4.7 us, both latency.
 
 // 2^t for -1020 <= t <= 0: t = n + f with |f| <= 1/2, 1 + f q(f) with q interpolating (2^f - 1) / f at 7 Chebyshev points (off by at
-// most 1.2e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of u = t + 1.5 * 2^52 as its low word.
+// most 1.1e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of u = t + 1.5 * 2^52 as its low word.
 __device__ __forceinline__ double beam_poly(double f, double u) {
     double p = 1.5297323765018243e-05;
     p = __builtin_fma(p, f, 0.00015461444698569867);

@@ -368,15 +368,16 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
 
 /* No counterpart in the reference: one step of a beam search over n_group independent groups of n_beam (1 .. GEMVQ_BEAM_MAX)
  * beams, rows g * n_beam + b, at most 65535 rows; on caller-owned device memory, under the rules of the calls above.
- * Selection: candidate v of beam b has the value score[b] + logit[b][v] - log(sum of e^logit[b]), formed in 64 bits; the
- * n_beam best candidates of a group, in descending order: score_out (rounded to FP32), token, and parent (the beam in the
- * group it continues); of equal ones the lower b * n_vocab + v first (among one beam's logits, the larger logit first). A
- * beam whose last token (last[row], or last NULL) is eos has ended: it has the one candidate eos, at its score, whatever
- * its logits (which are there all the same); eos outside the vocabulary: none ends. The candidates of a beam with score
- * -inf (the beams after the first, at a search's start) come after all others. NaN logits and scores count as -inf, +inf
- * logits as the largest finite number. logits: FP32 rows row_stride >= n_vocab floats apart, 1 <= n_vocab <=
- * GEMVQ_BEAM_MAX_VOCAB, 4-byte aligned. score_out may be score, token may be last. work: gemvq_beam_work() bytes, 16-byte
- * aligned, contents do not matter. */
+ * Selection: candidate v of beam b has the value score[b] + logit[b][v] - log(sum of e^logit[b]), formed in 64 bits, the
+ * logarithm to within 6e-10 (two beams' candidates that are closer than twice that may change places; beams with the same
+ * logits have the same logarithm); the n_beam best candidates of a group, in descending order: score_out (rounded to FP32),
+ * token, and parent (the beam in the group it continues); of equal ones the lower b * n_vocab + v first (among one beam's
+ * logits, the larger logit first; -0 and +0 are equal). A beam whose last token (last[row], or last NULL) is eos has ended: it
+ * has the one candidate eos, at its score, whatever its logits (which are there all the same); eos outside the vocabulary: none
+ * ends. The candidates of a beam with score -inf (the beams after the first, at a search's start) come after all others. NaN
+ * logits and scores count as -inf, +inf logits as the largest finite number. logits: FP32 rows row_stride >= n_vocab floats
+ * apart, 1 <= n_vocab <= GEMVQ_BEAM_MAX_VOCAB, 4-byte aligned. score_out may be score, token may be last. work:
+ * gemvq_beam_work() bytes, 16-byte aligned, contents do not matter. */
 #define GEMVQ_BEAM_MAX 32
 #define GEMVQ_BEAM_MAX_VOCAB (1 << 20)
 uint64_t gemvq_beam_work(int n_group, int n_beam, int n_vocab);

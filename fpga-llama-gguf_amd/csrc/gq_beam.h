@@ -42,7 +42,7 @@ __host__ __device__ inline uint32_t beam_order(float x) {
 }
 __host__ __device__ inline float beam_number(uint32_t o) { return __builtin_bit_cast(float, o & 0x80000000u ? o & 0x7fffffffu : ~o); }
 
-constexpr int BEAM_SLACK = 4;  // lanes beyond n_beam that a bound may let pass (24.4, 24.6 and 25.1 us with 4, 8 and 16 at 8 groups of 8 of 151936)
+constexpr int BEAM_SLACK = 4;  // lanes beyond n_beam that a bound may let pass (25.1, 25.2 and 25.6 us with 4, 8 and 16 at 8 groups of 8 of 151936)
 
 // A bound on a wave's words, of which at_least(w) lanes' are w or more (0: none; low: the smallest, high: the largest): at least k of
 // them are >= it, and no more than k + BEAM_SLACK if equal ones do not forbid that; with fewer than k words: 1. n: how many pass.

@@ -14,9 +14,9 @@ namespace {
 // lists n_beam times (or, of many, merges them). Values are 64-bit from the logits on (candidates of two beams may lie next to each
 // other). A list entry is one word that orders as the candidates of one row do: the logit's bits made monotone, above the token
 // inverted.
-// 8 groups of 8 beams of 151936 logits (39 MB): 16.3 us (2.4 TB/s: a workgroup's own way of read, reduce and rank is 7 us, the 64-bit
-// exponentials another 5, partly behind the reads) and 8.4 us, of which n_beam steps of about 0.4 us that wait for one another; one
-// group of 4: 7.0 and 4.7 us, both latency.
+// 8 groups of 8 beams of 151936 logits (39 MB): 16.2 us (2.4 TB/s: a workgroup's own way of read, reduce and rank is 7 us, the 64-bit
+// exponentials another 5, partly behind the reads) and 8.6 us, of which n_beam steps of about 0.4 us that wait for one another; one
+// group of 4: 6.8 and 4.7 us, both latency. (Kernel times by rocprofv3; those of the rules below are calls replayed in a graph.)
 
 // 2^t for -1020 <= t <= 0: t = n + f with |f| <= 1/2, 1 + f q(f) with q interpolating (2^f - 1) / f at 7 Chebyshev points (off by at
 // most 1.1e-10 of 2^f, exact at 0), and n added to the exponent. n comes out of u = t + 1.5 * 2^52 as its low word.
@@ -613,9 +613,9 @@ __global__ void beam_next_kernel(BeamNextArgs a) {
 
 int beam_chunks(int n_vocab, int per) { return (n_vocab + 256 * per - 1) / (256 * per); }
 // Logits a thread of the first kernel takes: 8, the shorter way through one workgroup, or 32 where those would give the second kernel
-// 192 lists a group or the first more workgroups than the device holds at once. Both kernels with 8 and 32: 10.2 and 11.6 us at one
-// group of 4 of 32000, 10.5 and 11.3 at one of 2 of 151936, 15.4 and 18.0 at 70 of 8 of 4000; 12.8 and 12.2 at one of 4 of 151936, 17.8
-// and 15.6 at one of 12 of 32000, 17.0 and 14.9 at 20 of 5 of 32003, 41.4 and 26.4 at 8 of 8 of 151936.
+// 192 lists a group or the first more workgroups than the device holds at once. Both kernels with 8 and 32: 10.0 and 11.0 us at one
+// group of 4 of 32000, 10.4 and 10.8 at one of 2 of 151936, 14.6 and 16.5 at 70 of 8 of 4000; 12.6 and 11.6 at one of 4 of 151936, 15.5
+// and 14.4 at one of 12 of 32000, 16.0 and 14.1 at 20 of 5 of 32003, 41.6 and 25.0 at 8 of 8 of 151936.
 int beam_per(int n_group, int n_beam, int n_vocab) {
     const int lists = n_beam * beam_chunks(n_vocab, 8);
     return lists >= 192 || (long long)n_group * lists >= 1536 ? 32 : 8;
@@ -630,9 +630,9 @@ size_t beam_work(int n_group, int n_beam, int n_vocab) {
 }
 
 // Winners from which on the lists are merged; also where a group has more lists than a wave's registers take the heads of. Both
-// kernels, winners one by one and merged: 25.3 and 26.1 us at 8 groups of 8 of 151936, 18.4 and 17.5 at one of 10 of 151936, 29.2 and
-// 26.3 at 4 of 12, 57 and 38 at one of 32; 32.3 and 25.3 at 17 of 29 of 4687. One by one with 2 and 5 lists a lane: 12.5 and 13.9 us at
-// one of 8 of 32000.
+// kernels, winners one by one and merged: 11.6 and 14.5 us at one group of 4 of 151936, 25.4 and 25.5 at 8 of 8, 18.2 and 17.0 at one of
+// 10, 28.7 and 25.5 at 4 of 12; 27.3 and 20.0 at 17 of 29 of 4687. One by one with 2 and 5 lists a lane: 12.1 and 13.6 us at one of 8 of
+// 32000.
 constexpr int BEAM_MANY = 10;
 hipError_t launch_beam_select(const BeamSelectArgs & args, hipStream_t s) {
     BeamSelectArgs a = args;

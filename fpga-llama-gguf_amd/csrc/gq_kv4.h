@@ -75,18 +75,19 @@ struct Kv4AttnArgs {
     int group;           // set at launch: n_head / n_head_kv
 };
 
+// Times of these rules, here and in gq_kv4.hip: a call alone (attention and joining; storing and reading back) replayed in a graph.
 // Workgroups of the attention a CU holds at once (nq groups of 16 query rows each): three where the registers can be kept to that (32
-// sequences of up to 8192, 32/8 heads of 128: 52 us, 58 with two). A call's records are dealt to as many as the device holds, each with
-// its share: twice as many, each with half of it, are 21.6 us in place of 19.9 (4 sequences of 8192, 32/8 heads of 128), 27.7 and 23.3
-// (8 of 5 tokens at 8000, 32/8 heads of 64), 30.7 and 24.7 (8 of 8 tokens, 16/4 heads of 128); 26.2 and 21.5 (one of 32768, 16/4 heads
-// of 256).
+// ragged sequences of up to 8192, 32/8 heads of 128: 46 us, 51 with two). A call's records are dealt to as many as the device holds, each
+// with its share: twice as many, each with half of it, are 25.1 us in place of 20.1 (4 sequences of 8192, 32/8 heads of 128), 32.5 and
+// 27.6 (8 of 5 tokens at 8000, 32/8 heads of 64), 37.0 and 29.3 (8 of 8 tokens at 8184, 16/4 heads of 128); 23.5 and 18.4 (one of 32768,
+// 16/4 heads of 256).
 __host__ __device__ constexpr int kv4_resident(int hd, int nq) { return hd * nq <= 128 ? 3 : 2; }
 constexpr int KV4_GROUPS = 768;   // at most
 constexpr int KV4_LEAST = 4;      // records of a range at least: one a wave
 // Records times head_dim up to which a cache's sequences are not split, which needs no second launch: its waves' few records more take
 // less than joining. Half as many where the cache is longer, but no sequence in it (us whole, whole with the second launch, and split:
-// one sequence of 320, 16/4 heads of 256, 12.7 / 14.2 / 12.8; 4 of 1500 19.7 / - / 13.8; 32 of 256, 32/8 heads of 128, 10.2 / 13.3 /
-// 16.6; 7 of 5 tokens in a window of 1000, 8 heads of 64, - / 14.3 / 13.3).
+// one sequence of 320, 16/4 heads of 256, 10.2 / 11.5 / 10.3, of 640 13.5 / 15.0 / 10.4; 4 of 1500 26.0 / 27.9 / 14.8; 32 of 256, 32/8
+// heads of 128, in caches of 8192, 7.7 / 10.2 / 12.8; 7 of 5 tokens in a window of 1000, 8 heads of 64, 10.5 / 12.8 / 11.1).
 constexpr int KV4_ALONE = 2048;
 bool kv4_joins(const Kv4AttnArgs & a);  // the launch is followed by that of kv4_join_kernel
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head);

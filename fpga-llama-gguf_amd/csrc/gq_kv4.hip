@@ -58,7 +58,7 @@ __device__ __forceinline__ uint8_t * kv4_rec(const Kv4Cache & c, int s, int h, i
 // 1983 tokens of 4 heads of 256 (18.5 MB): 8.0 us, 2.3 TB/s; 512 of them 4.9 us; one token of each of 32 sequences, 8 heads of 128, 3 us.
 // The launch and one trip to memory are 3 to 4 us of each; behind them the largest is bound by the shuffles and conversions of its
 // blocks.
-constexpr int KV4_STORE = 256;  // threads (1983 tokens as below with their reading back: 17.9, 15.7 and 14.6 us with 64, 128 and 256)
+constexpr int KV4_STORE = 256;  // threads (1983 tokens of 4 heads of 256 with their reading back: 17.6, 15.3 and 14.3 us with 64, 128 and 256)
 template <int HD>
 __global__ __launch_bounds__(KV4_STORE) void kv4_store_kernel(Kv4RowsArgs a) {
     using L = Kv4Layout<HD>;
@@ -265,12 +265,12 @@ __global__ __launch_bounds__(256) void kv4_load_records_kernel(Kv4RowsArgs a) {
 // its range in turn and join at the end; ranges of one sequence are joined by kv4_join_kernel.
 // A record and 16 rows, heads of 256, are 64 matrix instructions and about 540 others, half of them unpacking; wider heads than 128
 // leave no registers for more than 16 rows to share that. What bounds it, by the counters:
-//   512 tokens at 7680, 16/4 heads of 256: 179 us, 370 TFLOP/s of the formula's 66.6 GFLOP (twice that in parts). Vector instructions
-//     are issued in 64 % of the cycles, and without any matrix instruction it would still be 159 us: each hundred instructions less a
-//     record are 21 us.
-//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 39 us, 3.9 TB/s; vector instructions in 47 %, matrix instructions in 16 %,
+//   512 tokens at 7680, 16/4 heads of 256: 180 us, 370 TFLOP/s of the formula's 66.6 GFLOP (twice that in parts). Vector instructions
+//     are issued in 64 % of the cycles, and without any matrix instruction it would still be 160 us: each hundred instructions less a
+//     record are 21 us. (Kernel times, here and below, by rocprofv3.)
+//   32 sequences of up to 8192, 32/8 heads of 128 (152 MB): 40 us, 3.8 TB/s; vector instructions in 47 %, matrix instructions in 16 %,
 //     the rest the beginnings and ends of workgroups that have some ten records a wave.
-//   one sequence of 32768, 16/4 heads of 256 (38 MB): 14.5 us, 2.6 TB/s, two records a wave: the chain of position, record, sums and
+//   one sequence of 32768, 16/4 heads of 256 (38 MB): 14.6 us, 2.6 TB/s, two records a wave: the chain of position, record, sums and
 //     joining is half of it; of 640: 7.2 us, that chain alone.
 // Tried and taken back, for the 512 tokens, then at 202 us: workgroups whose waves share one record's unpacking for 64 rows through LDS
 // (two barriers a record; 190 us and 16 us of joining); 32 rows a wave at heads of 256 with one wave a SIMD (244 us). A raised wave
@@ -482,7 +482,7 @@ __device__ __forceinline__ bool kv4_find(const Kv4AttnArgs & a, int range, int &
     }
     int per = kv4_per(sum, a.ranges, a.t.n_seq, most, a.c.head_dim);
     // That leaves room for a short range of every sequence; less will do. Worth its 0.3 us where the sequences are many (32 of up to
-    // 8192, 32/8 heads of 128: 53.0 and 58.2 us).
+    // 8192, 32/8 heads of 128: 46 and 51 us).
     if (a.t.n_seq <= 64 && 8 * a.t.n_seq > a.ranges && per < most) {
         int low = max(int((sum + a.ranges - 1) / a.ranges), KV4_LEAST);
         for (int i = 0; i < 4 && low < per; ++i) {
@@ -542,7 +542,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     u32x4(*ql)[64] = reinterpret_cast<u32x4(*)[64]>(both);              // the queries' parts
     float(*part)[ROWS][PAD] = reinterpret_cast<float(*)[ROWS][PAD]>(both);  // later the waves' sums
     // The queries' parts that stay in registers, as many as leave room for two waves a SIMD (512 tokens at 7680, us with two, one and
-    // none: 16/4 heads of 256 184.9 / 187.8 / 192.4, 32/8 of 128 no room / 172.1 / 176.5). The others are read from LDS for every
+    // none: 16/4 heads of 256 178.8 / 181.6 / 185.7, 32/8 of 128 no room / 167.3 / 170.7). The others are read from LDS for every
     // record.
     constexpr int QR = NQ == 1 || HD * NQ <= 128 ? 2 : 1;
     __shared__ float kqs[ROWS], cs[4][ROWS], ls[4][ROWS];
@@ -927,8 +927,7 @@ __global__ __launch_bounds__(256) void kv4_join_kernel(Kv4AttnArgs a) {
 }
 
 // The same for many rows (q heads of tokens): a wave `per_wave` of them one after another, its lanes HD / 4 to a set. What each
-// workgroup does before its first row (finding the sequence's ranges, 2 us) is shared by its rows. 3 sequences of 360 tokens of 8 heads
-// of 64: 14 us.
+// workgroup does before its first row (finding the sequence's ranges, 2 us) is shared by its rows.
 template <int HD>
 __global__ __launch_bounds__(256) void kv4_join_rows_kernel(Kv4AttnArgs a, int per_wave) {
     constexpr int PER = HD / 4, SETS = 64 / PER;
@@ -1005,7 +1004,7 @@ hipError_t launch_kv4_store(const Kv4RowsArgs & a, hipStream_t s) {
 }
 
 // Rows (KV heads of tokens) from which on the records are read whole, where a sequence has tokens for half a record; us with single
-// rows and records, and the storing before: 8.1 and 9.3 at 400 rows, 10.5 and 10.6 at 2048, 10.2 and 8.9 at 4096, 18.2 and 15.5 at 7932.
+// rows and records, and the storing before: 6.6 and 7.6 at 400 rows, 8.5 and 8.8 at 2048, 9.4 and 8.1 at 4096, 16.7 and 14.2 at 7932.
 constexpr int KV4_RECORDS = 2048;
 hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s) {
     const unsigned span = unsigned((a.t.n_tok + KV4_TILE - 2) / KV4_TILE + 1);  // records that n_tok positions can touch
@@ -1032,8 +1031,8 @@ int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     const long long records = (long long)n_seq * kv4_tiles(c.n_ctx), most = (long long)n_seq * ((kv4_tiles(c.n_ctx) + KV4_LEAST - 1) / KV4_LEAST);
     long long ranges = std::max<long long>(n_seq, std::min(groups / units, most));
     // Few long ranges for sequences of unlike lengths come out unlike themselves: twice as many (3 sequences of 96 tokens at up to
-    // 10776, 32/8 heads of 128: 58 and 79 us; one of 512 at 7680, 16/4 heads of 256, 192 and 185; 3 of 360 at 1451, 8 heads of 64, 49
-    // and 42).
+    // 10776, 32/8 heads of 128: 54 us, 76 without). Of others twice as many are no gain (187 and 179 us at one of 512 at 7680, 16/4 heads
+    // of 256; 25.0 and 23.6 at 3 of 360 at up to 1451, 8 heads of 64; 28.0 and 22.0 at 8 of 8 at up to 8184, 16/4 heads of 128).
     if (n_seq > 1 && records >= 128 * ranges) ranges = std::max<long long>(ranges, std::min<long long>(2 * ranges, KV4_GROUPS));
     return int(std::min<long long>(ranges, 65535));
 }
@@ -1046,8 +1045,8 @@ size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
 bool kv4_joins(const Kv4AttnArgs & a) { return a.work && kv4_ranges(a.c, a.t.n_seq, a.t.n_tok, a.n_head) > a.t.n_seq; }
 
 // Rows (q heads of tokens) up to which each has workgroups of its own: several up to half as many. us with several, one, and a wave's
-// share of one: 26.7 / 24.7 / 25.3 at 320 rows, 30.8 / 30.4 / 32.2 at 352 (of 23 sets), 47.7 / 45.2 / 45.5 at 512, 55.6 / 51.4 / 49.7
-// at 1024, - / 61.2 / 41.7 at 8640.
+// share of one: 22.9 / 22.0 / 24.1 at 320 rows (20 tokens at 8172, 16/4 heads of 256), 12.9 / 12.9 / 12.6 at 320 (40 at 1411, 8 heads of 64),
+// 22.1 / 20.8 / 20.9 at 512, 51.4 / 48.5 / 46.6 at 1024, 35.9 / 35.9 / 24.0 at 8640.
 constexpr int KV4_FEW = 512;
 hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
     Kv4AttnArgs a = args;

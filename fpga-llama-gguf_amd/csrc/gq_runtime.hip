@@ -2184,6 +2184,7 @@ int gemvq_kv_create(gemvq_ctx * c, int n_ctx, int n_head_kv, int head_dim) {
     b.head_dim = head_dim;
     if (c->kv_type == GEMVQ_KV_Q4_0) {
         if (!kv4_dim_ok(head_dim)) return einval(c, "gemvq_kv_create: a 4-bit buffer takes heads of 32, 64, 128 or 256");
+        if (n_head_kv > 0xffff) return einval(c, "gemvq_kv_create: shape");  // (what ATTN can name; sizes below stay below 2^56)
         // whole records for each of up to GEMM_MAX_TOK sequences' regions
         b.q4_records = size_t(kv4_tiles(n_ctx)) + GEMM_MAX_TOK;
         const size_t bytes = b.q4_records * n_head_kv * kv4_record(head_dim);

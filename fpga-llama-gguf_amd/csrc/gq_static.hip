@@ -51,10 +51,13 @@ bool rows_ok(const void * p, int64_t stride, int64_t least) {
 
 constexpr int GRID_MAX = 65535;
 
-bool kv4_sizes_ok(const gemvq_kv4 * c) {
-    return c && c->n_seq > 0 && c->n_seq <= GRID_MAX && c->n_ctx > 0 && c->n_head_kv > 0 && c->n_head_kv <= GRID_MAX &&
-           kv4_dim_ok(c->head_dim);
+// Bytes of a cache; 0: sizes that are not served (2^46 bytes and more among them, whose offsets would pass 64 bits).
+uint64_t kv4_bytes(int n_seq, int n_ctx, int n_head_kv, int head_dim) {
+    if (n_seq < 1 || n_seq > GRID_MAX || n_ctx < 1 || n_head_kv < 1 || n_head_kv > GRID_MAX || !kv4_dim_ok(head_dim)) return 0;
+    const uint64_t records = uint64_t(n_seq) * uint64_t(n_head_kv) * uint64_t(kv4_tiles(n_ctx));
+    return records < (uint64_t(1) << 46) / kv4_record(head_dim) ? records * kv4_record(head_dim) : 0;
 }
+bool kv4_sizes_ok(const gemvq_kv4 * c) { return c && kv4_bytes(c->n_seq, c->n_ctx, c->n_head_kv, c->head_dim); }
 // Query rows of a sequence: their workgroups fit a grid.
 bool kv4_heads_ok(const gemvq_kv4 * c, int n_tok, int n_head) {
     return n_tok >= 1 && n_tok <= GEMVQ_KV4_MAX_TOK && n_head >= 1 && n_head <= GRID_MAX && n_head % c->n_head_kv == 0 &&
@@ -133,10 +136,7 @@ extern "C" int gemvq_gemm_static(int type, int rows, int cols, const void * w, c
 
 extern "C" {
 
-uint64_t gemvq_kv4_bytes(int n_seq, int n_ctx, int n_head_kv, int head_dim) {
-    if (n_seq < 1 || n_seq > GRID_MAX || n_ctx < 1 || n_head_kv < 1 || n_head_kv > GRID_MAX || !kv4_dim_ok(head_dim)) return 0;
-    return uint64_t(n_seq) * uint64_t(n_head_kv) * uint64_t(kv4_tiles(n_ctx)) * kv4_record(head_dim);
-}
+uint64_t gemvq_kv4_bytes(int n_seq, int n_ctx, int n_head_kv, int head_dim) { return kv4_bytes(n_seq, n_ctx, n_head_kv, head_dim); }
 
 int gemvq_kv4_store_static(const gemvq_kv4 * kv, const float * k, const float * v, int64_t row_stride, int n_tok,
                            const int32_t * pos, const int32_t * num, void * stream) {

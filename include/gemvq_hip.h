@@ -342,7 +342,7 @@ typedef struct {
     void * data;
     int32_t n_seq, n_ctx, n_head_kv, head_dim;
 } gemvq_kv4;
-/* 0 for sizes that are not served. */
+/* 0 for sizes that are not served (2^46 bytes and more among them). */
 uint64_t gemvq_kv4_bytes(int n_seq, int n_ctx, int n_head_kv, int head_dim);
 /* Quantizes the tokens' keys and values (KV head h of a row at h * head_dim) into the cache, in FP32 as ggml does: d the
  * element of largest magnitude over -8, each value min(15, trunc(x * (1 / d) + 8.5)); a block with a NaN, or with more than fp16 holds as d, reads

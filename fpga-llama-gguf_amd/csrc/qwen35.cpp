@@ -746,6 +746,7 @@ int gemvq_qwen35_batch_set_beam(gemvq_qwen35 * m, int n_beam, int eos) {
 
 int gemvq_qwen35_batch_scores(gemvq_qwen35 * m, float * out) {
     if (!m || !out || !m->n_beam) return GEMVQ_EINVAL;
+    if (m->beams_changed) return set_err(m->ctx, "gemvq_qwen35_batch_scores: gemvq_qwen35_batch_set_beam takes a reset first");
     std::vector<float> slots(size_t(m->n_seq) * 16);
     const int st = gemvq_act_read(m->ctx, m->sscore, slots.data(), slots.size());
     for (int s = 0; s < m->n_seq && !st; ++s) out[s] = slots[size_t(s) * 16];

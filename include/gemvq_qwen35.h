@@ -92,7 +92,7 @@ int gemvq_qwen35_batch_reset(gemvq_qwen35 * m, const int32_t * prompts, const in
 int gemvq_qwen35_batch_tokens(gemvq_qwen35 * m, int seq, int32_t * out, int n);
 int gemvq_qwen35_batch_logits(gemvq_qwen35 * m, int seq, float * out);
 /* Beam search over a batch model (no counterpart in the reference): its sequences become n_seq / n_beam groups of n_beam beams
- * (sequences g * n_beam + b). It takes a gemvq_qwen35_batch_reset next (a step before it is refused), with the same
+ * (sequences g * n_beam + b). It takes a gemvq_qwen35_batch_reset next (a step or _scores before it are refused), with the same
  * prompt for all beams of a group. Steps read the prompt as before, and behind it select the n_beam best continuations
  * of each group (BEAM), let states, conv windows, caches and ids follow their parents (BEAM_MOVE) and append the new
  * tokens, all in the step's graph. Beams are in descending order of their scores (sums of the tokens' log

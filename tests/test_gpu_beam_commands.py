@@ -1,6 +1,8 @@
-"""The beam search's commands in lists: groups that read their prompts."""
+"""The beam search's commands in lists and in the model driver at their edges."""
 import numpy as np
 import pytest
+
+from test_gpu_kv4_commands import small
 
 pytestmark = pytest.mark.gpu
 F = np.float32
@@ -57,3 +59,22 @@ def test_beam_under_a_scratch_limit(gq, monkeypatch):
             best = np.argsort(-lp.ravel(), kind="stable")[:2]
             assert np.array_equal(ctx.read(192, 32, np.int32)[::16], best % v)
             assert np.array_equal(ctx.read(128, 32, np.int32)[::16], best // v)
+
+
+def test_no_scores_of_an_earlier_search(gq):
+    """Between set_beam and reset there are no scores: those in memory are another search's, in other groups."""
+    import qwen35
+
+    with qwen35.BatchModel(qwen35.generate(small(qwen35), seed=5), 4) as bm:
+        bm.set_beam(2)
+        with pytest.raises(gq.GemvqError, match="reset first"):
+            bm.scores()
+        bm.reset([[1, 2]] * 4)
+        assert np.array_equal(bm.scores(), F([0, -np.inf, 0, -np.inf]))
+        bm.step(3)
+        assert np.isfinite(bm.scores()).all()
+        bm.set_beam(4)
+        with pytest.raises(gq.GemvqError, match="reset first"):
+            bm.scores()
+        bm.reset([[1, 2]] * 4)
+        assert np.array_equal(bm.scores(), F([0, -np.inf, -np.inf, -np.inf]))

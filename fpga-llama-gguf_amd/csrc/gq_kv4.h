@@ -77,7 +77,7 @@ struct Kv4AttnArgs {
 
 // Times of these rules, here and in gq_kv4.hip: a call alone (attention and joining; storing and reading back) replayed in a graph.
 // Workgroups of the attention a CU holds at once (nq groups of 16 query rows each): three where the registers can be kept to that (32
-// ragged sequences of up to 8192, 32/8 heads of 128: 46 us, 51 with two). A call's records are dealt to as many as the device holds, each
+// ragged sequences of up to 8192, 32/8 heads of 128: 46 us, 50 with two). A call's records are dealt to as many as the device holds, each
 // with its share: twice as many, each with half of it, are 25.1 us in place of 20.1 (4 sequences of 8192, 32/8 heads of 128), 32.5 and
 // 27.6 (8 of 5 tokens at 8000, 32/8 heads of 64), 37.0 and 29.3 (8 of 8 tokens at 8184, 16/4 heads of 128); 23.5 and 18.4 (one of 32768,
 // 16/4 heads of 256).

@@ -251,12 +251,12 @@ __global__ __launch_bounds__(256) void kv4_load_records_kernel(Kv4RowsArgs a) {
 //                 multiplied by its scales in FP32. (The quants' bits as they are, 2^-24 n, with the 8 taken off through the
 //                 accumulator's start, are a tenth fewer vector instructions, but the instruction's sums of such small factors keep
 //                 several bits less: results are off by 5e-6 in place of 3e-7.)
-//   P = 2^(S - c) in FP32, c = m - 7 with m the query's running maximum, taken anew when a score passes it by 2 (so P <= 2^9). P is the
-//                 sum of two fp16 numbers: 22 bits, but no finer than 2^-24, at most 2^-31 of the largest weight. (FP32 would keep 24
-//                 bits of the smallest ones too, in three parts: half as many matrix instructions again. The nearer P is to the end of
-//                 fp16's range, the less is lost, and the more often maxima are taken anew: 512 tokens at 7680, 16/4 heads of 256,
-//                 178.6 us with m - 4 and 4 more, 180.0 with m - 6 and 3, 180.8 so.) Lane 16 g + q holds query q's weights of the 8
-//                 positions that it feeds to
+//   P = 2^(S - c) in FP32, c = m - 4 with m the query's running maximum, or m - 7 where that is far above the one before it, taken anew
+//                 when a score passes c by 9 (so P <= 2^9). P is the sum of two fp16 numbers: 22 bits, but no finer than 2^-24: at most
+//                 2^-28 of the largest weight, and 2^-31 where one position is 2^9 above all others and the sum is made of small
+//                 weights beside it. (FP32 would keep 24 bits of the smallest ones too, in three parts: half as many matrix instructions
+//                 again. m - 7 always: 512 tokens at 7680, us with m - 4, so, and m - 7: 16/4 heads of 256 175.0 / 174.9 / 178.1,
+//                 16/2 of 64 59.8 / 60.4 / 63.9.) Lane 16 g + q holds query q's weights of the 8 positions that it feeds to
 //   O^T += V^T P^T: the quants minus 8 again; a block's scales go to the weights, P d = h + l: h the rounded product of d and P's upper
 //                 part, l, by two fused multiply-adds, what that rounding left and the lower part's product (22 bits). The scales
 //                 are brought up by a power of two 2^e common to the wave, the largest so far to 2^6..2^7, its 11 bits below 2^7, so
@@ -542,7 +542,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     u32x4(*ql)[64] = reinterpret_cast<u32x4(*)[64]>(both);              // the queries' parts
     float(*part)[ROWS][PAD] = reinterpret_cast<float(*)[ROWS][PAD]>(both);  // later the waves' sums
     // The queries' parts that stay in registers, as many as leave room for two waves a SIMD (512 tokens at 7680, us with two, one and
-    // none: 16/4 heads of 256 178.8 / 181.6 / 185.7, 32/8 of 128 no room / 167.3 / 170.7). The others are read from LDS for every
+    // none: 16/4 heads of 256 175.0 / 178.8 / 182.9, 32/8 of 128 no room / 161.3 / 164.9). The others are read from LDS for every
     // record.
     constexpr int QR = NQ == 1 || HD * NQ <= 128 ? 2 : 1;
     __shared__ float kqs[ROWS], cs[4][ROWS], ls[4][ROWS];
@@ -756,7 +756,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
             for (int n = 0; n < NQ; ++n) {
                 float m = fmaxf(top[n], __shfl_xor(top[n], 16, WAVE));
                 m = fmaxf(m, __shfl_xor(m, 32, WAVE));
-                const float c2 = fmaxf(m - 7.0f, c[n]), f = __builtin_amdgcn_exp2f(c[n] - c2);
+                const float c2 = fmaxf(m - (m - c[n] > 13.0f ? 7.0f : 4.0f), c[n]), f = __builtin_amdgcn_exp2f(c[n] - c2);
                 c[n] = c2;
                 l[n] *= f;
                 if (sums)
@@ -1031,8 +1031,8 @@ int kv4_ranges(const Kv4Cache & c, int n_seq, int n_tok, int n_head) {
     const long long records = (long long)n_seq * kv4_tiles(c.n_ctx), most = (long long)n_seq * ((kv4_tiles(c.n_ctx) + KV4_LEAST - 1) / KV4_LEAST);
     long long ranges = std::max<long long>(n_seq, std::min(groups / units, most));
     // Few long ranges for sequences of unlike lengths come out unlike themselves: twice as many (3 sequences of 96 tokens at up to
-    // 10776, 32/8 heads of 128: 54 us, 76 without). Of others twice as many are no gain (187 and 179 us at one of 512 at 7680, 16/4 heads
-    // of 256; 25.0 and 23.6 at 3 of 360 at up to 1451, 8 heads of 64; 28.0 and 22.0 at 8 of 8 at up to 8184, 16/4 heads of 128).
+    // 10776, 32/8 heads of 128: 53 us, 74 without). Of others twice as many are no gain (182 and 175 us at one of 512 at 7680, 16/4 heads
+    // of 256; 25.1 and 23.7 at 3 of 360 at up to 1451, 8 heads of 64; 28.0 and 21.8 at 8 of 8 at up to 8184, 16/4 heads of 128).
     if (n_seq > 1 && records >= 128 * ranges) ranges = std::max<long long>(ranges, std::min<long long>(2 * ranges, KV4_GROUPS));
     return int(std::min<long long>(ranges, 65535));
 }

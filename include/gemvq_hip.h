@@ -356,8 +356,9 @@ int gemvq_kv4_load_static(const gemvq_kv4 * kv, float * k, float * v, int64_t ro
  * max(0, p - window + 1) with window > 0, to p (store the tokens' own keys and values first). q head h of a row starts at
  * h * q_head_stride and reads KV head h / (n_head / n_head_kv); y's heads are packed. q enters as it is (no rounding to 16
  * bits); scores, softmax statistics and sums are FP32. The matrix instructions' factors are sums of two fp16 numbers: queries
- * (22 bits of their row's largest element) and softmax weights times value scales (22 bits, but weights no finer than 2^-31 of
- * the row's largest, and scales no finer than 2^-30 of the largest among the positions read together). A block of values that
+ * (22 bits of their row's largest element) and softmax weights times value scales (22 bits, but weights no finer than 2^-28 of
+ * the row's largest, or 2^-31 where that is 2^9 above all others, and scales no finer than 2^-30 of the largest among the
+ * positions read together). A block of values that
  * has no finite scale comes out NaN in the rows that see its position; what other positions hold does not reach a row. work:
  * gemvq_kv4_attn_work() bytes of device memory, 16-byte aligned, whose contents do not matter before or after; calls that may
  * overlap need one each. */

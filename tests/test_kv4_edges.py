@@ -58,7 +58,8 @@ def test_scores_of_any_size(gq, hip, nh, nkv, hd, size, first, n_tok):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("hd,n_tok", [(32, 1), (64, 40), (128, 1), (128, 20), (256, 3)])
-def test_a_dominant_position_without_values(gq, hip, hd, n_tok):
+@pytest.mark.parametrize("at", [11, 500])
+def test_a_dominant_position_without_values(gq, hip, hd, n_tok, at):
     """One position far above all others, whose values are zero: the output is made of the others' weights alone. All of them are equal, so
     what rounding leaves of one adds up. A weight is held no finer than 2^-31 of the largest (off by half of that), a weight times a
     value scale no finer than 2^-24 beside a largest product of at least 2^7 * 2^6 (8 quants of the largest scale: 2^-35 of the values)."""
@@ -67,7 +68,7 @@ def test_a_dominant_position_without_values(gq, hip, hd, n_tok):
     first = n - n_tok
     k = np.zeros((1, n, nkv, hd), np.float32)
     v = rng.uniform(0.5, 1.5, (1, n, nkv, hd)).astype(np.float32)
-    k[0, 11, :, 3], v[0, 11] = 1, 0
+    k[0, at, :, 3], v[0, at] = 1, 0
     q = rng.standard_normal((1, n_tok, nh, hd)).astype(np.float32)
     q[..., 3] = np.linspace(9, 22, n_tok * nh).reshape(n_tok, nh)  # how far above, in nats
     kv, _ = _cache(gq, hip, 1, n, nkv, hd)

@@ -1215,7 +1215,8 @@ struct Compiler {
         // joins the launch before it: same parents, nothing of either met by the other
         const int32_t * parent = reinterpret_cast<const int32_t *>(A(k[6]));
         BeamReorderArgs * l = moves.open ? std::get<LBeamMove>(out.back()).a.get() : nullptr;
-        if (l && (l->parent != parent || l->n_beam != int(nb) || l->n_group != int(ng) || l->n + nm > BEAM_MOVES || (l->n && l->m[l->n - 1].end + groups > BEAM_GRID) ||
+        if (l && (l->parent != parent || l->n_beam != int(nb) || l->n_group != int(ng) || l->n + nm > BEAM_MOVES ||
+                  (l->n && l->m[l->n - 1].end + groups > BEAM_GRID) ||
                   meet_any(io.wr, moves.wr) || meet_any(io.wr, moves.rd) || meet_any(io.rd, moves.wr) || meet_any(io.state, moves.state) ||
                   (!io.kv.empty() && std::find(moves.kv.begin(), moves.kv.end(), io.kv[0]) != moves.kv.end())))
             l = nullptr;

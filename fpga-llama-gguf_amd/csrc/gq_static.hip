@@ -4,14 +4,17 @@
 // process ends). Nothing here allocates: the array's address on a device is looked up once, on the first call on
 // that device, and kept.
 // The 4-bit KV cache (gemvq_kv4_*_static) and the beam search's step (gemvq_beam_*_static) on caller-owned memory: their arguments'
-// checks and launches.
+// checks and launches. So for rotary positions (gemvq_rope_*) and the verification of drafted tokens (gemvq_draft_*).
 #include "gemvq_hip.h"
 #include "gq_beam.h"
+#include "gq_draft.h"
 #include "gq_kernels.h"
 #include "gq_kv4.h"
+#include "gq_rope.h"
 
 #include <hip/hip_runtime.h>
 
+#include <cmath>
 #include <mutex>
 
 using namespace gq;
@@ -274,6 +277,94 @@ int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, con
         if (e != hipSuccess) return -int(e);
     }
     return 0;
+}
+
+}  // extern "C"
+
+static_assert(GEMVQ_ROPE_MAX_ARRAYS == ROPE_ARRAYS && GEMVQ_ROPE_MAX_DIM == ROPE_MAX_DIM, "limits in the header");
+static_assert(GEMVQ_DRAFT_MAX == DRAFT_MAX && GEMVQ_DRAFT_MAX_VOCAB == DRAFT_MAX_VOCAB, "limits in the header");
+
+extern "C" {
+
+int gemvq_rope_freqs(int n_rot, double base, double factor, int yarn_ctx, double beta_fast, double beta_slow, const double * factors,
+                     double * freqs) {
+    if (n_rot < 2 || n_rot % 2 || n_rot > ROPE_MAX_DIM || !freqs) return GEMVQ_EINVAL;
+    if (!(base > 1) || !std::isfinite(base) || !(factor > 0) || !std::isfinite(factor) || yarn_ctx < 0) return GEMVQ_EINVAL;
+    if (yarn_ctx && !(beta_slow > 0 && beta_fast >= beta_slow && std::isfinite(beta_fast))) return GEMVQ_EINVAL;
+    for (int i = 0; factors && i < n_rot / 2; ++i)
+        if (!(factors[i] > 0) || !std::isfinite(factors[i])) return GEMVQ_EINVAL;
+    rope_table(n_rot, base, factor, yarn_ctx, beta_fast, beta_slow, factors, freqs);
+    return 0;
+}
+
+int gemvq_rope_static(const gemvq_rope_rows * arrays, int n_arrays, int n_seq, int n_tok, int head_dim, int n_rot, int layout,
+                      const double * freqs, const int32_t * pos, const int32_t * num, void * stream) {
+    if (!arrays || n_arrays < 1 || n_arrays > ROPE_ARRAYS || n_seq < 1 || n_tok < 1 || int64_t(n_seq) * n_tok > (int64_t(1) << 30))
+        return GEMVQ_EINVAL;
+    if (head_dim < 4 || head_dim % 4 || head_dim > ROPE_MAX_DIM || n_rot < 2 || n_rot % 2 || n_rot > head_dim) return GEMVQ_EINVAL;
+    if ((layout != GEMVQ_ROPE_HALF && layout != GEMVQ_ROPE_PAIRS) || !freqs || !aligned(freqs, 8) || !pos || !aligned(pos, 4) || !aligned(num, 4))
+        return GEMVQ_EINVAL;
+    RotaryArgs a{};
+    int64_t heads = 0;
+    for (int i = 0; i < n_arrays; ++i) {
+        const gemvq_rope_rows & r = arrays[i];
+        if (r.n_head < 1 || r.n_head > GRID_MAX || (heads += r.n_head) > GRID_MAX) return GEMVQ_EINVAL;
+        if (!rows_ok(r.x, r.x_row, head_dim) || !rows_ok(r.y, r.y_row, head_dim) || !rows_ok(r.x, r.x_head, head_dim) || !rows_ok(r.y, r.y_head, head_dim))
+            return GEMVQ_EINVAL;
+        if (r.x == r.y && (r.x_row != r.y_row || r.x_head != r.y_head)) return GEMVQ_EINVAL;
+        a.a[i] = {r.x, r.y, r.x_row, r.x_head, r.y_row, r.y_head, r.n_head, 0};
+    }
+    a.freqs = freqs;
+    a.pos = pos;
+    a.num = num;
+    a.n = n_arrays;
+    a.n_seq = n_seq;
+    a.n_tok = n_tok;
+    a.head_dim = head_dim;
+    a.n_rot = n_rot;
+    a.pairs = layout == GEMVQ_ROPE_PAIRS;
+    const hipError_t e = launch_rotary(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : -int(e);
+}
+
+uint64_t gemvq_draft_work(int n_seq, int n_draft, int n_vocab) {
+    if (n_seq < 1 || n_draft < 0 || n_draft > DRAFT_MAX || int64_t(n_seq) * (2 * n_draft + 1) > GRID_MAX || n_vocab < 1 || n_vocab > DRAFT_MAX_VOCAB)
+        return 0;
+    return draft_work(n_seq, n_draft, n_vocab);
+}
+
+int gemvq_draft_verify_static(const float * target, int64_t target_stride, const float * draft, int64_t draft_stride, int n_vocab,
+                              int n_seq, int n_draft, const int32_t * token, const int32_t * num, const float * uniform,
+                              double temperature, double draft_temperature, int32_t * n_accept, int32_t * out, float * logp, void * work,
+                              uint64_t work_bytes, void * stream) {
+    const uint64_t need = gemvq_draft_work(n_seq, n_draft, n_vocab);
+    const int64_t most = int64_t(1) << 40;
+    if (!need || !target || target_stride < n_vocab || target_stride > most || !n_accept || !out || !work || work_bytes < need) return GEMVQ_EINVAL;
+    if (draft && (draft_stride < n_vocab || draft_stride > most)) return GEMVQ_EINVAL;
+    if ((n_draft && !token) || !(temperature >= 0.0) || !std::isfinite(temperature) || (temperature > 0.0 && !uniform)) return GEMVQ_EINVAL;
+    if (temperature > 0.0 && draft && (!(draft_temperature > 0.0) || !std::isfinite(draft_temperature))) return GEMVQ_EINVAL;
+    if (!aligned(target, 4) || !aligned(draft, 4) || !aligned(token, 4) || !aligned(num, 4) || !aligned(uniform, 4) || !aligned(n_accept, 4) ||
+        !aligned(out, 4) || !aligned(logp, 4) || !aligned(work, 16))
+        return GEMVQ_EINVAL;
+    DraftArgs a{};
+    a.target = target;
+    a.draft = n_draft ? draft : nullptr;
+    a.target_stride = target_stride;
+    a.draft_stride = draft_stride;
+    a.token = token;
+    a.num = num;
+    a.uniform = uniform;
+    a.n_accept = n_accept;
+    a.out = out;
+    a.logp = logp;
+    a.temperature = temperature;
+    a.draft_temperature = draft_temperature;
+    a.n_vocab = n_vocab;
+    a.n_seq = n_seq;
+    a.n_draft = n_draft;
+    a.work = work;
+    const hipError_t e = launch_draft(a, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : -int(e);
 }
 
 }  // extern "C"

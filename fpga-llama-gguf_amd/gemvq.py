@@ -25,6 +25,7 @@ OP_ATTN, OP_GET_ROWS, OP_ARGMAX, OP_NEXT_TOKEN, OP_FILL, OP_GEMM = 12, 13, 14, 1
 OP_BEAM, OP_BEAM_MOVE, OP_BEAM_NEXT = 18, 19, 20
 BEAM_ACT, BEAM_STATE, BEAM_KV = 0, 1, 2
 KV_F16, KV_Q4_0 = 1, 2
+ROPE_HALF, ROPE_PAIRS = 0, 1
 GEMM_MAX_TOK = 32
 GEMV_SWIGLU, GEMV_CONV, GEMV_ADD, GEMV_ARGMAX, GEMV_SILU = 0x100, 0x200, 0x400, 0x800, 0x1000
 GDN_WITH_GEMV, GDN_L2_QK, GDN_GATED, GDN_GATES, GDN_WITH_OUT, GDN_Z_SILU, GDN_SEQS = 1, 2, 4, 8, 16, 32, 64
@@ -168,6 +169,12 @@ class BeamArray(C.Structure):  # gemvq_beam_array
                 ("used", C.c_void_p), ("used_stride", C.c_int32)]
 
 
+class RopeRows(C.Structure):  # gemvq_rope_rows
+    """Rows of heads that rope_static turns: addresses, strides in floats, heads a row."""
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("x_row", C.c_int64), ("x_head", C.c_int64), ("y_row", C.c_int64),
+                ("y_head", C.c_int64), ("n_head", C.c_int32)]
+
+
 class LaunchStat(C.Structure):  # gemvq_launch_stat
     _fields_ = [("name", C.c_char * 40), ("first_cmd", C.c_int32), ("n_cmds", C.c_int32), ("bytes", C.c_uint64),
                 ("us", C.c_double)]
@@ -230,6 +237,11 @@ def hip_lib() -> C.CDLL:
         _c_fn(lib, "gemvq_beam_work", u64, i, i, i)
         _c_fn(lib, "gemvq_beam_select_static", i, vp, i64, i, i, i, vp, vp, i, vp, vp, vp, vp, u64, vp)
         _c_fn(lib, "gemvq_beam_reorder_static", i, C.POINTER(BeamArray), i, vp, i, i, vp)
+        f64 = C.c_double
+        _c_fn(lib, "gemvq_rope_freqs", i, i, f64, f64, i, f64, f64, vp, vp)
+        _c_fn(lib, "gemvq_rope_static", i, C.POINTER(RopeRows), i, i, i, i, i, i, vp, vp, vp, vp)
+        _c_fn(lib, "gemvq_draft_work", u64, i, i, i)
+        _c_fn(lib, "gemvq_draft_verify_static", i, vp, i64, vp, i64, i, i, i, vp, vp, vp, f64, f64, vp, vp, vp, vp, u64, vp)
         _hip = lib
     return _hip
 
@@ -363,6 +375,41 @@ def beam_reorder_static(arrays, parent: int, n_group: int, n_beam: int, stream: 
     if not isinstance(arrays, C.Array):
         arrays = (BeamArray * len(arrays))(*arrays)
     _ok(hip_lib().gemvq_beam_reorder_static(arrays, len(arrays), parent, n_group, n_beam, stream), "beam reordering")
+
+
+def rope_freqs(n_rot: int, base: float, factor: float = 1.0, yarn_ctx: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0,
+               factors=None) -> np.ndarray:
+    """The table of rope_static (turns per position of each pair, then the magnitude), to be copied to the device."""
+    if factors is not None:
+        factors = np.ascontiguousarray(factors, dtype=np.float64)
+        if factors.size != n_rot // 2:
+            raise GemvqError("rope table: a factor for each pair")
+    out = np.empty(max(n_rot // 2, 0) + 1, dtype=np.float64)
+    _ok(hip_lib().gemvq_rope_freqs(n_rot, base, factor, yarn_ctx, beta_fast, beta_slow, None if factors is None else _ptr(factors),
+                                   _ptr(out)), "rope table")
+    return out
+
+
+def rope_static(arrays, n_seq: int, n_tok: int, head_dim: int, n_rot: int, layout: int, freqs: int, pos: int, num: int = 0,
+                stream: int = 0) -> None:
+    """Rotary positions pos[s] + t of the arrays' (RopeRows) heads."""
+    if not isinstance(arrays, C.Array):
+        arrays = (RopeRows * len(arrays))(*arrays)
+    _ok(hip_lib().gemvq_rope_static(arrays, len(arrays), n_seq, n_tok, head_dim, n_rot, layout, freqs, pos, num, stream), "rope")
+
+
+def draft_work(n_seq: int, n_draft: int, n_vocab: int) -> int:
+    """Bytes of workspace of draft_verify_static (0: sizes that are not served)."""
+    return hip_lib().gemvq_draft_work(n_seq, n_draft, n_vocab)
+
+
+def draft_verify_static(target: int, target_stride: int, draft: int, draft_stride: int, n_vocab: int, n_seq: int, n_draft: int,
+                        token: int, num: int, uniform: int, temperature: float, draft_temperature: float, n_accept: int, out: int,
+                        logp: int, work: int, work_bytes: int, stream: int = 0) -> None:
+    """How many of the drafted tokens stand, and the token behind them."""
+    _ok(hip_lib().gemvq_draft_verify_static(target, target_stride, draft, draft_stride, n_vocab, n_seq, n_draft, token, num, uniform,
+                                            temperature, draft_temperature, n_accept, out, logp, work, work_bytes, stream),
+        "draft verification")
 
 
 class Context:

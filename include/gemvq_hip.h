@@ -402,6 +402,61 @@ typedef struct {
 int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, const int32_t * parent, int n_group, int n_beam,
                               void * stream);
 
+/* No counterpart in the reference (its ROPE command takes a table of cosines and sines): rotary positions of rows of heads on
+ * caller-owned device memory, under the rules of the calls above. A head's first n_rot of head_dim elements turn in pairs (i,
+ * i + n_rot / 2) (GEMVQ_ROPE_HALF) or (2 i, 2 i + 1) (GEMVQ_ROPE_PAIRS), x0' = m (x0 cos - x1 sin), x1' = m (x0 sin + x1 cos), by
+ * (pos[s] + t) * freqs[i] full turns; the others are copied. Angles are in 64 bits, products in FP32.
+ * The table: n_rot / 2 turns per position, then m. gemvq_rope_freqs() fills it on the host; the call takes a copy in device memory,
+ * 8-byte aligned. Pair i's angle a position is base^(-2 i / n_rot), over factors[i] (NULL: 1), and with yarn_ctx 0 over `factor`
+ * (1: none). With yarn_ctx (YaRN: the context the model was trained on), pairs that turn more than beta_fast times over it keep
+ * their angle, those that turn less than beta_slow times have it over `factor`, the ones between a share of both that goes up
+ * linearly with i, between floor and ceiling of the pairs that turn beta_fast and beta_slow times, n_rot ln(yarn_ctx / (2 pi
+ * beta)) / (2 ln base), within 0 and n_rot - 1; m is 0.1 ln(factor) + 1, else 1.
+ * Up to GEMVQ_ROPE_MAX_ARRAYS arrays (q and k) in one launch: row s * n_tok + t of x at x_row floats a row, its head h at x_head
+ * floats a head, y likewise; y may be x with the same strides, else memory of its own. Rows of tokens t >= num[s], or at
+ * positions below 0, are left as they were in y. head_dim: a multiple of 4, at most GEMVQ_ROPE_MAX_DIM; n_rot even; rows start at
+ * multiples of 16 bytes. */
+#define GEMVQ_ROPE_HALF 0
+#define GEMVQ_ROPE_PAIRS 1
+#define GEMVQ_ROPE_MAX_ARRAYS 4
+#define GEMVQ_ROPE_MAX_DIM 1024
+typedef struct {
+    const float * x;
+    float * y;
+    int64_t x_row, x_head, y_row, y_head;
+    int32_t n_head;
+} gemvq_rope_rows;
+int gemvq_rope_freqs(int n_rot, double base, double factor, int yarn_ctx, double beta_fast, double beta_slow, const double * factors,
+                     double * freqs);
+int gemvq_rope_static(const gemvq_rope_rows * arrays, int n_arrays, int n_seq, int n_tok, int head_dim, int n_rot, int layout,
+                      const double * freqs, const int32_t * pos, const int32_t * num, void * stream);
+
+/* No counterpart in the reference: speculative sampling's verification of drafted tokens, on caller-owned device memory, under the
+ * rules of the calls above. Sequence s has num[s] <= n_draft drafted tokens d_t = token[s * n_draft + t] (num NULL: n_draft each;
+ * larger: n_draft; below 0: the sequence is not in use, and its outputs are left as they were), target logits in rows s *
+ * (n_draft + 1) + t for t = 0 .. num[s] (row t is what the target says of d_t, the last row of the token behind them), and the
+ * draft's logits in rows s * n_draft + t (draft NULL: its tokens are certain, q_t is 1 at d_t and 0 elsewhere). p_t and q_t are the
+ * distributions e^(logit / temperature) / sum, in 64 bits. d_t is accepted if u_t q_t(d_t) < p_t(d_t), u_t = uniform[s * (n_draft +
+ * 1) + t] in [0, 1), and all before it are. A new token follows: at the first d_t that is not accepted from max(p_t - q_t, 0)
+ * over its sum (p_t where nothing is left), behind the last from the last row's p: the first token whose weights up to and with its own sum to
+ * more than uniform[s * (n_draft + 1) + n_draft] times the sum of all (none does: the last with a weight). n_accept[s]: how many
+ * stand; out[s * (n_draft + 1) + ..]: they, the new token, then -1; logp (or NULL): log p_t of each, then 0. So the tokens are
+ * distributed as the target's own.
+ * temperature 0: d_t is accepted if it has the row's largest logit (of equal ones the lowest index), which is also the new token;
+ * draft and uniform are not read (uniform may be NULL); logp is of temperature 1.
+ * n_draft 0: one token of each sequence is sampled. d_t outside the vocabulary are not accepted. NaN logits count as -inf, +inf as
+ * the largest finite number; a row of nothing but -inf accepts no token and has none: -1, logp 0 (as a draft row: q is 0).
+ * FP32 rows `stride` >= n_vocab floats apart, 4-byte aligned; 0 <= n_draft <= GEMVQ_DRAFT_MAX, n_seq * (2 n_draft + 1) <= 65535,
+ * 1 <= n_vocab <= GEMVQ_DRAFT_MAX_VOCAB. work: gemvq_draft_work() bytes, 16-byte aligned, contents do not matter; calls that may
+ * overlap need one each. Outputs do not overlap inputs. */
+#define GEMVQ_DRAFT_MAX 32
+#define GEMVQ_DRAFT_MAX_VOCAB (1 << 20)
+uint64_t gemvq_draft_work(int n_seq, int n_draft, int n_vocab);
+int gemvq_draft_verify_static(const float * target, int64_t target_stride, const float * draft, int64_t draft_stride, int n_vocab,
+                              int n_seq, int n_draft, const int32_t * token, const int32_t * num, const float * uniform,
+                              double temperature, double draft_temperature, int32_t * n_accept, int32_t * out, float * logp, void * work,
+                              uint64_t work_bytes, void * stream);
+
 #ifdef __cplusplus
 }
 #endif

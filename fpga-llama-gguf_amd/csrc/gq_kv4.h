@@ -92,6 +92,23 @@ constexpr int KV4_ALONE = 2048;
 bool kv4_joins(const Kv4AttnArgs & a);  // the launch is followed by that of kv4_join_kernel
 size_t kv4_work_floats(const Kv4Cache & c, int n_seq, int n_tok, int n_head);
 
+// Attention with sinks, and with a prefix that groups of sequences share: the token at place p of its sequence's own cache is
+// position P + p, P = pre_len of its group (0 without a prefix; n_seq / members groups of consecutive sequences), and sees the
+// positions up to its own, with window > 0 only the last `window` of them and the first `sinks`. Positions below P are in the group's
+// region of the prefix. The regions that a call reads (segments: the groups', then the sequences' own) are split into ranges of
+// records, and every range is taken for all rows that see it, 16 * NQ at a time.
+struct Kv4PartsArgs {
+    Kv4AttnArgs a;  // c: the sequences' own caches; ranges is not used, group as there
+    Kv4Cache pre;   // data NULL: none
+    const int32_t * pre_len;
+    int members, sinks;
+    int target;     // set at launch: workgroups that the ranges are dealt to
+    int whole;      // set at launch: every segment is one range
+};
+// n_group: groups with a prefix, 0 without one.
+size_t kv4_parts_floats(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head);
+long long kv4_parts_grid(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head);
+
 // The ATTN command's part before the attention: every q head and new key normalized and rotated (gq_kernels.h, AttnArgs; q stays FP32
 // in qr), the keys and values stored. Tokens as t says.
 struct Kv4AppendArgs {
@@ -112,5 +129,6 @@ hipError_t launch_kv4_append(const Kv4AppendArgs & a, hipStream_t s);
 hipError_t launch_kv4_store(const Kv4RowsArgs & a, hipStream_t s);
 hipError_t launch_kv4_load(const Kv4RowsArgs & a, hipStream_t s);
 hipError_t launch_kv4_attn(const Kv4AttnArgs & a, hipStream_t s);
+hipError_t launch_kv4_parts(const Kv4PartsArgs & a, hipStream_t s);
 
 }  // namespace gq

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cfloat>
+#include <climits>
 #include <type_traits>
 
 namespace gq {
@@ -532,8 +533,43 @@ __device__ __forceinline__ void kv4_out(const Kv4AttnArgs & a, size_t row, int h
     *reinterpret_cast<f32x4 *>(a.y + row * size_t(a.y_row) + size_t(hq) * HD + e) = y;
 }
 
-template <int HD, int NQ>
-__global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4AttnArgs a) {
+// Which rows and records a workgroup has: those of one sequence's range of records (kv4_attn_kernel).
+struct Kv4Rows {
+    int s, h, G, row0, p0, t_lo, t_hi, n_tok, n_head, window, range;  // tokens t_lo .. t_hi are in the rows and have positions
+    int lo, hi;       // the positions that they see
+    int first, last;  // the range's records of those
+    bool alone;       // the sequence's one range
+    const uint8_t * head;
+    float * work;
+    __device__ __forceinline__ int record(int at) const { return at; }
+    // Row i of the workgroup: whether it has a position, its token's row and its q head (of some row with a position otherwise).
+    __device__ __forceinline__ bool row(int i, size_t & token, int & hq) const {
+        const int r = row0 + i, t = int(unsigned(r) / unsigned(G));
+        const bool ok = t >= t_lo && t <= t_hi;
+        token = size_t(s) * n_tok + (ok ? t : t_lo);
+        hq = h * G + (ok ? r - t * G : 0);
+        return ok;
+    }
+    // The positions from..to that row i sees, to -1: none.
+    __device__ __forceinline__ void limits(int i, int & from, int & to) const {
+        const int t = int(unsigned(row0 + i) / unsigned(G));
+        const bool ok = t >= t_lo && t <= t_hi;
+        to = ok ? p0 + t : -1;
+        from = ok && window ? p0 + t - window + 1 : 0;
+    }
+    __device__ __forceinline__ bool sees(int p, int from, int to) const { return p >= from && p <= to; }
+    __device__ __forceinline__ bool hidden(int p, int from, int to) const { return p < from || p > to; }
+    __device__ __forceinline__ bool unseen(int p) const { return p < lo || p > hi; }  // by any row
+    // Some row does not see all of the record at position `from`.
+    __device__ __forceinline__ bool edge(int from) const { return from < (window ? p0 + t_hi - window + 1 : 0) || from + KV4_TILE - 1 > p0 + t_lo; }
+    // This range's set of a row: [range][token][head][HD + 4], C and L behind the sums.
+    __device__ __forceinline__ float * set(int, size_t token, int hq, int hd) const {
+        return work + ((size_t(range) * n_tok + (token - size_t(s) * n_tok)) * n_head + hq) * (hd + 4);
+    }
+};
+
+template <int HD, int NQ, typename Rows>
+__device__ __forceinline__ void kv4_attend(const Kv4AttnArgs & a, const Rows & rows) {
     constexpr int NB = HD / 32, ROWS = 16 * NQ;
     // Blocks of 32 elements that the waves' sums are joined in at a time; threads of a row there.
     constexpr int JB = NQ == 1 ? NB : 1, PAD = 32 * JB + 4, JT = 256 / ROWS;
@@ -548,33 +584,14 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     __shared__ float kqs[ROWS], cs[4][ROWS], ls[4][ROWS];
     __shared__ __align__(16) uint32_t scales[4][HD];  // a wave's record's key scales, then its value scales: [g][block][8] each
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane >> 4, col = lane & 15;
-    // Workgroup (KV head, group of rows behind it | range): the groups of one KV head, which read the same records, stay on an XCD or
-    // a few. Rows of the KV head: token row / G, q head row % G
-    const int G = a.group, h = int(unsigned(blockIdx.x) % unsigned(a.c.n_head_kv)), row0 = int(unsigned(blockIdx.x) / unsigned(a.c.n_head_kv)) * ROWS;
-    const int range = blockIdx.y;
-    int s = 0;
-    Kv4Range r;
-    if (!kv4_find<true>(a, range, s, r)) return;
-    s = __builtin_amdgcn_readfirstlane(s);
-    const int p0 = __builtin_amdgcn_readfirstlane(int(r.p0));
-    // tokens -p0 (where p0 < 0) .. live - 1 have positions
-    const int live = int(min((long long)__builtin_amdgcn_readfirstlane(r.n), (long long)a.c.n_ctx - p0));
-    const int t_lo = max(int(unsigned(row0) / unsigned(G)), -p0), t_hi = min(int(unsigned(row0 + ROWS - 1) / unsigned(G)), live - 1);
-    if (t_lo > t_hi) return;
-    // the group's positions: lo .. hi, the rows' own ranges within them
-    const int lo = a.window ? max(0, p0 + t_lo - a.window + 1) : 0, hi = p0 + t_hi;
-    const int j = range - r.slot;
-    const bool alone = __builtin_amdgcn_readfirstlane(int(r.tiles <= r.per));  // the sequence's one range
-    const int first = __builtin_amdgcn_readfirstlane(max(r.first + j * r.per, lo / KV4_TILE));
-    const int last = __builtin_amdgcn_readfirstlane(min(r.first + min((j + 1) * r.per, r.tiles) - 1, hi / KV4_TILE));
-    if (first > last) return;  // none of the range's positions are seen
-    const uint8_t * head = kv4_rec(a.c, s, h, 0);
+    const int first = rows.first, last = rows.last;
+    const uint8_t * head = rows.head;
     const Kv4Const k4;
 
     Kv4Tile<HD> tile;
     int at = first + wave;
     {
-        const uint8_t * rec = head + size_t(min(at, last)) * kv4_record(HD);
+        const uint8_t * rec = head + size_t(rows.record(min(at, last))) * kv4_record(HD);
         tile.load_scales(rec, lane);
         tile.load_keys(rec, lane);
         tile.load_values(rec, lane);
@@ -583,9 +600,11 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
         constexpr int NP = HD >= 64 ? HD / 64 : 1;
-        const int row = row0 + n * 16 + (tid >> 4), t = int(unsigned(row) / unsigned(G)), pc = tid & 15;
-        const bool ok = t >= t_lo && t <= t_hi;
-        const float * src = a.q + (size_t(s) * a.t.n_tok + (ok ? t : t_lo)) * size_t(a.q_row) + size_t(h * G + (ok ? row - t * G : 0)) * size_t(a.q_head);
+        const int pc = tid & 15;
+        size_t token;
+        int hq;
+        rows.row(n * 16 + (tid >> 4), token, hq);
+        const float * src = a.q + token * size_t(a.q_row) + size_t(hq) * size_t(a.q_head);
         f32x4 x[NP];
         float top = 0.0f;
 #pragma unroll
@@ -627,10 +646,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     float c[NQ], l[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-        const int t = int(unsigned(row0 + n * 16 + col) / unsigned(G));
-        const bool ok = t >= t_lo && t <= t_hi;
-        my_hi[n] = ok ? p0 + t : -1;
-        my_lo[n] = ok && a.window ? p0 + t - a.window + 1 : 0;
+        rows.limits(n * 16 + col, my_lo[n], my_hi[n]);
         kq[n] = kqs[n * 16 + col];
         c[n] = KV4_LOW;
         l[n] = 0.0f;
@@ -644,14 +660,14 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
     bool sums = false;  // o holds something
     int e = 15;  // the value scales' exponent: the largest so far times 2^e is below 2^7 (scales below 2^-8 keep 2^15)
     for (; at <= last; at += 4) {
-        const uint8_t * ahead = head + size_t(min(at + 4, last)) * kv4_record(HD);  // (the last one again where there is none)
-        const int from = at * KV4_TILE;
-        const bool edge = from < (a.window ? p0 + t_hi - a.window + 1 : 0) || from + KV4_TILE - 1 > p0 + t_lo;  // some row does not see all of it
+        const uint8_t * ahead = head + size_t(rows.record(min(at + 4, last))) * kv4_record(HD);  // (the last one again where there is none)
+        const int from = rows.record(at) * KV4_TILE;
+        const bool edge = rows.edge(from);
         if (edge) {  // positions that no row sees may never have been stored: their scales become 0
 #pragma unroll
             for (int i = 0; i < Kv4Tile<HD>::NS; ++i) {
                 const int p = from + Kv4Tile<HD>::at(lane, i);
-                if (p < lo || p > hi) tile.d[i / 2] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
+                if (rows.unseen(p)) tile.d[i / 2] &= i & 1 ? 0x0000ffffu : 0xffff0000u;
             }
         }
         uint32_t dtop = 0;  // the largest value scale's magnitude, as fp16 bits
@@ -673,7 +689,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 #pragma unroll
                         for (int i = 0; i < 8; ++i) {  // word i / 2: positions 0 and 2, 1 and 3 of the lane's four, and 16 further
                             const int p = from + (i >> 2) * 16 + 4 * g + ((i >> 1) & 1) + 2 * (i & 1);
-                            hit |= p >= my_lo[n] && p <= my_hi[n] && (vd[i >> 1] >> 16 * (i & 1) & 0x7c00u) == 0x7c00u;
+                            hit |= rows.sees(p, my_lo[n], my_hi[n]) && (vd[i >> 1] >> 16 * (i & 1) & 0x7c00u) == 0x7c00u;
                         }
                         unsigned long long hits = __ballot(hit);
                         hits |= hits >> 32;
@@ -746,7 +762,7 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int p = from + (i >> 2) * 16 + 4 * g + (i & 3);
-                    if (p < my_lo[n] || p > my_hi[n]) sc[n][i] = -__builtin_inff();
+                    if (rows.hidden(p, my_lo[n], my_hi[n])) sc[n][i] = -__builtin_inff();
                 }
             top[n] = fmaxf(fmaxf(fmaxf(sc[n][0], sc[n][1]), fmaxf(sc[n][2], sc[n][3])), fmaxf(fmaxf(sc[n][4], sc[n][5]), fmaxf(sc[n][6], sc[n][7]))) * kq[n];
             again |= bool(__any(top[n] - c[n] > 9.0f));  // (not c + 9, which may round to the maximum)
@@ -821,9 +837,10 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
             ls[wave][n * 16 + col] = l[n];
         }
     }
-    const int rj = tid / JT, row = row0 + rj, tj = int(unsigned(row) / unsigned(G)), hq = h * G + row - tj * G;
-    const bool mine = tj >= t_lo && tj <= t_hi;
-    const size_t orow = size_t(s) * a.t.n_tok + tj;
+    const int rj = tid / JT;
+    size_t token;
+    int hq;
+    const bool mine = rows.row(rj, token, hq);
     float f[4] = {0.0f, 0.0f, 0.0f, 0.0f}, C = KV4_LOW, L = 0.0f;
 #pragma unroll
     for (int b0 = 0; b0 < NB; b0 += JB) {
@@ -852,10 +869,10 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 #pragma unroll
             for (int w = 0; w < 4; ++w) y += *reinterpret_cast<const f32x4 *>(&part[w][rj][ej]) * f[w];
             const int el = b0 * 32 + ej;
-            if (alone) {
-                kv4_out<HD>(a, orow, hq, el, y, L);
-            } else {  // this range's set: [range][token][head][HD + 4], C and L behind the sums
-                float * w = a.work + ((size_t(range) * a.t.n_tok + tj) * a.n_head + hq) * (HD + 4);
+            if (rows.alone) {
+                kv4_out<HD>(a, token, hq, el, y, L);
+            } else {
+                float * w = rows.set(rj, token, hq, HD);
                 *reinterpret_cast<f32x4 *>(w + el) = y;
                 if (el == 0) {
                     w[HD] = C;
@@ -864,6 +881,348 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
             }
         }
     }
+}
+
+template <int HD, int NQ>
+__global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4AttnArgs a) {
+    constexpr int ROWS = 16 * NQ;
+    // Workgroup (KV head, group of rows behind it | range): the groups of one KV head, which read the same records, stay on an XCD or
+    // a few. Rows of the KV head: token row / G, q head row % G
+    const int G = a.group, h = int(unsigned(blockIdx.x) % unsigned(a.c.n_head_kv)), row0 = int(unsigned(blockIdx.x) / unsigned(a.c.n_head_kv)) * ROWS;
+    const int range = blockIdx.y;
+    int s = 0;
+    Kv4Range r;
+    if (!kv4_find<true>(a, range, s, r)) return;
+    s = __builtin_amdgcn_readfirstlane(s);
+    const int p0 = __builtin_amdgcn_readfirstlane(int(r.p0));
+    // tokens -p0 (where p0 < 0) .. live - 1 have positions
+    const int live = int(min((long long)__builtin_amdgcn_readfirstlane(r.n), (long long)a.c.n_ctx - p0));
+    const int t_lo = max(int(unsigned(row0) / unsigned(G)), -p0), t_hi = min(int(unsigned(row0 + ROWS - 1) / unsigned(G)), live - 1);
+    if (t_lo > t_hi) return;
+    // the group's positions: lo .. hi, the rows' own ranges within them
+    const int lo = a.window ? max(0, p0 + t_lo - a.window + 1) : 0, hi = p0 + t_hi;
+    const int j = range - r.slot;
+    const bool alone = __builtin_amdgcn_readfirstlane(int(r.tiles <= r.per));  // the sequence's one range
+    const int first = __builtin_amdgcn_readfirstlane(max(r.first + j * r.per, lo / KV4_TILE));
+    const int last = __builtin_amdgcn_readfirstlane(min(r.first + min((j + 1) * r.per, r.tiles) - 1, hi / KV4_TILE));
+    if (first > last) return;  // none of the range's positions are seen
+    kv4_attend<HD, NQ>(a, Kv4Rows{s, h, G, row0, p0, t_lo, t_hi, a.t.n_tok, a.n_head, a.window, range, lo, hi, first, last, alone, kv4_rec(a.c, s, h, 0), a.work});
+}
+
+// ---- attention with a prefix and sinks ----
+// Segments: the groups' prefixes (number g), then the sequences' own caches (n_group + s). A segment has `units` workgroups (KV heads
+// times groups of rows) for each range of its records.
+struct Kv4Seg {
+    // Records that some row sees: n_sink from 0 on, and those from `rest` on, `tiles` in all.
+    int n_sink, rest, tiles;
+};
+
+__device__ __forceinline__ int kv4_groups(const Kv4PartsArgs & x) { return x.pre.data ? int(unsigned(x.a.t.n_seq) / unsigned(x.members)) : 0; }
+__device__ __forceinline__ int kv4_prefix(const Kv4PartsArgs & x, int group) { return x.pre.data ? max(0, min(x.pre_len[group], x.pre.n_ctx)) : 0; }
+__device__ __forceinline__ int kv4_units(const Kv4PartsArgs & x, bool pre, int rows) {
+    return int((unsigned(x.a.t.n_tok) * unsigned(x.a.group) * unsigned(pre ? x.members : 1) + rows - 1) / unsigned(rows)) * x.a.c.n_head_kv;
+}
+
+// The records of a segment of which the positions from .. to - 1 and the first `sinks` are seen.
+__device__ __forceinline__ Kv4Seg kv4_records(long long from, long long to, long long sinks) {
+    if (to <= 0) return {0, 0, 0};
+    const int end = int((to - 1) / KV4_TILE) + 1, rest = from >= to ? end : int(max(from, 0ll) / KV4_TILE);
+    const int n_sink = int(min((min(max(sinks, 0ll), to) + KV4_TILE - 1) / KV4_TILE, (long long)rest));
+    return {n_sink, rest, n_sink + end - rest};
+}
+// The positions of a sequence's live tokens in its own cache: low .. high - 1, none: high 0.
+__device__ __forceinline__ void kv4_live(const Kv4PartsArgs & x, int s, long long & low, long long & high) {
+    long long p0;
+    int n;
+    kv4_span(x.a.t, s, p0, n);
+    low = p0 < 0 ? 0 : p0;
+    high = p0 + n < x.a.c.n_ctx ? p0 + n : x.a.c.n_ctx;
+    if (low >= high) high = 0;
+}
+__device__ __forceinline__ Kv4Seg kv4_own_seg(const Kv4PartsArgs & x, int s) {
+    long long low, high;
+    kv4_live(x, s, low, high);
+    const int window = x.a.window;
+    const long long sinks = window ? x.sinks - (x.pre.data ? kv4_prefix(x, int(unsigned(s) / unsigned(x.members))) : 0) : 0;
+    return kv4_records(window ? low - window + 1 : 0, high, sinks);
+}
+__device__ __forceinline__ Kv4Seg kv4_prefix_seg(const Kv4PartsArgs & x, int group) {
+    const int n = kv4_prefix(x, group);
+    if (!x.a.window || !n) return kv4_records(0, n, 0);
+    long long least = -1;  // the group's first live position
+    for (int i = 0; i < x.members; ++i) {
+        long long low, high;
+        kv4_live(x, group * x.members + i, low, high);
+        if (high && (least < 0 || low < least)) least = low;
+    }
+    return least < 0 ? Kv4Seg{0, 0, 0} : kv4_records(n + least - x.a.window + 1, n, x.sinks);
+}
+
+// The workspace: every segment's first workgroup and number of ranges, then the workgroups' sets, [workgroup][row][HD + 4] each.
+__host__ __device__ inline size_t kv4_table_floats(long long segs) { return size_t(segs + 1) / 2 * 4; }
+__device__ __forceinline__ float * kv4_sets(const Kv4PartsArgs & x) { return x.a.work + kv4_table_floats(kv4_groups(x) + (long long)x.a.t.n_seq); }
+
+// What a workgroup has to do, the same in every lane: a unit of a range of a segment.
+struct Kv4Piece {
+    int seg, unit, from, to;  // records from .. to - 1 of the segment's
+    Kv4Seg r;
+};
+
+// Workgroup `id`'s piece; false: it has none. Every wave's lanes look at the segments together, 64 at a time (the groups, then the
+// sequences): first at all records times units, for the ranges' length, then for the segment that the workgroup falls into.
+__device__ __forceinline__ bool kv4_place(const Kv4PartsArgs & x, int id, int rows, Kv4Piece & piece) {
+    const int lane = threadIdx.x & 63, n_group = kv4_groups(x), n_seq = x.a.t.n_seq;
+    const int pre_units = n_group ? kv4_units(x, true, rows) : 0, own_units = kv4_units(x, false, rows);
+    const int pre_batches = (n_group + 63) / 64, batches = pre_batches + (n_seq + 63) / 64;
+    const bool few = n_seq <= 64;  // at most one batch of each, looked at once
+    const auto look = [&](int b) {
+        const int i = (b < pre_batches ? b : b - pre_batches) * 64 + lane;
+        if (b < pre_batches) return i < n_group ? kv4_prefix_seg(x, i) : Kv4Seg{0, 0, 0};
+        return i < n_seq ? kv4_own_seg(x, i) : Kv4Seg{0, 0, 0};
+    };
+    Kv4Seg pre = {0, 0, 0}, own = {0, 0, 0};
+    if (few) {
+        if (n_group) pre = look(0);
+        own = look(pre_batches);
+    }
+    const auto seg = [&](int b) { return few ? b < pre_batches ? pre : own : look(b); };
+    int per = INT_MAX;
+    if (!x.whole) {
+        long long sum = 0;
+        for (int b = 0; b < batches; ++b) sum += (long long)seg(b).tiles * (b < pre_batches ? pre_units : own_units);
+#pragma unroll
+        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, WAVE);
+        per = int(min((sum + x.target - 1) / x.target, (long long)INT_MAX / 4));
+        per = max(per, KV4_LEAST);
+    }
+    const auto ranges = [&](int tiles) { return tiles ? per == INT_MAX ? 1 : int(unsigned(tiles + per - 1) / unsigned(per)) : 0; };
+    if (id == 0 && x.a.work) {
+        int before = 0;
+        for (int b = 0; b < batches; ++b) {
+            const int units = b < pre_batches ? pre_units : own_units, n = ranges(seg(b).tiles);
+            int upto = n * units;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const int y = __shfl_up(upto, d, WAVE);
+                if (lane >= d) upto += y;
+            }
+            const int i = (b < pre_batches ? b : b - pre_batches) * 64 + lane;
+            if (threadIdx.x < 64 && i < (b < pre_batches ? n_group : n_seq))
+                reinterpret_cast<int2 *>(x.a.work)[(b < pre_batches ? 0 : n_group) + i] = int2{before + upto - n * units, n};
+            before += __shfl(upto, 63, WAVE);
+        }
+    }
+    int before = 0;
+    for (int b = 0; b < batches; ++b) {
+        const Kv4Seg y = seg(b);
+        const int units = b < pre_batches ? pre_units : own_units, n = ranges(y.tiles);
+        int upto = n * units;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int z = __shfl_up(upto, d, WAVE);
+            if (lane >= d) upto += z;
+        }
+        const int all = __shfl(upto, 63, WAVE);
+        if (id - before < all) {
+            const int l = __ffsll(__ballot(before + upto > id)) - 1;
+            const auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
+            const int k = id - before - get(upto - n * units), m = get(n), tiles = get(y.tiles);  // workgroup k of the segment's m * units
+            const int j = int(unsigned(k) / unsigned(units));
+            piece.seg = (b < pre_batches ? b * 64 : n_group + (b - pre_batches) * 64) + l;
+            piece.unit = k - j * units;
+            piece.r = {get(y.n_sink), get(y.rest), tiles};
+            piece.from = int((long long)tiles * j / m);  // ranges of a segment are alike
+            piece.to = int((long long)tiles * (j + 1) / m);
+            return true;
+        }
+        before += all;
+    }
+    return false;
+}
+
+// The rows and records of kv4_parts_kernel's workgroup.
+struct Kv4PartRows {
+    int h, G, row0, sink;
+    int lo, hi;                       // positions (of the segment's cache) that some row sees, besides the first `sink`
+    int lo_most, hi_least;            // every row sees those
+    int first, last, n_sink, skip;    // records: `first` on, from number n_sink on `skip` further
+    bool alone, pre, windowed;
+    int len, window;
+    const uint8_t * head;
+    float * sets;
+    const int2 * at;                  // in LDS: a row's token row (-1: none) and place in its own cache
+
+    __device__ __forceinline__ bool find(const Kv4PartsArgs & x, int ROWS, int2 * at_) {
+        const Kv4AttnArgs & a = x.a;
+        Kv4Piece p;
+        if (!kv4_place(x, int(blockIdx.x), ROWS, p)) return false;
+        const int tid = threadIdx.x, n_group = kv4_groups(x);
+        const int seg = __builtin_amdgcn_readfirstlane(p.seg), unit = __builtin_amdgcn_readfirstlane(p.unit);
+        pre = seg < n_group;
+        const int id = pre ? seg : seg - n_group, members = pre ? x.members : 1;
+        G = a.group;
+        h = int(unsigned(unit) % unsigned(a.c.n_head_kv));
+        row0 = int(unsigned(unit) / unsigned(a.c.n_head_kv)) * ROWS;
+        len = n_group ? __builtin_amdgcn_readfirstlane(kv4_prefix(x, pre ? id : int(unsigned(id) / unsigned(x.members)))) : 0;
+        window = a.window;
+        windowed = window != 0;
+        sink = !windowed ? 0 : pre ? min(x.sinks, len) : max(x.sinks - len, 0);
+        // every lane a row (ROWS are at most 64), the workgroup's positions from all of them
+        const int rows = members * a.t.n_tok * G, i = tid & (ROWS - 1);
+        const bool in = row0 + i < rows;
+        const int token = id * members * a.t.n_tok + int(unsigned(in ? row0 + i : 0) / unsigned(G));
+        const int sq = int(unsigned(token) / unsigned(a.t.n_tok)), t = token - sq * a.t.n_tok;
+        long long p0;
+        int n;
+        kv4_span(a.t, sq, p0, n);
+        const bool ok = in && t < n && p0 + t >= 0 && p0 + t < a.c.n_ctx;
+        const int place = int(p0 + t);
+        if (tid < ROWS) at_[tid] = int2{ok ? token : -1, place};
+        at = at_;
+        int from = 0, to = -1;
+        if (ok) span(place, from, to);
+        int v[4] = {ok ? from : INT_MAX, ok ? -to : INT_MAX, ok ? -from : INT_MAX, ok ? to : INT_MAX};
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1)
+            if (d < ROWS)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[k] = min(v[k], __shfl_xor(v[k], d, WAVE));
+        lo = __builtin_amdgcn_readfirstlane(v[0]);
+        hi = -__builtin_amdgcn_readfirstlane(v[1]);
+        lo_most = -__builtin_amdgcn_readfirstlane(v[2]);
+        hi_least = __builtin_amdgcn_readfirstlane(v[3]);
+        if (hi_least == INT_MAX) return false;  // no row has a position
+        // the range's records of the sinks, then those behind them, as far as the rows see any
+        const Kv4Seg r = {__builtin_amdgcn_readfirstlane(p.r.n_sink), __builtin_amdgcn_readfirstlane(p.r.rest), __builtin_amdgcn_readfirstlane(p.r.tiles)};
+        const int f = __builtin_amdgcn_readfirstlane(p.from), e = __builtin_amdgcn_readfirstlane(p.to), end = hi / KV4_TILE + 1;
+        const int s1 = min(min(e, r.n_sink), end);
+        int b0 = max(f, r.n_sink) - r.n_sink + r.rest;
+        const int b1 = min(e - r.n_sink + r.rest, end);
+        if ((long long)b0 * KV4_TILE >= sink) b0 = max(b0, lo / KV4_TILE);  // (there are sinks behind it otherwise)
+        const int sinks = max(s1 - f, 0), others = max(b1 - b0, 0);
+        first = sinks ? f : b0;
+        last = first + sinks + others - 1;
+        n_sink = sinks ? f + sinks : INT_MAX;
+        skip = sinks ? b0 - (f + sinks) : 0;
+        alone = !a.work || (!len && r.tiles == e - f);
+        head = pre ? kv4_rec(x.pre, id, h, 0) : kv4_rec(a.c, id, h, 0);
+        sets = a.work ? kv4_sets(x) + size_t(blockIdx.x) * ROWS * (a.c.head_dim + 4) : nullptr;
+        __syncthreads();  // the rows' places are there
+        if (first <= last) return true;
+        if (!alone && tid < ROWS && at[tid].x >= 0) {  // the rows see nothing of the range
+            sets[tid * (a.c.head_dim + 4) + a.c.head_dim] = KV4_LOW;
+            sets[tid * (a.c.head_dim + 4) + a.c.head_dim + 1] = 0.0f;
+        }
+        return false;
+    }
+    // The positions of the segment that a token at that place sees, besides the sinks.
+    __device__ __forceinline__ void span(int place, int & from, int & to) const {
+        to = pre ? len - 1 : place;
+        from = windowed ? int(min(max((pre ? (long long)len : 0ll) + place - window + 1, 0ll), (long long)INT_MAX - 1)) : 0;
+    }
+    __device__ __forceinline__ int record(int i) const { return i < n_sink ? i : i + skip; }
+    __device__ __forceinline__ bool row(int i, size_t & token, int & hq) const {
+        const int t = at[i].x;
+        token = size_t(max(t, 0));
+        hq = t < 0 ? 0 : h * G + int(unsigned(row0 + i) % unsigned(G));
+        return t >= 0;
+    }
+    __device__ __forceinline__ void limits(int i, int & from, int & to) const {
+        const int2 x = at[i];
+        from = 0;
+        to = -1;
+        if (x.x >= 0) span(x.y, from, to);
+    }
+    __device__ __forceinline__ bool sees(int p, int from, int to) const { return (p >= from || p < sink) && p <= to; }
+    __device__ __forceinline__ bool hidden(int p, int from, int to) const { return !sees(p, from, to); }
+    __device__ __forceinline__ bool unseen(int p) const { return (p < lo && p >= sink) || p > hi; }
+    __device__ __forceinline__ bool edge(int from) const { return (from < lo_most && from + KV4_TILE > sink) || from + KV4_TILE - 1 > hi_least; }
+    __device__ __forceinline__ float * set(int i, size_t, int, int hd) const { return sets + size_t(i) * (hd + 4); }
+};
+
+template <int HD, int NQ>
+__global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_parts_kernel(Kv4PartsArgs x) {
+    __shared__ int2 at[16 * NQ];
+    Kv4PartRows rows;
+    if (rows.find(x, 16 * NQ, at)) kv4_attend<HD, NQ>(x.a, rows);
+}
+
+// Workgroup (rows: q heads of tokens): WAVES waves a row, each its share of the row's sets, lanes HD / 4 to a set; WAVES 1: four rows
+// a workgroup.
+template <int HD, int WAVES>
+__global__ __launch_bounds__(256) void kv4_parts_join_kernel(Kv4PartsArgs x, int rows) {
+    constexpr int PER = HD / 4, SETS = 64 / PER, AHEAD = 4;
+    __shared__ float cl[4][2];
+    __shared__ __align__(16) float part[4][HD];
+    const Kv4AttnArgs & a = x.a;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / PER, e = lane % PER * 4;
+    const long long all = (long long)a.t.n_seq * a.t.n_tok * a.n_head, at = WAVES == 1 ? blockIdx.x * 4ll + wave : blockIdx.x;
+    if (at >= all) return;
+    const int token = int(at / a.n_head), hq = int(at - (long long)token * a.n_head), s = int(unsigned(token) / unsigned(a.t.n_tok)), t = token - s * a.t.n_tok;
+    const int n_group = kv4_groups(x), group = n_group ? int(unsigned(s) / unsigned(x.members)) : 0, G = a.group, h = int(unsigned(hq) / unsigned(G));
+    const int2 * table = reinterpret_cast<const int2 *>(a.work);
+    const int2 own = table[n_group + s], pre = n_group ? table[group] : int2{0, 0};
+    const int len = n_group ? kv4_prefix(x, group) : 0;
+    long long p0;
+    int n_tok;
+    kv4_span(a.t, s, p0, n_tok);
+    if (t >= n_tok || p0 + t < 0 || p0 + t >= a.c.n_ctx || (!len && own.y == 1)) return;
+    // its place in its workgroups: in that of the sequence's own ranges and in that of the prefix's
+    constexpr size_t SET = HD + 4;
+    const int orow = t * G + hq - h * G, prow = orow + (s - group * x.members) * a.t.n_tok * G;
+    const float * sets = kv4_sets(x);
+    const auto first = [&](int base, int row) { return sets + (size_t(base + row / rows * a.c.n_head_kv + h) * rows + row % rows) * SET; };
+    const float * ow = first(own.x, orow), * pw = first(pre.x, n_group ? prow : 0);
+    const size_t ostep = kv4_units(x, false, rows) * size_t(rows) * SET, pstep = n_group ? kv4_units(x, true, rows) * size_t(rows) * SET : 0;
+    const int n = pre.y + own.y, n0 = WAVES == 1 ? 0 : n * wave / WAVES, n1 = WAVES == 1 ? n : n * (wave + 1) / WAVES;
+    const auto set = [&](int j) { return j < pre.y ? pw + j * pstep : ow + (j - pre.y) * ostep; };
+    f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
+    float C = KV4_LOW, L = 0.0f;
+    for (int b = n0; b < n1; b += 64) {  // 64 sets (often all) at a time
+        const float2 c = b + lane < n1 ? *reinterpret_cast<const float2 *>(set(b + lane) + HD) : float2{KV4_LOW, 0.0f};
+        const float top = fmaxf(wave_max(c.x), C), old = __builtin_amdgcn_exp2f(C - top), f = __builtin_amdgcn_exp2f(c.x - top);
+        C = top;
+        L = L * old + c.y * f;  // the lane's own sets'
+        y *= old;
+        const int m = min(n1 - b, 64);
+        for (int j0 = sub; j0 < m + sub; j0 += AHEAD * SETS) {  // (as often in every lane)
+            f32x4 v[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                v[i] = j0 + i * SETS < m ? *reinterpret_cast<const f32x4 *>(set(b + j0 + i * SETS) + e) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i) {
+                const int j = (j0 + i * SETS) & 63;
+                const float fj = __shfl(f, j, WAVE), lj = __shfl(c.y, j, WAVE);
+                if (j0 + i * SETS < m && !(lj == 0.0f)) y += v[i] * fj;  // (sets of nothing have no sums)
+            }
+        }
+    }
+#pragma unroll
+    for (int d = 32; d >= 1; d >>= 1) L += __shfl_xor(L, d, WAVE);
+#pragma unroll
+    for (int d = 32; d >= PER; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) y[i] += __shfl_xor(y[i], d, WAVE);
+    if constexpr (WAVES > 1) {
+        if (lane == 0) {
+            cl[wave][0] = C;
+            cl[wave][1] = L;
+        }
+        if (sub == 0) *reinterpret_cast<f32x4 *>(&part[wave][e]) = y;
+        __syncthreads();
+        if (wave) return;
+        float top = KV4_LOW;
+        for (int w = 0; w < WAVES; ++w) top = fmaxf(top, cl[w][0]);
+        y = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        L = 0.0f;
+        for (int w = 0; w < WAVES; ++w) {
+            const float f = __builtin_amdgcn_exp2f(cl[w][0] - top);
+            y += *reinterpret_cast<const f32x4 *>(&part[w][e]) * f;
+            L += cl[w][1] * f;
+        }
+    }
+    if (sub == 0) kv4_out<HD>(a, token, hq, e, y, L);
 }
 
 // Workgroup (q head and EL of its elements, token, sequence): the sets of a sequence with several ranges. The factors of all sets
@@ -1071,6 +1430,57 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
             const int per_wave = int(std::min<long long>(std::max<long long>(all / 4096, 1), 16));
             GQ_LAUNCH(kv4_join_rows_kernel<hd.value>, dim3(unsigned((rows + 4 * per_wave - 1) / (4 * per_wave)), a.t.n_seq), dim3(256), 0, s, a, per_wave);
         }
+    });
+}
+
+// How a call with a prefix or sinks is launched: groups of 16 rows a workgroup, the workgroups that its ranges are dealt to and the
+// most that they can come to (every segment's units once more), and whether every segment is one range.
+struct Kv4Plan {
+    int nq, target;
+    bool whole;
+    long long grid;
+};
+static Kv4Plan kv4_plan(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head, int window, int sinks) {
+    const long long per_kv = n_tok * (long long)(n_head / c.n_head_kv);
+    Kv4Plan p;
+    p.nq = kv4_nq(c.head_dim, n_tok, n_head / c.n_head_kv);
+    p.target = 256 * kv4_resident(c.head_dim, p.nq);
+    const int rows = 16 * p.nq;
+    const long long own = (per_kv + rows - 1) / rows * c.n_head_kv * n_seq;
+    const long long pre = n_group ? (per_kv * (n_seq / n_group) + rows - 1) / rows * c.n_head_kv * n_group : 0;
+    long long tiles = kv4_tiles(c.n_ctx);  // records of a sequence that its tokens see
+    if (window) tiles = std::min(tiles, (long long)window / KV4_TILE + n_tok / KV4_TILE + 3 + sinks / KV4_TILE);
+    p.whole = !n_group && (own >= p.target || tiles <= KV4_ALONE / c.head_dim);
+    p.grid = own + pre + (p.whole ? 0 : p.target);
+    return p;
+}
+
+size_t kv4_parts_floats(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head) {
+    const Kv4Plan p = kv4_plan(c, n_group, n_seq, n_tok, n_head, 0, 0);
+    return p.whole ? 0 : kv4_table_floats((long long)n_group + n_seq) + size_t(p.grid) * (16 * p.nq) * (c.head_dim + 4);
+}
+long long kv4_parts_grid(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head) {
+    return kv4_plan(c, n_group, n_seq, n_tok, n_head, 0, 0).grid;
+}
+
+hipError_t launch_kv4_parts(const Kv4PartsArgs & args, hipStream_t s) {
+    Kv4PartsArgs x = args;
+    Kv4AttnArgs & a = x.a;
+    const Kv4Plan p = kv4_plan(a.c, x.pre.data ? a.t.n_seq / x.members : 0, a.t.n_seq, a.t.n_tok, a.n_head, a.window, x.sinks);
+    x.target = p.target;
+    x.whole = p.whole;
+    a.group = a.n_head / a.c.n_head_kv;
+    const dim3 grid{unsigned(p.grid)};
+    return by_dim(a.c.head_dim, [&](auto hd) {
+        if (p.nq == 1) GQ_LAUNCH((kv4_parts_kernel<hd.value, 1>), grid, dim3(256), 0, s, x);
+        if constexpr (hd.value < 256)
+            if (p.nq == 2) GQ_LAUNCH((kv4_parts_kernel<hd.value, 2>), grid, dim3(256), 0, s, x);
+        if constexpr (hd.value < 128)
+            if (p.nq == 4) GQ_LAUNCH((kv4_parts_kernel<hd.value, 4>), grid, dim3(256), 0, s, x);
+        if (p.whole) return;
+        const long long rows = (long long)a.t.n_seq * a.t.n_tok * a.n_head;
+        if (rows <= KV4_FEW) GQ_LAUNCH((kv4_parts_join_kernel<hd.value, 4>), dim3(unsigned(rows)), dim3(256), 0, s, x, 16 * p.nq);
+        else GQ_LAUNCH((kv4_parts_join_kernel<hd.value, 1>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, s, x, 16 * p.nq);
     });
 }
 

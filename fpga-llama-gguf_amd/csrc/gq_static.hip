@@ -192,6 +192,76 @@ int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_strid
 
 }  // extern "C"
 
+namespace {
+
+// Sizes of a call with parts: rows and workgroups fit one-dimensional grids.
+bool kv4_parts_ok(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int n_head) {
+    if (!kv4_sizes_ok(kv) || !kv4_heads_ok(kv, n_tok, n_head) || int64_t(kv->n_seq) * n_tok * n_head > GEMVQ_KV4_MAX_PART_ROWS) return false;
+    if (prefix && (!kv4_sizes_ok(prefix) || prefix->n_head_kv != kv->n_head_kv || prefix->head_dim != kv->head_dim || kv->n_seq % prefix->n_seq)) return false;
+    return kv4_parts_grid(kv4_cache(kv), prefix ? prefix->n_seq : 0, kv->n_seq, n_tok, n_head) < (1 << 24);  // below 2^32 threads
+}
+uint64_t kv4_parts_work(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int n_head) {
+    return kv4_parts_floats(kv4_cache(kv), prefix ? prefix->n_seq : 0, kv->n_seq, n_tok, n_head) * sizeof(float);
+}
+
+int kv4_parts(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, const int32_t * prefix_len, const float * q, int64_t q_stride,
+              int64_t q_head_stride, float * y, int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num,
+              int window, int sinks, float scale, void * work, uint64_t work_bytes, void * stream) {
+    Kv4PartsArgs x{};
+    if (!kv4_ok(kv) || !kv4_tokens(kv, n_tok, pos, num, x.a.t) || !kv4_parts_ok(kv, prefix, n_tok, n_head) || window < 0 || sinks < 0) return GEMVQ_EINVAL;
+    if (prefix && (!kv4_ok(prefix) || !prefix_len || !aligned(prefix_len, 4))) return GEMVQ_EINVAL;
+    const uint64_t need = kv4_parts_work(kv, prefix, n_tok, n_head);
+    if (work_bytes < need || (need && (!work || !aligned(work, 16)))) return GEMVQ_EINVAL;
+    const int64_t hd = kv->head_dim;
+    if (!rows_ok(q, q_stride, hd) || q_head_stride % 4 || q_head_stride < hd || q_head_stride > (int64_t(1) << 40) ||
+        !rows_ok(y, y_stride, n_head * hd))
+        return GEMVQ_EINVAL;
+    x.a.c = kv4_cache(kv);
+    x.a.q = q;
+    x.a.y = y;
+    x.a.q_row = q_stride;
+    x.a.q_head = q_head_stride;
+    x.a.y_row = y_stride;
+    x.a.n_head = n_head;
+    x.a.window = window;
+    x.a.scale = scale;
+    x.a.work = need ? static_cast<float *>(work) : nullptr;
+    if (prefix) x.pre = kv4_cache(prefix);
+    x.pre_len = prefix_len;
+    x.members = prefix ? kv->n_seq / prefix->n_seq : 1;
+    x.sinks = sinks;
+    const hipError_t e = launch_kv4_parts(x, static_cast<hipStream_t>(stream));
+    return e == hipSuccess ? 0 : -int(e);
+}
+
+}  // namespace
+
+extern "C" {
+
+uint64_t gemvq_kv4_attn_sink_work(const gemvq_kv4 * kv, int n_tok, int n_head) {
+    return kv4_parts_ok(kv, nullptr, n_tok, n_head) ? kv4_parts_work(kv, nullptr, n_tok, n_head) : 0;
+}
+
+int gemvq_kv4_attn_sink_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
+                               int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,
+                               int sinks, float scale, void * work, uint64_t work_bytes, void * stream) {
+    return kv4_parts(kv, nullptr, nullptr, q, q_stride, q_head_stride, y, y_stride, n_tok, n_head, pos, num, window, sinks, scale, work, work_bytes, stream);
+}
+
+uint64_t gemvq_kv4_attn_shared_work(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int n_head) {
+    return prefix && kv4_parts_ok(kv, prefix, n_tok, n_head) ? kv4_parts_work(kv, prefix, n_tok, n_head) : 0;
+}
+
+int gemvq_kv4_attn_shared_static(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, const int32_t * prefix_len, const float * q,
+                                 int64_t q_stride, int64_t q_head_stride, float * y, int64_t y_stride, int n_tok, int n_head,
+                                 const int32_t * pos, const int32_t * num, int window, int sinks, float scale, void * work,
+                                 uint64_t work_bytes, void * stream) {
+    if (!prefix) return GEMVQ_EINVAL;
+    return kv4_parts(kv, prefix, prefix_len, q, q_stride, q_head_stride, y, y_stride, n_tok, n_head, pos, num, window, sinks, scale, work, work_bytes, stream);
+}
+
+}  // extern "C"
+
 static_assert(GEMVQ_BEAM_MAX == BEAM_MAX && GEMVQ_BEAM_MAX_VOCAB == BEAM_MAX_VOCAB, "limits in the header");
 
 namespace {

@@ -238,6 +238,10 @@ def hip_lib() -> C.CDLL:
         _c_fn(lib, "gemvq_beam_select_static", i, vp, i64, i, i, i, vp, vp, i, vp, vp, vp, vp, u64, vp)
         _c_fn(lib, "gemvq_beam_reorder_static", i, C.POINTER(BeamArray), i, vp, i, i, vp)
         f64 = C.c_double
+        _c_fn(lib, "gemvq_kv4_attn_sink_work", u64, kvp, i, i)
+        _c_fn(lib, "gemvq_kv4_attn_sink_static", i, kvp, vp, i64, i64, vp, i64, i, i, vp, vp, i, i, C.c_float, vp, u64, vp)
+        _c_fn(lib, "gemvq_kv4_attn_shared_work", u64, kvp, kvp, i, i)
+        _c_fn(lib, "gemvq_kv4_attn_shared_static", i, kvp, kvp, vp, vp, i64, i64, vp, i64, i, i, vp, vp, i, i, C.c_float, vp, u64, vp)
         _c_fn(lib, "gemvq_rope_freqs", i, i, f64, f64, i, f64, f64, vp, vp)
         _c_fn(lib, "gemvq_rope_static", i, C.POINTER(RopeRows), i, i, i, i, i, i, vp, vp, vp, vp)
         _c_fn(lib, "gemvq_draft_work", u64, i, i, i)
@@ -356,6 +360,32 @@ def kv4_attn_static(kv: Kv4, q: int, q_stride: int, q_head_stride: int, y: int, 
     """Attention of the tokens at positions pos[s] + t over the cache (their own keys and values stored before)."""
     _ok(hip_lib().gemvq_kv4_attn_static(kv, q, q_stride, q_head_stride, y, y_stride, n_tok, n_head, pos, num, window, scale,
                                         work, work_bytes, stream), "kv4 attention")
+
+
+def kv4_attn_sink_work(kv: Kv4, n_tok: int, n_head: int) -> int:
+    """Bytes of workspace of kv4_attn_sink_static."""
+    return hip_lib().gemvq_kv4_attn_sink_work(kv, n_tok, n_head)
+
+
+def kv4_attn_sink_static(kv: Kv4, q: int, q_stride: int, q_head_stride: int, y: int, y_stride: int, n_tok: int, n_head: int,
+                         pos: int, num: int = 0, window: int = 0, sinks: int = 0, scale: float = 1.0, work: int = 0,
+                         work_bytes: int = 0, stream: int = 0) -> None:
+    """Attention over the last `window` positions and the first `sinks`."""
+    _ok(hip_lib().gemvq_kv4_attn_sink_static(kv, q, q_stride, q_head_stride, y, y_stride, n_tok, n_head, pos, num, window, sinks,
+                                             scale, work, work_bytes, stream), "kv4 attention with sinks")
+
+
+def kv4_attn_shared_work(kv: Kv4, prefix: Kv4, n_tok: int, n_head: int) -> int:
+    """Bytes of workspace of kv4_attn_shared_static (0: sizes that are not served)."""
+    return hip_lib().gemvq_kv4_attn_shared_work(kv, prefix, n_tok, n_head)
+
+
+def kv4_attn_shared_static(kv: Kv4, prefix: Kv4, prefix_len: int, q: int, q_stride: int, q_head_stride: int, y: int, y_stride: int,
+                           n_tok: int, n_head: int, pos: int, num: int = 0, window: int = 0, sinks: int = 0, scale: float = 1.0,
+                           work: int = 0, work_bytes: int = 0, stream: int = 0) -> None:
+    """Attention of groups of sequences, each over its group's prefix and its own cache behind it."""
+    _ok(hip_lib().gemvq_kv4_attn_shared_static(kv, prefix, prefix_len, q, q_stride, q_head_stride, y, y_stride, n_tok, n_head, pos,
+                                               num, window, sinks, scale, work, work_bytes, stream), "kv4 attention with a prefix")
 
 
 def beam_work(n_group: int, n_beam: int, n_vocab: int) -> int:

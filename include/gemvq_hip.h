@@ -366,6 +366,24 @@ uint64_t gemvq_kv4_attn_work(const gemvq_kv4 * kv, int n_tok, int n_head);
 int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
                           int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,
                           float scale, void * work, uint64_t work_bytes, void * stream);
+/* Attention with sinks: as gemvq_kv4_attn_static, the token at position p seeing the positions j <= p with j < sinks or j > p -
+ * window (window 0: all of them). n_seq * n_tok * n_head <= GEMVQ_KV4_MAX_PART_ROWS. work: gemvq_kv4_attn_sink_work() bytes. */
+#define GEMVQ_KV4_MAX_PART_ROWS (1 << 22)
+uint64_t gemvq_kv4_attn_sink_work(const gemvq_kv4 * kv, int n_tok, int n_head);
+int gemvq_kv4_attn_sink_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
+                               int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,
+                               int sinks, float scale, void * work, uint64_t work_bytes, void * stream);
+/* Attention of groups of sequences that share a prefix, whose records are read and unpacked for all of a group's rows together.
+ * prefix: a cache with a region for each group, of kv's n_head_kv and head_dim; group g are the sequences g * m .. g * m + m - 1, m =
+ * kv->n_seq / prefix->n_seq (a whole number). Positions 0 .. P - 1 of a sequence are the first P = prefix_len[g] (int32 in device
+ * memory, taken within 0 .. prefix->n_ctx) of its group's region, the others those of its own region of kv: token t stands at
+ * place pos[s] + t there (0 .. kv->n_ctx - 1), its position is P + pos[s] + t. It sees the positions j up to its own with j < sinks or j >
+ * position - window (window 0: all of them). Everything else as in the calls above. */
+uint64_t gemvq_kv4_attn_shared_work(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int n_head);
+int gemvq_kv4_attn_shared_static(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, const int32_t * prefix_len, const float * q,
+                                 int64_t q_stride, int64_t q_head_stride, float * y, int64_t y_stride, int n_tok, int n_head,
+                                 const int32_t * pos, const int32_t * num, int window, int sinks, float scale, void * work,
+                                 uint64_t work_bytes, void * stream);
 
 /* No counterpart in the reference: one step of a beam search over n_group independent groups of n_beam (1 .. GEMVQ_BEAM_MAX)
  * beams, rows g * n_beam + b, at most 65535 rows; on caller-owned device memory, under the rules of the calls above.

@@ -9,7 +9,7 @@ constexpr int DRAFT_MAX_VOCAB = 1 << 20;
 
 // Sequence s has tokens d_0 .. d_{k-1} drafted (k = num[s], at most n_draft; below 0: not in use), the target's rows s * (n_draft + 1) + t
 // for t = 0 .. k (row k follows the last token) and the draft's rows s * n_draft + t. p_t and q_t are the rows' distributions,
-// e^((x - max x) / temperature) over their sum, in 64 bits; without draft rows q_t is 1 at d_t. Token t is accepted if u_t q_t(d_t) <
+// e^((x - max x) / temperature) over their sum (below 2^-1000 of the largest: 0); without draft rows q_t is 1 at d_t. Token t is accepted if u_t q_t(d_t) <
 // p_t(d_t) and all before it are. At the first that is not, a new token comes from max(p_t - q_t, 0) (from p_t where nothing is left),
 // behind the last from p_k: the first whose weights' sum up to it is above u_{n_draft} times the sum of all. Temperature 0: the
 // target's largest logit, the lowest index of equal ones, is what a token is compared with and what is new; log-probabilities are
@@ -27,8 +27,8 @@ struct DraftArgs {
     double temperature, draft_temperature;
     int n_vocab, n_seq, n_draft;
     void * work;
-    int per;     // set at launch: logits a thread takes at a time
-    int chunks;  // set at launch: workgroups a row
+    int chunks;  // set at launch: the first kernel's workgroups a row
+    int parts;   // set at launch: the second one's workgroups a sequence
 };
 
 size_t draft_work(int n_seq, int n_draft, int n_vocab);

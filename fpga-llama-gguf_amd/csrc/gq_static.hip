@@ -397,6 +397,9 @@ int gemvq_rope_static(const gemvq_rope_rows * arrays, int n_arrays, int n_seq, i
     return e == hipSuccess ? 0 : -int(e);
 }
 
+// Differences of logits over it, and its reciprocal, are 64-bit numbers.
+static bool draft_temperature_ok(double t) { return t >= 1e-30 && t <= 1e30; }
+
 uint64_t gemvq_draft_work(int n_seq, int n_draft, int n_vocab) {
     if (n_seq < 1 || n_draft < 0 || n_draft > DRAFT_MAX || int64_t(n_seq) * (2 * n_draft + 1) > GRID_MAX || n_vocab < 1 || n_vocab > DRAFT_MAX_VOCAB)
         return 0;
@@ -411,8 +414,8 @@ int gemvq_draft_verify_static(const float * target, int64_t target_stride, const
     const int64_t most = int64_t(1) << 40;
     if (!need || !target || target_stride < n_vocab || target_stride > most || !n_accept || !out || !work || work_bytes < need) return GEMVQ_EINVAL;
     if (draft && (draft_stride < n_vocab || draft_stride > most)) return GEMVQ_EINVAL;
-    if ((n_draft && !token) || !(temperature >= 0.0) || !std::isfinite(temperature) || (temperature > 0.0 && !uniform)) return GEMVQ_EINVAL;
-    if (temperature > 0.0 && draft && (!(draft_temperature > 0.0) || !std::isfinite(draft_temperature))) return GEMVQ_EINVAL;
+    if ((n_draft && !token) || (temperature != 0.0 && (!draft_temperature_ok(temperature) || !uniform))) return GEMVQ_EINVAL;
+    if (temperature != 0.0 && draft && !draft_temperature_ok(draft_temperature)) return GEMVQ_EINVAL;
     if (!aligned(target, 4) || !aligned(draft, 4) || !aligned(token, 4) || !aligned(num, 4) || !aligned(uniform, 4) || !aligned(n_accept, 4) ||
         !aligned(out, 4) || !aligned(logp, 4) || !aligned(work, 16))
         return GEMVQ_EINVAL;

@@ -36,18 +36,19 @@ __device__ __forceinline__ float2 rope_turn(double t, double m) {
 }
 
 // Workgroup (token rows | heads): the angles of its rows once, to LDS, 64-bit work that all heads share; then its elements, WIDE in
-// pieces of four pairs (or of 16 bytes that stay), else pair by pair. The first pieces are read before the angles are there. Memory
-// bounds it.
+// pieces of four pairs, or of 16 bytes that stay, else pair by pair. The first pieces are
+// read before the angles are there. Memory bounds it.
 template <bool WIDE, bool PAIRS>
 __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
-    constexpr int AHEAD = 4, W = WIDE ? 4 : 1;
+    // pairs of a piece (elements of one that stays), its elements, pieces that a thread has on their way
+    constexpr int W = WIDE ? 4 : 1, N = 2 * W, AHEAD = 4;
     __shared__ float2 cs[ROPE_MAX_DIM / 2];  // tokens * n_rot / 2 of them
     __shared__ int live[256];                // rows with a position
     const int tid = threadIdx.x, half = a.n_rot / 2, tail = a.head_dim - a.n_rot;
-    const int per = half / W + tail / W;  // pieces of a head
+    const int turn = half / W, per = turn + tail / W;  // pieces of a head
     const int row0 = int(blockIdx.x) * a.tokens, rows = min(a.tokens, a.n_seq * a.n_tok - row0);
     const int head0 = int(blockIdx.y) * a.heads, heads = min(a.heads, a.a[a.n - 1].end - head0);
-    const int items = rows * heads * per;
+    const int items = rows * heads * per, second = PAIRS ? W : half;  // where a piece's second 16 bytes (or element) are
 
     struct Piece {
         const float * x;
@@ -56,7 +57,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
     };
     const auto find = [&](int i) {
         Piece p;
-        const int rh = int(unsigned(i) / unsigned(per)), r = int(unsigned(rh) / unsigned(heads));
+        // quotients of numbers whose product with the divisor is below 2^32
+        const int rh = a.per_mul ? int(__umulhi(unsigned(i), a.per_mul)) : i, r = heads == 1 ? rh : heads == a.heads ? int(__umulhi(unsigned(rh), a.heads_mul)) : int(unsigned(rh) / unsigned(heads));
         int h = head0 + rh - r * heads, k = 0;
         p.c = i - rh * per;
         p.r = i < items ? r : -1;
@@ -68,64 +70,48 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
         const long long row = row0 + r;
         p.x = m.x + row * m.x_row + h * m.x_head;
         p.y = m.y + row * m.y_row + h * m.y_head;
-        if (p.x == p.y && p.c >= half / W) p.r = -1;  // in place: nothing to copy
+        if (p.x == p.y && p.c >= turn) p.r = -1;  // in place: nothing to copy
+        const int at = p.c >= turn ? a.n_rot + (p.c - turn) * W : PAIRS ? N * p.c : W * p.c;
+        p.x += at;
+        p.y += at;
         return p;
     };
-    const auto load = [&](const Piece & p, float * v) {  // its pairs' first elements, then the second ones
+    const auto load = [&](const Piece & p, float * v) {  // of halves the first elements, then the second ones
         if (p.r < 0) return;
-        const int o = p.c * W;
         if constexpr (WIDE) {
-            f32x4 lo, hi;
-            if (o >= half) {
-                lo = *reinterpret_cast<const f32x4 *>(p.x + a.n_rot + o - half);
-                hi = lo;
-            } else if (PAIRS) {
-                lo = *reinterpret_cast<const f32x4 *>(p.x + 2 * o);
-                hi = *reinterpret_cast<const f32x4 *>(p.x + 2 * o + 4);
-            } else {
-                lo = *reinterpret_cast<const f32x4 *>(p.x + o);
-                hi = *reinterpret_cast<const f32x4 *>(p.x + half + o);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                v[e] = lo[e];
-                v[4 + e] = hi[e];
-            }
+            *reinterpret_cast<f32x4 *>(v) = *reinterpret_cast<const f32x4 *>(p.x);
+            if (p.c < turn) *reinterpret_cast<f32x4 *>(v + 4) = *reinterpret_cast<const f32x4 *>(p.x + second);
         } else {
-            v[0] = p.x[o >= half ? a.n_rot + o - half : PAIRS ? 2 * o : o];
-            v[1] = o >= half ? 0.0f : p.x[PAIRS ? 2 * o + 1 : half + o];
+            v[0] = p.x[0];
+            if (p.c < turn) v[1] = p.x[second];
         }
     };
     const auto put = [&](const Piece & p, const float * v) {
         if (p.r < 0 || !live[p.r]) return;
-        const int o = p.c * W;
-        float z[2 * W];
-        if (o < half) {
+        const bool turns = p.c < turn;
+        float z[N];
+#pragma unroll
+        for (int e = 0; e < N; ++e) z[e] = v[e];
+        if (turns) {
 #pragma unroll
             for (int e = 0; e < W; ++e) {
-                const float2 t = cs[p.r * half + o + e];
-                const int i0 = WIDE && PAIRS ? 2 * e : e, i1 = WIDE && PAIRS ? 2 * e + 1 : W + e;
+                const float2 t = cs[p.r * half + p.c * W + e];
+                const int i0 = PAIRS ? 2 * e : e, i1 = PAIRS ? 2 * e + 1 : W + e;
                 z[i0] = v[i0] * t.x - v[i1] * t.y;
                 z[i1] = v[i0] * t.y + v[i1] * t.x;
             }
         }
         if constexpr (WIDE) {
-            if (o >= half) {
-                *reinterpret_cast<f32x4 *>(p.y + a.n_rot + o - half) = f32x4{v[0], v[1], v[2], v[3]};
-            } else {
-                *reinterpret_cast<f32x4 *>(p.y + (PAIRS ? 2 * o : o)) = f32x4{z[0], z[1], z[2], z[3]};
-                *reinterpret_cast<f32x4 *>(p.y + (PAIRS ? 2 * o + 4 : half + o)) = f32x4{z[4], z[5], z[6], z[7]};
-            }
-        } else if (o >= half) {
-            p.y[a.n_rot + o - half] = v[0];
+            *reinterpret_cast<f32x4 *>(p.y) = f32x4{z[0], z[1], z[2], z[3]};
+            if (turns) *reinterpret_cast<f32x4 *>(p.y + second) = f32x4{z[4], z[5], z[6], z[7]};
         } else {
-            p.y[PAIRS ? 2 * o : o] = z[0];
-            p.y[PAIRS ? 2 * o + 1 : half + o] = z[1];
+            p.y[0] = z[0];
+            if (turns) p.y[second] = z[1];
         }
     };
 
     Piece p[AHEAD];
-    float v[AHEAD][2 * W];
+    float v[AHEAD][N];
 #pragma unroll
     for (int j = 0; j < AHEAD; ++j) {
         p[j] = find(tid + 256 * j);
@@ -160,13 +146,16 @@ hipError_t launch_rotary(const RotaryArgs & args, hipStream_t s) {
     int heads = 0;
     for (int i = 0; i < a.n; ++i) a.a[i].end = heads += a.a[i].n_head;
     const bool wide = a.n_rot % 8 == 0;
-    const int w = wide ? 4 : 1, per = a.n_rot / 2 / w + (a.head_dim - a.n_rot) / w;
+    const int per = (a.n_rot / 2 + a.head_dim - a.n_rot) / (wide ? 4 : 1);  // pieces of a head
     const long long rows = (long long)a.n_seq * a.n_tok;
     a.tokens = std::max(1, 512 / a.n_rot);
-    // pieces of a workgroup: four a thread, or one where that leaves the device's 256 CUs less than two workgroups each
-    const long long all = rows * heads * per;
-    const int pieces = all >= 512 * 1024 ? 1024 : 256;
+    // Pieces of a workgroup: one a thread, or, where that is more than the device has room for, eight. us with one, four and eight: 4.3 /
+    // 4.4 / 4.1 at 1 token of 16/4 heads of 256, 4.3 / 4.8 / 6.6 at 8 of 32/8 of 128, 62 / 42 / 38.5 at 4096 of them.
+    const int pieces = rows * heads * per >= 512 * 1024 ? 2048 : 256;
     a.heads = std::min(heads, std::max(1, pieces / (a.tokens * per)));
+    const auto mul = [](int d) { return d > 1 ? unsigned((0x100000000ull + unsigned(d) - 1) / unsigned(d)) : 0u; };
+    a.per_mul = mul(per);
+    a.heads_mul = mul(a.heads);
     const dim3 grid(unsigned((rows + a.tokens - 1) / a.tokens), unsigned((heads + a.heads - 1) / a.heads));
     if (wide && a.pairs) GQ_LAUNCH((rope_kernel<true, true>), grid, dim3(256), 0, s, a);
     else if (wide) GQ_LAUNCH((rope_kernel<true, false>), grid, dim3(256), 0, s, a);

@@ -37,7 +37,8 @@ __device__ __forceinline__ float2 rope_turn(double t, double m) {
 
 // Workgroup (token rows | heads): the angles of its rows once, to LDS, 64-bit work that all heads share; then its elements, WIDE in
 // pieces of four pairs, or of 16 bytes that stay, else pair by pair. The first pieces are
-// read before the angles are there. Memory bounds it.
+// read before the angles are there. Memory bounds it: 4096 tokens of 32/8 heads of 128
+// (168 MB) are 29.4 us, 5.7 TB/s, neighbours 35.7, where a wave's access covers every other 16 bytes; one token 4.3, a launch and two trips.
 template <bool WIDE, bool PAIRS>
 __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
     // pairs of a piece (elements of one that stays), its elements, pieces that a thread has on their way
@@ -86,6 +87,10 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
             if (p.c < turn) v[1] = p.x[second];
         }
     };
+    const auto store = [&](f32x4 z, float * to) {
+        if (a.many) __builtin_nontemporal_store(z, reinterpret_cast<f32x4 *>(to));
+        else *reinterpret_cast<f32x4 *>(to) = z;
+    };
     const auto put = [&](const Piece & p, const float * v) {
         if (p.r < 0 || !live[p.r]) return;
         const bool turns = p.c < turn;
@@ -102,8 +107,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
             }
         }
         if constexpr (WIDE) {
-            *reinterpret_cast<f32x4 *>(p.y) = f32x4{z[0], z[1], z[2], z[3]};
-            if (turns) *reinterpret_cast<f32x4 *>(p.y + second) = f32x4{z[4], z[5], z[6], z[7]};
+            store(f32x4{z[0], z[1], z[2], z[3]}, p.y);
+            if (turns) store(f32x4{z[4], z[5], z[6], z[7]}, p.y + second);
         } else {
             p.y[0] = z[0];
             if (turns) p.y[second] = z[1];
@@ -150,8 +155,10 @@ hipError_t launch_rotary(const RotaryArgs & args, hipStream_t s) {
     const long long rows = (long long)a.n_seq * a.n_tok;
     a.tokens = std::max(1, 512 / a.n_rot);
     // Pieces of a workgroup: one a thread, or, where that is more than the device has room for, eight. us with one, four and eight: 4.3 /
-    // 4.4 / 4.1 at 1 token of 16/4 heads of 256, 4.3 / 4.8 / 6.6 at 8 of 32/8 of 128, 62 / 42 / 38.5 at 4096 of them.
-    const int pieces = rows * heads * per >= 512 * 1024 ? 2048 : 256;
+    // 4.4 / 4.1 at 1 token of 16/4 heads of 256, 4.3 / 4.8 / 6.6 at 8 of 32/8 of 128, 62 / 42 / 38.5 at 4096 of them (29.4 with stores
+    // that pass the caches by, which these, 16 MB and more, do not fit; loads that do are 3 us longer).
+    a.many = rows * heads * per >= 512 * 1024;
+    const int pieces = a.many ? 2048 : 256;
     a.heads = std::min(heads, std::max(1, pieces / (a.tokens * per)));
     const auto mul = [](int d) { return d > 1 ? unsigned((0x100000000ull + unsigned(d) - 1) / unsigned(d)) : 0u; };
     a.per_mul = mul(per);

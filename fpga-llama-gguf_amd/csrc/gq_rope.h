@@ -27,7 +27,6 @@ struct RotaryArgs {
     int pairs;       // 0: halves, 1: neighbours
     int tokens;      // set at launch: token rows of a workgroup
     int heads;       // set at launch: heads of a workgroup
-    int many;        // set at launch: more than the caches hold
     unsigned per_mul, heads_mul;  // set at launch: i / d = the high word of i * mul, for the pieces of a head and for heads; 0: d is 1
 };
 hipError_t launch_rotary(const RotaryArgs & a, hipStream_t s);

@@ -39,7 +39,7 @@ __device__ __forceinline__ float2 rope_turn(double t, double m) {
 // pieces of four pairs, or of 16 bytes that stay, else pair by pair. The first pieces are
 // read before the angles are there. Memory bounds it: 4096 tokens of 32/8 heads of 128
 // (168 MB) are 29.4 us, 5.7 TB/s, neighbours 35.7, where a wave's access covers every other 16 bytes; one token 4.3, a launch and two trips.
-template <bool WIDE, bool PAIRS>
+template <bool WIDE, bool PAIRS, bool MANY>
 __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
     // pairs of a piece (elements of one that stays), its elements, pieces that a thread has on their way
     constexpr int W = WIDE ? 4 : 1, N = 2 * W, AHEAD = 4;
@@ -88,7 +88,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
         }
     };
     const auto store = [&](f32x4 z, float * to) {
-        if (a.many) __builtin_nontemporal_store(z, reinterpret_cast<f32x4 *>(to));
+        if constexpr (MANY) __builtin_nontemporal_store(z, reinterpret_cast<f32x4 *>(to));
         else *reinterpret_cast<f32x4 *>(to) = z;
     };
     const auto put = [&](const Piece & p, const float * v) {
@@ -157,17 +157,19 @@ hipError_t launch_rotary(const RotaryArgs & args, hipStream_t s) {
     // Pieces of a workgroup: one a thread, or, where that is more than the device has room for, eight. us with one, four and eight: 4.3 /
     // 4.4 / 4.1 at 1 token of 16/4 heads of 256, 4.3 / 4.8 / 6.6 at 8 of 32/8 of 128, 62 / 42 / 38.5 at 4096 of them (29.4 with stores
     // that pass the caches by, which these, 16 MB and more, do not fit; loads that do are 3 us longer).
-    a.many = rows * heads * per >= 512 * 1024;
-    const int pieces = a.many ? 2048 : 256;
+    const bool many = rows * heads * per >= 512 * 1024;
+    const int pieces = many ? 2048 : 256;
     a.heads = std::min(heads, std::max(1, pieces / (a.tokens * per)));
     const auto mul = [](int d) { return d > 1 ? unsigned((0x100000000ull + unsigned(d) - 1) / unsigned(d)) : 0u; };
     a.per_mul = mul(per);
     a.heads_mul = mul(a.heads);
     const dim3 grid(unsigned((rows + a.tokens - 1) / a.tokens), unsigned((heads + a.heads - 1) / a.heads));
-    if (wide && a.pairs) GQ_LAUNCH((rope_kernel<true, true>), grid, dim3(256), 0, s, a);
-    else if (wide) GQ_LAUNCH((rope_kernel<true, false>), grid, dim3(256), 0, s, a);
-    else if (a.pairs) GQ_LAUNCH((rope_kernel<false, true>), grid, dim3(256), 0, s, a);
-    else GQ_LAUNCH((rope_kernel<false, false>), grid, dim3(256), 0, s, a);
+    if (wide && a.pairs && many) GQ_LAUNCH((rope_kernel<true, true, true>), grid, dim3(256), 0, s, a);
+    else if (wide && many) GQ_LAUNCH((rope_kernel<true, false, true>), grid, dim3(256), 0, s, a);
+    else if (wide && a.pairs) GQ_LAUNCH((rope_kernel<true, true, false>), grid, dim3(256), 0, s, a);
+    else if (wide) GQ_LAUNCH((rope_kernel<true, false, false>), grid, dim3(256), 0, s, a);
+    else if (a.pairs) GQ_LAUNCH((rope_kernel<false, true, false>), grid, dim3(256), 0, s, a);
+    else GQ_LAUNCH((rope_kernel<false, false, false>), grid, dim3(256), 0, s, a);
     return hipGetLastError();
 }
 

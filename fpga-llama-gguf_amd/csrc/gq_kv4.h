@@ -102,12 +102,17 @@ struct Kv4PartsArgs {
     Kv4Cache pre;   // data NULL: none
     const int32_t * pre_len;
     int members, sinks;
-    int target;     // set at launch: workgroups that the ranges are dealt to
-    int whole;      // set at launch: every segment is one range
+    // set at launch: groups with a prefix; the high word of s * member_mul is s / members (0: members is 1); rows of a workgroup, groups
+    // of them in a prefix's and in a sequence's rows, workgroups of a range; workgroups that the ranges are dealt to; every segment is
+    // one range
+    int n_group;
+    unsigned member_mul;
+    int rows, pre_groups, own_groups, pre_units, own_units;
+    int target, whole;
 };
-// n_group: groups with a prefix, 0 without one.
-size_t kv4_parts_floats(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head);
-long long kv4_parts_grid(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head);
+// n_group: groups with a prefix of up to pre_ctx positions, 0 without one.
+size_t kv4_parts_floats(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head);
+long long kv4_parts_grid(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head);
 
 // The ATTN command's part before the attention: every q head and new key normalized and rotated (gq_kernels.h, AttnArgs; q stays FP32
 // in qr), the keys and values stored. Tokens as t says.

@@ -910,69 +910,103 @@ __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_attn_kernel(Kv4
 }
 
 // ---- attention with a prefix and sinks ----
-// Segments: the groups' prefixes (number g), then the sequences' own caches (n_group + s). A segment has `units` workgroups (KV heads
-// times groups of rows) for each range of its records.
+// Segments: the groups' prefixes (number g), then the sequences' own caches (n_group + s). Each range of a segment's records has a
+// workgroup for every KV head and group of rows.
 struct Kv4Seg {
     // Records that some row sees: n_sink from 0 on, and those from `rest` on, `tiles` in all.
     int n_sink, rest, tiles;
 };
 
-__device__ __forceinline__ int kv4_groups(const Kv4PartsArgs & x) { return x.pre.data ? int(unsigned(x.a.t.n_seq) / unsigned(x.members)) : 0; }
-__device__ __forceinline__ int kv4_prefix(const Kv4PartsArgs & x, int group) { return x.pre.data ? max(0, min(x.pre_len[group], x.pre.n_ctx)) : 0; }
-__device__ __forceinline__ int kv4_units(const Kv4PartsArgs & x, bool pre, int rows) {
-    return int((unsigned(x.a.t.n_tok) * unsigned(x.a.group) * unsigned(pre ? x.members : 1) + rows - 1) / unsigned(rows)) * x.a.c.n_head_kv;
-}
+__device__ __forceinline__ int kv4_group_of(const Kv4PartsArgs & x, int s) { return x.member_mul ? int(__umulhi(unsigned(s), x.member_mul)) : s; }
+__device__ __forceinline__ int kv4_prefix(const Kv4PartsArgs & x, int group) { return max(0, min(x.pre_len[group], x.pre.n_ctx)); }
 
 // The records of a segment of which the positions from .. to - 1 and the first `sinks` are seen.
-__device__ __forceinline__ Kv4Seg kv4_records(long long from, long long to, long long sinks) {
+__device__ __forceinline__ Kv4Seg kv4_records(int from, int to, int sinks) {
     if (to <= 0) return {0, 0, 0};
-    const int end = int((to - 1) / KV4_TILE) + 1, rest = from >= to ? end : int(max(from, 0ll) / KV4_TILE);
-    const int n_sink = int(min((min(max(sinks, 0ll), to) + KV4_TILE - 1) / KV4_TILE, (long long)rest));
+    const int end = (to - 1) / KV4_TILE + 1, rest = from >= to ? end : max(from, 0) / KV4_TILE;
+    const int n_sink = min(sinks > 0 ? (min(sinks, to) - 1) / KV4_TILE + 1 : 0, rest);
     return {n_sink, rest, n_sink + end - rest};
 }
 // The positions of a sequence's live tokens in its own cache: low .. high - 1, none: high 0.
-__device__ __forceinline__ void kv4_live(const Kv4PartsArgs & x, int s, long long & low, long long & high) {
-    long long p0;
-    int n;
-    kv4_span(x.a.t, s, p0, n);
-    low = p0 < 0 ? 0 : p0;
-    high = p0 + n < x.a.c.n_ctx ? p0 + n : x.a.c.n_ctx;
-    if (low >= high) high = 0;
+__device__ __forceinline__ void kv4_live(const Kv4PartsArgs & x, int s, int & low, int & high) {
+    const int p0 = x.a.t.pos[s], n = x.a.t.num ? min(x.a.t.num[s], x.a.t.n_tok) : x.a.t.n_tok;
+    low = max(p0, 0);
+    high = n > 0 && p0 < x.a.c.n_ctx && p0 > -n ? p0 + min(n, p0 < 0 ? n : x.a.c.n_ctx - p0) : 0;
+    high = min(high, x.a.c.n_ctx);
 }
 __device__ __forceinline__ Kv4Seg kv4_own_seg(const Kv4PartsArgs & x, int s) {
-    long long low, high;
+    int low, high;
     kv4_live(x, s, low, high);
-    const int window = x.a.window;
-    const long long sinks = window ? x.sinks - (x.pre.data ? kv4_prefix(x, int(unsigned(s) / unsigned(x.members))) : 0) : 0;
-    return kv4_records(window ? low - window + 1 : 0, high, sinks);
+    if (!x.a.window) return kv4_records(0, high, 0);
+    // (a window begins at -2^31 + 1 or after)
+    return kv4_records(low - x.a.window + 1, high, x.n_group ? x.sinks - kv4_prefix(x, kv4_group_of(x, s)) : x.sinks);
 }
 __device__ __forceinline__ Kv4Seg kv4_prefix_seg(const Kv4PartsArgs & x, int group) {
     const int n = kv4_prefix(x, group);
     if (!x.a.window || !n) return kv4_records(0, n, 0);
-    long long least = -1;  // the group's first live position
+    int least = INT_MAX;  // the group's first live position
     for (int i = 0; i < x.members; ++i) {
-        long long low, high;
+        int low, high;
         kv4_live(x, group * x.members + i, low, high);
-        if (high && (least < 0 || low < least)) least = low;
+        if (high) least = min(least, low);
     }
-    return least < 0 ? Kv4Seg{0, 0, 0} : kv4_records(n + least - x.a.window + 1, n, x.sinks);
+    return least == INT_MAX ? Kv4Seg{0, 0, 0} : kv4_records(int(min((long long)n + least - x.a.window + 1, (long long)INT_MAX)), n, x.sinks);
 }
 
 // The workspace: every segment's first workgroup and number of ranges, then the workgroups' sets, [workgroup][row][HD + 4] each.
 __host__ __device__ inline size_t kv4_table_floats(long long segs) { return size_t(segs + 1) / 2 * 4; }
-__device__ __forceinline__ float * kv4_sets(const Kv4PartsArgs & x) { return x.a.work + kv4_table_floats(kv4_groups(x) + (long long)x.a.t.n_seq); }
+__device__ __forceinline__ float * kv4_sets(const Kv4PartsArgs & x) { return x.a.work + kv4_table_floats(x.n_group + (long long)x.a.t.n_seq); }
 
-// What a workgroup has to do, the same in every lane: a unit of a range of a segment.
+// A segment's workgroups: its ranges times KV heads, 8 of these side by side, for every group of rows in turn: the groups that read the
+// same records are on one XCD, close in time (workgroups are dealt to the 8 XCDs in turn).
+struct Kv4Order {
+    int n, groups;  // ranges times KV heads, groups of rows
+    __device__ __forceinline__ int to(int q, int group) const {
+        const int c = q & ~7;
+        return c * groups + group * min(8, n - c) + (q & 7);
+    }
+    __device__ __forceinline__ void from(int k, int & q, int & group) const {
+        const int c = int(unsigned(k) / unsigned(8 * groups)), rest = k - c * 8 * groups, width = min(8, n - 8 * c);
+        group = int(unsigned(rest) / unsigned(width));
+        q = 8 * c + rest - group * width;
+    }
+};
+
+// What a workgroup has to do, the same in every lane: a group of rows and a KV head of a range of a segment.
 struct Kv4Piece {
-    int seg, unit, from, to;  // records from .. to - 1 of the segment's
+    int seg, head, group, from, to;  // records from .. to - 1 of the segment's
     Kv4Seg r;
 };
 
+// Sums of a wave's lanes up to each (DPP: within rows of 16, then row 15 into the next and 31 into the upper half).
+__device__ __forceinline__ int wave_upto(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);
+    return x;
+}
+__device__ __forceinline__ float wave_sum_f(float x) {
+    const auto step = [&](auto ctrl, auto rows) {
+        x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl.value, rows.value, 0xf, rows.value == 0xf));
+    };
+    step(std::integral_constant<int, 0x111>(), std::integral_constant<int, 0xf>());
+    step(std::integral_constant<int, 0x112>(), std::integral_constant<int, 0xf>());
+    step(std::integral_constant<int, 0x114>(), std::integral_constant<int, 0xf>());
+    step(std::integral_constant<int, 0x118>(), std::integral_constant<int, 0xf>());
+    step(std::integral_constant<int, 0x142>(), std::integral_constant<int, 0xa>());
+    step(std::integral_constant<int, 0x143>(), std::integral_constant<int, 0xc>());
+    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+__device__ __forceinline__ int kv4_parts_of(int tiles, int per) { return int(unsigned(tiles + per - 1) / unsigned(per)); }
+
 // Workgroup `id`'s piece; false: it has none. Every wave's lanes look at the segments together, 64 at a time (the groups, then the
-// sequences): first at all records times units, for the ranges' length, then for the segment that the workgroup falls into.
-__device__ __forceinline__ bool kv4_place(const Kv4PartsArgs & x, int id, int rows, Kv4Piece & piece) {
-    const int lane = threadIdx.x & 63, n_group = kv4_groups(x), n_seq = x.a.t.n_seq;
-    const int pre_units = n_group ? kv4_units(x, true, rows) : 0, own_units = kv4_units(x, false, rows);
+// sequences): first at all records times workgroups, for the ranges' length, then for the segment that the workgroup falls into. The
+// last workgroup, which mostly has no piece, writes the table of them.
+__device__ __forceinline__ bool kv4_place(const Kv4PartsArgs & x, int id, Kv4Piece & piece) {
+    const int lane = threadIdx.x & 63, n_group = x.n_group, n_seq = x.a.t.n_seq, heads = x.a.c.n_head_kv;
     const int pre_batches = (n_group + 63) / 64, batches = pre_batches + (n_seq + 63) / 64;
     const bool few = n_seq <= 64;  // at most one batch of each, looked at once
     const auto look = [&](int b) {
@@ -982,62 +1016,68 @@ __device__ __forceinline__ bool kv4_place(const Kv4PartsArgs & x, int id, int ro
     };
     Kv4Seg pre = {0, 0, 0}, own = {0, 0, 0};
     if (few) {
-        if (n_group) pre = look(0);
         own = look(pre_batches);
+        if (n_group) pre = look(0);
     }
     const auto seg = [&](int b) { return few ? b < pre_batches ? pre : own : look(b); };
-    int per = INT_MAX;
+    int per = 1 << 30;
     if (!x.whole) {
-        long long sum = 0;
-        for (int b = 0; b < batches; ++b) sum += (long long)seg(b).tiles * (b < pre_batches ? pre_units : own_units);
-#pragma unroll
-        for (int d = 32; d >= 1; d >>= 1) sum += __shfl_xor(sum, d, WAVE);
-        per = int(min((sum + x.target - 1) / x.target, (long long)INT_MAX / 4));
-        per = max(per, KV4_LEAST);
-    }
-    const auto ranges = [&](int tiles) { return tiles ? per == INT_MAX ? 1 : int(unsigned(tiles + per - 1) / unsigned(per)) : 0; };
-    if (id == 0 && x.a.work) {
-        int before = 0;
-        for (int b = 0; b < batches; ++b) {
-            const int units = b < pre_batches ? pre_units : own_units, n = ranges(seg(b).tiles);
-            int upto = n * units;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const int y = __shfl_up(upto, d, WAVE);
-                if (lane >= d) upto += y;
-            }
-            const int i = (b < pre_batches ? b : b - pre_batches) * 64 + lane;
-            if (threadIdx.x < 64 && i < (b < pre_batches ? n_group : n_seq))
-                reinterpret_cast<int2 *>(x.a.work)[(b < pre_batches ? 0 : n_group) + i] = int2{before + upto - n * units, n};
-            before += __shfl(upto, 63, WAVE);
+        float sum = 0.0f;
+        if (few) {
+            sum = float(own.tiles) * float(x.own_units) + (n_group ? float(pre.tiles) * float(x.pre_units) : 0.0f);
+        } else {
+            double all = 0.0;
+            for (int b = 0; b < batches; ++b) all += double(seg(b).tiles) * (b < pre_batches ? x.pre_units : x.own_units);
+            sum = float(all);
         }
+        // (roundings to FP32 are within 2^-17: the ranges are never more than the target and one a segment)
+        const float each = wave_sum_f(sum) * (1.00002f / float(x.target));
+        per = max(each < 1e9f ? int(each) + 1 : 1 << 30, KV4_LEAST);
+        // That leaves room for a short range of every segment, and a few workgroups that start when the others are done cost more
+        // than they bring: the shortest ranges, nearly, that are all there at once (us with the ones above and so: 30 and 25 at 32
+        // sequences behind 8192, 32/8 heads of 128, 22 and 18 at windows of 1024 of them; twice as many ranges 35 and 24).
+        if (few)
+            for (int k = 0, low = per, high = 2 * min(per, 1 << 29); k < 5 && low < high; ++k) {
+                const int mid = k ? (low + high) >> 1 : low;
+                const int n = kv4_parts_of(own.tiles, mid) * x.own_units + (n_group ? kv4_parts_of(pre.tiles, mid) * x.pre_units : 0);
+                const bool fits = __builtin_amdgcn_readlane(wave_upto(n), 63) <= x.target;
+                per = fits ? mid : per;
+                if (fits) high = mid;
+                else low = mid + 1;
+                if (!fits && k == 4) per = high;
+            }
     }
+    const bool table = id == int(gridDim.x) - 1 && x.a.work;
+    bool found = false;
     int before = 0;
     for (int b = 0; b < batches; ++b) {
         const Kv4Seg y = seg(b);
-        const int units = b < pre_batches ? pre_units : own_units, n = ranges(y.tiles);
-        int upto = n * units;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int z = __shfl_up(upto, d, WAVE);
-            if (lane >= d) upto += z;
+        const bool is_pre = b < pre_batches;
+        const int units = is_pre ? x.pre_units : x.own_units, n = kv4_parts_of(y.tiles, per), upto = wave_upto(n * units);
+        const int all = __builtin_amdgcn_readlane(upto, 63);
+        if (table) {
+            const int i = (is_pre ? b : b - pre_batches) * 64 + lane;
+            if (threadIdx.x < 64 && i < (is_pre ? n_group : n_seq))
+                reinterpret_cast<int2 *>(x.a.work)[(is_pre ? 0 : n_group) + i] = int2{before + upto - n * units, n};
         }
-        const int all = __shfl(upto, 63, WAVE);
-        if (id - before < all) {
+        if (!found && id - before < all) {
             const int l = __ffsll(__ballot(before + upto > id)) - 1;
             const auto get = [&](int v) { return __builtin_amdgcn_readlane(v, l); };
-            const int k = id - before - get(upto - n * units), m = get(n), tiles = get(y.tiles);  // workgroup k of the segment's m * units
-            const int j = int(unsigned(k) / unsigned(units));
-            piece.seg = (b < pre_batches ? b * 64 : n_group + (b - pre_batches) * 64) + l;
-            piece.unit = k - j * units;
+            const int k = id - before - get(upto - n * units), m = get(n), tiles = get(y.tiles);
+            int q;
+            Kv4Order{m * heads, is_pre ? x.pre_groups : x.own_groups}.from(k, q, piece.group);
+            const int j = int(unsigned(q) / unsigned(heads)), each = int(unsigned(tiles) / unsigned(m)), more = tiles - each * m;
+            piece.seg = (is_pre ? b * 64 : n_group + (b - pre_batches) * 64) + l;
+            piece.head = q - j * heads;
             piece.r = {get(y.n_sink), get(y.rest), tiles};
-            piece.from = int((long long)tiles * j / m);  // ranges of a segment are alike
-            piece.to = int((long long)tiles * (j + 1) / m);
-            return true;
+            piece.from = each * j + min(j, more);  // ranges of a segment are alike
+            piece.to = piece.from + each + (j < more);
+            found = true;
+            if (!table) return true;
         }
         before += all;
     }
-    return false;
+    return found;
 }
 
 // The rows and records of kv4_parts_kernel's workgroup.
@@ -1052,26 +1092,24 @@ struct Kv4PartRows {
     float * sets;
     const int2 * at;                  // in LDS: a row's token row (-1: none) and place in its own cache
 
-    __device__ __forceinline__ bool find(const Kv4PartsArgs & x, int ROWS, int2 * at_) {
+    template <int ROWS>
+    __device__ __forceinline__ bool find(const Kv4PartsArgs & x, const Kv4Piece & p, int2 * at_) {
         const Kv4AttnArgs & a = x.a;
-        Kv4Piece p;
-        if (!kv4_place(x, int(blockIdx.x), ROWS, p)) return false;
-        const int tid = threadIdx.x, n_group = kv4_groups(x);
-        const int seg = __builtin_amdgcn_readfirstlane(p.seg), unit = __builtin_amdgcn_readfirstlane(p.unit);
+        const int tid = threadIdx.x, n_group = x.n_group, seg = __builtin_amdgcn_readfirstlane(p.seg);
         pre = seg < n_group;
         const int id = pre ? seg : seg - n_group, members = pre ? x.members : 1;
         G = a.group;
-        h = int(unsigned(unit) % unsigned(a.c.n_head_kv));
-        row0 = int(unsigned(unit) / unsigned(a.c.n_head_kv)) * ROWS;
-        len = n_group ? __builtin_amdgcn_readfirstlane(kv4_prefix(x, pre ? id : int(unsigned(id) / unsigned(x.members)))) : 0;
+        h = __builtin_amdgcn_readfirstlane(p.head);
+        row0 = __builtin_amdgcn_readfirstlane(p.group) * ROWS;
+        len = n_group ? __builtin_amdgcn_readfirstlane(kv4_prefix(x, pre ? id : kv4_group_of(x, id))) : 0;
         window = a.window;
         windowed = window != 0;
         sink = !windowed ? 0 : pre ? min(x.sinks, len) : max(x.sinks - len, 0);
         // every lane a row (ROWS are at most 64), the workgroup's positions from all of them
         const int rows = members * a.t.n_tok * G, i = tid & (ROWS - 1);
         const bool in = row0 + i < rows;
-        const int token = id * members * a.t.n_tok + int(unsigned(in ? row0 + i : 0) / unsigned(G));
-        const int sq = int(unsigned(token) / unsigned(a.t.n_tok)), t = token - sq * a.t.n_tok;
+        const int token = id * members * a.t.n_tok + (G == 1 ? in ? row0 + i : 0 : int(unsigned(in ? row0 + i : 0) / unsigned(G)));
+        const int sq = a.t.n_tok == 1 ? token : int(unsigned(token) / unsigned(a.t.n_tok)), t = token - sq * a.t.n_tok;
         long long p0;
         int n;
         kv4_span(a.t, sq, p0, n);
@@ -1106,7 +1144,7 @@ struct Kv4PartRows {
         skip = sinks ? b0 - (f + sinks) : 0;
         alone = !a.work || (!len && r.tiles == e - f);
         head = pre ? kv4_rec(x.pre, id, h, 0) : kv4_rec(a.c, id, h, 0);
-        sets = a.work ? kv4_sets(x) + size_t(blockIdx.x) * ROWS * (a.c.head_dim + 4) : nullptr;
+        sets = a.work ? kv4_sets(x) + size_t(blockIdx.x) * x.rows * (a.c.head_dim + 4) : nullptr;
         __syncthreads();  // the rows' places are there
         if (first <= last) return true;
         if (!alone && tid < ROWS && at[tid].x >= 0) {  // the rows see nothing of the range
@@ -1140,17 +1178,23 @@ struct Kv4PartRows {
     __device__ __forceinline__ float * set(int i, size_t, int, int hd) const { return sets + size_t(i) * (hd + 4); }
 };
 
+// Times (rocprofv3): 32 sequences behind 8192 positions and up to 1024 of their own, 32/8 heads of 128 27 us, two groups of 16 behind
+// 30000, 16/4 heads of 256 71 us (a wave takes 2.6 to 3.3 us for a record, with one or two waves a SIMD: 600 instructions, one after
+// another); windows of 1024 and 64 sinks of 32 sequences, 32/8 heads of 128 18 us; of 512 tokens, 16/4 of 256 40 us; 4 sequences behind
+// 512 positions 10.5 us, a chain of four trips to memory around one record. More rows of a group's together (32 or 64, as
+// kv4_attn_kernel takes of a long prompt) change less than 5 % either way.
 template <int HD, int NQ>
 __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_parts_kernel(Kv4PartsArgs x) {
     __shared__ int2 at[16 * NQ];
+    Kv4Piece p;
     Kv4PartRows rows;
-    if (rows.find(x, 16 * NQ, at)) kv4_attend<HD, NQ>(x.a, rows);
+    if (kv4_place(x, int(blockIdx.x), p) && rows.find<16 * NQ>(x, p, at)) kv4_attend<HD, NQ>(x.a, rows);
 }
 
 // Workgroup (rows: q heads of tokens): WAVES waves a row, each its share of the row's sets, lanes HD / 4 to a set; WAVES 1: four rows
 // a workgroup.
 template <int HD, int WAVES>
-__global__ __launch_bounds__(256) void kv4_parts_join_kernel(Kv4PartsArgs x, int rows) {
+__global__ __launch_bounds__(256) void kv4_parts_join_kernel(Kv4PartsArgs x) {
     constexpr int PER = HD / 4, SETS = 64 / PER, AHEAD = 4;
     __shared__ float cl[4][2];
     __shared__ __align__(16) float part[4][HD];
@@ -1158,8 +1202,8 @@ __global__ __launch_bounds__(256) void kv4_parts_join_kernel(Kv4PartsArgs x, int
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, sub = lane / PER, e = lane % PER * 4;
     const long long all = (long long)a.t.n_seq * a.t.n_tok * a.n_head, at = WAVES == 1 ? blockIdx.x * 4ll + wave : blockIdx.x;
     if (at >= all) return;
-    const int token = int(at / a.n_head), hq = int(at - (long long)token * a.n_head), s = int(unsigned(token) / unsigned(a.t.n_tok)), t = token - s * a.t.n_tok;
-    const int n_group = kv4_groups(x), group = n_group ? int(unsigned(s) / unsigned(x.members)) : 0, G = a.group, h = int(unsigned(hq) / unsigned(G));
+    const int token = int(unsigned(at) / unsigned(a.n_head)), hq = int(at) - token * a.n_head, s = int(unsigned(token) / unsigned(a.t.n_tok)), t = token - s * a.t.n_tok;
+    const int n_group = x.n_group, group = n_group ? kv4_group_of(x, s) : 0, G = a.group, h = int(unsigned(hq) / unsigned(G));
     const int2 * table = reinterpret_cast<const int2 *>(a.work);
     const int2 own = table[n_group + s], pre = n_group ? table[group] : int2{0, 0};
     const int len = n_group ? kv4_prefix(x, group) : 0;
@@ -1167,35 +1211,43 @@ __global__ __launch_bounds__(256) void kv4_parts_join_kernel(Kv4PartsArgs x, int
     int n_tok;
     kv4_span(a.t, s, p0, n_tok);
     if (t >= n_tok || p0 + t < 0 || p0 + t >= a.c.n_ctx || (!len && own.y == 1)) return;
-    // its place in its workgroups: in that of the sequence's own ranges and in that of the prefix's
+    // its row in its workgroups: those of the sequence's own ranges and those of the prefix's
     constexpr size_t SET = HD + 4;
     const int orow = t * G + hq - h * G, prow = orow + (s - group * x.members) * a.t.n_tok * G;
+    const int og = int(unsigned(orow) / unsigned(x.rows)), pg = n_group ? int(unsigned(prow) / unsigned(x.rows)) : 0;
+    const Kv4Order oo{own.y * a.c.n_head_kv, x.own_groups}, po{pre.y * a.c.n_head_kv, x.pre_groups};
     const float * sets = kv4_sets(x);
-    const auto first = [&](int base, int row) { return sets + (size_t(base + row / rows * a.c.n_head_kv + h) * rows + row % rows) * SET; };
-    const float * ow = first(own.x, orow), * pw = first(pre.x, n_group ? prow : 0);
-    const size_t ostep = kv4_units(x, false, rows) * size_t(rows) * SET, pstep = n_group ? kv4_units(x, true, rows) * size_t(rows) * SET : 0;
     const int n = pre.y + own.y, n0 = WAVES == 1 ? 0 : n * wave / WAVES, n1 = WAVES == 1 ? n : n * (wave + 1) / WAVES;
-    const auto set = [&](int j) { return j < pre.y ? pw + j * pstep : ow + (j - pre.y) * ostep; };
+    const auto set = [&](int j) {
+        const bool first = j < pre.y;
+        const int q = (first ? j : j - pre.y) * a.c.n_head_kv + h;
+        const int k = first ? pre.x + po.to(q, pg) : own.x + oo.to(q, og), row = first ? prow - pg * x.rows : orow - og * x.rows;
+        return sets + (size_t(k) * x.rows + row) * SET;
+    };
     f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f};
     float C = KV4_LOW, L = 0.0f;
-    for (int b = n0; b < n1; b += 64) {  // 64 sets (often all) at a time
+    for (int b = n0; b < n1; b += 64) {  // 64 sets (often all) at a time: their statistics and the first sums read together
         const float2 c = b + lane < n1 ? *reinterpret_cast<const float2 *>(set(b + lane) + HD) : float2{KV4_LOW, 0.0f};
+        const int m = min(n1 - b, 64);
+        f32x4 v[AHEAD];
+        const auto fetch = [&](int j0) {
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                v[i] = j0 + i * SETS < m ? *reinterpret_cast<const f32x4 *>(set(b + j0 + i * SETS) + e) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        };
+        fetch(sub);
         const float top = fmaxf(wave_max(c.x), C), old = __builtin_amdgcn_exp2f(C - top), f = __builtin_amdgcn_exp2f(c.x - top);
         C = top;
         L = L * old + c.y * f;  // the lane's own sets'
         y *= old;
-        const int m = min(n1 - b, 64);
         for (int j0 = sub; j0 < m + sub; j0 += AHEAD * SETS) {  // (as often in every lane)
-            f32x4 v[AHEAD];
-#pragma unroll
-            for (int i = 0; i < AHEAD; ++i)
-                v[i] = j0 + i * SETS < m ? *reinterpret_cast<const f32x4 *>(set(b + j0 + i * SETS) + e) : f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i) {
                 const int j = (j0 + i * SETS) & 63;
                 const float fj = __shfl(f, j, WAVE), lj = __shfl(c.y, j, WAVE);
                 if (j0 + i * SETS < m && !(lj == 0.0f)) y += v[i] * fj;  // (sets of nothing have no sums)
             }
+            if (j0 + AHEAD * SETS < m + sub) fetch(j0 + AHEAD * SETS);
         }
     }
 #pragma unroll
@@ -1433,40 +1485,53 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
     });
 }
 
-// How a call with a prefix or sinks is launched: groups of 16 rows a workgroup, the workgroups that its ranges are dealt to and the
-// most that they can come to (every segment's units once more), and whether every segment is one range.
+// How a call with a prefix or sinks is launched: groups of 16 rows a workgroup, groups of those in a prefix's rows and in a sequence's,
+// the workgroups that its ranges are dealt to and the most that they can come to (every segment's workgroups of one range more),
+// and whether every segment is one range.
 struct Kv4Plan {
-    int nq, target;
+    int nq, pre_groups, own_groups, target;
     bool whole;
     long long grid;
 };
-static Kv4Plan kv4_plan(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head, int window, int sinks) {
-    const long long per_kv = n_tok * (long long)(n_head / c.n_head_kv);
+static Kv4Plan kv4_plan(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head, int window, int sinks) {
+    const int members = n_group ? n_seq / n_group : 1, per_kv = n_head / c.n_head_kv;
+    const long long rows = n_tok * (long long)per_kv;
     Kv4Plan p;
-    p.nq = kv4_nq(c.head_dim, n_tok, n_head / c.n_head_kv);
+    p.nq = kv4_nq(c.head_dim, n_tok, per_kv);
+    p.own_groups = int((rows + 16 * p.nq - 1) / (16 * p.nq));
+    p.pre_groups = n_group ? int((rows * members + 16 * p.nq - 1) / (16 * p.nq)) : 0;
     p.target = 256 * kv4_resident(c.head_dim, p.nq);
-    const int rows = 16 * p.nq;
-    const long long own = (per_kv + rows - 1) / rows * c.n_head_kv * n_seq;
-    const long long pre = n_group ? (per_kv * (n_seq / n_group) + rows - 1) / rows * c.n_head_kv * n_group : 0;
+    const long long own = (long long)p.own_groups * c.n_head_kv * n_seq, pre = (long long)p.pre_groups * c.n_head_kv * n_group;
     long long tiles = kv4_tiles(c.n_ctx);  // records of a sequence that its tokens see
-    if (window) tiles = std::min(tiles, (long long)window / KV4_TILE + n_tok / KV4_TILE + 3 + sinks / KV4_TILE);
+    if (window) tiles = std::min(tiles, (long long)window / KV4_TILE + n_tok / KV4_TILE + 4 + sinks / KV4_TILE);
     p.whole = !n_group && (own >= p.target || tiles <= KV4_ALONE / c.head_dim);
     p.grid = own + pre + (p.whole ? 0 : p.target);
+    if (!p.whole) {  // no more than the longest segments could have
+        const auto most = [](int n_ctx) { return (kv4_tiles(n_ctx) + KV4_LEAST - 1) / KV4_LEAST; };
+        p.grid = std::min(p.grid, own * most(c.n_ctx) + pre * most(pre_ctx));
+    }
     return p;
 }
 
-size_t kv4_parts_floats(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head) {
-    const Kv4Plan p = kv4_plan(c, n_group, n_seq, n_tok, n_head, 0, 0);
+size_t kv4_parts_floats(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head) {
+    const Kv4Plan p = kv4_plan(c, n_group, pre_ctx, n_seq, n_tok, n_head, 0, 0);
     return p.whole ? 0 : kv4_table_floats((long long)n_group + n_seq) + size_t(p.grid) * (16 * p.nq) * (c.head_dim + 4);
 }
-long long kv4_parts_grid(const Kv4Cache & c, int n_group, int n_seq, int n_tok, int n_head) {
-    return kv4_plan(c, n_group, n_seq, n_tok, n_head, 0, 0).grid;
+long long kv4_parts_grid(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head) {
+    return kv4_plan(c, n_group, pre_ctx, n_seq, n_tok, n_head, 0, 0).grid;
 }
 
 hipError_t launch_kv4_parts(const Kv4PartsArgs & args, hipStream_t s) {
     Kv4PartsArgs x = args;
     Kv4AttnArgs & a = x.a;
-    const Kv4Plan p = kv4_plan(a.c, x.pre.data ? a.t.n_seq / x.members : 0, a.t.n_seq, a.t.n_tok, a.n_head, a.window, x.sinks);
+    const Kv4Plan p = kv4_plan(a.c, x.pre.data ? a.t.n_seq / x.members : 0, x.pre.n_ctx, a.t.n_seq, a.t.n_tok, a.n_head, a.window, x.sinks);
+    x.rows = 16 * p.nq;
+    x.n_group = x.pre.data ? a.t.n_seq / x.members : 0;
+    x.member_mul = x.members > 1 ? unsigned((0x100000000ull + unsigned(x.members) - 1) / unsigned(x.members)) : 0;  // (exact: s below 2^16)
+    x.pre_groups = p.pre_groups;
+    x.own_groups = p.own_groups;
+    x.pre_units = p.pre_groups * a.c.n_head_kv;
+    x.own_units = p.own_groups * a.c.n_head_kv;
     x.target = p.target;
     x.whole = p.whole;
     a.group = a.n_head / a.c.n_head_kv;
@@ -1479,8 +1544,8 @@ hipError_t launch_kv4_parts(const Kv4PartsArgs & args, hipStream_t s) {
             if (p.nq == 4) GQ_LAUNCH((kv4_parts_kernel<hd.value, 4>), grid, dim3(256), 0, s, x);
         if (p.whole) return;
         const long long rows = (long long)a.t.n_seq * a.t.n_tok * a.n_head;
-        if (rows <= KV4_FEW) GQ_LAUNCH((kv4_parts_join_kernel<hd.value, 4>), dim3(unsigned(rows)), dim3(256), 0, s, x, 16 * p.nq);
-        else GQ_LAUNCH((kv4_parts_join_kernel<hd.value, 1>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, s, x, 16 * p.nq);
+        if (rows <= KV4_FEW) GQ_LAUNCH((kv4_parts_join_kernel<hd.value, 4>), dim3(unsigned(rows)), dim3(256), 0, s, x);
+        else GQ_LAUNCH((kv4_parts_join_kernel<hd.value, 1>), dim3(unsigned((rows + 3) / 4)), dim3(256), 0, s, x);
     });
 }
 

@@ -198,10 +198,10 @@ namespace {
 bool kv4_parts_ok(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int n_head) {
     if (!kv4_sizes_ok(kv) || !kv4_heads_ok(kv, n_tok, n_head) || int64_t(kv->n_seq) * n_tok * n_head > GEMVQ_KV4_MAX_PART_ROWS) return false;
     if (prefix && (!kv4_sizes_ok(prefix) || prefix->n_head_kv != kv->n_head_kv || prefix->head_dim != kv->head_dim || kv->n_seq % prefix->n_seq)) return false;
-    return kv4_parts_grid(kv4_cache(kv), prefix ? prefix->n_seq : 0, kv->n_seq, n_tok, n_head) < (1 << 24);  // below 2^32 threads
+    return kv4_parts_grid(kv4_cache(kv), prefix ? prefix->n_seq : 0, prefix ? prefix->n_ctx : 0, kv->n_seq, n_tok, n_head) < (1 << 24);  // below 2^32 threads
 }
 uint64_t kv4_parts_work(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int n_head) {
-    return kv4_parts_floats(kv4_cache(kv), prefix ? prefix->n_seq : 0, kv->n_seq, n_tok, n_head) * sizeof(float);
+    return kv4_parts_floats(kv4_cache(kv), prefix ? prefix->n_seq : 0, prefix ? prefix->n_ctx : 0, kv->n_seq, n_tok, n_head) * sizeof(float);
 }
 
 int kv4_parts(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, const int32_t * prefix_len, const float * q, int64_t q_stride,

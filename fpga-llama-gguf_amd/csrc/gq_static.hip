@@ -369,7 +369,7 @@ int gemvq_rope_freqs(int n_rot, double base, double factor, int yarn_ctx, double
 
 int gemvq_rope_static(const gemvq_rope_rows * arrays, int n_arrays, int n_seq, int n_tok, int head_dim, int n_rot, int layout,
                       const double * freqs, const int32_t * pos, const int32_t * num, void * stream) {
-    if (!arrays || n_arrays < 1 || n_arrays > ROPE_ARRAYS || n_seq < 1 || n_tok < 1 || int64_t(n_seq) * n_tok > (int64_t(1) << 30))
+    if (!arrays || n_arrays < 1 || n_arrays > ROPE_ARRAYS || n_seq < 1 || n_tok < 1 || int64_t(n_seq) * n_tok >= GEMVQ_ROPE_MAX_ROWS)
         return GEMVQ_EINVAL;
     if (head_dim < 4 || head_dim % 4 || head_dim > ROPE_MAX_DIM || n_rot < 2 || n_rot % 2 || n_rot > head_dim) return GEMVQ_EINVAL;
     if ((layout != GEMVQ_ROPE_HALF && layout != GEMVQ_ROPE_PAIRS) || !freqs || !aligned(freqs, 8) || !pos || !aligned(pos, 4) || !aligned(num, 4))

@@ -432,12 +432,13 @@ int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, con
  * beta)) / (2 ln base), within 0 and n_rot - 1; m is 0.1 ln(factor) + 1, else 1.
  * Up to GEMVQ_ROPE_MAX_ARRAYS arrays (q and k) in one launch: row s * n_tok + t of x at x_row floats a row, its head h at x_head
  * floats a head, y likewise; y may be x with the same strides, else memory of its own. Rows of tokens t >= num[s], or at
- * positions below 0, are left as they were in y. head_dim: a multiple of 4, at most GEMVQ_ROPE_MAX_DIM; n_rot even; rows start at
- * multiples of 16 bytes. */
+ * positions below 0, are left as they were in y. head_dim: a multiple of 4, at most GEMVQ_ROPE_MAX_DIM; n_rot even; n_seq * n_tok below
+ * GEMVQ_ROPE_MAX_ROWS; rows start at multiples of 16 bytes. */
 #define GEMVQ_ROPE_HALF 0
 #define GEMVQ_ROPE_PAIRS 1
 #define GEMVQ_ROPE_MAX_ARRAYS 4
 #define GEMVQ_ROPE_MAX_DIM 1024
+#define GEMVQ_ROPE_MAX_ROWS (1 << 24) /* a launch has fewer than 2^32 threads */
 typedef struct {
     const float * x;
     float * y;

@@ -269,3 +269,40 @@ def test_refusals(gq):
         assert lib.gemvq_draft_verify_static(*{**ok, **b}.values(), 0) == gq.EINVAL, b
     with pytest.raises(gq.GemvqError):
         gq.draft_verify_static(0, 10, 0, 10, 10, 1, 1, P, 0, P, 1.0, 1.0, P, P, P, P, 1 << 20)
+
+
+@pytest.mark.gpu
+def test_rows_far_apart(gq, hip):
+    """Rows 2 GiB apart: the last ones beyond 32 bits of bytes and of floats."""
+    rng = np.random.default_rng(10)
+    s, k, n = 2, 2, 3000
+    x = inputs(rng, s, k, n)
+    stride = (1 << 29) + 64
+    big = hip.alloc(4 * (5 * stride + n))
+    for r in range(6):
+        hip.write(big + 4 * r * stride, x[0].reshape(6, n)[r])
+    na, out, lp = hip.alloc(8), hip.alloc(24), hip.alloc(24)
+    nw = gq.draft_work(s, k, n)
+    gq.draft_verify_static(big, stride, hip.upload(x[1]), n, n, s, k, hip.upload(x[2]), 0, hip.upload(x[3]), 1.0, 1.0, na, out, lp, hip.alloc(nw), nw)
+    check((hip.download(na, (s,), np.int32), hip.download(out, (s, k + 1), np.int32), hip.download(lp, (s, k + 1), np.float32)),
+          reference(*x[:3], None, x[3], 1.0, 1.0))
+
+
+@pytest.mark.gpu
+def test_calls_at_once(gq, hip):
+    """Calls on two streams with workspaces of their own, many times over, do not disturb one another."""
+    rng = np.random.default_rng(11)
+    s, k, n = 6, 3, 9000
+    streams = [hip.stream(), hip.stream()]
+    sides, wants = [], []
+    for _ in range(2):
+        x = inputs(rng, s, k, n)
+        nw = gq.draft_work(s, k, n)
+        sides.append([hip.upload(x[0]), hip.upload(x[1]), hip.upload(x[2]), hip.upload(x[3]), hip.alloc(4 * s), hip.alloc(4 * s * (k + 1)),
+                      hip.alloc(4 * s * (k + 1)), hip.alloc(nw), nw])
+        wants.append(reference(*x[:3], None, x[3], 1.0, 1.0))
+    for _ in range(20):
+        for (t, d, tok, u, na, out, lp, w, nw), stream in zip(sides, streams):
+            gq.draft_verify_static(t, n, d, n, n, s, k, tok, 0, u, 1.0, 1.0, na, out, lp, w, nw, stream)
+    for (_, _, _, _, na, out, lp, _, _), want in zip(sides, wants):
+        check((hip.download(na, (s,), np.int32), hip.download(out, (s, k + 1), np.int32), hip.download(lp, (s, k + 1), np.float32)), want)

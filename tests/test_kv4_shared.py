@@ -358,3 +358,47 @@ def test_refusals(gq):
         gq.kv4_attn_sink_static(kv(0), P, 256, 64, P, 256, 4, 4, P)
     with pytest.raises(gq.GemvqError):
         gq.kv4_attn_shared_static(kv(), kv(n_seq=3), P, P, 256, 64, P, 256, 4, 4, P)
+
+
+@pytest.mark.gpu
+def test_far_into_large_caches(gq, hip):
+    """A prefix of which the last KV heads lie beyond 4 GiB, seen by its sinks and a window at its end."""
+    nh, nkv, hd, plen, window, sinks = 8, 8, 256, 2200000, 60, 3
+    rng = np.random.default_rng(13)
+    nb = gq.kv4_bytes(1, plen, nkv, hd)
+    assert nb // nkv * (nkv - 1) > 4 << 30
+    prefix = gq.Kv4(hip.alloc(nb), 1, plen, nkv, hd)
+    kv, _ = _cache(gq, hip, 2, 40, nkv, hd)
+    tail = 70
+    pk, pv = _data(rng, 1, sinks + tail, nkv, hd)
+    k, v = _data(rng, 2, 40, nkv, hd)
+    q = rng.standard_normal((2, 2, nh, hd)).astype(np.float32)
+    _store(gq, hip, prefix, pk[:, :sinks], pv[:, :sinks], [0])
+    _store(gq, hip, prefix, pk[:, sinks:], pv[:, sinks:], [plen - tail])
+    _store(gq, hip, kv, k, v, [0, 0])
+    pos = [0, 30]
+    y = attend(gq, hip, kv, q, pos, None, window, sinks, hd ** -0.5, prefix, [plen])
+    kk, vv, ppk, ppv = (ref.values(x) for x in (k, v, pk, pv))
+    for s in range(2):
+        for t in range(2):
+            p = pos[s] + t
+            first = plen + p - window + 1  # of the window: some of it in the prefix
+            from_prefix = np.concatenate([np.arange(sinks), sinks + tail - (plen - first) + np.arange(plen - first)])
+            for h in range(nh):
+                want, tol = want_of(q[s, t, h].astype(np.float64), np.concatenate([ppk[0, from_prefix, h], kk[s, :p + 1, h]]),
+                                    np.concatenate([ppv[0, from_prefix, h], vv[s, :p + 1, h]]), hd ** -0.5)
+                assert (np.abs(y[s, t, h] - want) <= tol).all(), (s, t, h)
+
+
+@pytest.mark.gpu
+def test_numbers_of_tokens_that_are_too_large(gq, hip):
+    """num above n_tok counts as n_tok; prefix lengths below 0 as none."""
+    shared(gq, hip, 2, 2, 2, (4, 2, 64), 100, 50, [-5, 60], [3, 10, 0, 44], [2, 2, 2, 2], [(0, 0), (30, 2)], 3)
+    nh, nkv, hd = 4, 2, 64
+    rng = np.random.default_rng(14)
+    k, v = _data(rng, 2, 60, nkv, hd)
+    q = rng.standard_normal((2, 2, nh, hd)).astype(np.float32)
+    kv, _ = _cache(gq, hip, 2, 60, nkv, hd)
+    _store(gq, hip, kv, k, v, [0, 0])
+    y = attend(gq, hip, kv, q, [20, 50], [9, 70000], 16, 2, 0.1)
+    check(q, ref.values(k), ref.values(v), y, [20, 50], None, 16, 2, 0.1)

@@ -163,7 +163,7 @@ def test_refusals(gq):
     bad = [dict(arrays=[rows(**b)]) for b in (dict(x=0), dict(y=0), dict(x=P + 4), dict(y=P + 8), dict(xr=124), dict(xr=1022), dict(xh=126), dict(xh=64),
                                               dict(yr=64), dict(yh=130), dict(yh=-128), dict(h=0), dict(h=65536), dict(y=P, yr=2048),
                                               dict(xr=1 << 41))]
-    bad += [dict(arrays=[rows()] * 5), dict(arrays=[rows(h=40000)] * 2), dict(n_seq=0), dict(n_tok=0), dict(n_seq=1 << 16, n_tok=1 << 15), dict(dim=0),
+    bad += [dict(arrays=[rows()] * 5), dict(arrays=[rows(h=40000)] * 2), dict(n_seq=0), dict(n_tok=0), dict(n_seq=1 << 16, n_tok=1 << 15), dict(n_seq=1 << 12, n_tok=1 << 12), dict(dim=0),
             dict(dim=126, n_rot=64), dict(dim=1028), dict(n_rot=0), dict(n_rot=63), dict(n_rot=130), dict(layout=2), dict(layout=-1),
             dict(freqs=0), dict(freqs=P + 4), dict(pos=0), dict(pos=P + 2), dict(num=P + 1)]
     for b in bad:

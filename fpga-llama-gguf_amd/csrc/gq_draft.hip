@@ -5,7 +5,7 @@
 // by chance: a token is found where a sum of up to 2^20 terms passes a given number, and the borders of all of them have to be where
 // they belong.
 // 32 sequences of 4 tokens, 151936 logits (175 MB, 39 MB of them twice): 41 us (4.3 TB/s; reading them alone 31 us, the exponentials
-// without reading 25) and 21 us; one of them: 5.4 and 11 us, the second a chain of six trips to memory.
+// without reading 25) and 22 us; one of them: 5.4 and 11 us, the second a chain of six trips to memory.
 #include "gq_device.h"
 #include "gq_draft.h"
 

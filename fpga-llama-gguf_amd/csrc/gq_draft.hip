@@ -49,10 +49,10 @@ constexpr double DRAFT_NONE = 1e-290;
 // low bits.
 struct DraftExp {
     double m, c, unit;
-    float ch, cl, base, low;
+    float top, ch, cl, base, low;
     bool fast;
     __device__ __forceinline__ DraftExp(float max, double c_, const double * table) {
-        m = max;
+        m = top = max;
         c = c_;
         const double t = m * c, k = rint(t);
         fast = fabs(t) < 8192.0 && c < 1e30 && c > 1e-30;
@@ -63,19 +63,22 @@ struct DraftExp {
         unit = fast ? quick(max, table) : 1.0;
     }
     __device__ __forceinline__ double quick(float x, const double * table) const {
-        x = fminf(fmaxf(x, low), float(m));
+        x = __builtin_amdgcn_fmed3f(x, low, top);  // (NaN: low)
         const float p = x * ch, e = __builtin_fmaf(x, cl, __builtin_fmaf(x, ch, -p));
         const float u = __builtin_fmaf(p, 256.0f, base), r = __builtin_fmaf(u - base, -1.0f / 256.0f, p) + e;
         const float E = r * __builtin_fmaf(r, __builtin_fmaf(r, 0.0555041086648216f, 0.240226506959101f), 0.693147180559945f);
         const uint32_t n = __float_as_uint(u);
         const double t = table[n & 255u];
-        const double v = __hiloint2double(int(uint32_t(__double2hiint(t)) + ((n & ~255u) << 12)), __double2loint(t));
+        const double v = __hiloint2double(int(uint32_t(__double2hiint(t)) + (n << 12)), __double2loint(t));  // (N / 256 in the exponent's place)
         return __builtin_fma(v, double(E), v);
     }
     __device__ __forceinline__ double slow(float x) const { return draft_term(x, m, c); }
 };
-// The table, by all threads of the workgroup (before a barrier).
-__device__ __forceinline__ void draft_table(double * table) { table[threadIdx.x] = draft_exp2(double(threadIdx.x) / 256.0); }
+// The table, by all threads of the workgroup (before a barrier): of 2^(i / 256) with i / 256 taken off where an exponent is added.
+__device__ __forceinline__ void draft_table(double * table) {
+    const double t = draft_exp2(double(threadIdx.x) / 256.0);
+    table[threadIdx.x] = __hiloint2double(int(uint32_t(__double2hiint(t)) - (threadIdx.x << 12)), __double2loint(t));
+}
 
 __device__ __forceinline__ float draft_clean(float x) { return x == x ? fminf(x, FLT_MAX) : -__builtin_inff(); }
 __device__ __forceinline__ double draft_scale(double temperature) {

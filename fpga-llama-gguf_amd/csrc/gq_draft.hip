@@ -51,15 +51,15 @@ struct DraftExp {
     double m, c, unit;
     float top, ch, cl, base, low;
     bool fast;
-    __device__ __forceinline__ DraftExp(float max, double c_, const double * table) {
+    __device__ __forceinline__ DraftExp(float max, const DraftScale & s, const double * table) {
         m = top = max;
-        c = c_;
+        c = s.c;
         const double t = m * c, k = rint(t);
-        fast = fabs(t) < 8192.0 && c < 1e30 && c > 1e-30;
-        ch = float(c);
-        cl = float(c - double(ch));
+        fast = fabs(t) < 8192.0 && s.fast;
+        ch = s.ch;
+        cl = s.cl;
         base = 12582912.0f - 256.0f * float(fast ? k : 0.0);
-        low = float(m - 1000.0 / c);
+        low = float(m - s.reach);
         unit = fast ? quick(max, table) : 1.0;
     }
     __device__ __forceinline__ double quick(float x, const double * table) const {
@@ -81,10 +81,6 @@ __device__ __forceinline__ void draft_table(double * table) {
 }
 
 __device__ __forceinline__ float draft_clean(float x) { return x == x ? fminf(x, FLT_MAX) : -__builtin_inff(); }
-__device__ __forceinline__ double draft_scale(double temperature) {
-    return 1.4426950408889634 / (temperature > 0.0 ? temperature : 1.0);
-}
-
 // Over aligned groups of 2^SH lanes (8 to 64): DPP within rows of 16, then across them.
 template <typename F>
 __device__ __forceinline__ float over_lanes(float x, int sh, F f) {
@@ -184,7 +180,8 @@ __global__ __launch_bounds__(256) void draft_scan_kernel(DraftArgs a) {
     const int num = draft_num(a, s), token = t < a.n_draft ? a.token[(long long)s * a.n_draft + t] : -1;
     if (own ? t > num : t >= num) return;
     const float * x = own ? a.target + row * a.target_stride : a.draft + row * a.draft_stride;
-    const double c = draft_scale(own ? a.temperature : a.draft_temperature);
+    const DraftScale & sc = own ? a.scale : a.draft_scale;
+    const double c = sc.c;
     float v[PER];
     draft_load<PER>(x, a.n_vocab, chunk, v);
     draft_table(table);
@@ -202,7 +199,7 @@ __global__ __launch_bounds__(256) void draft_scan_kernel(DraftArgs a) {
 #pragma unroll
         for (int j = 0; j < PER; ++j) v[j] = draft_clean(v[j]);
     }
-    if (a.temperature == 0.0) {
+    if (a.greedy) {
 #pragma unroll
         for (int j = PER - 1; j >= 0; --j) at = v[j] == m ? draft_place<PER>(chunk, j >> 2) + (j & 3) : at;
 #pragma unroll
@@ -217,7 +214,7 @@ __global__ __launch_bounds__(256) void draft_scan_kernel(DraftArgs a) {
     m = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(m)));
     double sum = 0.0;
     if (m > -__builtin_inff()) {
-        const DraftExp e(m, c, table);
+        const DraftExp e(m, sc, table);
         if (e.fast) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) sum += e.quick(v[j], table);
@@ -247,9 +244,9 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(DraftArgs a) {
     __shared__ double total[ROWS], red[4], rest, table[256];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, chunk = blockIdx.x, s = blockIdx.y;
     const int num = draft_num(a, s);
-    const bool greedy = a.temperature == 0.0, rows_of_draft = a.draft && !greedy;
+    const bool greedy = a.greedy, rows_of_draft = a.draft && !greedy;
     const DraftWork w = draft_at(a);
-    const double c = draft_scale(a.temperature), cq = draft_scale(a.draft_temperature);
+    const double c = a.scale.c, cq = a.draft_scale.c;
     const long long trow = (long long)s * (a.n_draft + 1), drow = (long long)s * a.n_draft, trows = (long long)a.n_seq * (a.n_draft + 1);
     draft_table(table);
     // the drafted tokens, and their logits (read whether or not there are as many)
@@ -346,7 +343,7 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(DraftArgs a) {
     float px[PER], qx[PER];
     draft_load<PER>(xp, a.n_vocab, chunk, px);
     if (less) draft_load<PER>(xq, a.n_vocab, chunk, qx);
-    const DraftExp ep(m, c, table), eq(less ? top[n1 + k] : m, less ? cq : c, table);
+    const DraftExp ep(m, a.scale, table), eq(less ? top[n1 + k] : m, less ? a.draft_scale : a.scale, table);
     const double share = less ? total[k] * ep.unit / (total[n1 + k] * eq.unit) : 0.0;
     const bool fast = ep.fast && eq.fast;
     const auto weight = [&](float p, float q, int token, bool whole) {
@@ -492,6 +489,16 @@ int draft_chunks(int n_vocab, int each) { return (n_vocab + each - 1) / each; }
 
 }  // namespace
 
+DraftScale draft_scale(double temperature) {
+    DraftScale s;
+    s.c = 1.4426950408889634 / temperature;
+    s.reach = 1000.0 / s.c;
+    s.fast = s.c < 1e30 && s.c > 1e-30;
+    s.ch = s.fast ? float(s.c) : 0.0f;
+    s.cl = s.fast ? float(s.c - double(s.ch)) : 0.0f;
+    return s;
+}
+
 size_t draft_work(int n_seq, int n_draft, int n_vocab) {
     const DraftSizes z = draft_sizes(n_seq, n_draft, n_vocab);
     return size_t(n_seq) * (size_t(2 * n_draft + 1) * (sizeof(DraftStat) * draft_chunks(n_vocab, z.scan) + sizeof(float)) +
@@ -503,7 +510,7 @@ hipError_t launch_draft(const DraftArgs & args, hipStream_t s) {
     const DraftSizes z = draft_sizes(a.n_seq, a.n_draft, a.n_vocab);
     a.chunks = draft_chunks(a.n_vocab, z.scan);
     a.parts = draft_chunks(a.n_vocab, z.pick);
-    const bool draft = a.draft && a.temperature > 0.0;
+    const bool draft = a.draft && !a.greedy;
     const dim3 rows(unsigned(a.chunks), unsigned(a.n_seq * (a.n_draft + 1 + (draft ? a.n_draft : 0)))), seqs(unsigned(a.parts), unsigned(a.n_seq));
     if (z.scan == 8192) GQ_LAUNCH(draft_scan_kernel<32>, rows, dim3(256), 0, s, a);
     else GQ_LAUNCH(draft_scan_kernel<16>, rows, dim3(256), 0, s, a);

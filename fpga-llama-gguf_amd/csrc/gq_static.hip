@@ -430,8 +430,9 @@ int gemvq_draft_verify_static(const float * target, int64_t target_stride, const
     a.n_accept = n_accept;
     a.out = out;
     a.logp = logp;
-    a.temperature = temperature;
-    a.draft_temperature = draft_temperature;
+    a.greedy = temperature == 0.0;
+    a.scale = draft_scale(a.greedy ? 1.0 : temperature);
+    a.draft_scale = draft_scale(a.greedy || !draft ? 1.0 : draft_temperature);
     a.n_vocab = n_vocab;
     a.n_seq = n_seq;
     a.n_draft = n_draft;

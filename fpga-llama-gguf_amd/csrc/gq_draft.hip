@@ -4,8 +4,8 @@
 // from; the last workgroup of the sequence to be done finds the token. Sums are in 64 bits and their terms good to 2.2e-10, up and down
 // by chance: a token is found where a sum of up to 2^20 terms passes a given number, and the borders of all of them have to be where
 // they belong.
-// 32 sequences of 4 tokens, 151936 logits (175 MB, 39 MB of them twice): 41 us (4.3 TB/s; reading them alone 31 us, the exponentials
-// without reading 25) and 22 us; one of them: 5.4 and 11 us, the second a chain of six trips to memory.
+// 32 sequences of 4 tokens, 151936 logits (175 MB, 39 MB of them twice): 35 us (5.0 TB/s; reading them alone 31 us) and 21 us; one of
+// them: 5.4 and 11 us, the second a chain of six trips to memory.
 #include "gq_device.h"
 #include "gq_draft.h"
 
@@ -43,10 +43,10 @@ constexpr double DRAFT_NONE = 1e-290;
 
 // The same for many logits of a row, most of it in FP32: instructions in 64 bits are what the kernels wait for otherwise (16 of them a
 // logit: 32 x 4 of 151936 took 43 us without reading anything, 31 us to read without them). x c in two parts, p + e, whose sum has 40
-// bits and more; p = N / 256 + r exactly; 2^(r + e) = 1 + E with |E| < 0.0014 in FP32, to 1e-10; 2^(N / 256) from a table of 256 in 64
-// bits, its exponent moved. The reference is 2^K, K the whole number next to c times the row's maximum, and `unit`
-// what the maximum itself gives (so that a row of one token has the probability 1). Only where |c max| is below 8192 (`fast`): N comes out of u = 256 p + 1.5 * 2^23 - 256 K, as its
-// low bits.
+// bits and more; p = N / 256 + r exactly; 2^(r + e) = 1 + E with |E| < 0.0014 in FP32, to 2.2e-10; 2^(N / 256) from a table of 256 in
+// 64 bits, its exponent moved. The reference is 2^K, K the whole number next to c times the row's maximum, and `unit` what the
+// maximum itself gives (so that a row of one token has the probability 1). Only where |c max| is below 8192 (`fast`): N comes out of
+// u = 256 p + 1.5 * 2^23 - 256 K, as its low bits.
 struct DraftExp {
     double m, c, unit;
     float top, ch, cl, base, low;
@@ -477,7 +477,7 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(DraftArgs a) {
 
 // Logits of a chunk in either kernel: the longer ones where there are enough to fill the device with them. Both kernels, us, with
 // 4096 and 2048 / 8192 and 4096: 5.4 + 11.1 / 6.2 + 11.2 at 1 x 4 of 151936, 11.2 + 11.6 / 12.1 + 10.4 at 61 x 3 of 32003 (certain,
-// half of them there), 45 + 28 / 41 + 21 at 32 x 4 of 151936.
+// half of them there), 45 + 28 / 41 + 21 at 32 x 4 of 151936, before the last steps (5.4 + 11.3, 10.3 + 10.3 and 35 + 21 now).
 struct DraftSizes {
     int scan, pick;
 };

@@ -1179,8 +1179,8 @@ struct Kv4PartRows {
 };
 
 // Times (rocprofv3): 32 sequences behind 8192 positions and up to 1024 of their own, 32/8 heads of 128 27 us, two groups of 16 behind
-// 30000, 16/4 heads of 256 73 us (a wave takes 2.6 to 3.3 us for a record, with one or two waves a SIMD: 600 instructions, one after
-// another); windows of 1024 and 64 sinks of 32 sequences, 32/8 heads of 128 18 us; of 512 tokens, 16/4 of 256 41 us; 4 sequences behind
+// 30000, 16/4 heads of 256 72 us (a wave takes 2.6 to 3.3 us for a record, with one or two waves a SIMD: 600 instructions, one after
+// another); windows of 1024 and 64 sinks of 32 sequences, 32/8 heads of 128 18 us; of 512 tokens, 16/4 of 256 40 us; 4 sequences behind
 // 512 positions 10.5 us, a chain of four trips to memory around one record. More rows of a group's together (32 or 64, as
 // kv4_attn_kernel takes of a long prompt) change less than 5 % either way.
 template <int HD, int NQ>

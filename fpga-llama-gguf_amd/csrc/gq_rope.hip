@@ -36,17 +36,19 @@ __device__ __forceinline__ float2 rope_turn(double t, double m) {
 }
 
 // Workgroup (token rows | heads): the angles of its rows once, to LDS, 64-bit work that all heads share; then its elements, WIDE in
-// pieces of four pairs, or of 16 bytes that stay, else pair by pair. The first pieces are
-// read before the angles are there. Memory bounds it: 4096 tokens of 32/8 heads of 128
-// (168 MB) are 29.4 us, 5.7 TB/s, neighbours 35.7, where a wave's access covers every other 16 bytes; one token 4.3, a launch and two trips.
+// pieces of four pairs of halves (two times 16 bytes), two neighbouring pairs (16 bytes) or 16 bytes that stay, else pair by pair. The
+// first pieces are read before the angles are there. Memory bounds it: 4096 tokens of 32/8 heads of 128 (168 MB) are 29.1 us, 5.8 TB/s,
+// of neighbours 31.4 (35.6 with four pairs a piece, where a wave's access covers every other 16 bytes); one token 4.3, a launch and two
+// trips.
 template <bool WIDE, bool PAIRS, bool MANY>
 __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
-    // pairs of a piece (elements of one that stays), its elements, pieces that a thread has on their way
-    constexpr int W = WIDE ? 4 : 1, N = 2 * W, AHEAD = 4;
+    // pairs of a piece, its elements, elements of a piece that stays, pieces that a thread has on their way; ONE: 16 bytes a piece
+    constexpr bool ONE = WIDE && PAIRS;
+    constexpr int W = !WIDE ? 1 : PAIRS ? 2 : 4, N = 2 * W, TAIL = WIDE ? 4 : 1, AHEAD = ONE ? 8 : 4;
     __shared__ float2 cs[ROPE_MAX_DIM / 2];  // tokens * n_rot / 2 of them
     __shared__ int live[256];                // rows with a position
     const int tid = threadIdx.x, half = a.n_rot / 2, tail = a.head_dim - a.n_rot;
-    const int turn = half / W, per = turn + tail / W;  // pieces of a head
+    const int turn = half / W, per = turn + tail / TAIL;  // pieces of a head
     const int row0 = int(blockIdx.x) * a.tokens, rows = min(a.tokens, a.n_seq * a.n_tok - row0);
     const int head0 = int(blockIdx.y) * a.heads, heads = min(a.heads, a.a[a.n - 1].end - head0);
     const int items = rows * heads * per, second = PAIRS ? W : half;  // where a piece's second 16 bytes (or element) are
@@ -59,7 +61,8 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
     const auto find = [&](int i) {
         Piece p;
         // quotients of numbers whose product with the divisor is below 2^32
-        const int rh = a.per_mul ? int(__umulhi(unsigned(i), a.per_mul)) : i, r = heads == 1 ? rh : heads == a.heads ? int(__umulhi(unsigned(rh), a.heads_mul)) : int(unsigned(rh) / unsigned(heads));
+        const int rh = a.per_mul ? int(__umulhi(unsigned(i), a.per_mul)) : i;
+        const int r = heads == 1 ? rh : heads == a.heads ? int(__umulhi(unsigned(rh), a.heads_mul)) : int(unsigned(rh) / unsigned(heads));
         int h = head0 + rh - r * heads, k = 0;
         p.c = i - rh * per;
         p.r = i < items ? r : -1;
@@ -72,7 +75,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
         p.x = m.x + row * m.x_row + h * m.x_head;
         p.y = m.y + row * m.y_row + h * m.y_head;
         if (p.x == p.y && p.c >= turn) p.r = -1;  // in place: nothing to copy
-        const int at = p.c >= turn ? a.n_rot + (p.c - turn) * W : PAIRS ? N * p.c : W * p.c;
+        const int at = p.c >= turn ? a.n_rot + (p.c - turn) * TAIL : PAIRS ? N * p.c : W * p.c;
         p.x += at;
         p.y += at;
         return p;
@@ -81,7 +84,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
         if (p.r < 0) return;
         if constexpr (WIDE) {
             *reinterpret_cast<f32x4 *>(v) = *reinterpret_cast<const f32x4 *>(p.x);
-            if (p.c < turn) *reinterpret_cast<f32x4 *>(v + 4) = *reinterpret_cast<const f32x4 *>(p.x + second);
+            if (!ONE && p.c < turn) *reinterpret_cast<f32x4 *>(v + N - 4) = *reinterpret_cast<const f32x4 *>(p.x + second);
         } else {
             v[0] = p.x[0];
             if (p.c < turn) v[1] = p.x[second];
@@ -108,7 +111,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RotaryArgs a) {
         }
         if constexpr (WIDE) {
             store(f32x4{z[0], z[1], z[2], z[3]}, p.y);
-            if (turns) store(f32x4{z[4], z[5], z[6], z[7]}, p.y + second);
+            if (!ONE && turns) store(f32x4{z[N - 4], z[N - 3], z[N - 2], z[N - 1]}, p.y + second);
         } else {
             p.y[0] = z[0];
             if (turns) p.y[second] = z[1];
@@ -151,14 +154,14 @@ hipError_t launch_rotary(const RotaryArgs & args, hipStream_t s) {
     int heads = 0;
     for (int i = 0; i < a.n; ++i) a.a[i].end = heads += a.a[i].n_head;
     const bool wide = a.n_rot % 8 == 0;
-    const int per = (a.n_rot / 2 + a.head_dim - a.n_rot) / (wide ? 4 : 1);  // pieces of a head
+    const int per = a.n_rot / 2 / (wide ? a.pairs ? 2 : 4 : 1) + (a.head_dim - a.n_rot) / (wide ? 4 : 1);  // pieces of a head
     const long long rows = (long long)a.n_seq * a.n_tok;
     a.tokens = std::max(1, 512 / a.n_rot);
-    // Pieces of a workgroup: one a thread, or, where that is more than the device has room for, eight. us with one, four and eight: 4.3 /
-    // 4.4 / 4.1 at 1 token of 16/4 heads of 256, 4.3 / 4.8 / 6.6 at 8 of 32/8 of 128, 62 / 42 / 38.5 at 4096 of them (29.4 with stores
-    // that pass the caches by, which these, 16 MB and more, do not fit; loads that do are 3 us longer).
-    const bool many = rows * heads * per >= 512 * 1024;
-    const int pieces = many ? 2048 : 256;
+    // Pieces of a workgroup: one a thread, or, where that is more than the device has room for, eight (16 of 16 bytes). us with one,
+    // four and eight: 4.3 / 4.4 / 4.1 at 1 token of 16/4 heads of 256, 4.3 / 4.8 / 6.6 at 8 of 32/8 of 128, 62 / 42 / 38.5 at 4096 of them
+    // (29.4 with stores that pass the caches by, which these, 16 MB and more, do not fit; loads that do are 3 us longer).
+    const bool many = rows * heads * a.head_dim >= 4 << 20;
+    const int pieces = many ? a.pairs ? 4096 : 2048 : 256;
     a.heads = std::min(heads, std::max(1, pieces / (a.tokens * per)));
     const auto mul = [](int d) { return d > 1 ? unsigned((0x100000000ull + unsigned(d) - 1) / unsigned(d)) : 0u; };
     a.per_mul = mul(per);

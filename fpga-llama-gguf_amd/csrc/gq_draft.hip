@@ -44,14 +44,14 @@ constexpr double DRAFT_NONE = 1e-290;
 // The same for many logits of a row, most of it in FP32: instructions in 64 bits are what the kernels wait for otherwise (16 of them a
 // logit: 32 x 4 of 151936 took 43 us without reading anything, 31 us to read without them). x c in two parts, p + e, whose sum has 40
 // bits and more; p = N / 256 + r exactly; 2^(r + e) = 1 + E with |E| < 0.0014 in FP32, to 2.2e-10; 2^(N / 256) from a table of 256 in
-// 64 bits, its exponent moved. The reference is 2^K, K the whole number next to c times the row's maximum, and `unit` what the
-// maximum itself gives (so that a row of one token has the probability 1). Only where |c max| is below 8192 (`fast`): N comes out of
-// u = 256 p + 1.5 * 2^23 - 256 K, as its low bits.
+// 64 bits, its exponent moved. The reference is 2^K, K the whole number next to c times the row's maximum, `unit` the exact
+// 2^(c max - K): a term is the same whatever maximum it is formed with, so a row's sums and its weights have the same errors. Only where
+// |c max| is below 8192 (`fast`): N comes out of u = 256 p + 1.5 * 2^23 - 256 K, as its low bits.
 struct DraftExp {
     double m, c, unit;
     float top, ch, cl, base, low;
     bool fast;
-    __device__ __forceinline__ DraftExp(float max, const DraftScale & s, const double * table) {
+    __device__ __forceinline__ DraftExp(float max, const DraftScale & s) {
         m = top = max;
         c = s.c;
         const double t = m * c, k = rint(t);
@@ -60,7 +60,7 @@ struct DraftExp {
         cl = s.cl;
         base = 12582912.0f - 256.0f * float(fast ? k : 0.0);
         low = float(m - s.reach);
-        unit = fast ? quick(max, table) : 1.0;
+        unit = fast ? draft_exp2(t - k) : 1.0;
     }
     __device__ __forceinline__ double quick(float x, const double * table) const {
         x = __builtin_amdgcn_fmed3f(x, low, top);  // (NaN: low)
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(256) void draft_scan_kernel(DraftArgs a) {
     m = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(m)));
     double sum = 0.0;
     if (m > -__builtin_inff()) {
-        const DraftExp e(m, sc, table);
+        const DraftExp e(m, sc);
         if (e.fast) {
 #pragma unroll
             for (int j = 0; j < PER; ++j) sum += e.quick(v[j], table);
@@ -302,13 +302,13 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(DraftArgs a) {
             ok = d == arg[lane];
         } else if (ok) {
             const double p = (double(xt) - top[lane]) * c > -1000.0 ? draft_term(xt, top[lane], c) : 0.0;
-            double q = 1.0, qs = 1.0;  // e and sums: u q / qs < p / total
+            double q = 1.0, qs = 1.0;  // e and sums, which are no less: u q / qs < p / total
             if (a.draft) {
                 const float m = top[n1 + lane];
                 q = (double(xd) - m) * cq > -1000.0 ? draft_term(xd, m, cq) : 0.0;
-                qs = m > -__builtin_inff() ? total[n1 + lane] : 1.0;
+                qs = m > -__builtin_inff() ? fmax(total[n1 + lane], q) : 1.0;
             }
-            ok = double(u) * q * total[lane] < p * qs;
+            ok = double(u) * q * fmax(total[lane], p) < p * qs;
         }
         const unsigned long long no = ~__ballot(ok);
         if (lane == 0) accepted = __ffsll(no) - 1;  // (lanes from num on say no)
@@ -328,7 +328,7 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(DraftArgs a) {
             if (lane == k) xt = draft_clean(a.target[(trow + k) * a.target_stride + tok]);
             l = (double(xt) - top[lane]) * c * 0.6931471805599453 - logsum;
         }
-        a.logp[trow + lane] = float(l);
+        a.logp[trow + lane] = float(fmin(l, 0.0));
     };
     if (greedy || !(m > -__builtin_inff())) {
         if (chunk == 0 && a.logp && lane <= k) logsum = log(total[lane]);
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(DraftArgs a) {
     float px[PER], qx[PER];
     draft_load<PER>(xp, a.n_vocab, chunk, px);
     if (less) draft_load<PER>(xq, a.n_vocab, chunk, qx);
-    const DraftExp ep(m, a.scale, table), eq(less ? top[n1 + k] : m, less ? a.draft_scale : a.scale, table);
+    const DraftExp ep(m, a.scale), eq(less ? top[n1 + k] : m, less ? a.draft_scale : a.scale);
     const double share = less ? total[k] * ep.unit / (total[n1 + k] * eq.unit) : 0.0;
     const bool fast = ep.fast && eq.fast;
     const auto weight = [&](float p, float q, int token, bool whole) {

@@ -478,12 +478,13 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(DraftArgs a) {
 // Logits of a chunk in either kernel: the longer ones where there are enough to fill the device with them. Both kernels, us, with
 // 4096 and 2048 / 8192 and 4096: 5.4 + 11.1 / 6.2 + 11.2 at 1 x 4 of 151936, 11.2 + 11.6 / 12.1 + 10.4 at 61 x 3 of 32003 (certain,
 // half of them there), 45 + 28 / 41 + 21 at 32 x 4 of 151936, before the last steps (5.4 + 11.3, 10.3 + 10.3 and 35 + 21 now).
+constexpr int DRAFT_SCAN = 4096, DRAFT_PICK = 2048;  // the shorter ones
 struct DraftSizes {
     int scan, pick;
 };
 DraftSizes draft_sizes(int n_seq, int n_draft, int n_vocab) {
     const long long row = (long long)n_seq * n_vocab;
-    return {row * (2 * n_draft + 1) >= 16 << 20 ? 8192 : 4096, row >= 1 << 20 ? 4096 : 2048};
+    return {row * (2 * n_draft + 1) >= 16 << 20 ? 2 * DRAFT_SCAN : DRAFT_SCAN, row >= 1 << 20 ? 2 * DRAFT_PICK : DRAFT_PICK};
 }
 int draft_chunks(int n_vocab, int each) { return (n_vocab + each - 1) / each; }
 
@@ -499,10 +500,10 @@ DraftScale draft_scale(double temperature) {
     return s;
 }
 
+// Of the shorter chunks whatever a call's own are (twice as many numbers at most): what a call needs never falls as its sizes grow.
 size_t draft_work(int n_seq, int n_draft, int n_vocab) {
-    const DraftSizes z = draft_sizes(n_seq, n_draft, n_vocab);
-    return size_t(n_seq) * (size_t(2 * n_draft + 1) * (sizeof(DraftStat) * draft_chunks(n_vocab, z.scan) + sizeof(float)) +
-                            4 * sizeof(double) * draft_chunks(n_vocab, z.pick) + DRAFT_LINE * sizeof(unsigned));
+    return size_t(n_seq) * (size_t(2 * n_draft + 1) * (sizeof(DraftStat) * draft_chunks(n_vocab, DRAFT_SCAN) + sizeof(float)) +
+                            4 * sizeof(double) * draft_chunks(n_vocab, DRAFT_PICK) + DRAFT_LINE * sizeof(unsigned));
 }
 
 hipError_t launch_draft(const DraftArgs & args, hipStream_t s) {
@@ -512,11 +513,11 @@ hipError_t launch_draft(const DraftArgs & args, hipStream_t s) {
     a.parts = draft_chunks(a.n_vocab, z.pick);
     const bool draft = a.draft && !a.greedy;
     const dim3 rows(unsigned(a.chunks), unsigned(a.n_seq * (a.n_draft + 1 + (draft ? a.n_draft : 0)))), seqs(unsigned(a.parts), unsigned(a.n_seq));
-    if (z.scan == 8192) GQ_LAUNCH(draft_scan_kernel<32>, rows, dim3(256), 0, s, a);
+    if (z.scan > DRAFT_SCAN) GQ_LAUNCH(draft_scan_kernel<32>, rows, dim3(256), 0, s, a);
     else GQ_LAUNCH(draft_scan_kernel<16>, rows, dim3(256), 0, s, a);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
-    if (z.pick == 4096) GQ_LAUNCH(draft_pick_kernel<16>, seqs, dim3(256), 0, s, a);
+    if (z.pick > DRAFT_PICK) GQ_LAUNCH(draft_pick_kernel<16>, seqs, dim3(256), 0, s, a);
     else GQ_LAUNCH(draft_pick_kernel<8>, seqs, dim3(256), 0, s, a);
     return hipGetLastError();
 }

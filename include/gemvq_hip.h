@@ -467,8 +467,8 @@ int gemvq_rope_static(const gemvq_rope_rows * arrays, int n_arrays, int n_seq, i
  * n_draft 0: one token of each sequence is sampled. d_t outside the vocabulary are not accepted. NaN logits count as -inf, +inf as
  * the largest finite number; a row of nothing but -inf accepts no token and has none: -1, logp 0 (as a draft row: q is 0).
  * FP32 rows `stride` >= n_vocab floats apart, 4-byte aligned; 0 <= n_draft <= GEMVQ_DRAFT_MAX, n_seq * (2 n_draft + 1) <= 65535,
- * 1 <= n_vocab <= GEMVQ_DRAFT_MAX_VOCAB. work: gemvq_draft_work() bytes, 16-byte aligned, contents do not matter; calls that may
- * overlap need one each. Outputs do not overlap inputs. */
+ * 1 <= n_vocab <= GEMVQ_DRAFT_MAX_VOCAB. work: gemvq_draft_work() bytes (0: sizes that are not served), 16-byte aligned, contents do
+ * not matter; what serves some sizes serves smaller ones. Calls that may overlap need one each. Outputs do not overlap inputs. */
 #define GEMVQ_DRAFT_MAX 32
 #define GEMVQ_DRAFT_MAX_VOCAB (1 << 20)
 uint64_t gemvq_draft_work(int n_seq, int n_draft, int n_vocab);

@@ -110,8 +110,10 @@ struct Kv4PartsArgs {
     int rows, pre_groups, own_groups, pre_units, own_units;
     int target, whole;
 };
-// n_group: groups with a prefix of up to pre_ctx positions, 0 without one.
+// n_group: groups with a prefix of up to pre_ctx positions, 0 without one. The workspace is for this call and those of smaller sizes
+// (0: no such call needs one); whole: this one needs none whatever its window.
 size_t kv4_parts_floats(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head);
+bool kv4_parts_whole(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head);
 long long kv4_parts_grid(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head);
 
 // The ATTN command's part before the attention: every q head and new key normalized and rotated (gq_kernels.h, AttnArgs; q stays FP32

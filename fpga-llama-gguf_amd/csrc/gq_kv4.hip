@@ -1513,9 +1513,27 @@ static Kv4Plan kv4_plan(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq,
     return p;
 }
 
+// No less than any call needs that has as much of something as this one and no more of anything: of sequences, groups, positions and
+// tokens. Fewer tokens may mean fewer rows a workgroup (nq), whose one group of rows is then full; groups of a prefix's rows are counted
+// as if each prefix's last one held a single row; a call without a prefix needs nothing once its sequences' workgroups are the target
+// or more, so no more than one less counts.
 size_t kv4_parts_floats(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head) {
-    const Kv4Plan p = kv4_plan(c, n_group, pre_ctx, n_seq, n_tok, n_head, 0, 0);
-    return p.whole ? 0 : kv4_table_floats((long long)n_group + n_seq) + size_t(p.grid) * (16 * p.nq) * (c.head_dim + 4);
+    const long long own_tiles = kv4_tiles(c.n_ctx), pre_tiles = kv4_tiles(pre_ctx), all_rows = n_tok * (long long)(n_head / c.n_head_kv);
+    if (!n_group && own_tiles <= KV4_ALONE / c.head_dim) return 0;
+    size_t floats = 0;
+    for (int nq = 1, most_nq = kv4_nq(c.head_dim, n_tok, n_head / c.n_head_kv); nq <= most_nq; nq *= 2) {
+        const long long size = 16 * nq, rows = nq < most_nq ? size : all_rows, target = 256 * kv4_resident(c.head_dim, nq);
+        long long own = (rows + size - 1) / size * c.n_head_kv * n_seq;
+        if (!n_group) own = std::min(own, target - 1);
+        const long long pre = (rows * n_seq + (size - 1) * n_group) / size * c.n_head_kv;
+        const auto ranges = [](long long tiles) { return (tiles + KV4_LEAST - 1) / KV4_LEAST; };
+        const long long grid = n_group ? std::min(own + pre + target, own * ranges(own_tiles) + pre * ranges(pre_tiles)) : std::min(own + target, own * ranges(own_tiles));
+        floats = std::max(floats, size_t(grid * size) * (c.head_dim + 4));
+    }
+    return kv4_table_floats((long long)n_group + n_seq) + floats;
+}
+bool kv4_parts_whole(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head) {
+    return kv4_plan(c, n_group, pre_ctx, n_seq, n_tok, n_head, 0, 0).whole;
 }
 long long kv4_parts_grid(const Kv4Cache & c, int n_group, int pre_ctx, int n_seq, int n_tok, int n_head) {
     return kv4_plan(c, n_group, pre_ctx, n_seq, n_tok, n_head, 0, 0).grid;

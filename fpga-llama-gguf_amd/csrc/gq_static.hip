@@ -14,6 +14,7 @@
 
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <mutex>
 
@@ -200,8 +201,9 @@ bool kv4_parts_ok(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int
     if (prefix && (!kv4_sizes_ok(prefix) || prefix->n_head_kv != kv->n_head_kv || prefix->head_dim != kv->head_dim || kv->n_seq % prefix->n_seq)) return false;
     return kv4_parts_grid(kv4_cache(kv), prefix ? prefix->n_seq : 0, prefix ? prefix->n_ctx : 0, kv->n_seq, n_tok, n_head) < (1 << 24);  // below 2^32 threads
 }
+// At least 16 bytes (0 says that sizes are not served).
 uint64_t kv4_parts_work(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int n_head) {
-    return kv4_parts_floats(kv4_cache(kv), prefix ? prefix->n_seq : 0, prefix ? prefix->n_ctx : 0, kv->n_seq, n_tok, n_head) * sizeof(float);
+    return std::max<uint64_t>(16, kv4_parts_floats(kv4_cache(kv), prefix ? prefix->n_seq : 0, prefix ? prefix->n_ctx : 0, kv->n_seq, n_tok, n_head) * sizeof(float));
 }
 
 int kv4_parts(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, const int32_t * prefix_len, const float * q, int64_t q_stride,
@@ -210,7 +212,8 @@ int kv4_parts(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, const int32_t * pr
     Kv4PartsArgs x{};
     if (!kv4_ok(kv) || !kv4_tokens(kv, n_tok, pos, num, x.a.t) || !kv4_parts_ok(kv, prefix, n_tok, n_head) || window < 0 || sinks < 0) return GEMVQ_EINVAL;
     if (prefix && (!kv4_ok(prefix) || !prefix_len || !aligned(prefix_len, 4))) return GEMVQ_EINVAL;
-    const uint64_t need = kv4_parts_work(kv, prefix, n_tok, n_head);
+    const bool none = kv4_parts_whole(kv4_cache(kv), prefix ? prefix->n_seq : 0, prefix ? prefix->n_ctx : 0, kv->n_seq, n_tok, n_head);
+    const uint64_t need = none ? 0 : kv4_parts_work(kv, prefix, n_tok, n_head);
     if (work_bytes < need || (need && (!work || !aligned(work, 16)))) return GEMVQ_EINVAL;
     const int64_t hd = kv->head_dim;
     if (!rows_ok(q, q_stride, hd) || q_head_stride % 4 || q_head_stride < hd || q_head_stride > (int64_t(1) << 40) ||

@@ -363,7 +363,7 @@ def kv4_attn_static(kv: Kv4, q: int, q_stride: int, q_head_stride: int, y: int, 
 
 
 def kv4_attn_sink_work(kv: Kv4, n_tok: int, n_head: int) -> int:
-    """Bytes of workspace of kv4_attn_sink_static."""
+    """Bytes of workspace of kv4_attn_sink_static, and of its calls of smaller sizes (0: sizes that are not served)."""
     return hip_lib().gemvq_kv4_attn_sink_work(kv, n_tok, n_head)
 
 
@@ -376,7 +376,7 @@ def kv4_attn_sink_static(kv: Kv4, q: int, q_stride: int, q_head_stride: int, y: 
 
 
 def kv4_attn_shared_work(kv: Kv4, prefix: Kv4, n_tok: int, n_head: int) -> int:
-    """Bytes of workspace of kv4_attn_shared_static (0: sizes that are not served)."""
+    """Bytes of workspace of kv4_attn_shared_static, and of its calls of smaller sizes (0: sizes that are not served)."""
     return hip_lib().gemvq_kv4_attn_shared_work(kv, prefix, n_tok, n_head)
 
 
@@ -429,7 +429,7 @@ def rope_static(arrays, n_seq: int, n_tok: int, head_dim: int, n_rot: int, layou
 
 
 def draft_work(n_seq: int, n_draft: int, n_vocab: int) -> int:
-    """Bytes of workspace of draft_verify_static (0: sizes that are not served)."""
+    """Bytes of workspace of draft_verify_static, and of its calls of smaller sizes (0: sizes that are not served)."""
     return hip_lib().gemvq_draft_work(n_seq, n_draft, n_vocab)
 
 

@@ -360,14 +360,15 @@ int gemvq_kv4_load_static(const gemvq_kv4 * kv, float * k, float * v, int64_t ro
  * the row's largest, or 2^-31 where that is 2^9 above all others, and scales no finer than 2^-30 of the largest among the
  * positions read together). A block of values that
  * has no finite scale comes out NaN in the rows that see its position; what other positions hold does not reach a row. work:
- * gemvq_kv4_attn_work() bytes of device memory, 16-byte aligned, whose contents do not matter before or after; calls that may
- * overlap need one each. */
+ * gemvq_kv4_attn_work() bytes of device memory (for these very sizes: fewer sequences or tokens may need more; 0 also where none is
+ * needed), 16-byte aligned, whose contents do not matter before or after; calls that may overlap need one each. */
 uint64_t gemvq_kv4_attn_work(const gemvq_kv4 * kv, int n_tok, int n_head);
 int gemvq_kv4_attn_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
                           int64_t y_stride, int n_tok, int n_head, const int32_t * pos, const int32_t * num, int window,
                           float scale, void * work, uint64_t work_bytes, void * stream);
 /* Attention with sinks: as gemvq_kv4_attn_static, the token at position p seeing the positions j <= p with j < sinks or j > p -
- * window (window 0: all of them). n_seq * n_tok * n_head <= GEMVQ_KV4_MAX_PART_ROWS. work: gemvq_kv4_attn_sink_work() bytes. */
+ * window (window 0: all of them). n_seq * n_tok * n_head <= GEMVQ_KV4_MAX_PART_ROWS. work: gemvq_kv4_attn_sink_work() bytes (0:
+ * sizes that are not served); what serves some sizes serves smaller ones, with fewer sequences, positions or tokens of the same heads. */
 #define GEMVQ_KV4_MAX_PART_ROWS (1 << 22)
 uint64_t gemvq_kv4_attn_sink_work(const gemvq_kv4 * kv, int n_tok, int n_head);
 int gemvq_kv4_attn_sink_static(const gemvq_kv4 * kv, const float * q, int64_t q_stride, int64_t q_head_stride, float * y,
@@ -378,7 +379,8 @@ int gemvq_kv4_attn_sink_static(const gemvq_kv4 * kv, const float * q, int64_t q_
  * kv->n_seq / prefix->n_seq (a whole number). Positions 0 .. P - 1 of a sequence are the first P = prefix_len[g] (int32 in device
  * memory, taken within 0 .. prefix->n_ctx) of its group's region, the others those of its own region of kv: token t stands at
  * place pos[s] + t there (0 .. kv->n_ctx - 1), its position is P + pos[s] + t. It sees the positions j up to its own with j < sinks or j >
- * position - window (window 0: all of them). Everything else as in the calls above. */
+ * position - window (window 0: all of them). Everything else as in the calls above (work: gemvq_kv4_attn_shared_work() bytes, which
+ * serve fewer groups and shorter prefixes too). */
 uint64_t gemvq_kv4_attn_shared_work(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, int n_tok, int n_head);
 int gemvq_kv4_attn_shared_static(const gemvq_kv4 * kv, const gemvq_kv4 * prefix, const int32_t * prefix_len, const float * q,
                                  int64_t q_stride, int64_t q_head_stride, float * y, int64_t y_stride, int n_tok, int n_head,

@@ -366,7 +366,11 @@ int gemvq_rope_freqs(int n_rot, double base, double factor, int yarn_ctx, double
     if (yarn_ctx && !(beta_slow > 0 && beta_fast >= beta_slow && std::isfinite(beta_fast))) return GEMVQ_EINVAL;
     for (int i = 0; factors && i < n_rot / 2; ++i)
         if (!(factors[i] > 0) || !std::isfinite(factors[i])) return GEMVQ_EINVAL;
-    rope_table(n_rot, base, factor, yarn_ctx, beta_fast, beta_slow, factors, freqs);
+    double table[ROPE_MAX_DIM / 2 + 1];
+    rope_table(n_rot, base, factor, yarn_ctx, beta_fast, beta_slow, factors, table);
+    for (int i = 0; i <= n_rot / 2; ++i)
+        if (!std::isfinite(table[i])) return GEMVQ_EINVAL;  // divisors next to 0
+    std::copy(table, table + n_rot / 2 + 1, freqs);
     return 0;
 }
 

@@ -389,6 +389,8 @@ int gemvq_rope_static(const gemvq_rope_rows * arrays, int n_arrays, int n_seq, i
         if (!rows_ok(r.x, r.x_row, head_dim) || !rows_ok(r.y, r.y_row, head_dim) || !rows_ok(r.x, r.x_head, head_dim) || !rows_ok(r.y, r.y_head, head_dim))
             return GEMVQ_EINVAL;
         if (r.x == r.y && (r.x_row != r.y_row || r.x_head != r.y_head)) return GEMVQ_EINVAL;
+        for (int j = 0; j < i; ++j)  // one array's first head is written while another's is read or written
+            if (r.y == arrays[j].y || r.y == arrays[j].x || r.x == arrays[j].y) return GEMVQ_EINVAL;
         a.a[i] = {r.x, r.y, r.x_row, r.x_head, r.y_row, r.y_head, r.n_head, 0};
     }
     a.freqs = freqs;

@@ -433,7 +433,8 @@ int gemvq_beam_reorder_static(const gemvq_beam_array * arrays, int n_arrays, con
  * linearly with i, between floor and ceiling of the pairs that turn beta_fast and beta_slow times, n_rot ln(yarn_ctx / (2 pi
  * beta)) / (2 ln base), within 0 and n_rot - 1; m is 0.1 ln(factor) + 1, else 1. Refused where that is not finite.
  * Up to GEMVQ_ROPE_MAX_ARRAYS arrays (q and k) in one launch: row s * n_tok + t of x at x_row floats a row, its head h at x_head
- * floats a head, y likewise; y may be x with the same strides, else memory of its own. Rows of tokens t >= num[s], or at
+ * floats a head, y likewise; y may be x with the same strides, else memory of its own: no head of any y overlaps another head, or an
+ * x that is not its own (an array that is named twice is refused). Rows of tokens t >= num[s], or at
  * positions below 0, are left as they were in y. head_dim: a multiple of 4, at most GEMVQ_ROPE_MAX_DIM; n_rot even; n_seq * n_tok below
  * GEMVQ_ROPE_MAX_ROWS; rows start at multiples of 16 bytes. */
 #define GEMVQ_ROPE_HALF 0

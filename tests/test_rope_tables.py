@@ -1,4 +1,5 @@
-"""Tables of rotary positions at the ends of what their arguments may be: finite, or refused. (No device is touched.)"""
+"""Rotary positions: tables at the ends of what their arguments may be are finite, or refused; so are arrays that name one another's
+memory. (No device is touched.)"""
 import math
 
 import numpy as np
@@ -23,3 +24,12 @@ def test_pairs_that_keep_their_angle_do_not_depend_on_the_factor(gq):
     plain, stretched = gq.rope_freqs(64, 1e4), gq.rope_freqs(64, 1e4, factor=1e300, yarn_ctx=4096)
     kept = max(math.floor(64 * math.log(4096 / (2 * math.pi * 32)) / (2 * math.log(1e4))), 0)
     assert kept > 0 and np.array_equal(plain[:kept + 1], stretched[:kept + 1])
+
+
+def test_an_array_named_twice_is_refused(gq):
+    """In place or not: its heads would turn twice, or be read while another workgroup writes them."""
+    lib, P = gq.hip_lib(), 1 << 20
+    a, b, c, d = P, 2 * P, 3 * P, 4 * P
+    for pairs in ([(a, a), (a, a)], [(a, b), (c, b)], [(a, b), (b, d)], [(b, d), (a, b)], [(a, b), (c, d), (P * 5, a)], [(a, a), (b, b), (c, c), (b, d)]):
+        arr = (gq.RopeRows * len(pairs))(*(gq.RopeRows(x, y, 1024, 128, 1024, 128, 8) for x, y in pairs))
+        assert lib.gemvq_rope_static(arr, len(arr), 2, 3, 128, 64, 0, P, P, P, 0) == gq.EINVAL, pairs

@@ -1,8 +1,8 @@
 // Verification of drafted tokens (gq_draft.h), in two launches. The first reads every logit once: the maximum and the sum of
 // exponentials of every chunk of a row (and, at temperature 0, the place of the maximum). In the second, every workgroup of a sequence
 // joins its rows' chunks, decides how many tokens stand, and sums what is left of one chunk of the one row that a new token comes
-// from; the last workgroup of the sequence to be done finds the token. Sums are in 64 bits and their terms good to 2.2e-10, up and down
-// by chance: a token is found where a sum of up to 2^20 terms passes a given number, and the borders of all of them have to be where
+// from; the last workgroup of the sequence to be done finds the token. Sums are in 64 bits and their terms good to 2.2e-10 (3.6e-10 where logits over the
+// temperature pass 1400), up and down by chance: a token is found where a sum of up to 2^20 terms passes a given number, and the borders of all of them have to be where
 // they belong.
 // 32 sequences of 4 tokens, 151936 logits (175 MB, 39 MB of them twice): 35 us (5.0 TB/s; reading them alone 31 us) and 21 us; one of
 // them: 5.4 and 11 us, the second a chain of six trips to memory.
@@ -43,10 +43,13 @@ constexpr double DRAFT_NONE = 1e-290;
 
 // The same for many logits of a row, most of it in FP32: instructions in 64 bits are what the kernels wait for otherwise (16 of them a
 // logit: 32 x 4 of 151936 took 43 us without reading anything, 31 us to read without them). x c in two parts, p + e, whose sum has 40
-// bits and more; p = N / 256 + r exactly; 2^(r + e) = 1 + E with |E| < 0.0014 in FP32, to 2.2e-10; 2^(N / 256) from a table of 256 in
-// 64 bits, its exponent moved. The reference is 2^K, K the whole number next to c times the row's maximum, `unit` the exact
-// 2^(c max - K): a term is the same whatever maximum it is formed with, so a row's sums and its weights have the same errors. Only where
-// |c max| is below 8192 (`fast`): N comes out of u = 256 p + 1.5 * 2^23 - 256 K, as its low bits.
+// bits and more; p = N / 256 + r exactly, |r| <= 2^-9; 2^(r + e) = 1 + E in FP32; 2^(N / 256) from a table of 256 in 64 bits, its
+// exponent moved. With X = |x c| (below 9192), |r + e| < 2^-9 + 2^-23 X < 0.0031. What is rounded, in parts of a term: r + e by 2^-33
+// (8.1e-11), its factor by 2^-25 and ln 2 in it by 1.9e-9 (times |r + e|), E, up to 0.0022, by 2^-33 (2^-34 below 2^-9), e by half a step of
+// 2^-23 X and c by 2^-48: 2.2e-10 for X up to 2024, 3.6e-10 for all (the most that was seen: 2.1e-10, 2.4e-10).
+// The reference is 2^K, K the whole number next to c times the row's maximum, `unit` the exact 2^(c max - K): a term is the same whatever
+// maximum it is formed with, so a row's sums and its weights have the same errors. Only where |c max| is below 8192 (`fast`): N comes
+// out of u = 256 p + 1.5 * 2^23 - 256 K, as its low bits.
 struct DraftExp {
     double m, c, unit;
     float top, ch, cl, base, low;

@@ -458,8 +458,8 @@ int gemvq_rope_static(const gemvq_rope_rows * arrays, int n_arrays, int n_seq, i
  * larger: n_draft; below 0: the sequence is not in use, and its outputs are left as they were), target logits in rows s *
  * (n_draft + 1) + t for t = 0 .. num[s] (row t is what the target says of d_t, the last row of the token behind them), and the
  * draft's logits in rows s * n_draft + t (draft NULL: its tokens are certain, q_t is 1 at d_t and 0 elsewhere). p_t and q_t are the
- * distributions e^(logit / temperature) / sum, summed in 64 bits, each term good to 2.2e-10 (temperatures of 1e-30 to 1e30; terms
- * below 2^-1000 of the row's largest count as 0). d_t is accepted if u_t q_t(d_t) < p_t(d_t), u_t = uniform[s * (n_draft +
+ * distributions e^(logit / temperature) / sum, summed in 64 bits, each term good to 2.2e-10, or 3.6e-10 where logits over the temperature
+ * pass 1400 either way (temperatures of 1e-30 to 1e30; terms below 2^-1000 of the row's largest count as 0). d_t is accepted if u_t q_t(d_t) < p_t(d_t), u_t = uniform[s * (n_draft +
  * 1) + t] in [0, 1), and all before it are. A new token follows: at the first d_t that is not accepted from max(p_t - q_t, 0)
  * over its sum (p_t where nothing is left), behind the last from the last row's p: the first token whose weights up to and with its own sum to
  * more than uniform[s * (n_draft + 1) + n_draft] times the sum of all (none does: the last with a weight). n_accept[s]: how many

@@ -4,7 +4,7 @@
 // from; the last workgroup of the sequence to be done finds the token. Sums are in 64 bits and their terms good to 2.2e-10 (3.6e-10 where logits over the
 // temperature pass 1400), up and down by chance: a token is found where a sum of up to 2^20 terms passes a given number, and the borders of all of them have to be where
 // they belong.
-// 32 sequences of 4 tokens, 151936 logits (175 MB, 39 MB of them twice): 35 us (5.0 TB/s; reading them alone 31 us) and 21 us; one of
+// 32 sequences of 4 tokens, 151936 logits (175 MB, 39 MB of them twice): 36 us (4.8 TB/s; reading them alone 31 us) and 22 us; one of
 // them: 5.4 and 11 us, the second a chain of six trips to memory.
 #include "gq_device.h"
 #include "gq_draft.h"
@@ -480,7 +480,7 @@ __global__ __launch_bounds__(256) void draft_pick_kernel(DraftArgs a) {
 
 // Logits of a chunk in either kernel: the longer ones where there are enough to fill the device with them. Both kernels, us, with
 // 4096 and 2048 / 8192 and 4096: 5.4 + 11.1 / 6.2 + 11.2 at 1 x 4 of 151936, 11.2 + 11.6 / 12.1 + 10.4 at 61 x 3 of 32003 (certain,
-// half of them there), 45 + 28 / 41 + 21 at 32 x 4 of 151936, before the last steps (5.4 + 11.3, 10.3 + 10.3 and 35 + 21 now).
+// half of them there), 45 + 28 / 41 + 21 at 32 x 4 of 151936, before the last steps (5.3 + 11.3, 9.9 + 10.4 and 36 + 22 now).
 constexpr int DRAFT_SCAN = 4096, DRAFT_PICK = 2048;  // the shorter ones
 struct DraftSizes {
     int scan, pick;

@@ -1180,9 +1180,11 @@ struct Kv4PartRows {
 
 // Times (rocprofv3): 32 sequences behind 8192 positions and up to 1024 of their own, 32/8 heads of 128 27 us, two groups of 16 behind
 // 30000, 16/4 heads of 256 72 us (a wave takes 2.6 to 3.3 us for a record, with one or two waves a SIMD: 600 instructions, one after
-// another); windows of 1024 and 64 sinks of 32 sequences, 32/8 heads of 128 18 us; of 512 tokens, 16/4 of 256 40 us; 4 sequences behind
-// 512 positions 10.5 us, a chain of four trips to memory around one record. More rows of a group's together (32 or 64, as
-// kv4_attn_kernel takes of a long prompt) change less than 5 % either way.
+// another); windows of 1024 and 64 sinks of 32 sequences, 32/8 heads of 128 18 us; of 512 tokens, 16/4 of 256 40 us (35 in calls one after
+// another); 4 sequences behind 512 positions 10.5 us, a chain of four trips to memory around one record. A group's rows are taken as many
+// at a time as one sequence's are (kv4_nq), whatever its members. With all members' rows counted, up to 32 or 64, a call alone in a graph:
+// 32 sequences behind 8192, 32/8 heads of 128, 35.0 and 38.9 us, 15 of 4 tokens behind 1503, heads of 64, 16.9 and 22.3; but 64 behind
+// 30000 138 and 113, of heads of 64 87 and 67.
 template <int HD, int NQ>
 __global__ __launch_bounds__(256, kv4_resident(HD, NQ)) void kv4_parts_kernel(Kv4PartsArgs x) {
     __shared__ int2 at[16 * NQ];
@@ -1487,7 +1489,10 @@ hipError_t launch_kv4_attn(const Kv4AttnArgs & args, hipStream_t s) {
 
 // How a call with a prefix or sinks is launched: groups of 16 rows a workgroup, groups of those in a prefix's rows and in a sequence's,
 // the workgroups that its ranges are dealt to and the most that they can come to (every segment's workgroups of one range more),
-// and whether every segment is one range.
+// and whether every segment is one range. That is so of short caches, and where the sequences' workgroups fill the device by themselves (us
+// so and split: 64 sequences at up to 8192, 32/8 heads of 256, 172 and 177, all at 8191 245 and 245; 256 at up to 4096, 32/8 of 128, 157 and
+// 164; 96 at up to 8192 139 and 137; a window of 1024 of 512 tokens, 16/4 of 256, 36.4 and 38.8). Rows are counted as n_tok says: one live
+// token of 512 at 30000 waits 363 us for its four workgroups, 26 in a call of one token.
 struct Kv4Plan {
     int nq, pre_groups, own_groups, target;
     bool whole;

@@ -159,7 +159,11 @@ hipError_t launch_rotary(const RotaryArgs & args, hipStream_t s) {
     a.tokens = std::max(1, 512 / a.n_rot);
     // Pieces of a workgroup: one a thread, or, where that is more than the device has room for, eight (16 of 16 bytes). us with one,
     // four and eight: 4.3 / 4.4 / 4.1 at 1 token of 16/4 heads of 256, 4.3 / 4.8 / 6.6 at 8 of 32/8 of 128, 62 / 42 / 38.5 at 4096 of them
-    // (29.4 with stores that pass the caches by, which these, 16 MB and more, do not fit; loads that do are 3 us longer).
+    // (29.4 with stores that pass the caches by, which these, 16 MB and more, do not fit; loads that do are 3 us longer). Few pieces and
+    // stores that stay, many and stores that pass by: 4.8 / 6.8 us at 128 of them (2 MB out), 8.2 / 7.2 at 512 (10 MB; neighbours 16.2 / 9.5),
+    // 13.1 / 9.7 at 1024 (20 MB; 29 / 12.9), 105 / 54 at 8192; with a kernel that reads the queries afterwards 13.5 / 12.0, 19.2 / 18.1 and
+    // 148 / 117. Where n_rot is no multiple of 8, element by element: 4096 of 32/8 heads, 58 of 128 58 us (neighbours 51), 122 of 256 155
+    // (140), for 33 and 66 at the rate of a copy; 64 of 256 53 (56).
     const bool many = rows * heads * a.head_dim >= 4 << 20;
     const int pieces = many ? a.pairs ? 4096 : 2048 : 256;
     a.heads = std::min(heads, std::max(1, pieces / (a.tokens * per)));

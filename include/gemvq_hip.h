@@ -376,8 +376,8 @@ int gemvq_kv4_attn_sink_static(const gemvq_kv4 * kv, const float * q, int64_t q_
                                int sinks, float scale, void * work, uint64_t work_bytes, void * stream);
 /* Attention of groups of sequences that share a prefix, which is held once a group and whose records are read and unpacked for 16 rows (q
  * heads behind a KV head, of tokens of the group's sequences) at a time; where one sequence alone has more than 16, for 32 (heads of up
- * to 128) or 64 (up to 64). prefix: a cache with a region for each group, of kv's n_head_kv and head_dim; group g are the sequences g * m .. g * m + m - 1, m =
- * kv->n_seq / prefix->n_seq (a whole number). Positions 0 .. P - 1 of a sequence are the first P = prefix_len[g] (int32 in device
+ * to 128) or 64 (up to 64). prefix: a cache with a region for each group, of kv's n_head_kv and head_dim; group g are the sequences
+ * g * m .. g * m + m - 1, m = kv->n_seq / prefix->n_seq (a whole number). Positions 0 .. P - 1 of a sequence are the first P = prefix_len[g] (int32 in device
  * memory, taken within 0 .. prefix->n_ctx) of its group's region, the others those of its own region of kv: token t stands at
  * place pos[s] + t there (0 .. kv->n_ctx - 1), its position is P + pos[s] + t. It sees the positions j up to its own with j < sinks or j >
  * position - window (window 0: all of them). Everything else as in the calls above (work: gemvq_kv4_attn_shared_work() bytes, which

@@ -107,3 +107,18 @@ def test_a_loop_of_verifications_with_the_workspace_of_its_largest(gq, hip):
         gq.draft_verify_static(bufs[0], n, bufs[1], n, n, few, k, bufs[2], 0, bufs[3], 1.0, 1.0, na, out, lp, work, nw)
         check_tokens((hip.download(na, (few,), np.int32), hip.download(out, (few, k + 1), np.int32), hip.download(lp, (few, k + 1), np.float32)),
                      reference(*(a[:few] for a in x[:3]), None, x[3][:few], 1.0, 1.0))
+
+
+@pytest.mark.gpu
+def test_calls_that_are_not_split_take_no_workspace(gq, hip):
+    """Short caches, and sequences enough to fill the device by themselves."""
+    for n_seq, own, (nh, nkv, hd) in ((3, 200, (8, 2, 128)), (96, 600, (32, 8, 128))):
+        rng = np.random.default_rng(18)
+        k, v = _data(rng, n_seq, own, nkv, hd)
+        kv, _ = _cache(gq, hip, n_seq, own, nkv, hd)
+        _store(gq, hip, kv, k, v, [0] * n_seq)
+        q, y = rng.standard_normal((n_seq, 1, nh, hd)).astype(np.float32), hip.alloc(4 * n_seq * nh * hd)
+        pos = rng.integers(0, own, n_seq)
+        gq.kv4_attn_sink_static(kv, hip.upload(q), nh * hd, hd, y, nh * hd, 1, nh, hip.upload(pos.astype(np.int32)), 0, 70, 3, 0.1)
+        few = slice(0, 5)
+        check(q[few], ref.values(k[few]), ref.values(v[few]), hip.download(y, q.shape, np.float32)[few], pos[few], None, 70, 3, 0.1)
